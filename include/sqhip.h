@@ -402,6 +402,89 @@ int sq_linear_small_from(const sq_matrix* mats, int32_t n_mats, const sq_produce
 int sq_linear_small_silu(const sq_matrix* mats, int32_t n_mats, const sq_producer* from, const void* x, int dtype, int64_t ldx,
                          void* out, int64_t ld_out, int32_t B, void* workspace, size_t ws_bytes, void* stream);
 
+/* ---- The heads of the q|k|v product, and attention ----
+ *
+ * What a decoder layer does between its q|k|v product and its o product (the reference's decode engine: rope_cache, attn, attn_rope,
+ * shapequant/kernels/decode_e2e.py:142-225, attn_prep, qwen35_kernels.py:50-190).  All pointers but those to the structs are device
+ * pointers; strides are in elements and of any sign for what is read; elements of a head are neighbours.
+ *
+ * sq_heads: heads in[t * in_token + h * in_head ..] of `dim` elements, written to out[t * out_token + h * out_head ..] (out may be in,
+ * with the same strides; otherwise what is written must not overlap what is read); w: norm weights [dim], or NULL.
+ * sq_rotation: of the first 2 * pairs elements of a head.  Pair i of token t turns by the angle positions[t] * freqs[i] (radians, worked
+ * out in 64 bits, so far positions are as exact as near ones) and is multiplied by scale:
+ *     a' = scale * (a cos - b sin),  b' = scale * (b cos + a sin)        (inverse: sin -> -sin)
+ * with a, b = elements i and pairs + i, or, interleaved, 2i and 2i + 1.  The other elements keep their values.  positions: int64 if
+ * positions_64, else int32; any sign.
+ * sq_cache: a layer's paged cache of keys and values; slot s of page p, head h at k + p * k_page + s * k_slot + h * k_head. */
+typedef struct sq_heads {
+    const void* in;
+    void* out;
+    const void* w;
+    int64_t in_token, in_head, out_token, out_head;
+    int32_t heads;
+} sq_heads;
+typedef struct sq_rotation {
+    const double* freqs;
+    const void* positions;
+    int32_t pairs, positions_64, interleaved, inverse;
+    float scale;
+} sq_rotation;
+typedef struct sq_cache {
+    void* k;
+    void* v;
+    int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
+    int32_t pages, page, heads, dim, dtype;
+} sq_cache;
+
+/* Rotation of the heads x of `tokens` tokens (x->w is not read); dtype: any of the three, 32-bit arithmetic, one rounding. */
+int sq_rotary(const sq_heads* x, int32_t tokens, int32_t dim, int dtype, const sq_rotation* rot, void* stream);
+
+/* RMS norm of each head of q and k (where w is not NULL), the rotation, and one rounding, in one pass:
+ *     u = x * rsqrt(mean(x^2) + eps) * (w + w_offset)      per head, in 32 bits; then the rotation of u
+ * q to q->out; k to k->out if not NULL, and, with a cache, k and the values v (as they are; v->out may be NULL) to the slots of the tokens:
+ * slots[t] = page * cache->page + slot in page, int64 if slots_64, else int32; tokens whose slot lies outside the cache (-1: padding) are not
+ * written there.  Two tokens must not name one slot.  cache NULL: v and slots NULL too.  cache->dtype = dtype. */
+int sq_qk_norm_rotary(const sq_heads* q, const sq_heads* k, const sq_heads* v, int32_t tokens, int32_t dim, int dtype, const sq_rotation* rot, int w_dtype,
+                      float eps, float w_offset, const sq_cache* cache, const void* slots, int slots_64, void* stream);
+
+/* Attention of new tokens over a paged cache that holds their own keys and values too.  Sequence b has lens[b] cached tokens and the
+ * new tokens starts[b] .. starts[b + 1] - 1 (rows of q and out), whose keys and values are in the slots behind the cached ones;
+ * slot s of sequence b is slot s % page of page table[b * ld_table + s / page].  starts NULL: most_new new tokens each.
+ * New token t of a sequence (t = 0 ..) sees all cached tokens, and new token j of its sequence if
+ *     mask NULL: j <= t (one token: a decode step; many: a chunk of a prompt)
+ *     otherwise: bit j % 64 of mask[row * ld_mask + j / 64] is set, row = starts[b] + t (a tree of drafted tokens: itself and its
+ *     ancestors); bits of j >= 64 * mask_words count as clear.
+ * Head h of q reads head h / (q_heads / cache->heads) of the cache:
+ *     s_j = scale * q . k_j,  out = sum_j softmax(s)_j v_j  over what the token sees,  lse = log(sum_j exp(s_j))  (lse NULL: not written)
+ * A token that sees nothing gets zeros and -inf.  Keys and values that a token does not see do not touch its result, whatever they hold.
+ * dtype = cache->dtype, SQ_F16 or SQ_BF16, is q's and out's type; lse is fp32 [tokens, q_heads].  dim: a multiple of 8 up to 256; q, k, v and out
+ * 16-byte aligned with strides that are multiples of 8.  Scores, softmax and sums in 32 bits, its weights rounded to dtype for
+ * the matrix instructions.  Rows of out outside starts[0] .. starts[seqs] - 1 and new tokens from the most_new-th of a sequence on are
+ * not written.  A sequence whose tokens do not fit its table row, or whose table names a page outside the cache, gets NaN.
+ * The workspace (sq_tree_attention_workspace_bytes, 256-byte aligned; may be 0) needs no preparation and is the call's own while it runs.
+ * Results do not depend on its content or on what else runs: no atomics. */
+typedef struct sq_attention {
+    const void* q;
+    void* out;
+    float* lse;
+    const int32_t* table;
+    const int32_t* lens;
+    const int32_t* starts;
+    const int64_t* mask;
+    int64_t q_token, q_head, out_token, out_head, ld_table, ld_mask;
+    int32_t tokens, seqs, most_new, q_heads, max_pages, mask_words;
+    float scale;
+} sq_attention;
+int sq_tree_attention(const sq_attention* a, const sq_cache* cache, void* workspace, size_t ws_bytes, void* stream);
+size_t sq_tree_attention_workspace_bytes(const sq_attention* a, const sq_cache* cache);
+
+/* The accepted path of a draft: row path[b * ld_path + i], i < min(counts[b], most), of sequence b's new tokens moves from slot
+ * lens[b] + path to slot lens[b] + i, in the keys and values of all `layers` (k_layer, v_layer elements apart from cache->k, cache->v).
+ * A path ascends; entries from the first one on that does not, that is negative, or whose slot is not in the table or in
+ * the cache, are ignored.  16-byte pieces where strides and addresses allow, single elements elsewhere; any dtype. */
+int sq_keep_drafted(const sq_cache* cache, int32_t layers, int64_t k_layer, int64_t v_layer, const int32_t* table, int64_t ld_table, int32_t max_pages,
+                    const int32_t* lens, const int32_t* path, int64_t ld_path, int32_t most, const int32_t* counts, int32_t seqs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

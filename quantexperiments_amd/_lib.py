@@ -40,6 +40,32 @@ class SqProducer(ctypes.Structure):
 SQ_FROM_ADDNORM, SQ_FROM_SILU_MUL = 1, 2
 
 
+class SqHeads(ctypes.Structure):
+    """struct sq_heads of include/sqhip.h."""
+    _fields_ = [("in_", ctypes.c_void_p), ("out", ctypes.c_void_p), ("w", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int64) for n in ("in_token", "in_head", "out_token", "out_head")] + [("heads", ctypes.c_int32)]
+
+
+class SqRotation(ctypes.Structure):
+    """struct sq_rotation of include/sqhip.h."""
+    _fields_ = [("freqs", ctypes.c_void_p), ("positions", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int32) for n in ("pairs", "positions_64", "interleaved", "inverse")] + [("scale", ctypes.c_float)]
+
+
+class SqCache(ctypes.Structure):
+    """struct sq_cache of include/sqhip.h."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int64) for n in ("k_page", "k_slot", "k_head", "v_page", "v_slot", "v_head")] + \
+               [(n, ctypes.c_int32) for n in ("pages", "page", "heads", "dim", "dtype")]
+
+
+class SqAttention(ctypes.Structure):
+    """struct sq_attention of include/sqhip.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "out", "lse", "table", "lens", "starts", "mask")] + \
+               [(n, ctypes.c_int64) for n in ("q_token", "q_head", "out_token", "out_head", "ld_table", "ld_mask")] + \
+               [(n, ctypes.c_int32) for n in ("tokens", "seqs", "most_new", "q_heads", "max_pages", "mask_words")] + [("scale", ctypes.c_float)]
+
+
 class SqError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"sqhip error {code}: {msg}")
@@ -126,6 +152,15 @@ def lib() -> ctypes.CDLL:
         L.sq_silu_mul.argtypes = [vp, vp, ctypes.c_int, i64, vp, i32, i32, i32, vp, vp]
         L.sq_linear_small_from.argtypes = [mp, i32, ctypes.POINTER(SqProducer), ctypes.c_int, vp, ctypes.c_int, i64, i32, vp, sz, vp]
         L.sq_linear_small_silu.argtypes = [mp, i32, ctypes.POINTER(SqProducer), vp, ctypes.c_int, i64, vp, i64, i32, vp, sz, vp]
+        hp, rp, cp = ctypes.POINTER(SqHeads), ctypes.POINTER(SqRotation), ctypes.POINTER(SqCache)
+        L.sq_rotary.argtypes = [hp, i32, i32, ctypes.c_int, rp, vp]
+        L.sq_qk_norm_rotary.argtypes = [hp, hp, hp, i32, i32, ctypes.c_int, rp, ctypes.c_int, ctypes.c_float, ctypes.c_float, cp, vp, ctypes.c_int, vp]
+        L.sq_tree_attention.argtypes = [ctypes.POINTER(SqAttention), cp, vp, sz, vp]
+        L.sq_tree_attention_workspace_bytes.argtypes = [ctypes.POINTER(SqAttention), cp]
+        L.sq_tree_attention_workspace_bytes.restype = sz
+        L.sq_keep_drafted.argtypes = [cp, i32, i64, i64, vp, i64, i32, vp, vp, i64, i32, vp, i32, vp]
+        for f in (L.sq_rotary, L.sq_qk_norm_rotary, L.sq_tree_attention, L.sq_keep_drafted):
+            f.restype = ctypes.c_int
         for f in (L.sq_dequant, L.sq_dequant_stack, L.sq_linear_small, L.sq_linear_gemm, L.sq_gemm_dense, L.sq_q8_linear, L.sq_q8_dequant,
                   L.sq_q4_embed, L.sq_addnorm, L.sq_silu_mul, L.sq_linear_small_from, L.sq_linear_small_silu, L.sq_workspace_status,
                   L.sq_workspace_reset, L.sq_noalloc_reset):
@@ -141,7 +176,8 @@ EXPORTS = ("sq_version", "sq_last_error", "sq_dequant", "sq_dequant_stack", "sq_
            "sq_workspace_status", "sq_workspace_reset", "sq_noalloc_reset", "sq_stream_spin_limit", "sq_codebook_balance",
            "sq_stream_bytes_books", "sq_stream_build_books", "sq_codebook_balance_books", "sq_stream_counts_bytes", "sq_stream_plan_device",
            "sq_stream_fill_device", "sq_stream_fill_stack_device", "sq_stream_plan_free", "sq_codebook_balance_device", "sq_codebook_relabel_device",
-           "sq_codebook_rebalance_bytes", "sq_codebook_rebalance_device")
+           "sq_codebook_rebalance_bytes", "sq_codebook_rebalance_device", "sq_rotary", "sq_qk_norm_rotary", "sq_tree_attention",
+           "sq_tree_attention_workspace_bytes", "sq_keep_drafted")
 
 
 _native = None

@@ -1,0 +1,549 @@
+// Attention of new tokens over a paged cache (sq_tree_attention): the kernels, built once per 16-bit type.
+//
+//   s_j = scale q . k_j over the keys j a token sees,  m = max s_j,  out = sum exp(s_j - m) v_j / sum exp(s_j - m)
+//
+// in one pass over the keys with the running maximum and sum.  The query heads that share a key head, of all new tokens of a
+// sequence, are the rows of one matrix (row = token * group + head in group), so a key is read once for all of them.
+//
+// A step is 32 keys.  v_mfma_f32_16x16x32 takes the keys as its A operand (lane l: key l % 16, elements 8 * (l / 16) ..) and the rows
+// as its B operand (lane l: row l % 16), so lane l holds, of row l % 16, the scores of keys 4 * (l / 16) .. + 3 and 16 + 4 * (l / 16) .. + 3: eight keys
+// which, taken in that order, are the eight consecutive k of the second product's B operand.  Its A operand, values with the
+// keys in the same order, is two transposing LDS reads (ds_read_b64_tr_b16: 16 lanes read 4 keys x 16 elements, lane i gets the 4 keys of element i).
+// So weights go from one product to the other in registers, rounded to the type once (half a step: 2^-9 of a weight in bf16, 2^-12 in fp16), and the
+// running maximum of a row, which its lanes share, scales the sums of that row without a shuffle.
+//
+// Keys and values reach LDS with global_load_lds, whole rows at a time (16 bytes per lane, a key's elements by neighbouring lanes), their
+// 16-byte pieces placed by XOR with the key's number so that 16 keys' pieces (first product) and 8 keys' pairs of pieces (transposing reads) lie in
+// different banks; the XOR is in the source address, the copy itself is linear.
+#pragma once
+#include "sq_common.h"
+
+namespace sq {
+
+struct AttnArgs {
+    const char* q;
+    char* out;
+    float* lse;
+    const char *kc, *vc;
+    const int32_t *table, *lens, *starts;
+    const int64_t* mask;
+    float* po;                   // splits > 1: sums [token, head, split, DP] and (maximum, total) [token, head, split]
+    float2v* pml;
+    int64_t q_t, q_h, o_t, o_h, k_page, k_slot, k_head, v_page, v_slot, v_head;      // bytes
+    int64_t ld_table, ld_mask;
+    int tokens, seqs, most_new, q_heads, kv_heads, group, dim, pages, page, max_pages, mask_words, row_blocks, splits;
+    int near;                    // slots of a page lie less than 2^24 bytes apart, in order
+    float scale2;                // scale * log2(e): weights are powers of two
+};
+
+constexpr int ATTN_STEP = 32;                // keys of a step
+constexpr int ATTN_KEYS_MAX = INT32_MAX - 4096;
+
+// A sequence's rows and keys.  What its arguments say beyond the buffers is cut off here: no index below leaves them.
+struct AttnSeq { int first, n, len, total; bool over; };
+__device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, int b) {
+    AttnSeq s;
+    int end;
+    if (a.starts) {
+        s.first = min(max(a.starts[b], 0), a.tokens);
+        end = min(max(a.starts[b + 1], s.first), a.tokens);
+    } else {
+        s.first = (int)min((int64_t)b * a.most_new, (int64_t)a.tokens);
+        end = (int)min((int64_t)s.first + a.most_new, (int64_t)a.tokens);
+    }
+    s.n = min(end - s.first, a.most_new);
+    s.len = max(a.lens[b], 0);
+    const int64_t cap = min((int64_t)a.max_pages * a.page, (int64_t)ATTN_KEYS_MAX), want = (int64_t)s.len + s.n;
+    s.over = want > cap;
+    s.total = (int)min(want, cap);
+    return s;
+}
+
+template <int DT> struct AttnType;
+template <> struct AttnType<SQ_F16> {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    static constexpr uint32_t INF = 0x7C00, ONE = 0x3C00;
+    static __device__ __forceinline__ float4v mfma(u32x4 x, u32x4 y, float4v c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, x), __builtin_bit_cast(v8, y), c, 0, 0, 0);
+    }
+    // (no f2h_x2: its empty asm would keep these in order)
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v){lo, hi}, half2v)); }
+    static __device__ __forceinline__ uint16_t one(float v) { return f2h(v); }
+};
+template <> struct AttnType<SQ_BF16> {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    static constexpr uint32_t INF = 0x7F80, ONE = 0x3F80;
+    static __device__ __forceinline__ float4v mfma(u32x4 x, u32x4 y, float4v c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, x), __builtin_bit_cast(v8, y), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return f2bf_x2(lo, hi); }
+    static __device__ __forceinline__ uint16_t one(float v) { return f2bf(v); }
+};
+
+typedef __attribute__((address_space(3))) char* lds_ptr;
+
+// Copies 16 bytes per lane to LDS, lane l's to `to` + 16 l, and waits for all but the newest N memory operations.  Written out, because the
+// compiler waits for every copy in flight before a transposing read; they write no register, and what reads LDS stays behind the waits (memory clobber).
+// (m0 is not the compiler's to keep anything in.)  What the compiler loads into registers itself it waits for as if these were not there, that is for more than it has to.
+__device__ __forceinline__ void attn_copy16(uint32_t to, const char* at, uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(at) : "memory");
+}
+__device__ __forceinline__ void attn_copy16(uint32_t to, const char* at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(at) : "memory");
+}
+__device__ __forceinline__ void attn_reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }      // before copies to where was read
+template <int N> __device__ __forceinline__ void attn_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// value of every lane 16, 32 and 48 lanes away combined: the four groups of lanes that hold one row
+template <typename F> __device__ __forceinline__ float groups_fold(float v, F f) {
+    const uint32_t a = __builtin_bit_cast(uint32_t, v);
+    const auto h = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+    v = f(__builtin_bit_cast(float, (uint32_t)h[0]), __builtin_bit_cast(float, (uint32_t)h[1]));
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    return f(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
+// Layout of a step's keys (or values) in LDS for heads of DP elements, and its copy
+template <int DP> struct AttnTile {
+    static constexpr int PIECES = DP / 8;                   // 16-byte pieces of a key
+    static constexpr int ROWS = 64 / PIECES;                // keys per copy
+    static constexpr int COPIES = ATTN_STEP / ROWS;
+    static constexpr int PITCH = DP * 2, BYTES = ATTN_STEP * PITCH;
+    static __device__ __forceinline__ constexpr int k_xor(int key) { return PIECES == 8 ? (key >> 1) & 7 : key & 15; }
+    static __device__ __forceinline__ constexpr int v_xor(int key) { return PIECES == 8 ? 2 * ((key >> 1) & 3) : 2 * (key & 7); }
+};
+
+// The pages of a wave's keys: 64 table entries at a time in a register, and the place of every key of one step
+struct AttnPages {
+    int window = -1;             // first page of the entries, -1: none
+    int entries;
+    int id, off;                 // lane l: of key l % 32 of the step looked up last
+    bool bad = false;
+};
+
+__device__ __forceinline__ void attn_lookup(const AttnArgs& a, const AttnSeq& s, int b, int step, int lane, AttnPages& p) {
+    const int key = min(step * ATTN_STEP + (lane & 31), s.total - 1);
+    const int pg = (int)((uint32_t)key / (uint32_t)a.page);
+    p.off = key - pg * a.page;
+    const int lo = __builtin_amdgcn_readfirstlane(pg), hi = __builtin_amdgcn_readlane(pg, 31);
+    if (p.window < 0 || lo < p.window || hi >= p.window + 64) {
+        p.window = lo;
+        p.entries = lo + lane < a.max_pages ? a.table[(int64_t)b * a.ld_table + lo + lane] : 0;
+    }
+    int id = __builtin_amdgcn_ds_bpermute((pg - p.window) * 4, p.entries);
+    if ((uint32_t)id >= (uint32_t)a.pages) id = 0, p.bad = true;
+    p.id = id;
+}
+
+// Copies the looked-up step's keys (or values) of one head to `to`: `base` is the head's first byte of the pool
+template <int DP, bool VALUES>
+__device__ __forceinline__ void attn_copy(const AttnArgs& a, const AttnSeq& s, int step, int lane, const AttnPages& p, const char* base, const char* to) {
+    typedef AttnTile<DP> T;
+    const int64_t page_b = VALUES ? a.v_page : a.k_page, slot_b = VALUES ? a.v_slot : a.k_slot;
+    const int row = lane / T::PIECES, pos = lane % T::PIECES, pieces = a.dim >> 3;
+    const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr)to);
+    auto piece = [&](int j) {                                // heads narrower than DP: their first piece again
+        const int c = pos ^ (VALUES ? T::v_xor(j * T::ROWS + row) : T::k_xor(j * T::ROWS + row));
+        return (c < pieces ? c : 0) * 16;
+    };
+    if (a.near && a.page % T::ROWS == 0 && (step + 1) * ATTN_STEP <= s.total) {       // the keys of a copy lie in one page
+#pragma unroll
+        for (int j = 0; j < T::COPIES; ++j) {
+            const int id = __builtin_amdgcn_readlane(p.id, j * T::ROWS), off = __builtin_amdgcn_readlane(p.off, j * T::ROWS);
+            attn_copy16(lds + j * 1024, base + id * page_b + off * slot_b, (uint32_t)(row * (int)slot_b + piece(j)));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < T::COPIES; ++j) {
+            const int id = __shfl(p.id, j * T::ROWS + row), off = __shfl(p.off, j * T::ROWS + row);
+            attn_copy16(lds + j * 1024, base + id * page_b + off * slot_b + piece(j));
+        }
+    }
+}
+
+// What a wave keeps of its MT * 16 rows
+template <int DP, int MT> struct AttnRows {
+    u32x4 q[MT][DP / 32];
+    float4v o[MT][DP / 16];      // lane l: row l % 16, elements 16 * i + 4 * (l / 16) .. + 3
+    float m[MT], l[MT];          // maximum (times scale2) of the row, this lane's part of the total
+    int tok[MT];                 // new token of the row
+};
+
+template <int DP, int MT>
+__device__ __forceinline__ void attn_rows_begin(const AttnArgs& a, const AttnSeq& s, int head, int row0, int lane, AttnRows<DP, MT>& r) {
+    const int rows = s.n * a.group;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int row = min(row0 + t * 16 + (lane & 15), rows - 1), tok = row / a.group;
+        const char* q = a.q + (int64_t)(s.first + tok) * a.q_t + (int64_t)(head * a.group + row - tok * a.group) * a.q_h;
+        r.tok[t] = tok;
+        r.m[t] = -INFINITY;
+        r.l[t] = 0.f;
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) {
+            const int e = c * 32 + (lane >> 4) * 8;
+            r.q[t][c] = e < a.dim ? *reinterpret_cast<const u32x4*>(q + e * 2) : u32x4{0u, 0u, 0u, 0u};
+        }
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) r.o[t][i] = float4v{0.f, 0.f, 0.f, 0.f};
+    }
+    // (here, or the loop over the keys waits for them, and so for all that is in flight, in every step)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) asm volatile("" : "+v"(r.q[t][c]));
+}
+
+// Which of a step's 32 keys a row sees
+__device__ __forceinline__ uint32_t attn_sees(const AttnArgs& a, const AttnSeq& s, int step, int tok) {
+    const int base = step * ATTN_STEP;
+    auto below = [&](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };         // keys base .. base + n - 1
+    const uint32_t there = below(s.total - base);
+    if (!a.mask) return there & below(s.len - base + tok + 1);
+    const int j = base - s.len;                              // new token of the step's first key
+    if (j <= -32) return there;
+    const int64_t* words = a.mask + (int64_t)(s.first + tok) * a.ld_mask;
+    auto word = [&](int i) { return i < a.mask_words ? (uint64_t)words[i] : 0ull; };
+    if (j < 0) return there & ((uint32_t)(word(0) << -j) | below(-j));
+    const int i = j >> 6, sh = j & 63;
+    uint64_t w = word(i) >> sh;
+    if (sh > 32) w |= word(i + 1) << (64 - sh);
+    return there & (uint32_t)w;
+}
+
+// scores of a step: keys at k
+template <int DT, int DP, int MT>
+__device__ __forceinline__ void attn_scores(const AttnRows<DP, MT>& r, const char* k, int lane, float4v (&st)[MT][2]) {
+    typedef AttnTile<DP> T;
+    const int g = lane >> 4, i16 = lane & 15;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) st[t][0] = st[t][1] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const u32x4 f = *reinterpret_cast<const u32x4*>(k + (h * 16 + i16) * T::PITCH + (((c * 4 + g) ^ T::k_xor(h * 16 + i16)) * 16));
+#pragma unroll
+            for (int t = 0; t < MT; ++t) st[t][h] = AttnType<DT>::mfma(f, r.q[t][c], st[t][h]);
+        }
+}
+
+// softmax weights of a step from its scores; the rows' maxima, totals and sums brought up to date.  sees: where masked (the same for
+// the wave; branches around little, as two whole versions of this and of attn_sums would keep the sums in registers twice)
+template <int DT, int DP, int MT>
+__device__ __forceinline__ void attn_weights(const AttnArgs& a, AttnRows<DP, MT>& r, float4v (&st)[MT][2], bool masked, const uint32_t (&sees)[MT], int lane, u32x4 (&p)[MT]) {
+    const int g = lane >> 4;
+    float mx[MT];
+    bool up = false;
+    if (masked)
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) st[t][h][i] = (sees[t] >> (h * 16 + g * 4 + i)) & 1 ? st[t][h][i] : -INFINITY;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        float v = fmaxf(fmaxf(fmaxf(st[t][0][0], st[t][0][1]), fmaxf(st[t][0][2], st[t][0][3])), fmaxf(fmaxf(st[t][1][0], st[t][1][1]), fmaxf(st[t][1][2], st[t][1][3])));
+        mx[t] = groups_fold(v, [](float x, float y) { return fmaxf(x, y); }) * a.scale2;
+        up |= mx[t] > r.m[t];
+    }
+    if (__any(up))
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const float m = fmaxf(r.m[t], mx[t]), by = r.m[t] == m ? 1.f : __builtin_amdgcn_exp2f(r.m[t] - m);
+            r.m[t] = m;
+            r.l[t] *= by;
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) r.o[t][i] *= by;
+        }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        // The exponent in one operation, exact but for its rounding, where m's own is of no account (a factor 2^(1/16) of all weights at
+        // most); of larger maxima it could reach past the largest float, so there a rounded product less m, which is zero at the maximum.
+        float m = r.m[t] == -INFINITY ? 0.f : r.m[t], by = a.scale2;      // (nothing seen so far)
+        if (__any(!(fabsf(m) <= 0x1p20f))) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float x = st[t][i >> 2][i & 3] * a.scale2;
+                asm("" : "+v"(x));                           // (not one operation again)
+                st[t][i >> 2][i & 3] = x - m;
+            }
+            m = 0.f; by = 1.f;
+        }
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][i >> 2][i & 3], by, -m));
+        r.l[t] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[t][i] = AttnType<DT>::pack(e[2 * i], e[2 * i + 1]);
+    }
+}
+
+// sums of a step: values at v.  Where masked, values that are not finite do not go through the product, whose zero weights would make NaN of
+// them in rows that do not see their keys: such elements are set to zero, the rows' keys that hold them are counted by products of zeros and ones,
+// and rows that see one get what it makes of their sum (an infinity, or NaN).
+template <int DT, int DP, int MT>
+__device__ __forceinline__ void attn_sums(AttnRows<DP, MT>& r, const char* v, int lane, const u32x4 (&p)[MT], bool masked, const uint32_t (&sees)[MT]) {
+    typedef AttnTile<DP> T;
+    typedef AttnType<DT> E;
+    typedef short short4v __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) short4v* tr_ptr;
+    const int g = lane >> 4, i16 = lane & 15, key = 4 * g + (i16 >> 2);
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+        u32x4 f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const char* at = v + (h * 16 + key) * T::PITCH + (((d * 2 + ((i16 & 3) >> 1)) ^ T::v_xor(h * 16 + key)) * 16) + (i16 & 1) * 8;
+            const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(lds_ptr)at));
+            f[2 * h] = w[0];
+            f[2 * h + 1] = w[1];
+        }
+        if (masked) {
+            u32x4 up, down;                                  // ones where a value is not below +inf, not above -inf
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t clean = 0, u = 0, n = 0;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const uint32_t b = (f[i] >> (16 * x)) & 0xFFFF;
+                    const bool nan = (b & 0x7FFF) > E::INF, inf = (b & 0x7FFF) == E::INF;
+                    if (nan || inf) any = true; else clean |= b << (16 * x);
+                    if (nan || (inf && !(b & 0x8000))) u |= E::ONE << (16 * x);
+                    if (nan || (inf && (b & 0x8000))) n |= E::ONE << (16 * x);
+                }
+                f[i] = clean; up[i] = u; down[i] = n;
+            }
+            if (__any(any))
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    u32x4 vis;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t two = sees[t] >> ((i >> 1) * 16 + g * 4 + (i & 1) * 2);
+                        vis[i] = (two & 1 ? E::ONE : 0u) | (two & 2 ? E::ONE << 16 : 0u);
+                    }
+                    const float4v zero = float4v{0.f, 0.f, 0.f, 0.f};
+                    const float4v cu = E::mfma(up, vis, zero), cd = E::mfma(down, vis, zero);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (cu[i] > 0.f) r.o[t][d][i] += INFINITY;
+                        if (cd[i] > 0.f) r.o[t][d][i] -= INFINITY;
+                    }
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) r.o[t][d] = E::mfma(f, p[t], r.o[t][d]);
+    }
+}
+
+// Joined and written: `parts` waves' sums of the same rows (each as parts x ROWS x PITCH floats in LDS), maxima and totals
+template <int DT, int DP>
+__device__ __forceinline__ void attn_write(const AttnArgs& a, const AttnSeq& s, int head, int row0, int rows_here, int split, const float* sums, const float2v* ml, int parts,
+                                           int ml_pitch, bool bad, int tid, int threads) {
+    constexpr int PITCH = DP + 4;
+    const int rows = min(s.n * a.group - row0, rows_here);
+    for (int i = tid; i < rows * (DP / 8); i += threads) {
+        const int row = i / (DP / 8), e = i % (DP / 8) * 8, all = row0 + row, tok = all / a.group, hq = head * a.group + all - tok * a.group;
+        float m = -INFINITY, l = 0.f;
+        for (int w = 0; w < parts; ++w) m = fmaxf(m, ml[w * ml_pitch + row][0]);
+        float v[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] = 0.f;
+        for (int w = 0; w < parts; ++w) {
+            const float2v one = ml[w * ml_pitch + row];
+            const float by = one[0] == m ? (m == -INFINITY ? 0.f : 1.f) : __builtin_amdgcn_exp2f(one[0] - m);
+            l += one[1] * by;
+            if (by == 0.f) continue;
+            const float4v* from = reinterpret_cast<const float4v*>(sums + (size_t)(w * rows_here + row) * PITCH + e);
+            const float4v x0 = from[0], x1 = from[1];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) { v[x] = __builtin_fmaf(x0[x], by, v[x]); v[4 + x] = __builtin_fmaf(x1[x], by, v[4 + x]); }
+        }
+        if (bad) l = NAN;
+        const int64_t tok_all = s.first + tok;
+        if (a.splits > 1) {
+            const int64_t at = (tok_all * a.q_heads + hq) * a.splits + split;
+            float4v* to = reinterpret_cast<float4v*>(a.po + at * DP + e);
+            to[0] = float4v{v[0], v[1], v[2], v[3]};
+            to[1] = float4v{v[4], v[5], v[6], v[7]};
+            if (e == 0) a.pml[at] = float2v{m, l};
+            continue;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (e < a.dim) {
+            u32x4 o;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[x] = (uint32_t)AttnType<DT>::one(v[2 * x] * inv) | ((uint32_t)AttnType<DT>::one(v[2 * x + 1] * inv) << 16);
+            *reinterpret_cast<u32x4*>(a.out + tok_all * a.o_t + (int64_t)hq * a.o_h + e * 2) = o;
+        }
+        if (e == 0 && a.lse) a.lse[tok_all * a.q_heads + hq] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+    }
+}
+
+template <int DP, int MT, int NW> constexpr int attn_lds() {
+    constexpr int ring = NW * 4 * AttnTile<DP>::BYTES, join = NW * MT * 16 * ((DP + 4) * 4 + 8) + 64;
+    return ring > join ? ring : join;
+}
+
+// Few rows (MT * 16 at a time): the waves of a workgroup share the rows and split its keys, each with two steps of keys and values of its
+// own in LDS, no barrier until the end, where their sums are joined.  Sequences are cut into `splits` workgroups too.
+template <int DT, int DP, int MT, int NW>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(1, 1))) void attn_kernel(AttnArgs a) {
+    typedef AttnTile<DP> T;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    constexpr int C = T::COPIES, ROWS = MT * 16;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int id = blockIdx.x;
+    const int split = id % a.splits; id /= a.splits;
+    const int head = id % a.kv_heads; id /= a.kv_heads;
+    const int row0 = id % a.row_blocks * ROWS, b = id / a.row_blocks;
+    const AttnSeq s = attn_seq(a, b);
+    const int rows = s.n * a.group;
+    if (row0 >= rows) return;
+    const int last = min(row0 + ROWS, rows) - 1;
+    const int seen = a.mask ? s.total : min(s.total, s.len + last / a.group + 1);            // keys that some row sees
+    const int whole = a.mask ? min(s.len, s.total) : min(s.total, s.len + row0 / a.group + 1);        // and that all do
+    const int steps = (seen + ATTN_STEP - 1) / ATTN_STEP;
+    const int per = max((steps + a.splits - 1) / a.splits, NW), begin = min(split * per, steps), end = min(begin + per, steps);
+    const int each = (end - begin + NW - 1) / NW, w0 = min(begin + wave * each, end), w1 = min(w0 + each, end);
+
+    AttnRows<DP, MT> r;
+    attn_rows_begin<DP, MT>(a, s, head, row0, lane, r);
+    AttnPages pages;
+    const char *kb = a.kc + head * a.k_head, *vb = a.vc + head * a.v_head;
+    char* ring = smem + wave * (4 * T::BYTES);
+    auto slot_k = [&](int i) { return ring + (i & 1) * T::BYTES; };
+    auto slot_v = [&](int i) { return ring + (2 + (i & 1)) * T::BYTES; };
+    auto get_k = [&](int i) {
+        attn_lookup(a, s, b, i, lane, pages);
+        attn_copy<DP, false>(a, s, i, lane, pages, kb, slot_k(i));
+    };
+    auto get_v = [&](int i) { attn_copy<DP, true>(a, s, i, lane, pages, vb, slot_v(i)); };
+    if (w0 < w1) { get_k(w0); get_v(w0); }
+    if (w0 + 1 < w1) { get_k(w0 + 1); get_v(w0 + 1); }
+    for (int i = w0; i < w1; ++i) {
+        float4v st[MT][2];
+        u32x4 p[MT];
+        uint32_t sees[MT] = {};
+        const bool masked = (i + 1) * ATTN_STEP > whole;
+        if (i + 1 < w1) attn_wait<3 * C>(); else attn_wait<C>();
+        attn_scores<DT, DP, MT>(r, slot_k(i), lane, st);
+        __builtin_amdgcn_sched_barrier(0);
+        attn_reads_done();
+        if (i + 2 < w1) get_k(i + 2);
+        if (masked)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) sees[t] = attn_sees(a, s, i, r.tok[t]);
+        attn_weights<DT, DP, MT>(a, r, st, masked, sees, lane, p);
+        if (i + 2 < w1) attn_wait<3 * C>(); else if (i + 1 < w1) attn_wait<2 * C>(); else attn_wait<0>();
+        attn_sums<DT, DP, MT>(r, slot_v(i), lane, p, masked, sees);
+        __builtin_amdgcn_sched_barrier(0);
+        attn_reads_done();
+        if (i + 2 < w1) get_v(i + 2);
+    }
+    // the waves' sums meet in LDS
+    __syncthreads();
+    constexpr int PITCH = DP + 4;
+    float* sums = reinterpret_cast<float*>(smem);
+    float2v* ml = reinterpret_cast<float2v*>(smem + NW * ROWS * PITCH * 4);
+    int* flags = reinterpret_cast<int*>(ml + NW * ROWS);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int row = t * 16 + (lane & 15);
+        const float l = groups_fold(r.l[t], [](float x, float y) { return x + y; });
+        if (lane < 16) ml[wave * ROWS + row] = float2v{r.m[t], l};
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+            *reinterpret_cast<float4v*>(sums + (size_t)(wave * ROWS + row) * PITCH + d * 16 + (lane >> 4) * 4) = r.o[t][d];
+    }
+    const bool bad = __any(pages.bad) || s.over;
+    if (lane == 0) flags[wave] = bad;
+    __syncthreads();
+    bool any = false;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) any |= flags[w] != 0;
+    attn_write<DT, DP>(a, s, head, row0, ROWS, split, sums, ml, NW, ROWS, any, tid, NW * 64);
+}
+
+// The splits of a row joined: DP / 4 lanes per row and part of the splits
+template <int DT, int DP>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+    constexpr int Q = DP / 4, G = 256 / Q;
+    __shared__ __attribute__((aligned(16))) float4v part[G][Q];
+    const int per = a.most_new * a.q_heads, b = blockIdx.x / per, r = blockIdx.x % per, tok = r / a.q_heads, hq = r % a.q_heads;
+    const AttnSeq s = attn_seq(a, b);
+    if (tok >= s.n) return;
+    const int64_t row = (int64_t)(s.first + tok) * a.q_heads + hq, at = row * a.splits;
+    const int q = threadIdx.x % Q, g = threadIdx.x / Q;
+    float m = -INFINITY, l = 0.f;
+    for (int i = 0; i < a.splits; ++i) m = fmaxf(m, a.pml[at + i][0]);
+    float4v v = float4v{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < a.splits; ++i) {
+        const float2v one = a.pml[at + i];
+        const float by = one[0] == m ? (m == -INFINITY ? 0.f : 1.f) : __builtin_amdgcn_exp2f(one[0] - m);
+        l += one[1] * by;
+        if (i % G == g && by != 0.f) v += reinterpret_cast<const float4v*>(a.po + (at + i) * DP)[q] * by;
+    }
+    part[g][q] = v;
+    __syncthreads();
+    if (g) return;
+#pragma unroll
+    for (int i = 1; i < G; ++i) v += part[i][q];
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (q * 4 < a.dim) {
+        u32x2 o;
+        o[0] = (uint32_t)AttnType<DT>::one(v[0] * inv) | ((uint32_t)AttnType<DT>::one(v[1] * inv) << 16);
+        o[1] = (uint32_t)AttnType<DT>::one(v[2] * inv) | ((uint32_t)AttnType<DT>::one(v[3] * inv) << 16);
+        *reinterpret_cast<u32x2*>(a.out + (int64_t)(s.first + tok) * a.o_t + (int64_t)hq * a.o_h + q * 8) = o;
+    }
+    if (q == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+}
+
+// ------------------------------------------------------------------------------------------ host
+
+struct AttnPlan { int dp, mt, row_blocks, splits; };
+constexpr int attn_waves(int dp) { return dp == 256 ? 2 : 4; }
+
+template <int DT, int DP, int MT>
+int attn_launch_one(const AttnArgs& a, unsigned grid, hipStream_t s) {
+    constexpr int NW = attn_waves(DP), LDS = attn_lds<DP, MT, NW>();
+    static bool raised[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (!raised[dev]) {
+        (void)hipFuncSetAttribute((const void*)attn_kernel<DT, DP, MT, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        raised[dev] = true;
+    }
+    hipLaunchKernelGGL((attn_kernel<DT, DP, MT, NW>), dim3(grid), dim3(NW * 64), LDS, s, a);
+    return check_launch("sq_tree_attention");
+}
+
+template <int DT, int DP>
+int attn_launch_dim(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
+    const unsigned grid = (unsigned)((int64_t)a.seqs * a.kv_heads * p.row_blocks * p.splits);
+    int rc;
+    if (p.mt == 1) rc = attn_launch_one<DT, DP, 1>(a, grid, s);
+    else if (p.mt == 2) rc = attn_launch_one<DT, DP, 2>(a, grid, s);
+    else {
+        if constexpr (DP < 256) rc = attn_launch_one<DT, DP, 4>(a, grid, s);
+        else rc = fail(SQ_EUNSUPPORTED, "sq_tree_attention: plan");
+    }
+    if (rc || p.splits == 1) return rc;
+    hipLaunchKernelGGL((attn_join_kernel<DT, DP>), dim3((unsigned)((int64_t)a.seqs * a.most_new * a.q_heads)), dim3(256), 0, s, a);
+    return check_launch("sq_tree_attention: join");
+}
+
+template <int DT>
+int attn_launch(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
+    if (p.dp == 64) return attn_launch_dim<DT, 64>(a, p, s);
+    if (p.dp == 128) return attn_launch_dim<DT, 128>(a, p, s);
+    return attn_launch_dim<DT, 256>(a, p, s);
+}
+int attn_launch_f16(const AttnArgs& a, const AttnPlan& p, hipStream_t s);
+int attn_launch_bf16(const AttnArgs& a, const AttnPlan& p, hipStream_t s);
+
+}  // namespace sq

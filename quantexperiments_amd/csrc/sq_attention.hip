@@ -1,0 +1,85 @@
+// sq_tree_attention: argument checks, and how a call is cut into workgroups.
+#include "sq_attention.h"
+
+namespace sq {
+
+// Rows of 16, 32 or 64 per workgroup; sequences cut until the chip has a workgroup per compute unit, into pieces of at least two steps
+// per wave.
+static AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
+    AttnPlan p;
+    p.dp = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
+    const int64_t rows = (int64_t)a.most_new * (a.q_heads / c.heads);
+    p.mt = rows <= 16 ? 1 : rows <= 32 || p.dp == 256 ? 2 : 4;
+    p.row_blocks = (int)((rows + p.mt * 16 - 1) / (p.mt * 16));
+    const int64_t base = (int64_t)a.seqs * c.heads * p.row_blocks, steps = ((int64_t)a.max_pages * c.page + ATTN_STEP - 1) / ATTN_STEP;
+    const int64_t most = steps / (2 * attn_waves(p.dp)), want = (device_cus() + base - 1) / base;
+    p.splits = (int)(want < most ? want : most);
+    if (p.splits < 1) p.splits = 1;
+    if (p.splits > 128) p.splits = 128;
+    return p;
+}
+
+static int check_attention(const char* who, const sq_attention* a, const sq_cache* c) {
+    if (!a || !c) return fail(SQ_EINVAL, "%s: null argument", who);
+    if (c->dtype != SQ_F16 && c->dtype != SQ_BF16) return fail(SQ_EINVAL, "%s: dtype %d (fp16 or bf16)", who, c->dtype);
+    if (c->dim < 8 || c->dim > 256 || c->dim % 8) return fail(SQ_EUNSUPPORTED, "%s: heads of %d elements (a multiple of 8 up to 256)", who, c->dim);
+    if (c->heads < 1 || a->q_heads < 1 || a->q_heads % c->heads) return fail(SQ_EINVAL, "%s: %d query heads for %d key heads", who, a->q_heads, c->heads);
+    if (a->tokens < 0 || a->seqs < 0 || a->most_new < 0 || a->q_heads > (1 << 16) || a->max_pages < 0 || c->pages < 0 || c->page < 1 || a->mask_words < 0 ||
+        a->ld_table < a->max_pages)
+        return fail(SQ_EINVAL, "%s: %d tokens, %d sequences, at most %d new, tables of %d (ld %lld), %d pages of %d", who, a->tokens, a->seqs, a->most_new, a->max_pages,
+                    (long long)a->ld_table, c->pages, c->page);
+    if (!(a->scale > 0.f) || a->scale > 3e38f) return fail(SQ_EINVAL, "%s: scale %g", who, (double)a->scale);
+    if (!a->starts && (int64_t)a->seqs * a->most_new != a->tokens)
+        return fail(SQ_EINVAL, "%s: %d tokens are not %d for each of %d sequences", who, a->tokens, a->most_new, a->seqs);
+    return SQ_OK;
+}
+
+static bool attn_nothing(const sq_attention& a) { return a.tokens == 0 || a.seqs == 0 || a.most_new == 0; }
+
+}  // namespace sq
+
+using namespace sq;
+
+extern "C" {
+
+size_t sq_tree_attention_workspace_bytes(const sq_attention* a, const sq_cache* cache) {
+    if (check_attention("sq_tree_attention_workspace_bytes", a, cache) || attn_nothing(*a)) return 0;
+    const AttnPlan p = attn_plan(*a, *cache);
+    if (p.splits == 1) return 0;
+    return (size_t)a->tokens * a->q_heads * p.splits * (p.dp * 4 + 8);
+}
+
+int sq_tree_attention(const sq_attention* a, const sq_cache* cache, void* workspace, size_t ws_bytes, void* stream) {
+    const char* who = "sq_tree_attention";
+    if (int rc = check_attention(who, a, cache)) return rc;
+    if (attn_nothing(*a)) return SQ_OK;
+    if (!a->max_pages || !cache->pages) return fail(SQ_EINVAL, "%s: new tokens without a page", who);
+    if (!a->q || !a->out || !a->table || !a->lens || !cache->k || !cache->v) return fail(SQ_EINVAL, "%s: null argument", who);
+    const int64_t strides = a->q_token | a->q_head | a->out_token | a->out_head | cache->k_page | cache->k_slot | cache->k_head | cache->v_page | cache->v_slot | cache->v_head;
+    if (strides % 8 || (((uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)cache->k | (uintptr_t)cache->v) & 15))
+        return fail(SQ_EUNSUPPORTED, "%s: q, out, keys and values need 16-byte aligned heads", who);
+    const AttnPlan p = attn_plan(*a, *cache);
+    if ((int64_t)a->seqs * cache->heads * p.row_blocks * p.splits > (1 << 23) || (int64_t)a->seqs * a->most_new * a->q_heads > (p.splits > 1 ? 1 << 23 : INT32_MAX))
+        return fail(SQ_EUNSUPPORTED, "%s: %d sequences of up to %d new tokens and %d heads at once", who, a->seqs, a->most_new, a->q_heads);
+    const size_t need = p.splits == 1 ? 0 : (size_t)a->tokens * a->q_heads * p.splits * (p.dp * 4 + 8);
+    if (ws_bytes < need || (need && (!workspace || ((uintptr_t)workspace & 255))))
+        return fail(SQ_EWORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who, need, ws_bytes);
+    AttnArgs k;
+    k.q = (const char*)a->q; k.out = (char*)a->out; k.lse = a->lse; k.kc = (const char*)cache->k; k.vc = (const char*)cache->v;
+    k.table = a->table; k.lens = a->lens; k.starts = a->starts; k.mask = a->mask;
+    k.po = (float*)workspace;
+    k.pml = (float2v*)((float*)workspace + (need ? (size_t)a->tokens * a->q_heads * p.splits * p.dp : 0));
+    k.q_t = a->q_token * 2; k.q_h = a->q_head * 2; k.o_t = a->out_token * 2; k.o_h = a->out_head * 2;
+    k.k_page = cache->k_page * 2; k.k_slot = cache->k_slot * 2; k.k_head = cache->k_head * 2;
+    k.v_page = cache->v_page * 2; k.v_slot = cache->v_slot * 2; k.v_head = cache->v_head * 2;
+    k.ld_table = a->ld_table; k.ld_mask = a->ld_mask;
+    k.tokens = a->tokens; k.seqs = a->seqs; k.most_new = a->most_new; k.q_heads = a->q_heads; k.kv_heads = cache->heads; k.group = a->q_heads / cache->heads;
+    k.dim = cache->dim; k.pages = cache->pages; k.page = cache->page; k.max_pages = a->max_pages; k.mask_words = a->mask_words;
+    k.row_blocks = p.row_blocks; k.splits = p.splits;
+    auto near = [](int64_t b) { return b >= 0 && b < (1 << 24); };
+    k.near = near(k.k_slot) && near(k.v_slot);
+    k.scale2 = a->scale * 1.4426950408889634f;
+    return cache->dtype == SQ_F16 ? attn_launch_f16(k, p, (hipStream_t)stream) : attn_launch_bf16(k, p, (hipStream_t)stream);
+}
+
+}  // extern "C"

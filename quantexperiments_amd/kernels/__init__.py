@@ -799,3 +799,6 @@ def linear_small_silu(pieces, x: torch.Tensor, out: torch.Tensor, *, x_out=None,
     _lib.check(rc)
     return out
 
+
+
+from .attention import keep_drafted, qk_norm_rotary, rotary, rotary_freqs, tree_attention  # noqa: E402,F401

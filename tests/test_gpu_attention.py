@@ -1,0 +1,415 @@
+"""Attention of new tokens over a paged cache, against its formula in 64 bits.
+
+Tolerance of a result, from what the kernel rounds.  Half a step of 32 bits is h = 2^-24, of the type u = finfo.eps / 2.  A score is a sum of D
+exact products, off by at most D h scale sum |q||k|, and a rounding of its scaled value and of the exponential: ds = (D + 4) h scale max_j sum |q||k|.  That is
+what weights are off by, relative, in numerator and denominator alike (2 ds).  The weights of the second product are rounded to the type (u), the sums
+of L terms and their joining in 32 bits add at most (L + 64) h, all relative to A = sum softmax |v|; the result is rounded once: u |out|.
+lse: ds, the total's (L + 64) h, and the logarithm's rounding, 4 h max(1, |lse|, |maximum|)."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "f16": torch.float16}
+H = 2.0 ** -24
+
+
+def words_of(sees):
+    """Truth values [N, n] as 64-bit words [N, ceil(n / 64)]."""
+    n, w = sees.shape[1], max(1, -(-sees.shape[1] // 64))
+    out = np.zeros((sees.shape[0], w), dtype=np.uint64)
+    s = sees.numpy()
+    for j in range(n):
+        out[:, j // 64] |= s[:, j].astype(np.uint64) << np.uint64(j % 64)
+    return torch.from_numpy(out.view(np.int64))
+
+
+def tree_of(n, g):
+    """Ancestors-and-self of a random tree, [n, n]."""
+    sees = torch.eye(n, dtype=torch.bool)
+    for t in range(1, n):
+        p = int(torch.randint(-1, t, (1,), generator=g))
+        if p >= 0:
+            sees[t] |= sees[p]
+    return sees
+
+
+class Setup:
+    """Sequences of `lens` cached and `news` new tokens in a paged cache of slots that otherwise hold NaN."""
+
+    def __init__(self, lens, news, hq, hk, d, page, dtype="bf16", tree=False, seed=0, extra_rows=0, scale=2.0, spare=3):
+        g = torch.Generator().manual_seed(seed)
+        self.g, self.lens, self.news, self.hq, self.hk, self.d, self.page, self.dt = g, lens, news, hq, hk, d, page, DT[dtype]
+        need = [-(-(a + b) // page) for a, b in zip(lens, news)]
+        order = torch.randperm(sum(need) + spare, generator=g)
+        self.table = torch.full((len(lens), max(need) + 1), -7, dtype=torch.int32)
+        at = 0
+        self.k, self.v = [], []
+        self.kc, self.vc = (torch.full((len(order), page, hk, d), float("nan"), dtype=self.dt) for _ in range(2))
+        for b, (l, n) in enumerate(zip(lens, news)):
+            self.table[b, :need[b]] = order[at:at + need[b]].int()
+            at += need[b]
+            k, v = (torch.randn(l + n, hk, d, generator=g).to(self.dt) for _ in range(2))
+            self.k.append(k)
+            self.v.append(v)
+        self.put()
+        self.starts = [0]
+        for n in news:
+            self.starts.append(self.starts[-1] + n)
+        self.n = self.starts[-1] + extra_rows
+        self.q = (torch.randn(self.n, hq, d, generator=g) * scale).to(self.dt)
+        self.sees = [tree_of(n, g) if tree else torch.ones(n, n, dtype=torch.bool).tril() for n in news]
+        self.tree = tree
+        self.scale = d ** -0.5
+
+    def put(self):
+        for b, (k, v) in enumerate(zip(self.k, self.v)):
+            s = torch.arange(len(k))
+            pg = self.table[b, s // self.page].long()
+            self.kc[pg, s % self.page], self.vc[pg, s % self.page] = k, v
+
+    def mask(self):
+        if not self.tree:
+            return None
+        most = max(1, max(self.news))
+        rows = torch.zeros(self.n, most, dtype=torch.bool)
+        for b, s in enumerate(self.sees):
+            rows[self.starts[b]:self.starts[b + 1], :s.shape[1]] = s
+        return words_of(rows).cuda()
+
+    def device(self):
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+        return dict(q=self.q.cuda(), k_cache=self.kc.cuda(), v_cache=self.vc.cuda(), table=self.table.cuda(), lens=i32(self.lens), starts=i32(self.starts),
+                    most_new=max(self.news), mask=self.mask(), scale=self.scale)
+
+    def reference(self):
+        """(out, tolerance, lse, tolerance), rows of no sequence NaN."""
+        hq, hk, d = self.hq, self.hk, self.d
+        out, tol = (torch.full((self.n, hq, d), float("nan"), dtype=torch.float64) for _ in range(2))
+        lse, ltol = (torch.full((self.n, hq), float("nan"), dtype=torch.float64) for _ in range(2))
+        u = torch.finfo(self.dt).eps / 2
+        for b, (l, n) in enumerate(zip(self.lens, self.news)):
+            k, v = self.k[b].double(), self.v[b].double()
+            sees = torch.cat((torch.ones(n, l, dtype=torch.bool), self.sees[b]), 1)
+            for h in range(hq):
+                q = self.q[self.starts[b]:self.starts[b + 1], h].double()
+                kk, vv = k[:, h // (hq // hk)], v[:, h // (hq // hk)]
+                for t in range(n):
+                    see = sees[t]
+                    r = self.starts[b] + t
+                    if not see.any():
+                        out[r, h], tol[r, h], lse[r, h], ltol[r, h] = 0, 0, -math.inf, 0
+                        continue
+                    s = kk[see] @ q[t] * self.scale
+                    ds = (d + 4) * H * self.scale * float((kk[see].abs() @ q[t].abs()).max())
+                    p = torch.softmax(s, 0)
+                    big = (p[:, None] * vv[see].abs()).sum(0)
+                    out[r, h] = p @ vv[see]
+                    tol[r, h] = (u * 1.01 + 2 * ds + (len(s) + 64) * H) * big + u * out[r, h].abs() + torch.finfo(self.dt).tiny * torch.finfo(self.dt).eps
+                    lse[r, h] = torch.logsumexp(s, 0)
+                    ltol[r, h] = ds + (len(s) + 64) * H + 4 * H * max(1.0, abs(float(lse[r, h])), abs(float(s.max())))
+        return out, tol, lse, ltol
+
+    def check(self, got, got_lse=None):
+        out, tol, lse, ltol = self.reference()
+        rows = self.starts[-1]
+        got = got.cpu().double()[:rows]
+        off = (got - out[:rows]).abs()
+        assert bool((off <= tol[:rows]).all()), (float((off / tol[:rows]).nan_to_num(posinf=1e30).max()), int((~(off <= tol[:rows])).sum()))
+        if got_lse is not None:
+            gl = got_lse.cpu().double()[:rows]
+            same = (gl == lse[:rows]) | ((gl - lse[:rows]).abs() <= ltol[:rows])
+            assert bool(same.all()), float((gl - lse[:rows]).abs().nan_to_num().max())
+
+
+def attend(s, **kw):
+    from quantexperiments_amd.kernels import tree_attention
+    lse = torch.full((s.n, s.hq), 5.0, device="cuda")
+    a = {**s.device(), **kw}
+    return tree_attention(**a, lse=lse), lse
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("d", [8, 64, 72, 96, 128, 136, 256])
+@pytest.mark.parametrize("lens,news,hq,hk,page,tree", [
+    ([0], [1], 1, 1, 16, False), ([1], [1], 7, 1, 16, False), ([30, 31, 32, 33], [1, 1, 1, 1], 4, 2, 16, False), ([200], [1], 14, 2, 1, False),
+    ([130, 0, 65], [3, 0, 17], 6, 3, 24, True), ([40], [70], 2, 1, 64, True), ([5, 300], [40, 2], 5, 1, 100, False)])
+def test_matches_the_formula(lens, news, hq, hk, page, tree, d, dtype):
+    s = Setup(lens, news, hq, hk, d, page, dtype, tree, seed=d + len(lens))
+    s.check(*attend(s))
+
+
+@pytest.mark.parametrize("page", [1, 2, 3, 5, 16, 31, 32, 33, 64, 1000])
+def test_pages_of_any_size(page):
+    s = Setup([77, 255, 256, 1], [1, 5, 2, 9], 4, 2, 128, page, tree=True, seed=page)
+    s.check(*attend(s))
+
+
+@pytest.mark.parametrize("length", [15, 127, 128, 129, 1023, 2500, 9001])
+@pytest.mark.parametrize("hq,hk,new", [(7, 1, 1), (2, 2, 4), (16, 1, 9)])
+def test_long_caches_cut_into_parts_and_joined(length, hq, hk, new):
+    s = Setup([length], [new], hq, hk, 128, 16, "f16", tree=new > 1, seed=length)
+    s.check(*attend(s))
+    s = Setup([length, 3], [new, 1], hq, hk, 64, 8, "bf16", tree=new > 1, seed=length + 1)
+    s.check(*attend(s))
+
+
+@pytest.mark.parametrize("lens,news", [([0], [300]), ([100, 7], [150, 129]), ([33], [257])])
+@pytest.mark.parametrize("d,hq,hk", [(128, 7, 1), (64, 3, 3), (256, 4, 2)])
+def test_chunks_of_a_prompt(lens, news, d, hq, hk):
+    s = Setup(lens, news, hq, hk, d, 16, seed=d)
+    s.check(*attend(s))
+
+
+def test_trees_wider_than_words_and_masks_that_leave_a_row_nothing():
+    s = Setup([0, 10, 0], [65, 130, 3], 4, 2, 128, 16, tree=True, seed=5)
+    s.sees[0][3] = False
+    s.sees[0][64] = False
+    s.sees[1][7] = False                                     # (still sees the cached ones)
+    s.sees[2][:] = False
+    out, lse = attend(s)
+    s.check(out, lse)
+    assert bool((out[3] == 0).all()) and bool((lse[3] == -math.inf).all()) and bool((out[-3:] == 0).all())
+    s.sees = [t[:, :64].clone() for t in s.sees]             # a mask of one word: new tokens beyond it are seen by nobody
+    s.sees = [torch.cat((t, torch.zeros(len(t), max(0, n - t.shape[1]), dtype=torch.bool)), 1) for t, n in zip(s.sees, s.news)]
+    m = s.mask()[:, :1]
+    s.check(*attend(s, mask=m))
+    s.check(*attend(s, mask=s.mask()))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_what_a_token_does_not_see_does_not_touch_it(value, dtype):
+    s = Setup([37, 0], [6, 40], 4, 2, 128, 16, dtype, tree=True, seed=9)
+    clean, clean_lse = attend(s)
+    s.check(clean, clean_lse)
+    # new token 2 of either sequence holds what is not finite; some see it, others do not
+    s.sees[0][4, 2], s.sees[0][5, 2] = True, False
+    s.sees[1][:, 2] = False
+    s.sees[1][30, 2] = True
+    clean, clean_lse = attend(s)
+    for b, (l, where) in enumerate(((37, "k"), (0, "v"))):
+        (s.k if where == "k" else s.v)[b][l + 2, 1, 5] = value
+    s.put()
+    out, lse = attend(s)
+    blind = torch.ones(s.n, dtype=torch.bool)
+    for b in range(2):
+        blind[s.starts[b]:s.starts[b + 1]] = ~s.sees[b][:, 2]
+    assert torch.equal(out[blind.cuda()], clean[blind.cuda()]) and torch.equal(lse[blind.cuda()], clean_lse[blind.cuda()])
+    saw = s.starts[1] + 30                                   # a value: its element of the heads that read it, nothing else
+    row = out[saw].cpu()
+    assert torch.equal(row[:2], clean[saw].cpu()[:2]) and torch.equal(row[2:, :5], clean[saw].cpu()[2:, :5]) and torch.equal(row[2:, 6:], clean[saw].cpu()[2:, 6:])
+    bad = row[2:, 5]
+    assert bool(bad.isnan().all() if math.isnan(value) else (bad == value).all())
+    assert torch.equal(lse[saw], clean_lse[saw])
+
+
+def test_scores_at_the_ends_of_the_range():
+    s = Setup([64], [1], 2, 1, 64, 16, "f16", seed=4)
+    s.k[0][:] = 0
+    s.k[0][5, 0, 0] = 60000.0
+    s.q[0, 0], s.q[0, 1] = 0, 0
+    s.q[0, 0, 0], s.q[0, 1, 0] = 60000.0, -60000.0           # one key has everything; it has nothing and the others share alike
+    s.put()
+    s.scale = 1.0
+    out, lse = attend(s)
+    assert torch.equal(out[0, 0].cpu(), s.v[0][5, 0]) and abs(float(lse[0, 0]) - 3.6e9) <= 4 * H * 3.6e9      # (four factors and products of 32 bits)
+    rest = torch.cat((s.v[0][:5, 0], s.v[0][6:, 0])).double()
+    assert float((out[0, 1].cpu().double() - rest.mean(0)).abs().max()) <= 2 ** -11 * float(rest.abs().mean(0).max()) * 2.2
+    assert abs(float(lse[0, 1]) - math.log(64)) < 1e-5
+    s.k[0][:] = torch.finfo(torch.float16).min               # all scores alike, and far below zero
+    s.q[0] = 1.0
+    s.put()
+    out, lse = attend(s)
+    assert float((out[0, 0].cpu().double() - s.v[0][:, 0].double().mean(0)).abs().max()) <= 2 ** -11 * 2.2
+    assert float(lse[0, 0]) == pytest.approx(-65504.0 * 64, rel=1e-6)
+
+
+def test_strides_orders_and_rows_of_no_sequence():
+    s = Setup([50, 0, 9], [2, 3, 4], 6, 2, 128, 16, tree=True, seed=6, extra_rows=3)
+    a = s.device()
+    want, want_lse = attend(s, out=torch.full(s.q.shape, 9.0, dtype=s.dt, device="cuda"))
+    s.check(want, want_lse)
+    assert bool((want[-3:] == 9).all()) and bool((want_lse[-3:] == 5).all())
+    stacked = torch.empty(s.n, 10, 128, dtype=s.dt, device="cuda")
+    stacked[:, 1:7] = a["q"]
+    out = torch.full((6, s.n, 160), 9.0, dtype=s.dt, device="cuda")
+    kt, vt = (c.transpose(1, 2).contiguous().transpose(1, 2) for c in (a["k_cache"], a["v_cache"]))
+    both = torch.stack((a["k_cache"], a["v_cache"]), 1)      # one pool of pages, keys and values of a page side by side
+    wide = torch.full((3, a["table"].shape[1] + 5), -1, dtype=torch.int32, device="cuda")
+    wide[:, :-5] = a["table"]
+    for k, v in ((kt, vt), (both[:, 0], both[:, 1]), (a["k_cache"], vt)):
+        o = out.transpose(0, 1)[..., 16:144]
+        o.fill_(9.0)
+        got, lse = attend(s, q=stacked[:, 1:7], k_cache=k, v_cache=v, out=o, table=wide[:, :-5])
+        assert got is o and torch.equal(o, want) and torch.equal(lse, want_lse)
+    assert bool((out[..., :16] == 9).all()) and bool((out[..., 144:] == 9).all())
+    flipped = a["k_cache"].flip(0).contiguous().flip(0), a["v_cache"]
+    got, _ = attend(s, k_cache=flipped[0], out=torch.full(s.q.shape, 9.0, dtype=s.dt, device="cuda"))
+    assert torch.equal(got, want)
+
+
+def test_as_many_new_tokens_each_and_bounds_that_are_too_large():
+    s = Setup([100, 20, 3], [2, 2, 2], 4, 2, 64, 16, seed=8)
+    want, lse = attend(s)
+    s.check(want, lse)
+    got, _ = attend(s, starts=None)
+    assert torch.equal(got, want)
+    got, _ = attend(s, starts=None, most_new=None)
+    assert torch.equal(got, want)
+    s.check(*attend(s, most_new=None))                       # (as many as there are rows: another cut)
+    got, _ = attend(s, most_new=1, out=torch.full(s.q.shape, 9.0, dtype=s.dt, device="cuda"))
+    assert bool((got[1::2] == 9).all())                      # new tokens beyond the bound are left
+
+
+def test_a_contiguous_cache_is_a_page_per_sequence():
+    from quantexperiments_amd.kernels import tree_attention
+    g = torch.Generator().manual_seed(2)
+    k, v = (torch.randn(3, 200, 2, 128, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    q = torch.randn(3, 14, 128, generator=g).to(torch.bfloat16).cuda()
+    lens = torch.tensor([199, 0, 100], dtype=torch.int32).cuda()
+    out = tree_attention(q, k, v, torch.arange(3, dtype=torch.int32).cuda()[:, None], lens)
+    for b in range(3):
+        n = int(lens[b]) + 1
+        qq, kk, vv = q[b].double().cpu(), *(c[b, :n].double().cpu().repeat_interleave(7, 1) for c in (k, v))
+        p = torch.softmax(torch.einsum("hd,lhd->hl", qq, kk) * 128 ** -0.5, -1)
+        ref, big = torch.einsum("hl,lhd->hd", p, vv), torch.einsum("hl,lhd->hd", p, vv.abs())
+        ds = 132 * H * 128 ** -0.5 * float(torch.einsum("hd,lhd->hl", qq.abs(), kk.abs()).max())
+        assert bool(((out[b].double().cpu() - ref).abs() <= (2 ** -9 * 1.01 * 2 + 2 * ds + (n + 64) * H) * big + 2 ** -9 * 2 * ref.abs()).all())
+
+
+def test_wrong_tables_give_nan_for_their_sequence_alone():
+    s = Setup([100, 40, 60], [2, 2, 2], 4, 2, 128, 16, seed=3)
+    want, _ = attend(s)
+    for bad in (10 ** 6, -1, s.kc.shape[0]):
+        t = s.table.clone()
+        t[1, 1] = bad
+        out, lse = attend(s, table=t.cuda())
+        assert bool(out[2:4].isnan().all()) and bool(lse[2:4].isnan().all())
+        assert torch.equal(out[:2], want[:2]) and torch.equal(out[4:], want[4:])
+    out, _ = attend(s, lens=torch.tensor([100, 10 ** 6, 60], dtype=torch.int32).cuda(), table=s.table.clamp(min=0).cuda())   # more tokens than the table has slots
+    assert bool(out[2:4].isnan().all()) and torch.equal(out[:2], want[:2]) and torch.equal(out[4:], want[4:])
+    wild = torch.tensor([0, 2, 2 ** 31 - 1, -5], dtype=torch.int32).cuda()      # starts that leave the rows are cut off
+    out, _ = attend(s, starts=wild, most_new=2)
+    assert torch.equal(out[:2], want[:2])
+
+
+def test_offsets_beyond_32_bits():
+    from quantexperiments_amd.kernels import tree_attention
+    pages, page, hk, d = 3, 64, 2, 64
+    big = torch.empty(2, (1 << 31) + (1 << 21), dtype=torch.float16, device="cuda")       # pages 2^30 elements apart: offsets of 4 GiB
+    k, v = (t.as_strided((pages, page, hk, d), (1 << 30, hk * d, d, 1), t.storage_offset()) for t in big)
+    g = torch.Generator().manual_seed(1)
+    kh, vh = (torch.randn(pages, page, hk, d, generator=g).half() for _ in range(2))
+    k.copy_(kh)
+    v.copy_(vh)
+    q = torch.randn(1, 4, d, generator=g).half().cuda()
+    table, lens = torch.tensor([[2, 0, 1]], dtype=torch.int32).cuda(), torch.tensor([170], dtype=torch.int32).cuda()
+    got = tree_attention(q, k, v, table, lens)
+    want = tree_attention(q, kh.cuda(), vh.cuda(), table, lens)
+    assert torch.equal(got, want)
+    far_k, far_v = (t.as_strided((2, 3, hk, d), (1 << 20, 1 << 30, d, 1), t.storage_offset()) for t in big)      # slots that far apart
+    far_k.copy_(kh[:2, :3])
+    far_v.copy_(vh[:2, :3])
+    lens = torch.tensor([4], dtype=torch.int32).cuda()
+    table = torch.tensor([[1, 0]], dtype=torch.int32).cuda()
+    assert torch.equal(tree_attention(q, far_k, far_v, table, lens), tree_attention(q, kh[:2, :3].contiguous().cuda(), vh[:2, :3].contiguous().cuda(), table, lens))
+
+
+def test_the_same_bits_every_time_and_on_two_streams_at_once():
+    from quantexperiments_amd.kernels import tree_attention
+    s = Setup([3000], [4], 28, 4, 128, 16, tree=True, seed=1)
+    t = Setup([2000, 100], [4, 1], 28, 4, 128, 16, tree=True, seed=2)
+    a, b = s.device(), t.device()
+    want = tree_attention(**a), tree_attention(**b)
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, args in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(tree_attention(**args))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for os, w in zip(got, want) for o in os)
+
+
+def test_captured_twice_and_replayed_with_other_lengths():
+    from quantexperiments_amd.kernels import tree_attention
+    s = Setup([900, 30], [3, 1], 8, 2, 128, 16, tree=True, seed=3)
+    a = s.device()
+    outs = [torch.zeros_like(a["q"]) for _ in range(2)]
+    tree_attention(**a)
+    graphs = []
+    for o in outs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            tree_attention(**a, out=o)
+        graphs.append(g)
+    side = torch.cuda.Stream()
+    for lens in ([900, 30], [5, 0], [899, 29], [0, 0]):
+        a["lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+        a["q"].mul_(-1)
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        want = tree_attention(**a)
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+def test_a_drafted_step_equals_the_tokens_decoded_one_by_one():
+    """q|k|v heads of a draft tree through norm, rotation, cache, attention and the kept path; then the accepted tokens again, one at a time."""
+    from quantexperiments_amd.kernels import keep_drafted, qk_norm_rotary, rotary_freqs, tree_attention
+    hq, hk, d, page, n, layers = 8, 2, 64, 16, 6, 2
+    g = torch.Generator().manual_seed(11)
+    dt = torch.float16
+    lens0 = [37, 5]
+    table = torch.tensor([[0, 3, 1, 6], [2, 7, 4, 5]], dtype=torch.int32).cuda()
+    freqs, scale = rotary_freqs(d, 10000.0, {"type": "yarn", "factor": 4.0, "original": 4096})
+    qw, kw = ((torch.rand(d, generator=g) + 0.5).to(dt).cuda() for _ in range(2))
+    caches = [torch.zeros(layers, 8, page, hk, d, dtype=dt, device="cuda") for _ in range(2)]
+    past = torch.randn(layers, 2, max(lens0), hq + 2 * hk, d, generator=g).to(dt).cuda()
+    parents = [-1, 0, 0, 1, 2, 4]                            # accepted: 0, 2, 4, 5
+    sees = torch.eye(n, dtype=torch.bool)
+    depth = []
+    for t, p in enumerate(parents):
+        depth.append(0 if p < 0 else depth[p] + 1)
+        if p >= 0:
+            sees[t] |= sees[p]
+    mask = words_of(sees).repeat(2, 1).cuda()
+    draft = torch.randn(layers, 2, n, hq + 2 * hk, d, generator=g).to(dt).cuda()
+    slot = lambda b, s: int(table[b, s // page]) * page + s % page
+
+    def step(layer, y, b_of, pos, at, kc, vc):
+        slots = torch.tensor([slot(b, s) for b, s in zip(b_of, at)]).cuda()
+        return qk_norm_rotary(y[:, :hq], y[:, hq:hq + hk], torch.tensor(pos).cuda(), freqs, qw, kw, v=y[:, hq + hk:], k_cache=kc[layer], v_cache=vc[layer], slots=slots, scale=scale)[0]
+
+    for layer in range(layers):
+        for b, l in enumerate(lens0):
+            step(layer, past[layer, b, :l], [b] * l, list(range(l)), list(range(l)), *caches)
+    one_by_one = [c.clone() for c in caches]
+    lens = torch.tensor(lens0, dtype=torch.int32).cuda()
+    outs = []
+    for layer in range(layers):
+        b_of = [0] * n + [1] * n
+        q = step(layer, draft[layer].reshape(2 * n, -1, d), b_of, [lens0[b] + depth[i % n] for i, b in enumerate(b_of)], [lens0[b] + i % n for i, b in enumerate(b_of)], *caches)
+        outs.append(tree_attention(q, caches[0][layer], caches[1][layer], table, lens, mask=mask).view(2, n, hq, d))
+    path = torch.tensor([[0, 2, 4, 5]] * 2, dtype=torch.int32).cuda()
+    counts = torch.tensor([4, 3], dtype=torch.int32).cuda()
+    keep_drafted(*caches, table, lens, path, counts)
+    lens += counts
+    for b in range(2):
+        for i, t in enumerate((0, 2, 4, 5)[:int(counts[b])]):
+            for layer in range(layers):
+                q = step(layer, draft[layer, b, t:t + 1], [b], [lens0[b] + i], [lens0[b] + i], *one_by_one)
+                o = tree_attention(q, one_by_one[0][layer], one_by_one[1][layer], table[b:b + 1], torch.tensor([lens0[b] + i], dtype=torch.int32).cuda())
+                # the same keys in another order of additions: twice the tolerance of a result, with |v| < 5 and A < 5
+                assert float((o[0].double() - outs[layer][b, t].double()).abs().max()) <= 2 * (2 * 2 ** -11 * 5 + 2 * (d + 4) * H * 64 + 128 * H * 5)
+        total = lens0[b] + int(counts[b])
+        rows = torch.tensor([slot(b, s) for s in range(total)]).cuda()
+        for c, o in zip(caches, one_by_one):
+            assert torch.equal(c.view(layers, -1, hk, d)[:, rows], o.view(layers, -1, hk, d)[:, rows])
