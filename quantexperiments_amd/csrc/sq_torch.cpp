@@ -10,6 +10,7 @@
 // also words the errors.  Nothing is kept between calls but what a matrix is (its tensors and sizes, dropped by PackedLinear
 // whenever one of its attributes is set).
 #include <Python.h>
+#include <cmath>
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/hip/HIPFunctions.h>
@@ -471,6 +472,234 @@ PyObject* q4_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     )
 }
 
+// ------------------------------------------------------------------------------------------ heads of q|k|v, attention
+
+// A tensor these calls take as it is: on `dev`, strided, nothing that Python dispatches or that a gradient would be recorded for
+bool plain_on(const at::Tensor& t, int dev) {
+    return t.is_cuda() && t.get_device() == dev && t.layout() == at::kStrided && !t.unsafeGetTensorImpl()->is_python_dispatch() &&
+           !(t.requires_grad() && at::GradMode::is_enabled());
+}
+// An argument that may be None: NULL, or the tensor; false where it is neither
+bool maybe(PyObject* o, const at::Tensor*& t) {
+    t = nullptr;
+    if (o == Py_None) return true;
+    if (!THPVariable_Check(o)) return false;
+    t = &THPVariable_Unpack(o);
+    return true;
+}
+bool heads_on(const at::Tensor& t, int dev) { return t.dim() == 3 && plain_on(t, dev) && dtype_of(t) >= 0 && (t.stride(2) == 1 || t.size(2) == 1); }
+bool vector_on(const at::Tensor& t, int dev, int64_t n, at::ScalarType a, at::ScalarType b) {
+    return t.dim() == 1 && t.size(0) == n && (t.scalar_type() == a || t.scalar_type() == b) && plain_on(t, dev) && t.is_contiguous();
+}
+bool rows_on(const at::Tensor& t, int dev, int64_t n, at::ScalarType type) {
+    return t.dim() == 2 && t.size(0) == n && t.scalar_type() == type && plain_on(t, dev) && (t.stride(1) == 1 || t.size(1) <= 1) &&
+           (n <= 1 || t.stride(0) >= t.size(1));
+}
+bool apart(const at::Tensor& a, const at::Tensor& b) {       // no byte between the first and the last of both
+    auto ends = [](const at::Tensor& t, uintptr_t& lo, uintptr_t& hi) {
+        lo = hi = (uintptr_t)t.data_ptr();
+        for (int i = 0; i < t.dim(); ++i) (t.stride(i) > 0 ? hi : lo) += (t.size(i) - 1) * t.stride(i) * (int64_t)t.element_size();
+        hi += t.element_size();
+    };
+    uintptr_t al, ah, bl, bh;
+    ends(a, al, ah);
+    ends(b, bl, bh);
+    return ah <= bl || bh <= al;
+}
+// out is x, or apart from it, with x's shape and type
+bool out_ok(const at::Tensor& out, const at::Tensor& x, int dev) {
+    return heads_on(out, dev) && out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type() &&
+           ((out.data_ptr() == x.data_ptr() && out.strides() == x.strides()) || apart(out, x));
+}
+sq_heads part_of(const at::Tensor& x, const at::Tensor* out, const at::Tensor* w) {
+    const at::Tensor& o = out ? *out : x;
+    return {x.data_ptr(), out ? out->data_ptr() : nullptr, w ? w->data_ptr() : nullptr, x.stride(0), x.stride(1), o.stride(0), o.stride(1), (int32_t)x.size(1)};
+}
+bool rotation_of(const at::Tensor& pos, const at::Tensor& freqs, int64_t n, int64_t dim, bool interleaved, double scale, bool inverse, int dev, sq_rotation& r) {
+    if (!vector_on(pos, dev, n, at::kLong, at::kInt) || !vector_on(freqs, dev, freqs.numel(), at::kDouble, at::kDouble) || 2 * freqs.numel() > dim) return false;
+    r = {(const double*)freqs.data_ptr(), pos.data_ptr(), (int32_t)freqs.numel(), pos.scalar_type() == at::kLong, interleaved, inverse, (float)scale};
+    return true;
+}
+// the last four dimensions of a pair of caches; not where they are written and expanded
+bool cache_of(const at::Tensor& k, const at::Tensor& v, int dev, bool written, sq_cache& c) {
+    const int d = (int)k.dim();
+    if ((d != 4 && d != 5) || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type() || dtype_of(k) < 0 || !plain_on(k, dev) || !plain_on(v, dev) || k.numel() == 0 ||
+        k.numel() / k.size(d - 4) > INT32_MAX || k.size(d - 4) > INT32_MAX)
+        return false;
+    for (const at::Tensor* t : {&k, &v}) {
+        if (t->stride(d - 1) != 1 && t->size(d - 1) > 1) return false;
+        for (int i = 0; written && i < d; ++i) if (t->stride(i) == 0 && t->size(i) > 1) return false;
+    }
+    if (written && k.data_ptr() == v.data_ptr()) return false;
+    c = {k.data_ptr(), v.data_ptr(), k.stride(d - 4), k.stride(d - 3), k.stride(d - 2), v.stride(d - 4), v.stride(d - 3), v.stride(d - 2), (int32_t)k.size(d - 4),
+         (int32_t)k.size(d - 3), (int32_t)k.size(d - 2), (int32_t)k.size(d - 1), dtype_of(k)};
+    return true;
+}
+
+// rotary(x, positions, freqs, out, interleaved, scale, inverse) -> out, or a code
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const at::Tensor* given;
+    if (n != 7 || !tensors(a, 3) || !maybe(a[3], given)) return answer(NOT_COVERED);
+    SQ_GUARD(
+        const at::Tensor& x = THPVariable_Unpack(a[0]);
+        const double scale = PyFloat_AsDouble(a[5]);
+        const int inter = PyObject_IsTrue(a[4]); const int inverse = PyObject_IsTrue(a[6]);
+        if (PyErr_Occurred()) return nullptr;
+        if (x.dim() != 3 || !x.is_cuda() || x.numel() == 0 || x.size(0) > INT32_MAX || x.size(1) > INT32_MAX || x.size(2) > INT32_MAX) return answer(NOT_COVERED);
+        const int dev = x.get_device();
+        sq_rotation r;
+        if (!heads_on(x, dev) || !rotation_of(THPVariable_Unpack(a[1]), THPVariable_Unpack(a[2]), x.size(0), x.size(2), inter, scale, inverse, dev, r) ||
+            (given && !out_ok(*given, x, dev)))
+            return answer(NOT_COVERED);
+        OnDevice on(dev);
+        at::Tensor out = given ? *given : at::empty(x.sizes(), x.options());
+        const sq_heads h = part_of(x, &out, nullptr);
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = sq_rotary(&h, (int)x.size(0), (int)x.size(2), dtype_of(x), &r, on.stream);
+        Py_END_ALLOW_THREADS
+        return rc ? answer(rc) : THPVariable_Wrap(std::move(out));
+    )
+}
+
+// qk_norm_rotary(q, k, positions, freqs, q_w, k_w, eps, q_out, k_out, v, k_cache, v_cache, slots, interleaved, scale, offset) -> (q_out, k_out), or a code
+PyObject* qk_norm_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const at::Tensor *qw, *kw, *qg, *kg, *v, *kc, *vc, *slots;
+    if (n != 16 || !tensors(a, 4) || !maybe(a[4], qw) || !maybe(a[5], kw) || !maybe(a[7], qg) || !maybe(a[8], kg) || !maybe(a[9], v) || !maybe(a[10], kc) ||
+        !maybe(a[11], vc) || !maybe(a[12], slots))
+        return answer(NOT_COVERED);
+    SQ_GUARD(
+        const at::Tensor& q = THPVariable_Unpack(a[0]);
+        const at::Tensor& k = THPVariable_Unpack(a[1]);
+        const double eps = PyFloat_AsDouble(a[6]); const double scale = PyFloat_AsDouble(a[14]); const double offset = PyFloat_AsDouble(a[15]);
+        const int inter = PyObject_IsTrue(a[13]);
+        if (PyErr_Occurred()) return nullptr;
+        if (q.dim() != 3 || !q.is_cuda() || q.numel() == 0 || k.dim() != 3 || k.numel() == 0 || q.numel() > INT32_MAX || k.numel() > INT32_MAX) return answer(NOT_COVERED);
+        const int dev = q.get_device(); const int dt = dtype_of(q);
+        const int64_t rows = q.size(0); const int64_t d = q.size(2);
+        const bool cached = kc != nullptr;
+        sq_rotation r; sq_cache c;
+        if (!heads_on(q, dev) || !heads_on(k, dev) || k.scalar_type() != q.scalar_type() || k.size(0) != rows || k.size(2) != d || (vc != nullptr) != cached ||
+            (v != nullptr) != cached || (slots != nullptr) != cached ||
+            !rotation_of(THPVariable_Unpack(a[2]), THPVariable_Unpack(a[3]), rows, d, inter, scale, false, dev, r))
+            return answer(NOT_COVERED);
+        int wd = dt;
+        for (const at::Tensor* w : {qw, kw})
+            if (w && (dtype_of(*w) < 0 || !vector_on(*w, dev, d, w->scalar_type(), w->scalar_type()))) return answer(NOT_COVERED);
+        if (qw && kw && qw->scalar_type() != kw->scalar_type()) return answer(NOT_COVERED);
+        if (qw || kw) wd = dtype_of(qw ? *qw : *kw);
+        // (in place, or new: other outputs are told apart in Python)
+        for (int i = 0; i < 2; ++i) {
+            const at::Tensor* g = i ? kg : qg; const at::Tensor& x = i ? k : q;
+            if (!g || (heads_on(*g, dev) && g->data_ptr() == x.data_ptr() && g->strides() == x.strides() && g->sizes() == x.sizes() && g->scalar_type() == x.scalar_type()))
+                continue;
+            if (!out_ok(*g, x, dev) || !apart(*g, i ? q : k) || (v && !apart(*g, *v)) || (i && qg && !apart(*g, *qg))) return answer(NOT_COVERED);
+        }
+        if (cached) {
+            if (!heads_on(*v, dev) || v->sizes() != k.sizes() || v->scalar_type() != q.scalar_type() || !vector_on(*slots, dev, rows, at::kLong, at::kInt) || kc->dim() != 4 ||
+                !cache_of(*kc, *vc, dev, true, c) || c.dtype != dt || c.heads != k.size(1) || c.dim != d)
+                return answer(NOT_COVERED);
+            for (const at::Tensor* t : {&q, &k, v, qg, kg})
+                if (t && (!apart(*kc, *t) || !apart(*vc, *t))) return answer(NOT_COVERED);
+        }
+        OnDevice on(dev);
+        at::Tensor qo = qg ? *qg : at::empty(q.sizes(), q.options());
+        at::Tensor ko;
+        if (kg) ko = *kg; else if (!cached) ko = at::empty(k.sizes(), k.options());
+        const sq_heads hq = part_of(q, &qo, qw); const sq_heads hk = part_of(k, ko.defined() ? &ko : nullptr, kw);
+        sq_heads hv{};
+        if (cached) hv = part_of(*v, nullptr, nullptr);
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = sq_qk_norm_rotary(&hq, &hk, cached ? &hv : nullptr, (int)rows, (int)d, dt, &r, wd, (float)eps, (float)offset, cached ? &c : nullptr,
+                               cached ? slots->data_ptr() : nullptr, cached && slots->scalar_type() == at::kLong, on.stream);
+        Py_END_ALLOW_THREADS
+        if (rc) return answer(rc);
+        PyObject* both = PyTuple_New(2);
+        if (!both) return nullptr;
+        PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(std::move(qo)));
+        if (ko.defined()) PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(std::move(ko)));
+        else { Py_INCREF(Py_None); PyTuple_SET_ITEM(both, 1, Py_None); }
+        return both;
+    )
+}
+
+// tree_attention(q, k_cache, v_cache, table, lens, starts, most_new, mask, scale, out, lse) -> out, or a code
+PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const at::Tensor *starts, *mask, *given, *lse;
+    if (n != 11 || !tensors(a, 5) || !maybe(a[5], starts) || !maybe(a[7], mask) || !maybe(a[9], given) || !maybe(a[10], lse)) return answer(NOT_COVERED);
+    SQ_GUARD(
+        const at::Tensor& q = THPVariable_Unpack(a[0]);
+        const at::Tensor& kc = THPVariable_Unpack(a[1]);
+        const at::Tensor& vc = THPVariable_Unpack(a[2]);
+        const at::Tensor& table = THPVariable_Unpack(a[3]);
+        const at::Tensor& lens = THPVariable_Unpack(a[4]);
+        if (q.dim() != 3 || !q.is_cuda() || q.numel() == 0 || q.numel() > INT32_MAX || lens.dim() != 1 || lens.size(0) < 1 || lens.size(0) > INT32_MAX) return answer(NOT_COVERED);
+        const int dev = q.get_device();
+        const int64_t rows = q.size(0); const int64_t b = lens.size(0);
+        sq_cache c; sq_attention t{};
+        if (!heads_on(q, dev) || kc.dim() != 4 || !cache_of(kc, vc, dev, false, c) || c.dtype == SQ_F32 || c.dtype != dtype_of(q) || c.dim != q.size(2) ||
+            q.size(1) % c.heads || !vector_on(lens, dev, b, at::kInt, at::kInt) || !rows_on(table, dev, b, at::kInt) || table.size(1) > INT32_MAX ||
+            (starts && !vector_on(*starts, dev, b + 1, at::kInt, at::kInt)) || (!starts && rows % b) || (mask && (!rows_on(*mask, dev, rows, at::kLong) || mask->size(1) > INT32_MAX)) ||
+            (lse && (lse->scalar_type() != at::kFloat || lse->dim() != 2 || lse->size(0) != rows || lse->size(1) != q.size(1) || !plain_on(*lse, dev) || !lse->is_contiguous())))
+            return answer(NOT_COVERED);
+        int64_t most = starts ? rows : rows / b;
+        if (a[6] != Py_None) most = PyLong_AsLongLong(a[6]);
+        const double scale = a[8] == Py_None ? std::pow((double)c.dim, -0.5) : PyFloat_AsDouble(a[8]);
+        if (PyErr_Occurred()) return nullptr;
+        if (most < 0 || most > INT32_MAX || (!starts && most * b != rows) || !(scale > 0 && scale < 3e38)) return answer(NOT_COVERED);
+        if (given && (!heads_on(*given, dev) || given->sizes() != q.sizes() || given->scalar_type() != q.scalar_type() || !apart(*given, q) || !apart(*given, kc) || !apart(*given, vc) ||
+                      (given->stride(0) == 0 && rows > 1) || (given->stride(1) == 0 && q.size(1) > 1)))
+            return answer(NOT_COVERED);
+        OnDevice on(dev);
+        at::Tensor out = given ? *given : at::empty(q.sizes(), q.options());
+        t.q = q.data_ptr(); t.out = out.data_ptr(); t.lse = lse ? (float*)lse->data_ptr() : nullptr; t.table = (const int32_t*)table.data_ptr();
+        t.lens = (const int32_t*)lens.data_ptr(); t.starts = starts ? (const int32_t*)starts->data_ptr() : nullptr; t.mask = mask ? (const int64_t*)mask->data_ptr() : nullptr;
+        t.q_token = q.stride(0); t.q_head = q.stride(1); t.out_token = out.stride(0); t.out_head = out.stride(1);
+        t.ld_table = b > 1 ? table.stride(0) : table.size(1); t.ld_mask = mask ? rows > 1 ? mask->stride(0) : mask->size(1) : 0;
+        t.tokens = (int32_t)rows; t.seqs = (int32_t)b; t.most_new = (int32_t)most; t.q_heads = (int32_t)q.size(1); t.max_pages = (int32_t)table.size(1);
+        t.mask_words = mask ? (int32_t)mask->size(1) : 0; t.scale = (float)scale;
+        // (a buffer of the call's own: streams and captured graphs run side by side)
+        const size_t need = sq_tree_attention_workspace_bytes(&t, &c);
+        at::Tensor ws;
+        if (need) ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = sq_tree_attention(&t, &c, need ? ws.data_ptr() : nullptr, need, on.stream);
+        Py_END_ALLOW_THREADS
+        return rc ? answer(rc) : THPVariable_Wrap(std::move(out));
+    )
+}
+
+// keep_drafted(k_cache, v_cache, table, lens, path, counts)
+PyObject* keep_drafted(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 6 || !tensors(a, 6)) return answer(NOT_COVERED);
+    SQ_GUARD(
+        const at::Tensor& kc = THPVariable_Unpack(a[0]);
+        const at::Tensor& vc = THPVariable_Unpack(a[1]);
+        const at::Tensor& table = THPVariable_Unpack(a[2]);
+        const at::Tensor& lens = THPVariable_Unpack(a[3]);
+        const at::Tensor& path = THPVariable_Unpack(a[4]);
+        if (!kc.is_cuda() || lens.dim() != 1 || lens.size(0) < 1 || lens.size(0) > INT32_MAX) return answer(NOT_COVERED);
+        const int dev = kc.get_device();
+        const int64_t b = lens.size(0);
+        sq_cache c;
+        if (!cache_of(kc, vc, dev, true, c) || !vector_on(lens, dev, b, at::kInt, at::kInt) || !vector_on(THPVariable_Unpack(a[5]), dev, b, at::kInt, at::kInt) ||
+            !rows_on(table, dev, b, at::kInt) || !rows_on(path, dev, b, at::kInt) || table.size(1) > INT32_MAX || path.size(1) > INT32_MAX)
+            return answer(NOT_COVERED);
+        const bool stacked = kc.dim() == 5;
+        if (stacked && kc.size(0) > INT32_MAX) return answer(NOT_COVERED);
+        OnDevice on(dev);
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = sq_keep_drafted(&c, stacked ? (int)kc.size(0) : 1, stacked ? kc.stride(0) : 0, stacked ? vc.stride(0) : 0, (const int32_t*)table.data_ptr(),
+                             b > 1 ? table.stride(0) : table.size(1), (int)table.size(1), (const int32_t*)lens.data_ptr(), (const int32_t*)path.data_ptr(),
+                             b > 1 ? path.stride(0) : path.size(1), (int)path.size(1), (const int32_t*)THPVariable_Unpack(a[5]).data_ptr(), (int)b, on.stream);
+        Py_END_ALLOW_THREADS
+        return answer(rc);
+    )
+}
+
 // ------------------------------------------------------------------------------------------ torch.ops.shapequant.linear
 
 at::Tensor linear_op(const at::Tensor& x, int64_t handle) {
@@ -532,6 +761,7 @@ PyObject* install_op(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define SQ_FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"native", (PyCFunction)(void (*)(void))make_native, METH_FASTCALL, nullptr}, {"install", install, METH_O, nullptr}, SQ_FAST(install_op),
                          SQ_FAST(linear), SQ_FAST(forward), SQ_FAST(linear_from), SQ_FAST(linear_silu), SQ_FAST(addnorm), SQ_FAST(silu_mul), SQ_FAST(q8_linear), SQ_FAST(q4_rows),
+                         SQ_FAST(rotary), SQ_FAST(qk_norm_rotary), SQ_FAST(tree_attention), SQ_FAST(keep_drafted),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods};
 

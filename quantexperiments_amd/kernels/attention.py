@@ -171,6 +171,11 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, out: t
     a head, P = len(freqs), pair i turns by positions * freqs[i] radians (float64 [P], `rotary_freqs`) and is multiplied by `scale`; the pair is
     elements i and P + i, or 2i and 2i + 1 if interleaved; the other elements keep their values (sq_rotary).  out: x itself, or memory
     apart from it (default: new).  inverse turns back: the adjoint, for gradients, and the way to move rotated keys to other positions."""
+    done = _lib.native().rotary(x, positions, freqs, out, interleaved, scale, inverse)
+    if type(done) is not int:
+        return done
+    if done < 0:
+        _lib.check(done)
     who = "rotary"
     _heads3(who, "x", x)
     _no_grad(who, x, freqs, out)
@@ -198,6 +203,11 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, fr
     in one pass, in 32 bits, rounded once (sq_qk_norm_rotary).  q_out: q itself or memory apart (default: new).  With caches, keys and v
     [N, Hk, D] go to slots (int64 / int32 [N]: page * slots per page + slot in page, distinct; tokens with a slot outside the cache, as -1, are not
     written); k_out is then optional, without caches it is new by default.  Returns (q_out, k_out or None)."""
+    done = _lib.native().qk_norm_rotary(q, k, positions, freqs, q_w, k_w, eps, q_out, k_out, v, k_cache, v_cache, slots, interleaved, scale, weight_offset)
+    if type(done) is not int:
+        return done
+    if done < 0:
+        _lib.check(done)
     who = "qk_norm_rotary"
     _heads3(who, "q", q)
     n, hq, d = q.shape
@@ -258,6 +268,11 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     key head h / (Hq / Hk).  scale: default D ** -0.5.  out [N, Hq, D]: rows that belong to no sequence are left as they are (default: new, they
     hold anything); lse: fp32 [N, Hq] contiguous, log of the sum of exponentials.  A token that sees nothing: zeros, -inf.  D: a multiple
     of 8 up to 256, heads 16-byte aligned."""
+    done = _lib.native().tree_attention(q, k_cache, v_cache, table, lens, starts, most_new, mask, scale, out, lse)
+    if type(done) is not int:
+        return done
+    if done < 0:
+        _lib.check(done)
     who = "tree_attention"
     _heads3(who, "q", q)
     _no_grad(who, q, k_cache, v_cache, out, lse)
@@ -317,6 +332,11 @@ def keep_drafted(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tens
     heads, D] of all: new token path[b, i] (int32 [B, m], ascending) of sequence b, i < counts[b] (int32 [B]), moves from slot lens[b] + path[b, i] to
     slot lens[b] + i (sq_keep_drafted).  Entries from the first one on that does not ascend or has no slot are ignored; lens is left as it is.  Sequences
     must not share the pages that are written."""
+    done = _lib.native().keep_drafted(k_cache, v_cache, table, lens, path, counts)
+    if done <= 0:
+        if done:
+            _lib.check(done)
+        return
     who = "keep_drafted"
     _no_grad(who, k_cache, v_cache)
     dev = k_cache.device
