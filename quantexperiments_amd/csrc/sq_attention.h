@@ -38,6 +38,8 @@ struct AttnArgs {
 
 constexpr int ATTN_STEP = 32;                // keys of a step
 constexpr int ATTN_KEYS_MAX = INT32_MAX - 4096;
+constexpr float ATTN_SLACK = 8.f;
+constexpr float ATTN_NOTHING = -3e38f;       // maximum of no scores: weights of -inf are zero against it, and it is nothing beside any other
 
 // A sequence's rows and keys.  What its arguments say beyond the buffers is cut off here: no index below leaves them.
 struct AttnSeq { int first, n, len, total; bool over; };
@@ -114,19 +116,20 @@ template <int DP> struct AttnTile {
     static __device__ __forceinline__ constexpr int v_xor(int key) { return PIECES == 8 ? 2 * ((key >> 1) & 3) : 2 * (key & 7); }
 };
 
-// The pages of a wave's keys: 64 table entries at a time in a register, and the place of every key of one step
+// The pages of a wave's keys: 64 table entries at a time in a register, and the place of each of up to 32 keys
 struct AttnPages {
     int window = -1;             // first page of the entries, -1: none
     int entries;
-    int id, off;                 // lane l: of key l % 32 of the step looked up last
+    int id, off;                 // lane l: of key l % N of the keys looked up last
     bool bad = false;
 };
 
-__device__ __forceinline__ void attn_lookup(const AttnArgs& a, const AttnSeq& s, int b, int step, int lane, AttnPages& p) {
-    const int key = min(step * ATTN_STEP + (lane & 31), s.total - 1);
+template <int N>
+__device__ __forceinline__ void attn_lookup(const AttnArgs& a, const AttnSeq& s, int b, int first, int lane, AttnPages& p) {
+    const int key = min(first + (lane & (N - 1)), s.total - 1);
     const int pg = (int)((uint32_t)key / (uint32_t)a.page);
     p.off = key - pg * a.page;
-    const int lo = __builtin_amdgcn_readfirstlane(pg), hi = __builtin_amdgcn_readlane(pg, 31);
+    const int lo = __builtin_amdgcn_readfirstlane(pg), hi = __builtin_amdgcn_readlane(pg, N - 1);
     if (p.window < 0 || lo < p.window || hi >= p.window + 64) {
         p.window = lo;
         p.entries = lo + lane < a.max_pages ? a.table[(int64_t)b * a.ld_table + lo + lane] : 0;
@@ -136,26 +139,28 @@ __device__ __forceinline__ void attn_lookup(const AttnArgs& a, const AttnSeq& s,
     p.id = id;
 }
 
-// Copies the looked-up step's keys (or values) of one head to `to`: `base` is the head's first byte of the pool
-template <int DP, bool VALUES>
-__device__ __forceinline__ void attn_copy(const AttnArgs& a, const AttnSeq& s, int step, int lane, const AttnPages& p, const char* base, const char* to) {
+// Copies the N keys (or values) looked up, from `first` on, of one head to `to`: `base` is the head's first byte of the pool.  at: the first one's
+// place in its step
+template <int DP, bool VALUES, int N>
+__device__ __forceinline__ void attn_copy(const AttnArgs& a, const AttnSeq& s, int first, int place, int lane, const AttnPages& p, const char* base, const char* to) {
     typedef AttnTile<DP> T;
+    static_assert(N % T::ROWS == 0, "whole copies");
     const int64_t page_b = VALUES ? a.v_page : a.k_page, slot_b = VALUES ? a.v_slot : a.k_slot;
     const int row = lane / T::PIECES, pos = lane % T::PIECES, pieces = a.dim >> 3;
     const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr)to);
     auto piece = [&](int j) {                                // heads narrower than DP: their first piece again
-        const int c = pos ^ (VALUES ? T::v_xor(j * T::ROWS + row) : T::k_xor(j * T::ROWS + row));
+        const int key = place + j * T::ROWS + row, c = pos ^ (VALUES ? T::v_xor(key) : T::k_xor(key));
         return (c < pieces ? c : 0) * 16;
     };
-    if (a.near && a.page % T::ROWS == 0 && (step + 1) * ATTN_STEP <= s.total) {       // the keys of a copy lie in one page
+    if (a.near && a.page % T::ROWS == 0 && first + N <= s.total) {          // the keys of a copy lie in one page
 #pragma unroll
-        for (int j = 0; j < T::COPIES; ++j) {
+        for (int j = 0; j < N / T::ROWS; ++j) {
             const int id = __builtin_amdgcn_readlane(p.id, j * T::ROWS), off = __builtin_amdgcn_readlane(p.off, j * T::ROWS);
             attn_copy16(lds + j * 1024, base + id * page_b + off * slot_b, (uint32_t)(row * (int)slot_b + piece(j)));
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < T::COPIES; ++j) {
+        for (int j = 0; j < N / T::ROWS; ++j) {
             const int id = __shfl(p.id, j * T::ROWS + row), off = __shfl(p.off, j * T::ROWS + row);
             attn_copy16(lds + j * 1024, base + id * page_b + off * slot_b + piece(j));
         }
@@ -168,17 +173,19 @@ template <int DP, int MT> struct AttnRows {
     float4v o[MT][DP / 16];      // lane l: row l % 16, elements 16 * i + 4 * (l / 16) .. + 3
     float m[MT], l[MT];          // maximum (times scale2) of the row, this lane's part of the total
     int tok[MT];                 // new token of the row
+    bool far;                    // some maximum is none yet, or beyond 2^20 (the same for the wave)
 };
 
 template <int DP, int MT>
 __device__ __forceinline__ void attn_rows_begin(const AttnArgs& a, const AttnSeq& s, int head, int row0, int lane, AttnRows<DP, MT>& r) {
     const int rows = s.n * a.group;
+    r.far = true;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int row = min(row0 + t * 16 + (lane & 15), rows - 1), tok = row / a.group;
         const char* q = a.q + (int64_t)(s.first + tok) * a.q_t + (int64_t)(head * a.group + row - tok * a.group) * a.q_h;
         r.tok[t] = tok;
-        r.m[t] = -INFINITY;
+        r.m[t] = ATTN_NOTHING;
         r.l[t] = 0.f;
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
@@ -230,7 +237,9 @@ __device__ __forceinline__ void attn_scores(const AttnRows<DP, MT>& r, const cha
 }
 
 // softmax weights of a step from its scores; the rows' maxima, totals and sums brought up to date.  sees: where masked (the same for
-// the wave; branches around little, as two whole versions of this and of attn_sums would keep the sums in registers twice)
+// the wave; branches around little, as two whole versions of this and of attn_sums would keep the sums in registers twice).
+// What is taken off the exponents need not be the maximum itself: it is raised when a score is more than 2^ATTN_SLACK above it, so that most steps
+// neither fold their maxima over lanes nor scale the sums; weights stay below 2^ATTN_SLACK, far inside fp16 too.
 template <int DT, int DP, int MT>
 __device__ __forceinline__ void attn_weights(const AttnArgs& a, AttnRows<DP, MT>& r, float4v (&st)[MT][2], bool masked, const uint32_t (&sees)[MT], int lane, u32x4 (&p)[MT]) {
     const int g = lane >> 4;
@@ -245,25 +254,30 @@ __device__ __forceinline__ void attn_weights(const AttnArgs& a, AttnRows<DP, MT>
                 for (int i = 0; i < 4; ++i) st[t][h][i] = (sees[t] >> (h * 16 + g * 4 + i)) & 1 ? st[t][h][i] : -INFINITY;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        float v = fmaxf(fmaxf(fmaxf(st[t][0][0], st[t][0][1]), fmaxf(st[t][0][2], st[t][0][3])), fmaxf(fmaxf(st[t][1][0], st[t][1][1]), fmaxf(st[t][1][2], st[t][1][3])));
-        mx[t] = groups_fold(v, [](float x, float y) { return fmaxf(x, y); }) * a.scale2;
-        up |= mx[t] > r.m[t];
+        mx[t] = fmaxf(fmaxf(fmaxf(st[t][0][0], st[t][0][1]), fmaxf(st[t][0][2], st[t][0][3])), fmaxf(fmaxf(st[t][1][0], st[t][1][1]), fmaxf(st[t][1][2], st[t][1][3])));
+        up |= __builtin_fmaf(mx[t], a.scale2, -ATTN_SLACK) > r.m[t];
     }
-    if (__any(up))
+    if (__any(up)) {
+        bool far = false;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            const float m = fmaxf(r.m[t], mx[t]), by = r.m[t] == m ? 1.f : __builtin_amdgcn_exp2f(r.m[t] - m);
+            // (row by row, so that no row's bits depend on what the wave's other rows see)
+            const float top = groups_fold(mx[t], [](float x, float y) { return fmaxf(x, y); });
+            const float m = __builtin_fmaf(top, a.scale2, -ATTN_SLACK) > r.m[t] ? top * a.scale2 : r.m[t], by = __builtin_amdgcn_exp2f(r.m[t] - m);
             r.m[t] = m;
             r.l[t] *= by;
+            far |= !(fabsf(m) <= 0x1p20f);
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) r.o[t][i] *= by;
         }
+        r.far = __any(far);
+    }
+    // The exponent in one operation, exact but for its rounding, where the rounding of what is taken off is of no account (a factor of 2^(1/16) of all
+    // weights at most); of larger maxima it could reach past the largest float, so there a rounded product less the maximum, zero at it.
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        // The exponent in one operation, exact but for its rounding, where m's own is of no account (a factor 2^(1/16) of all weights at
-        // most); of larger maxima it could reach past the largest float, so there a rounded product less m, which is zero at the maximum.
-        float m = r.m[t] == -INFINITY ? 0.f : r.m[t], by = a.scale2;      // (nothing seen so far)
-        if (__any(!(fabsf(m) <= 0x1p20f))) {
+        float m = r.m[t], by = a.scale2;
+        if (r.far && !(fabsf(m) <= 0x1p20f)) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 float x = st[t][i >> 2][i & 3] * a.scale2;
@@ -348,14 +362,14 @@ __device__ __forceinline__ void attn_write(const AttnArgs& a, const AttnSeq& s, 
     const int rows = min(s.n * a.group - row0, rows_here);
     for (int i = tid; i < rows * (DP / 8); i += threads) {
         const int row = i / (DP / 8), e = i % (DP / 8) * 8, all = row0 + row, tok = all / a.group, hq = head * a.group + all - tok * a.group;
-        float m = -INFINITY, l = 0.f;
+        float m = ATTN_NOTHING, l = 0.f;
         for (int w = 0; w < parts; ++w) m = fmaxf(m, ml[w * ml_pitch + row][0]);
         float v[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x) v[x] = 0.f;
         for (int w = 0; w < parts; ++w) {
             const float2v one = ml[w * ml_pitch + row];
-            const float by = one[0] == m ? (m == -INFINITY ? 0.f : 1.f) : __builtin_amdgcn_exp2f(one[0] - m);
+            const float by = __builtin_amdgcn_exp2f(one[0] - m);
             l += one[1] * by;
             if (by == 0.f) continue;
             const float4v* from = reinterpret_cast<const float4v*>(sums + (size_t)(w * rows_here + row) * PITCH + e);
@@ -419,10 +433,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
     auto slot_k = [&](int i) { return ring + (i & 1) * T::BYTES; };
     auto slot_v = [&](int i) { return ring + (2 + (i & 1)) * T::BYTES; };
     auto get_k = [&](int i) {
-        attn_lookup(a, s, b, i, lane, pages);
-        attn_copy<DP, false>(a, s, i, lane, pages, kb, slot_k(i));
+        attn_lookup<ATTN_STEP>(a, s, b, i * ATTN_STEP, lane, pages);
+        attn_copy<DP, false, ATTN_STEP>(a, s, i * ATTN_STEP, 0, lane, pages, kb, slot_k(i));
     };
-    auto get_v = [&](int i) { attn_copy<DP, true>(a, s, i, lane, pages, vb, slot_v(i)); };
+    auto get_v = [&](int i) { attn_copy<DP, true, ATTN_STEP>(a, s, i * ATTN_STEP, 0, lane, pages, vb, slot_v(i)); };
     if (w0 < w1) { get_k(w0); get_v(w0); }
     if (w0 + 1 < w1) { get_k(w0 + 1); get_v(w0 + 1); }
     for (int i = w0; i < w1; ++i) {
@@ -469,6 +483,107 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
     attn_write<DT, DP>(a, s, head, row0, ROWS, split, sums, ml, NW, ROWS, any, tid, NW * 64);
 }
 
+// Stages of the many-row kernel: 64 keys and their values, copied by all waves
+template <int DP> constexpr int attn_stages() { return DP == 256 ? 2 : 3; }
+template <int DP> constexpr int attn_stage_bytes() { return 4 * AttnTile<DP>::BYTES; }
+template <int DP, int MT, int NW> constexpr int attn_tile_lds() { return attn_stages<DP>() * attn_stage_bytes<DP>() + 64; }
+
+// Many rows: each wave has MT * 16 of its own and all waves share the keys, a stage of 64 at a time.  One barrier per stage: behind it every wave's part
+// of the stage has arrived, and the stage before it has been read by all, so its place takes the copies of the one that comes stages - 1 later.
+template <int DT, int DP, int MT, int NW>
+__global__ __launch_bounds__(NW * 64, NW / 4) void attn_tile_kernel(AttnArgs a) {
+    typedef AttnTile<DP> T;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    constexpr int KEYS = 2 * ATTN_STEP, NB = attn_stages<DP>(), STAGE = attn_stage_bytes<DP>(), ROWS = NW * MT * 16, MINE = KEYS / NW, C = MINE / T::ROWS;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // the workgroups of one key head are dealt to as few dies as there are: neighbours are other heads'; last rows, which have most keys, first
+    int id = blockIdx.x;
+    const int groups = a.seqs * a.kv_heads, b = id % groups / a.kv_heads, head = id % groups % a.kv_heads;
+    id /= groups;
+    const int split = id % a.splits, row0 = (a.row_blocks - 1 - id / a.splits) * ROWS;
+    const AttnSeq s = attn_seq(a, b);
+    const int rows = s.n * a.group;
+    if (row0 >= rows) return;
+    const int last = min(row0 + ROWS, rows) - 1;
+    const int seen = a.mask ? s.total : min(s.total, s.len + last / a.group + 1);
+    const int stages = (seen + KEYS - 1) / KEYS, per = (stages + a.splits - 1) / a.splits, begin = min(split * per, stages), end = min(begin + per, stages);
+
+    AttnRows<DP, MT> r;
+    const int mine = row0 + wave * MT * 16;
+    attn_rows_begin<DP, MT>(a, s, head, mine, lane, r);
+    const int from = min(mine, rows - 1) / a.group, to = min(mine + MT * 16, rows) - 1;
+    const int whole = a.mask ? min(s.len, s.total) : min(s.total, s.len + from + 1);                  // keys that all of the wave's rows see
+    const int some = mine >= rows ? 0 : a.mask ? s.total : min(s.total, s.len + to / a.group + 1);    // and that any does
+    AttnPages pages;
+    const char *kb = a.kc + head * a.k_head, *vb = a.vc + head * a.v_head;
+    // (a stage: keys of two steps, values of two steps; this wave copies keys wave * MINE .. of the 64)
+    auto get = [&](int i) {
+        char* at = smem + (i - begin) % NB * STAGE + wave * MINE * T::PITCH;
+        const int first = i * KEYS + wave * MINE, place = wave * MINE % ATTN_STEP;
+        attn_lookup<MINE>(a, s, b, first, lane, pages);
+        attn_copy<DP, false, MINE>(a, s, first, place, lane, pages, kb, at);
+        attn_copy<DP, true, MINE>(a, s, first, place, lane, pages, vb, at + 2 * T::BYTES);
+    };
+#pragma unroll
+    for (int i = 0; i < NB - 1; ++i)
+        if (begin + i < end) get(begin + i);
+    for (int i = begin; i < end; ++i) {
+        if (i + NB - 1 <= end) attn_wait<2 * C * (NB - 2)>(); else attn_wait<0>();
+        attn_reads_done();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (i + NB - 1 < end) get(i + NB - 1);
+        const char* at = smem + (i - begin) % NB * STAGE;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int step = 2 * i + h;
+            if (step * ATTN_STEP >= some) continue;
+            float4v st[MT][2];
+            u32x4 p[MT];
+            uint32_t sees[MT] = {};
+            const bool masked = (step + 1) * ATTN_STEP > whole;
+            attn_scores<DT, DP, MT>(r, at + h * T::BYTES, lane, st);
+            if (masked)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) sees[t] = attn_sees(a, s, step, r.tok[t]);
+            attn_weights<DT, DP, MT>(a, r, st, masked, sees, lane, p);
+            attn_sums<DT, DP, MT>(r, at + (2 + h) * T::BYTES, lane, p, masked, sees);
+        }
+    }
+    int* flags = reinterpret_cast<int*>(smem + NB * STAGE);
+    if (lane == 0) flags[wave] = __any(pages.bad) || s.over;
+    __syncthreads();
+    bool bad = false;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) bad |= flags[w] != 0;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int row = mine + t * 16 + (lane & 15), tok = row / a.group, hq = head * a.group + row - tok * a.group, e = (lane >> 4) * 4;
+        float l = groups_fold(r.l[t], [](float x, float y) { return x + y; });
+        if (bad) l = NAN;
+        if (row >= rows) continue;
+        const int64_t tok_all = s.first + tok;
+        if (a.splits > 1) {
+            const int64_t to_row = (tok_all * a.q_heads + hq) * a.splits + split;
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) *reinterpret_cast<float4v*>(a.po + to_row * DP + d * 16 + e) = r.o[t][d];
+            if (lane < 16) a.pml[to_row] = float2v{r.m[t], l};
+            continue;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        char* out = a.out + tok_all * a.o_t + (int64_t)hq * a.o_h + e * 2;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+            if (d * 16 + e < a.dim) {
+                u32x2 o;
+                o[0] = (uint32_t)AttnType<DT>::one(r.o[t][d][0] * inv) | ((uint32_t)AttnType<DT>::one(r.o[t][d][1] * inv) << 16);
+                o[1] = (uint32_t)AttnType<DT>::one(r.o[t][d][2] * inv) | ((uint32_t)AttnType<DT>::one(r.o[t][d][3] * inv) << 16);
+                *reinterpret_cast<u32x2*>(out + d * 32) = o;
+            }
+        if (lane < 16 && a.lse) a.lse[tok_all * a.q_heads + hq] = l == 0.f ? -INFINITY : (r.m[t] + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+    }
+}
+
 // The splits of a row joined: DP / 4 lanes per row and part of the splits
 template <int DT, int DP>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
@@ -479,12 +594,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     if (tok >= s.n) return;
     const int64_t row = (int64_t)(s.first + tok) * a.q_heads + hq, at = row * a.splits;
     const int q = threadIdx.x % Q, g = threadIdx.x / Q;
-    float m = -INFINITY, l = 0.f;
+    float m = ATTN_NOTHING, l = 0.f;
     for (int i = 0; i < a.splits; ++i) m = fmaxf(m, a.pml[at + i][0]);
     float4v v = float4v{0.f, 0.f, 0.f, 0.f};
     for (int i = 0; i < a.splits; ++i) {
         const float2v one = a.pml[at + i];
-        const float by = one[0] == m ? (m == -INFINITY ? 0.f : 1.f) : __builtin_amdgcn_exp2f(one[0] - m);
+        const float by = __builtin_amdgcn_exp2f(one[0] - m);
         l += one[1] * by;
         if (i % G == g && by != 0.f) v += reinterpret_cast<const float4v*>(a.po + (at + i) * DP)[q] * by;
     }
@@ -505,20 +620,29 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 
 // ------------------------------------------------------------------------------------------ host
 
-struct AttnPlan { int dp, mt, row_blocks, splits; };
+struct AttnPlan { int dp, mt, nw, row_blocks, splits; };       // nw: waves of the many-row kernel; 0: the few-row one
 constexpr int attn_waves(int dp) { return dp == 256 ? 2 : 4; }
 
-template <int DT, int DP, int MT>
-int attn_launch_one(const AttnArgs& a, unsigned grid, hipStream_t s) {
-    constexpr int NW = attn_waves(DP), LDS = attn_lds<DP, MT, NW>();
-    static bool raised[64];
+inline void attn_raise(const void* kernel, int lds, bool (&raised)[64]) {
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
-    if (!raised[dev]) {
-        (void)hipFuncSetAttribute((const void*)attn_kernel<DT, DP, MT, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-        raised[dev] = true;
-    }
+    if (!raised[dev]) (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    raised[dev] = true;
+}
+template <int DT, int DP, int MT>
+int attn_launch_few(const AttnArgs& a, unsigned grid, hipStream_t s) {
+    constexpr int NW = attn_waves(DP), LDS = attn_lds<DP, MT, NW>();
+    static bool raised[64];
+    attn_raise((const void*)attn_kernel<DT, DP, MT, NW>, LDS, raised);
     hipLaunchKernelGGL((attn_kernel<DT, DP, MT, NW>), dim3(grid), dim3(NW * 64), LDS, s, a);
+    return check_launch("sq_tree_attention");
+}
+template <int DT, int DP, int MT, int NW>
+int attn_launch_many(const AttnArgs& a, unsigned grid, hipStream_t s) {
+    constexpr int LDS = attn_tile_lds<DP, MT, NW>();
+    static bool raised[64];
+    attn_raise((const void*)attn_tile_kernel<DT, DP, MT, NW>, LDS, raised);
+    hipLaunchKernelGGL((attn_tile_kernel<DT, DP, MT, NW>), dim3(grid), dim3(NW * 64), LDS, s, a);
     return check_launch("sq_tree_attention");
 }
 
@@ -526,12 +650,8 @@ template <int DT, int DP>
 int attn_launch_dim(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
     const unsigned grid = (unsigned)((int64_t)a.seqs * a.kv_heads * p.row_blocks * p.splits);
     int rc;
-    if (p.mt == 1) rc = attn_launch_one<DT, DP, 1>(a, grid, s);
-    else if (p.mt == 2) rc = attn_launch_one<DT, DP, 2>(a, grid, s);
-    else {
-        if constexpr (DP < 256) rc = attn_launch_one<DT, DP, 4>(a, grid, s);
-        else rc = fail(SQ_EUNSUPPORTED, "sq_tree_attention: plan");
-    }
+    if (p.nw) rc = p.mt == 1 ? attn_launch_many<DT, DP, 1, 8>(a, grid, s) : attn_launch_many<DT, DP, DP == 256 ? 1 : 2, 8>(a, grid, s);
+    else rc = p.mt == 1 ? attn_launch_few<DT, DP, 1>(a, grid, s) : attn_launch_few<DT, DP, 2>(a, grid, s);
     if (rc || p.splits == 1) return rc;
     hipLaunchKernelGGL((attn_join_kernel<DT, DP>), dim3((unsigned)((int64_t)a.seqs * a.most_new * a.q_heads)), dim3(256), 0, s, a);
     return check_launch("sq_tree_attention: join");
