@@ -16,6 +16,8 @@
 // 16-byte pieces placed by XOR with the key's number so that 16 keys' pieces (first product) and 8 keys' pairs of pieces (transposing reads) lie in
 // different banks; the XOR is in the source address, the copy itself is linear.
 #pragma once
+#include <type_traits>
+#include <utility>
 #include "sq_common.h"
 
 namespace sq {
@@ -174,6 +176,18 @@ template <int DP, int MT> struct AttnRows {
     float m[MT], l[MT];          // maximum (times scale2) of the row, this lane's part of the total
     int tok[MT];                 // new token of the row
     bool far;                    // some maximum is none yet, or beyond 2^20 (the same for the wave)
+
+    __device__ __forceinline__ AttnRows<DP, 1> tile(int t) const {
+        AttnRows<DP, 1> x;
+        for (int c = 0; c < DP / 32; ++c) x.q[0][c] = q[t][c];
+        for (int d = 0; d < DP / 16; ++d) x.o[0][d] = o[t][d];
+        x.m[0] = m[t]; x.l[0] = l[t]; x.tok[0] = tok[t]; x.far = true;
+        return x;
+    }
+    __device__ __forceinline__ void put(int t, const AttnRows<DP, 1>& x) {
+        for (int d = 0; d < DP / 16; ++d) o[t][d] = x.o[0][d];
+        m[t] = x.m[0]; l[t] = x.l[0];
+    }
 };
 
 template <int DP, int MT>
@@ -236,16 +250,15 @@ __device__ __forceinline__ void attn_scores(const AttnRows<DP, MT>& r, const cha
         }
 }
 
-// softmax weights of a step from its scores; the rows' maxima, totals and sums brought up to date.  sees: where masked (the same for
-// the wave; branches around little, as two whole versions of this and of attn_sums would keep the sums in registers twice).
+// softmax weights of a step from its scores; the rows' maxima, totals and sums brought up to date.  sees: where MASKED.
 // What is taken off the exponents need not be the maximum itself: it is raised when a score is more than 2^ATTN_SLACK above it, so that most steps
 // neither fold their maxima over lanes nor scale the sums; weights stay below 2^ATTN_SLACK, far inside fp16 too.
-template <int DT, int DP, int MT>
-__device__ __forceinline__ void attn_weights(const AttnArgs& a, AttnRows<DP, MT>& r, float4v (&st)[MT][2], bool masked, const uint32_t (&sees)[MT], int lane, u32x4 (&p)[MT]) {
+template <int DT, int DP, int MT, bool MASKED>
+__device__ __forceinline__ void attn_weights(const AttnArgs& a, AttnRows<DP, MT>& r, float4v (&st)[MT][2], const uint32_t (&sees)[MT], int lane, u32x4 (&p)[MT]) {
     const int g = lane >> 4;
     float mx[MT];
     bool up = false;
-    if (masked)
+    if constexpr (MASKED)
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -295,11 +308,11 @@ __device__ __forceinline__ void attn_weights(const AttnArgs& a, AttnRows<DP, MT>
     }
 }
 
-// sums of a step: values at v.  Where masked, values that are not finite do not go through the product, whose zero weights would make NaN of
+// sums of a step: values at v.  Where MASKED, values that are not finite do not go through the product, whose zero weights would make NaN of
 // them in rows that do not see their keys: such elements are set to zero, the rows' keys that hold them are counted by products of zeros and ones,
 // and rows that see one get what it makes of their sum (an infinity, or NaN).
-template <int DT, int DP, int MT>
-__device__ __forceinline__ void attn_sums(AttnRows<DP, MT>& r, const char* v, int lane, const u32x4 (&p)[MT], bool masked, const uint32_t (&sees)[MT]) {
+template <int DT, int DP, int MT, bool MASKED>
+__device__ __forceinline__ void attn_sums(AttnRows<DP, MT>& r, const char* v, int lane, const u32x4 (&p)[MT], const uint32_t (&sees)[MT]) {
     typedef AttnTile<DP> T;
     typedef AttnType<DT> E;
     typedef short short4v __attribute__((ext_vector_type(4)));
@@ -315,7 +328,7 @@ __device__ __forceinline__ void attn_sums(AttnRows<DP, MT>& r, const char* v, in
             f[2 * h] = w[0];
             f[2 * h + 1] = w[1];
         }
-        if (masked) {
+        if constexpr (MASKED) {
             u32x4 up, down;                                  // ones where a value is not below +inf, not above -inf
             bool any = false;
 #pragma unroll
@@ -432,33 +445,37 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
     char* ring = smem + wave * (4 * T::BYTES);
     auto slot_k = [&](int i) { return ring + (i & 1) * T::BYTES; };
     auto slot_v = [&](int i) { return ring + (2 + (i & 1)) * T::BYTES; };
-    auto get_k = [&](int i) {
+    auto get_k = [&](int i) __attribute__((always_inline)) {
         attn_lookup<ATTN_STEP>(a, s, b, i * ATTN_STEP, lane, pages);
         attn_copy<DP, false, ATTN_STEP>(a, s, i * ATTN_STEP, 0, lane, pages, kb, slot_k(i));
     };
-    auto get_v = [&](int i) { attn_copy<DP, true, ATTN_STEP>(a, s, i * ATTN_STEP, 0, lane, pages, vb, slot_v(i)); };
+    auto get_v = [&](int i) __attribute__((always_inline)) { attn_copy<DP, true, ATTN_STEP>(a, s, i * ATTN_STEP, 0, lane, pages, vb, slot_v(i)); };
     if (w0 < w1) { get_k(w0); get_v(w0); }
     if (w0 + 1 < w1) { get_k(w0 + 1); get_v(w0 + 1); }
-    for (int i = w0; i < w1; ++i) {
+    auto step = [&](int i, auto masked) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked)::value;
         float4v st[MT][2];
         u32x4 p[MT];
         uint32_t sees[MT] = {};
-        const bool masked = (i + 1) * ATTN_STEP > whole;
         if (i + 1 < w1) attn_wait<3 * C>(); else attn_wait<C>();
         attn_scores<DT, DP, MT>(r, slot_k(i), lane, st);
         __builtin_amdgcn_sched_barrier(0);
         attn_reads_done();
         if (i + 2 < w1) get_k(i + 2);
-        if (masked)
+        if constexpr (MASKED)
 #pragma unroll
             for (int t = 0; t < MT; ++t) sees[t] = attn_sees(a, s, i, r.tok[t]);
-        attn_weights<DT, DP, MT>(a, r, st, masked, sees, lane, p);
+        attn_weights<DT, DP, MT, MASKED>(a, r, st, sees, lane, p);
         if (i + 2 < w1) attn_wait<3 * C>(); else if (i + 1 < w1) attn_wait<2 * C>(); else attn_wait<0>();
-        attn_sums<DT, DP, MT>(r, slot_v(i), lane, p, masked, sees);
+        attn_sums<DT, DP, MT, MASKED>(r, slot_v(i), lane, p, sees);
         __builtin_amdgcn_sched_barrier(0);
         attn_reads_done();
         if (i + 2 < w1) get_v(i + 2);
-    }
+    };
+    // (two loops: one with a choice in it would keep two versions of the sums in registers)
+    const int clear = min(max(whole / ATTN_STEP, w0), w1);
+    for (int i = w0; i < clear; ++i) step(i, std::false_type());
+    for (int i = clear; i < w1; ++i) step(i, std::true_type());
     // the waves' sums meet in LDS
     __syncthreads();
     constexpr int PITCH = DP + 4;
@@ -483,19 +500,53 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
     attn_write<DT, DP>(a, s, head, row0, ROWS, split, sums, ml, NW, ROWS, any, tid, NW * 64);
 }
 
-// Stages of the many-row kernel: 64 keys and their values, copied by all waves
-template <int DP> constexpr int attn_stages() { return DP == 256 ? 2 : 3; }
-template <int DP> constexpr int attn_stage_bytes() { return 4 * AttnTile<DP>::BYTES; }
-template <int DP, int MT, int NW> constexpr int attn_tile_lds() { return attn_stages<DP>() * attn_stage_bytes<DP>() + 64; }
+// ------------------------------------------------------------------------------------------ many rows
 
-// Many rows: each wave has MT * 16 of its own and all waves share the keys, a stage of 64 at a time.  One barrier per stage: behind it every wave's part
-// of the stage has arrived, and the stage before it has been read by all, so its place takes the copies of the one that comes stages - 1 later.
-template <int DT, int DP, int MT, int NW>
-__global__ __launch_bounds__(NW * 64, NW / 4) void attn_tile_kernel(AttnArgs a) {
+// Waves of a workgroup (8, or 4 for fewer rows), tiles of 16 rows of a wave, steps of 32 keys in a stage, stages in LDS
+constexpr int attn_tiles(int dp) { return dp == 256 ? 1 : 2; }
+constexpr int attn_stage_steps(int dp, int nw) { return dp == 256 || nw == 4 ? 1 : 2; }
+constexpr int ATTN_STAGES = 4;
+template <int DP, int NW> constexpr int attn_stage_bytes() { return attn_stage_steps(DP, NW) * 2 * AttnTile<DP>::BYTES; }
+template <int DP, int NW> constexpr int attn_tile_lds() { return ATTN_STAGES * attn_stage_bytes<DP, NW>() + 64; }
+
+// In which order a region's instructions are issued: N times one matrix instruction, D LDS reads, V vector instructions, X exponentials
+template <int N, int V, int X, int D> __device__ __forceinline__ void attn_order() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if constexpr (D > 0) __builtin_amdgcn_sched_group_barrier(0x100, D, 0);
+        if constexpr (V > 0) __builtin_amdgcn_sched_group_barrier(0x002, V, 0);
+        if constexpr (X > 0) __builtin_amdgcn_sched_group_barrier(0x400, X, 0);
+    }
+}
+// Largest of eight scores (fmaxf would make each quiet first: twice the instructions)
+__device__ __forceinline__ float attn_most(float4v x, float4v y) {
+    float m;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(x[0]), "v"(x[1]), "v"(x[2]));
+    asm("v_max3_f32 %0, %0, %1, %2" : "+v"(m) : "v"(x[3]), "v"(y[0]));
+    asm("v_max3_f32 %0, %0, %1, %2" : "+v"(m) : "v"(y[1]), "v"(y[2]));
+    return fmaxf(m, y[3]);
+}
+// Many rows: each wave has MT tiles of 16 rows of its own and all waves share the keys, a stage at a time.  One barrier per stage: behind it every wave's
+// part of the stage has arrived, and all waves are done with the stage two before it, whose place takes the copies of the one that comes two later.
+//
+// A slot is one tile of one step: the products of its scores, the exponentials of the tile before it and the sums of the tile before that one, none of
+// which waits for another.  Keys and values of a step stay in registers for its tiles, and each register is filled again, for the next
+// step, right behind its last use.  Two waves per SIMD: with one of 48 rows (a third less to read from LDS) the compiler keeps the sums in the accumulation
+// registers and moves them around the branch that scales them, 1300 cycles a slot instead of 500.
+// The stages at a sequence's end that some row does not see whole go step by step, behind the pipeline, and all of them for heads wider than 128
+// elements, whose keys and values would take the registers of four tiles.
+template <int DT, int DP, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     typedef AttnTile<DP> T;
+    typedef AttnType<DT> E;
+    typedef short short4v __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) short4v* tr_ptr;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    constexpr int KEYS = 2 * ATTN_STEP, NB = attn_stages<DP>(), STAGE = attn_stage_bytes<DP>(), ROWS = NW * MT * 16, MINE = KEYS / NW, C = MINE / T::ROWS;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int MT = attn_tiles(DP), SK = attn_stage_steps(DP, NW), KEYS = SK * ATTN_STEP, NB = ATTN_STAGES, STAGE = attn_stage_bytes<DP, NW>(), ROWS = NW * MT * 16;
+    constexpr int MINE = KEYS / NW, C = MINE / T::ROWS, KC = DP / 32, VD = DP / 16;
+    constexpr bool PIPELINE = MT >= 2;                       // (a tile's maximum is raised while the sums of the tile before it are outstanding)
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, i16 = lane & 15;
     // the workgroups of one key head are dealt to as few dies as there are: neighbours are other heads'; last rows, which have most keys, first
     int id = blockIdx.x;
     const int groups = a.seqs * a.kv_heads, b = id % groups / a.kv_heads, head = id % groups % a.kv_heads;
@@ -514,40 +565,165 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_tile_kernel(AttnArgs a) 
     const int from = min(mine, rows - 1) / a.group, to = min(mine + MT * 16, rows) - 1;
     const int whole = a.mask ? min(s.len, s.total) : min(s.total, s.len + from + 1);                  // keys that all of the wave's rows see
     const int some = mine >= rows ? 0 : a.mask ? s.total : min(s.total, s.len + to / a.group + 1);    // and that any does
+    const int clear = !PIPELINE || mine >= rows ? begin : min(max(whole / KEYS, begin), end);
     AttnPages pages;
     const char *kb = a.kc + head * a.k_head, *vb = a.vc + head * a.v_head;
-    // (a stage: keys of two steps, values of two steps; this wave copies keys wave * MINE .. of the 64)
-    auto get = [&](int i) {
-        char* at = smem + (i - begin) % NB * STAGE + wave * MINE * T::PITCH;
-        const int first = i * KEYS + wave * MINE, place = wave * MINE % ATTN_STEP;
+    auto place = [&](int i) __attribute__((always_inline)) { return smem + (i - begin) % NB * STAGE; };      // keys of SK steps, values of SK steps
+    auto get = [&](int i) __attribute__((always_inline)) {           // this wave copies keys wave * MINE .. of a stage
+        char* at = place(i) + wave * MINE * T::PITCH;
+        const int first = i * KEYS + wave * MINE, in_step = wave * MINE % ATTN_STEP;
         attn_lookup<MINE>(a, s, b, first, lane, pages);
-        attn_copy<DP, false, MINE>(a, s, first, place, lane, pages, kb, at);
-        attn_copy<DP, true, MINE>(a, s, first, place, lane, pages, vb, at + 2 * T::BYTES);
+        attn_copy<DP, false, MINE>(a, s, first, in_step, lane, pages, kb, at);
+        attn_copy<DP, true, MINE>(a, s, first, in_step, lane, pages, vb, at + SK * T::BYTES);
     };
-#pragma unroll
-    for (int i = 0; i < NB - 1; ++i)
-        if (begin + i < end) get(begin + i);
-    for (int i = begin; i < end; ++i) {
-        if (i + NB - 1 <= end) attn_wait<2 * C * (NB - 2)>(); else attn_wait<0>();
+    auto arrive = [&](int i) __attribute__((always_inline)) {        // stage i is there
+        if (i + NB - 2 <= end) attn_wait<2 * C * (NB - 3)>(); else attn_wait<0>();
         attn_reads_done();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (i + NB - 1 < end) get(i + NB - 1);
-        const char* at = smem + (i - begin) % NB * STAGE;
+        if (i + NB - 2 < end) get(i + NB - 2);
+    };
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int step = 2 * i + h;
-            if (step * ATTN_STEP >= some) continue;
-            float4v st[MT][2];
-            u32x4 p[MT];
-            uint32_t sees[MT] = {};
-            const bool masked = (step + 1) * ATTN_STEP > whole;
-            attn_scores<DT, DP, MT>(r, at + h * T::BYTES, lane, st);
-            if (masked)
+    for (int i = 0; i < NB - 2; ++i)
+        if (begin + i < end) get(begin + i);
+
+    if constexpr (PIPELINE) if (begin < clear) {
+        // where this lane reads: piece c of key l % 16 (the step's other half 16 keys behind), elements 16 d .. of 4 keys (likewise)
+        int kat[KC], vat[VD];
 #pragma unroll
-                for (int t = 0; t < MT; ++t) sees[t] = attn_sees(a, s, step, r.tok[t]);
-            attn_weights<DT, DP, MT>(a, r, st, masked, sees, lane, p);
-            attn_sums<DT, DP, MT>(r, at + (2 + h) * T::BYTES, lane, p, masked, sees);
+        for (int c = 0; c < KC; ++c) kat[c] = i16 * T::PITCH + ((c * 4 + g) ^ T::k_xor(i16)) * 16;
+#pragma unroll
+        for (int d = 0; d < VD; ++d) vat[d] = (4 * g + (i16 >> 2)) * T::PITCH + ((d * 2 + ((i16 & 3) >> 1)) ^ T::v_xor(4 * g + (i16 >> 2))) * 16 + (i16 & 1) * 8;
+        u32x4 kf[KC][2], vf[VD], p = {0u, 0u, 0u, 0u};
+        float4v now[2], was[2], old[2];                      // scores of a slot's tile, of the tile before and the one two before
+        float e[8], by1 = a.scale2, less1 = 0.f, by2 = a.scale2, less2 = 0.f;         // exponents of the latter two: by * score - less
+#pragma unroll
+        for (int h = 0; h < 2; ++h) was[h] = old[h] = float4v{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < VD; ++d) vf[d] = u32x4{0u, 0u, 0u, 0u};
+        uint64_t far = ~0ull;                                // lanes with a maximum that is none yet, or beyond 2^20
+        constexpr int HALF = 6;                              // exponentials of a tile beside the sums, the others beside the scores
+        auto scores = [&](int t, auto last, const char* next) __attribute__((always_inline)) {    // last use of these keys: the next ones read behind it
+            now[0] = now[1] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    now[h] = E::mfma(kf[c][h], r.q[t][c], now[h]);
+                    if constexpr (decltype(last)::value) kf[c][h] = *reinterpret_cast<const u32x4*>(next + kat[c] + h * 16 * T::PITCH);
+                }
+        };
+        auto finish = [&](int t) __attribute__((always_inline)) {       // of the tile two before: the rest of its exponentials, its total and its weights
+#pragma unroll
+            for (int i = HALF; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(old[i >> 2][i & 3], by2, -less2));
+            r.l[t] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = E::pack(e[2 * i], e[2 * i + 1]);
+        };
+        auto raise = [&](int t, float mx) __attribute__((always_inline)) {      // of the tile before: its maximum against what is taken off
+            by1 = a.scale2;
+            less1 = r.m[t];
+            if ((__ballot(__builtin_fmaf(mx, a.scale2, -ATTN_SLACK) > r.m[t]) | far) != 0) {
+                const float top = groups_fold(mx, [](float x, float y) { return fmaxf(x, y); });
+                const float m = __builtin_fmaf(top, a.scale2, -ATTN_SLACK) > r.m[t] ? top * a.scale2 : r.m[t], f = __builtin_amdgcn_exp2f(r.m[t] - m);
+                r.m[t] = less1 = m;
+                r.l[t] *= f;
+#pragma unroll
+                for (int d = 0; d < VD; ++d) r.o[t][d] *= f;
+                far = 0;
+#pragma unroll
+                for (int i = 0; i < MT; ++i) far |= __ballot(!(fabsf(r.m[i]) <= 0x1p20f));
+                if (!(fabsf(m) <= 0x1p20f)) {                // (see attn_weights)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float x = was[i >> 2][i & 3] * a.scale2;
+                        asm("" : "+v"(x));
+                        was[i >> 2][i & 3] = x - m;
+                    }
+                    by1 = 1.f;
+                    less1 = 0.f;
+                }
+            }
+        };
+        auto sums = [&](int t, auto last, const char* next) __attribute__((always_inline)) {      // likewise
+#pragma unroll
+            for (int d = 0; d < VD; ++d) {
+                r.o[t][d] = E::mfma(vf[d], p, r.o[t][d]);
+                if constexpr (decltype(last)::value) {
+                    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(lds_ptr)(next + vat[d])));
+                    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(lds_ptr)(next + vat[d] + 16 * T::PITCH)));
+                    vf[d] = u32x4{x[0], x[1], y[0], y[1]};
+                }
+            }
+        };
+        auto half = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(was[i >> 2][i & 3], by1, -less1));
+        };
+        auto most = [&]() __attribute__((always_inline)) { return attn_most(was[0], was[1]); };
+        auto slot_end = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) { old[h] = was[h]; was[h] = now[h]; }
+            by2 = by1;
+            less2 = less1;
+        };
+        arrive(begin);
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) kf[c][h] = *reinterpret_cast<const u32x4*>(place(begin) + kat[c] + h * 16 * T::PITCH);
+        for (int i = begin; i < clear; ++i) {
+            const char *cur = place(i), *nxt = place(i + 1);
+            auto slot = [&](auto number) __attribute__((always_inline)) {
+                constexpr int n = decltype(number)::value, h = n / MT, t = n % MT, t1 = (t + MT - 1) % MT, t2 = (t + MT - 2) % MT;
+                if (n == SK * MT - 1 && i + 1 < clear) arrive(i + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                // (behind the last stage of the pipeline: whatever lies in the next one's place, for nothing)
+                scores(t, std::integral_constant<bool, t == MT - 1>(), h + 1 < SK ? cur + (h + 1) * T::BYTES : nxt);
+                finish(t2);
+                asm volatile("" : "+v"(p), "+v"(r.l[t2]));      // (here, not behind the branch)
+                const float mx = most();
+                attn_order<2 * KC, KC == 4 ? 2 : 4, 0, t == MT - 1>();
+                __builtin_amdgcn_sched_barrier(0);
+                raise(t1, mx);
+                __builtin_amdgcn_sched_barrier(0);
+                sums(t2, std::integral_constant<bool, t2 == MT - 1>(), cur + (SK + h) * T::BYTES);
+                half();
+                attn_order<VD, VD == 8 ? 1 : 2, VD == 8 ? 1 : 2, 2 * (t2 == MT - 1)>();
+                __builtin_amdgcn_sched_barrier(0);
+                slot_end();
+            };
+            [&]<int... N>(std::integer_sequence<int, N...>) __attribute__((always_inline)) { (slot(std::integral_constant<int, N>()), ...); }(std::make_integer_sequence<int, SK * MT>());
+        }
+        // the two tiles that are still on their way
+        finish(MT - 2);
+        raise(MT - 1, most());
+        sums(MT - 2, std::false_type(), nullptr);
+        half();
+        slot_end();
+        finish(MT - 1);
+        sums(MT - 1, std::false_type(), nullptr);
+    }
+    for (int i = clear; i < end; ++i) {
+        arrive(i);
+#pragma unroll 1
+        for (int h = 0; h < SK; ++h) {
+            const int step = SK * i + h;
+            if (step * ATTN_STEP >= some) break;
+            const char* at = place(i) + h * T::BYTES;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {                   // (a tile at a time: there are no registers for more)
+                AttnRows<DP, 1> one = r.tile(t);
+                float4v st[1][2];
+                u32x4 p[1];
+                uint32_t sees[1] = {attn_sees(a, s, step, r.tok[t])};
+                attn_scores<DT, DP, 1>(one, at, lane, st);
+                attn_weights<DT, DP, 1, true>(a, one, st, sees, lane, p);
+                attn_sums<DT, DP, 1, true>(one, at + SK * T::BYTES, lane, p, sees);
+                r.put(t, one);
+            }
         }
     }
     int* flags = reinterpret_cast<int*>(smem + NB * STAGE);
@@ -558,7 +734,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_tile_kernel(AttnArgs a) 
     for (int w = 0; w < NW; ++w) bad |= flags[w] != 0;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        const int row = mine + t * 16 + (lane & 15), tok = row / a.group, hq = head * a.group + row - tok * a.group, e = (lane >> 4) * 4;
+        const int row = mine + t * 16 + i16, tok = row / a.group, hq = head * a.group + row - tok * a.group, e = g * 4;
         float l = groups_fold(r.l[t], [](float x, float y) { return x + y; });
         if (bad) l = NAN;
         if (row >= rows) continue;
@@ -566,18 +742,18 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void attn_tile_kernel(AttnArgs a) 
         if (a.splits > 1) {
             const int64_t to_row = (tok_all * a.q_heads + hq) * a.splits + split;
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d) *reinterpret_cast<float4v*>(a.po + to_row * DP + d * 16 + e) = r.o[t][d];
+            for (int d = 0; d < VD; ++d) *reinterpret_cast<float4v*>(a.po + to_row * DP + d * 16 + e) = r.o[t][d];
             if (lane < 16) a.pml[to_row] = float2v{r.m[t], l};
             continue;
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
         char* out = a.out + tok_all * a.o_t + (int64_t)hq * a.o_h + e * 2;
 #pragma unroll
-        for (int d = 0; d < DP / 16; ++d)
+        for (int d = 0; d < VD; ++d)
             if (d * 16 + e < a.dim) {
                 u32x2 o;
-                o[0] = (uint32_t)AttnType<DT>::one(r.o[t][d][0] * inv) | ((uint32_t)AttnType<DT>::one(r.o[t][d][1] * inv) << 16);
-                o[1] = (uint32_t)AttnType<DT>::one(r.o[t][d][2] * inv) | ((uint32_t)AttnType<DT>::one(r.o[t][d][3] * inv) << 16);
+                o[0] = (uint32_t)E::one(r.o[t][d][0] * inv) | ((uint32_t)E::one(r.o[t][d][1] * inv) << 16);
+                o[1] = (uint32_t)E::one(r.o[t][d][2] * inv) | ((uint32_t)E::one(r.o[t][d][3] * inv) << 16);
                 *reinterpret_cast<u32x2*>(out + d * 32) = o;
             }
         if (lane < 16 && a.lse) a.lse[tok_all * a.q_heads + hq] = l == 0.f ? -INFINITY : (r.m[t] + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
@@ -620,7 +796,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 
 // ------------------------------------------------------------------------------------------ host
 
-struct AttnPlan { int dp, mt, nw, row_blocks, splits; };       // nw: waves of the many-row kernel; 0: the few-row one
+struct AttnPlan { int dp, mt, nw, row_blocks, splits; };       // nw: waves of the many-row kernel; 0: the few-row one, mt tiles of rows
 constexpr int attn_waves(int dp) { return dp == 256 ? 2 : 4; }
 
 inline void attn_raise(const void* kernel, int lds, bool (&raised)[64]) {
@@ -637,12 +813,12 @@ int attn_launch_few(const AttnArgs& a, unsigned grid, hipStream_t s) {
     hipLaunchKernelGGL((attn_kernel<DT, DP, MT, NW>), dim3(grid), dim3(NW * 64), LDS, s, a);
     return check_launch("sq_tree_attention");
 }
-template <int DT, int DP, int MT, int NW>
+template <int DT, int DP, int NW>
 int attn_launch_many(const AttnArgs& a, unsigned grid, hipStream_t s) {
-    constexpr int LDS = attn_tile_lds<DP, MT, NW>();
+    constexpr int LDS = attn_tile_lds<DP, NW>();
     static bool raised[64];
-    attn_raise((const void*)attn_tile_kernel<DT, DP, MT, NW>, LDS, raised);
-    hipLaunchKernelGGL((attn_tile_kernel<DT, DP, MT, NW>), dim3(grid), dim3(NW * 64), LDS, s, a);
+    attn_raise((const void*)attn_tile_kernel<DT, DP, NW>, LDS, raised);
+    hipLaunchKernelGGL((attn_tile_kernel<DT, DP, NW>), dim3(grid), dim3(NW * 64), LDS, s, a);
     return check_launch("sq_tree_attention");
 }
 
@@ -650,8 +826,8 @@ template <int DT, int DP>
 int attn_launch_dim(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
     const unsigned grid = (unsigned)((int64_t)a.seqs * a.kv_heads * p.row_blocks * p.splits);
     int rc;
-    if (p.nw) rc = p.mt == 1 ? attn_launch_many<DT, DP, 1, 8>(a, grid, s) : attn_launch_many<DT, DP, DP == 256 ? 1 : 2, 8>(a, grid, s);
-    else rc = p.mt == 1 ? attn_launch_few<DT, DP, 1>(a, grid, s) : attn_launch_few<DT, DP, 2>(a, grid, s);
+    if (p.nw) rc = p.nw == 4 ? attn_launch_many<DT, DP, 4>(a, grid, s) : attn_launch_many<DT, DP, 8>(a, grid, s);
+    else rc = p.mt == 1 ? attn_launch_few<DT, DP, 1>(a, grid, s) : attn_launch_few<DT, DP, DP == 256 ? 1 : 2>(a, grid, s);
     if (rc || p.splits == 1) return rc;
     hipLaunchKernelGGL((attn_join_kernel<DT, DP>), dim3((unsigned)((int64_t)a.seqs * a.most_new * a.q_heads)), dim3(256), 0, s, a);
     return check_launch("sq_tree_attention: join");

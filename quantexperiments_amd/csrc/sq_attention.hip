@@ -3,26 +3,26 @@
 
 namespace sq {
 
-// Up to 32 rows: one workgroup for all of them, its waves splitting the keys; more: waves with 16 or 32 rows each.  Sequences are cut until
-// the chip has a workgroup per compute unit.
+// Up to 32 rows (16 of wide heads): one workgroup for all of them, its waves splitting the keys; more: four or eight waves with 32 rows each (16).  Sequences are
+// cut until the chip has a workgroup per compute unit.
 static AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
     AttnPlan p;
     p.dp = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
     const int64_t rows = (int64_t)a.most_new * (a.q_heads / c.heads), steps = ((int64_t)a.max_pages * c.page + ATTN_STEP - 1) / ATTN_STEP;
     int64_t per, most;
-    if (rows <= 32) {
+    if (rows <= (p.dp == 256 ? 16 : 32)) {
         p.nw = 0;
         p.mt = rows <= 16 ? 1 : 2;
         per = p.mt * 16;
         most = steps / (2 * attn_waves(p.dp));
     } else {
-        p.nw = 8;
-        p.mt = rows <= 128 || p.dp == 256 ? 1 : 2;
-        per = p.mt * 128;
+        p.mt = attn_tiles(p.dp);
+        p.nw = rows <= 4 * 16 * p.mt ? 4 : 8;
+        per = p.mt * 16 * p.nw;
         most = steps / 4;
     }
     p.row_blocks = (int)((rows + per - 1) / per);
-    const int64_t base = (int64_t)a.seqs * c.heads * p.row_blocks, want = (device_cus() + base - 1) / base;
+    const int64_t base = (int64_t)a.seqs * c.heads * p.row_blocks, want = device_cus() / base;
     p.splits = (int)(want < most ? want : most);
     if (p.splits < 1) p.splits = 1;
     if (p.splits > 128) p.splits = 128;
