@@ -34,7 +34,7 @@ struct AttnArgs {
     int64_t q_t, q_h, o_t, o_h, k_page, k_slot, k_head, v_page, v_slot, v_head;      // bytes
     int64_t ld_table, ld_mask;
     int tokens, seqs, most_new, q_heads, kv_heads, group, dim, pages, page, max_pages, mask_words, row_blocks, splits;
-    int near;                    // slots of a page lie less than 2^24 bytes apart, in order
+    int near;                    // the slots of a page lie within 2^31 bytes, in order
     float scale2;                // scale * log2(e): weights are powers of two
 };
 
@@ -167,6 +167,35 @@ __device__ __forceinline__ void attn_copy(const AttnArgs& a, const AttnSeq& s, i
             attn_copy16(lds + j * 1024, base + id * page_b + off * slot_b + piece(j));
         }
     }
+}
+
+// The same for a run of stages of KEYS keys, N of each looked up and copied by this wave, where the N lie in one page (page % N == 0) and the slots of a page
+// near each other: the place of the next ones is walked to, and everything but a lane's own offset is worked out once for the wave.
+struct AttnWalk { int pg, off; };
+
+template <int DP, int N, int KEYS>
+__device__ __forceinline__ void attn_walk_copy(const AttnArgs& a, int b, int place, int lane, AttnPages& p, AttnWalk& w, const char* kb, const char* vb, const char* kto,
+                                               const char* vto) {
+    typedef AttnTile<DP> T;
+    if (p.window < 0 || w.pg < p.window || w.pg >= p.window + 64) {
+        p.window = w.pg;
+        p.entries = w.pg + lane < a.max_pages ? a.table[(int64_t)b * a.ld_table + w.pg + lane] : 0;
+    }
+    int id = __builtin_amdgcn_readlane(p.entries, w.pg - p.window);
+    if ((uint32_t)id >= (uint32_t)a.pages) id = 0, p.bad = true;
+    const int row = lane / T::PIECES, pos = lane % T::PIECES, pieces = a.dim >> 3, k_slot = (int)a.k_slot, v_slot = (int)a.v_slot;
+    const uint32_t kl = (uint32_t)(uintptr_t)(lds_ptr)kto, vl = (uint32_t)(uintptr_t)(lds_ptr)vto;
+    const char *kat = kb + id * a.k_page + (uint32_t)(w.off * k_slot), *vat = vb + id * a.v_page + (uint32_t)(w.off * v_slot);
+    auto piece = [&](int c) { return (c < pieces ? c : 0) * 16; };
+#pragma unroll
+    for (int j = 0; j < N / T::ROWS; ++j) {
+        const int key = place + j * T::ROWS + row;
+        attn_copy16(kl + j * 1024, kat, (uint32_t)((j * T::ROWS + row) * k_slot + piece(pos ^ T::k_xor(key))));
+        attn_copy16(vl + j * 1024, vat, (uint32_t)((j * T::ROWS + row) * v_slot + piece(pos ^ T::v_xor(key))));
+    }
+    w.pg += KEYS / a.page;
+    w.off += KEYS % a.page;
+    if (w.off >= a.page) { w.off -= a.page; ++w.pg; }
 }
 
 // What a wave keeps of its MT * 16 rows
@@ -568,10 +597,18 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     const int clear = !PIPELINE || mine >= rows ? begin : min(max(whole / KEYS, begin), end);
     AttnPages pages;
     const char *kb = a.kc + head * a.k_head, *vb = a.vc + head * a.v_head;
+    const bool easy = a.near && a.page % MINE == 0;
+    AttnWalk walk;
+    walk.pg = (begin * KEYS + wave * MINE) / a.page;
+    walk.off = begin * KEYS + wave * MINE - walk.pg * a.page;
     auto place = [&](int i) __attribute__((always_inline)) { return smem + (i - begin) % NB * STAGE; };      // keys of SK steps, values of SK steps
     auto get = [&](int i) __attribute__((always_inline)) {           // this wave copies keys wave * MINE .. of a stage
         char* at = place(i) + wave * MINE * T::PITCH;
         const int first = i * KEYS + wave * MINE, in_step = wave * MINE % ATTN_STEP;
+        if (easy && first + MINE <= s.total) {
+            attn_walk_copy<DP, MINE, KEYS>(a, b, in_step, lane, pages, walk, kb, vb, at, at + SK * T::BYTES);
+            return;
+        }
         attn_lookup<MINE>(a, s, b, first, lane, pages);
         attn_copy<DP, false, MINE>(a, s, first, in_step, lane, pages, kb, at);
         attn_copy<DP, true, MINE>(a, s, first, in_step, lane, pages, vb, at + SK * T::BYTES);

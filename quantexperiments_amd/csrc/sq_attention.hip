@@ -86,7 +86,7 @@ int sq_tree_attention(const sq_attention* a, const sq_cache* cache, void* worksp
     k.tokens = a->tokens; k.seqs = a->seqs; k.most_new = a->most_new; k.q_heads = a->q_heads; k.kv_heads = cache->heads; k.group = a->q_heads / cache->heads;
     k.dim = cache->dim; k.pages = cache->pages; k.page = cache->page; k.max_pages = a->max_pages; k.mask_words = a->mask_words;
     k.row_blocks = p.row_blocks; k.splits = p.splits;
-    auto near = [](int64_t b) { return b >= 0 && b < (1 << 24); };
+    auto near = [&](int64_t b) { return b >= 0 && b < (1 << 24) && b * (cache->page + 32) < INT32_MAX; };
     k.near = near(k.k_slot) && near(k.v_slot);
     k.scale2 = a->scale * 1.4426950408889634f;
     return cache->dtype == SQ_F16 ? attn_launch_f16(k, p, (hipStream_t)stream) : attn_launch_bf16(k, p, (hipStream_t)stream);
