@@ -40,6 +40,7 @@ struct AttnArgs {
 
 constexpr int ATTN_STEP = 32;                // keys of a step
 constexpr int ATTN_KEYS_MAX = INT32_MAX - 4096;
+constexpr int ATTN_SPLITS_MAX = 128;         // parts of a sequence
 constexpr float ATTN_SLACK = 8.f;
 constexpr float ATTN_NOTHING = -3e38f;       // maximum of no scores: weights of -inf are zero against it, and it is nothing beside any other
 
@@ -169,33 +170,41 @@ __device__ __forceinline__ void attn_copy(const AttnArgs& a, const AttnSeq& s, i
     }
 }
 
-// The same for a run of stages of KEYS keys, N of each looked up and copied by this wave, where the N lie in one page (page % N == 0) and the slots of a page
-// near each other: the place of the next ones is walked to, and everything but a lane's own offset is worked out once for the wave.
-struct AttnWalk { int pg, off; };
-
-template <int DP, int N, int KEYS>
-__device__ __forceinline__ void attn_walk_copy(const AttnArgs& a, int b, int place, int lane, AttnPages& p, AttnWalk& w, const char* kb, const char* vb, const char* kto,
-                                               const char* vto) {
-    typedef AttnTile<DP> T;
-    if (p.window < 0 || w.pg < p.window || w.pg >= p.window + 64) {
-        p.window = w.pg;
-        p.entries = w.pg + lane < a.max_pages ? a.table[(int64_t)b * a.ld_table + w.pg + lane] : 0;
+// The same where groups of keys that follow each other lie in one page and the slots of a page near each other: the place of the next group is walked to,
+// and everything but a lane's own offset is worked out once for the wave (with the above a step of 32 keys took 1.8 us of a wave's time, most
+// of it on addresses).
+struct AttnPlace { int64_t k, v; };          // a group's first key and value, bytes from the head's first
+struct AttnWalk {
+    int pg, off;
+    __device__ __forceinline__ void begin(const AttnArgs& a, int key) { pg = (int)((uint32_t)key / (uint32_t)a.page); off = key - pg * a.page; }
+    __device__ __forceinline__ void go(const AttnArgs& a, int pages, int slots) {      // pages * page + slots keys on, slots < page
+        pg += pages;
+        off += slots;
+        if (off >= a.page) { off -= a.page; ++pg; }
     }
-    int id = __builtin_amdgcn_readlane(p.entries, w.pg - p.window);
-    if ((uint32_t)id >= (uint32_t)a.pages) id = 0, p.bad = true;
-    const int row = lane / T::PIECES, pos = lane % T::PIECES, pieces = a.dim >> 3, k_slot = (int)a.k_slot, v_slot = (int)a.v_slot;
-    const uint32_t kl = (uint32_t)(uintptr_t)(lds_ptr)kto, vl = (uint32_t)(uintptr_t)(lds_ptr)vto;
-    const char *kat = kb + id * a.k_page + (uint32_t)(w.off * k_slot), *vat = vb + id * a.v_page + (uint32_t)(w.off * v_slot);
-    auto piece = [&](int c) { return (c < pieces ? c : 0) * 16; };
+    __device__ __forceinline__ AttnPlace find(const AttnArgs& a, int b, int lane, AttnPages& p) const {
+        if (p.window < 0 || pg < p.window || pg >= p.window + 64) {
+            p.window = pg;
+            p.entries = pg + lane < a.max_pages ? a.table[(int64_t)b * a.ld_table + pg + lane] : 0;
+        }
+        int id = __builtin_amdgcn_readlane(p.entries, pg - p.window);
+        if ((uint32_t)id >= (uint32_t)a.pages) id = 0, p.bad = true;
+        return {id * a.k_page + (uint32_t)(off * (int)a.k_slot), id * a.v_page + (uint32_t)(off * (int)a.v_slot)};
+    }
+};
+
+// Copies N keys (values) of one group; where: the first one's place in its step
+template <int DP, bool VALUES, int N>
+__device__ __forceinline__ void attn_copy_group(const AttnArgs& a, int where, int lane, const char* from, const char* to) {
+    typedef AttnTile<DP> T;
+    static_assert(N % T::ROWS == 0, "whole copies");
+    const int row = lane / T::PIECES, pos = lane % T::PIECES, pieces = a.dim >> 3, slot_b = (int)(VALUES ? a.v_slot : a.k_slot);
+    const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr)to);
 #pragma unroll
     for (int j = 0; j < N / T::ROWS; ++j) {
-        const int key = place + j * T::ROWS + row;
-        attn_copy16(kl + j * 1024, kat, (uint32_t)((j * T::ROWS + row) * k_slot + piece(pos ^ T::k_xor(key))));
-        attn_copy16(vl + j * 1024, vat, (uint32_t)((j * T::ROWS + row) * v_slot + piece(pos ^ T::v_xor(key))));
+        const int key = where + j * T::ROWS + row, c = pos ^ (VALUES ? T::v_xor(key) : T::k_xor(key));
+        attn_copy16(lds + j * 1024, from, (uint32_t)((j * T::ROWS + row) * slot_b + (c < pieces ? c : 0) * 16));
     }
-    w.pg += KEYS / a.page;
-    w.off += KEYS % a.page;
-    if (w.off >= a.page) { w.off -= a.page; ++w.pg; }
 }
 
 // What a wave keeps of its MT * 16 rows
@@ -238,7 +247,11 @@ __device__ __forceinline__ void attn_rows_begin(const AttnArgs& a, const AttnSeq
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) r.o[t][i] = float4v{0.f, 0.f, 0.f, 0.f};
     }
-    // (here, or the loop over the keys waits for them, and so for all that is in flight, in every step)
+}
+
+// The rows' loads waited for, behind the first copies: with the table's entries, which those wait for anyway.  (Not at all, the loop over the keys would wait for them, and so
+// for all that is in flight, in every step.)
+template <int DP, int MT> __device__ __forceinline__ void attn_rows_ready(AttnRows<DP, MT>& r) {
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -474,13 +487,34 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
     char* ring = smem + wave * (4 * T::BYTES);
     auto slot_k = [&](int i) { return ring + (i & 1) * T::BYTES; };
     auto slot_v = [&](int i) { return ring + (2 + (i & 1)) * T::BYTES; };
+    // (pages of whole groups of 16: a step is two groups, each in one page)
+    const bool easy = a.near && a.page % 16 == 0;
+    AttnWalk walk;
+    walk.begin(a, w0 * ATTN_STEP);
+    AttnPlace at[2];
     auto get_k = [&](int i) __attribute__((always_inline)) {
+        if (easy && (i + 1) * ATTN_STEP <= s.total) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                at[x] = walk.find(a, b, lane, pages);
+                attn_copy_group<DP, false, 16>(a, 16 * x, lane, kb + at[x].k, slot_k(i) + x * 16 * T::PITCH);
+                walk.go(a, 16 / a.page, 16 % a.page);
+            }
+            return;
+        }
         attn_lookup<ATTN_STEP>(a, s, b, i * ATTN_STEP, lane, pages);
         attn_copy<DP, false, ATTN_STEP>(a, s, i * ATTN_STEP, 0, lane, pages, kb, slot_k(i));
     };
-    auto get_v = [&](int i) __attribute__((always_inline)) { attn_copy<DP, true, ATTN_STEP>(a, s, i * ATTN_STEP, 0, lane, pages, vb, slot_v(i)); };
+    auto get_v = [&](int i) __attribute__((always_inline)) {
+        if (easy && (i + 1) * ATTN_STEP <= s.total) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) attn_copy_group<DP, true, 16>(a, 16 * x, lane, vb + at[x].v, slot_v(i) + x * 16 * T::PITCH);
+            return;
+        }
+        attn_copy<DP, true, ATTN_STEP>(a, s, i * ATTN_STEP, 0, lane, pages, vb, slot_v(i)); };
     if (w0 < w1) { get_k(w0); get_v(w0); }
     if (w0 + 1 < w1) { get_k(w0 + 1); get_v(w0 + 1); }
+    attn_rows_ready(r);
     auto step = [&](int i, auto masked) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked)::value;
         float4v st[MT][2];
@@ -599,14 +633,16 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     const char *kb = a.kc + head * a.k_head, *vb = a.vc + head * a.v_head;
     const bool easy = a.near && a.page % MINE == 0;
     AttnWalk walk;
-    walk.pg = (begin * KEYS + wave * MINE) / a.page;
-    walk.off = begin * KEYS + wave * MINE - walk.pg * a.page;
+    walk.begin(a, begin * KEYS + wave * MINE);
     auto place = [&](int i) __attribute__((always_inline)) { return smem + (i - begin) % NB * STAGE; };      // keys of SK steps, values of SK steps
     auto get = [&](int i) __attribute__((always_inline)) {           // this wave copies keys wave * MINE .. of a stage
         char* at = place(i) + wave * MINE * T::PITCH;
         const int first = i * KEYS + wave * MINE, in_step = wave * MINE % ATTN_STEP;
         if (easy && first + MINE <= s.total) {
-            attn_walk_copy<DP, MINE, KEYS>(a, b, in_step, lane, pages, walk, kb, vb, at, at + SK * T::BYTES);
+            const AttnPlace from = walk.find(a, b, lane, pages);
+            attn_copy_group<DP, false, MINE>(a, in_step, lane, kb + from.k, at);
+            attn_copy_group<DP, true, MINE>(a, in_step, lane, vb + from.v, at + SK * T::BYTES);
+            walk.go(a, KEYS / a.page, KEYS % a.page);
             return;
         }
         attn_lookup<MINE>(a, s, b, first, lane, pages);
@@ -623,6 +659,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < NB - 2; ++i)
         if (begin + i < end) get(begin + i);
+    attn_rows_ready(r);
 
     if constexpr (PIPELINE) if (begin < clear) {
         // where this lane reads: piece c of key l % 16 (the step's other half 16 keys behind), elements 16 d .. of 4 keys (likewise)
@@ -797,30 +834,60 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     }
 }
 
-// The splits of a row joined: DP / 4 lanes per row and part of the splits
-template <int DT, int DP>
+// The splits of a row joined: DP / 4 lanes per row and G parts of its splits, as many rows as that leaves room for.  (One row per workgroup took 15 us for
+// 10,752 rows of 4 splits, 22 MB, where this takes 6.)
+template <int DT, int DP, int G>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-    constexpr int Q = DP / 4, G = 256 / Q;
-    __shared__ __attribute__((aligned(16))) float4v part[G][Q];
-    const int per = a.most_new * a.q_heads, b = blockIdx.x / per, r = blockIdx.x % per, tok = r / a.q_heads, hq = r % a.q_heads;
-    const AttnSeq s = attn_seq(a, b);
-    if (tok >= s.n) return;
+    constexpr int Q = DP / 4, R = 256 / (Q * G);
+    static_assert(R >= 1, "a workgroup holds a row");
+    __shared__ __attribute__((aligned(16))) float4v part[R][G][Q];
+    const int tid = threadIdx.x, q = tid % Q, g = tid / Q % G, rr = tid / (Q * G);
+    const uint32_t per = (uint32_t)a.most_new * a.q_heads, i = blockIdx.x * R + rr, b = i / per, r = i - b * per, tok = r / a.q_heads, hq = r - tok * a.q_heads;
+    const AttnSeq s = attn_seq(a, min((int)b, a.seqs - 1));
+    const bool live = (int)b < a.seqs && (int)tok < s.n;
     const int64_t row = (int64_t)(s.first + tok) * a.q_heads + hq, at = row * a.splits;
-    const int q = threadIdx.x % Q, g = threadIdx.x / Q;
     float m = ATTN_NOTHING, l = 0.f;
-    for (int i = 0; i < a.splits; ++i) m = fmaxf(m, a.pml[at + i][0]);
     float4v v = float4v{0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < a.splits; ++i) {
-        const float2v one = a.pml[at + i];
-        const float by = __builtin_amdgcn_exp2f(one[0] - m);
-        l += one[1] * by;
-        if (i % G == g && by != 0.f) v += reinterpret_cast<const float4v*>(a.po + (at + i) * DP)[q] * by;
-    }
-    part[g][q] = v;
-    __syncthreads();
-    if (g) return;
+    const float4v* po = reinterpret_cast<const float4v*>(a.po + at * DP) + q;
+    if constexpr (G == 1) {
+        if (live) {
+            for (int x = 0; x < a.splits; ++x) m = fmaxf(m, a.pml[at + x][0]);
+            for (int x = 0; x < a.splits; ++x) {
+                const float2v one = a.pml[at + x];
+                const float by = __builtin_amdgcn_exp2f(one[0] - m);
+                l += one[1] * by;
+                if (by != 0.f) v += po[(size_t)x * Q] * by;
+            }
+        }
+    } else {
+        // (one row: its maxima and totals fetched at once, a split per thread)
+        __shared__ float2v ml[ATTN_SPLITS_MAX];
+        if (live && tid < a.splits) ml[tid] = a.pml[at + tid];
+        __syncthreads();
+        if (live) {
+            for (int x = 0; x < a.splits; ++x) m = fmaxf(m, ml[x][0]);
+            for (int x = 0; x < a.splits; ++x) l += ml[x][1] * __builtin_amdgcn_exp2f(ml[x][0] - m);
+            for (int x = g; x < a.splits; x += 4 * G) {
+                float4v y[4];
+                float by[4];
 #pragma unroll
-    for (int i = 1; i < G; ++i) v += part[i][q];
+                for (int k = 0; k < 4; ++k) {
+                    const int z = x + k * G;
+                    by[k] = z < a.splits ? __builtin_amdgcn_exp2f(ml[min(z, a.splits - 1)][0] - m) : 0.f;
+                    y[k] = po[(size_t)min(z, a.splits - 1) * Q];
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v += by[k] != 0.f ? y[k] * by[k] : float4v{0.f, 0.f, 0.f, 0.f};
+            }
+        }
+    }
+    if constexpr (G > 1) {
+        part[rr][g][q] = v;
+        __syncthreads();
+#pragma unroll
+        for (int x = 1; x < G; ++x) v += part[rr][(g + x) % G][q];
+    }
+    if (!live || g) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (q * 4 < a.dim) {
         u32x2 o;
@@ -866,7 +933,10 @@ int attn_launch_dim(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
     if (p.nw) rc = p.nw == 4 ? attn_launch_many<DT, DP, 4>(a, grid, s) : attn_launch_many<DT, DP, 8>(a, grid, s);
     else rc = p.mt == 1 ? attn_launch_few<DT, DP, 1>(a, grid, s) : attn_launch_few<DT, DP, DP == 256 ? 1 : 2>(a, grid, s);
     if (rc || p.splits == 1) return rc;
-    hipLaunchKernelGGL((attn_join_kernel<DT, DP>), dim3((unsigned)((int64_t)a.seqs * a.most_new * a.q_heads)), dim3(256), 0, s, a);
+    const int64_t all = (int64_t)a.seqs * a.most_new * a.q_heads;
+    constexpr int MOST = 1024 / DP;                          // parts of a row that fill a workgroup
+    if (a.splits > 8) hipLaunchKernelGGL((attn_join_kernel<DT, DP, MOST>), dim3((unsigned)all), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_join_kernel<DT, DP, 1>), dim3((unsigned)((all + MOST - 1) / MOST)), dim3(256), 0, s, a);
     return check_launch("sq_tree_attention: join");
 }
 

@@ -3,18 +3,23 @@
 
 namespace sq {
 
-// Up to 32 rows (16 of wide heads): one workgroup for all of them, its waves splitting the keys; more: four or eight waves with 32 rows each (16).  Sequences are
-// cut until the chip has a workgroup per compute unit.
+// Up to 32 rows (16 of wide heads): one workgroup for all of them, its waves splitting the keys; more: four or eight waves with 32 rows each (16).
+// Sequences are cut until the chip has a workgroup per compute unit, but not into less than two steps per wave, nor into two such parts (the joining
+// launch takes 3 us, as a step of 1 us does per wave: 500 slots whole 12.1, in two 12.9 us; 4000 in 15 parts 14.5, in 7 17.0 us).  Sequences of several lengths
+// are cut for two rounds of workgroups where a wave then still has 16 steps: 32 of 2,240 to 8,192 slots x 8 key heads 136 us, 163 in one round; but
+// 8 of 4000 x 4 heads 27 us in 480 parts, 23 in 224, and 64 of 500 27 us in 512, 18 in 256.
 static AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
     AttnPlan p;
     p.dp = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
     const int64_t rows = (int64_t)a.most_new * (a.q_heads / c.heads), steps = ((int64_t)a.max_pages * c.page + ATTN_STEP - 1) / ATTN_STEP;
+    const int waves = attn_waves(p.dp);
     int64_t per, most;
     if (rows <= (p.dp == 256 ? 16 : 32)) {
         p.nw = 0;
         p.mt = rows <= 16 ? 1 : 2;
         per = p.mt * 16;
-        most = steps / (2 * attn_waves(p.dp));
+        most = steps / (2 * waves);
+        if (most <= 2) most = 1;
     } else {
         p.mt = attn_tiles(p.dp);
         p.nw = rows <= 4 * 16 * p.mt ? 4 : 8;
@@ -22,10 +27,12 @@ static AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
         most = steps / 4;
     }
     p.row_blocks = (int)((rows + per - 1) / per);
-    const int64_t base = (int64_t)a.seqs * c.heads * p.row_blocks, want = device_cus() / base;
+    const int64_t base = (int64_t)a.seqs * c.heads * p.row_blocks, cus = device_cus();
+    int64_t want = cus / base;
+    if (a.seqs > 1 && !p.nw && 2 * cus / base > 1 && steps / (2 * cus / base) >= 16 * waves) want = 2 * cus / base;
     p.splits = (int)(want < most ? want : most);
     if (p.splits < 1) p.splits = 1;
-    if (p.splits > 128) p.splits = 128;
+    if (p.splits > ATTN_SPLITS_MAX) p.splits = ATTN_SPLITS_MAX;
     return p;
 }
 
