@@ -27,7 +27,7 @@ struct HeadsArgs {
     const double* freqs;
     const void* positions;
     const void* slots;
-    float scale, eps, w_offset, sign;
+    float scale, eps, w_offset, sign, inv_dim;
     int tokens, dim, pairs, interleaved, w_dtype, wide_positions, wide_slots, pages, page, lanes_log2, heads;
 };
 
@@ -106,14 +106,8 @@ template <int DT> __device__ __forceinline__ void narrow(Chunk<DT>& c, const flo
         else c.v[e >> 1] = f2bf_x2(v[e], v[e + 1]);
     }
 }
-__device__ __forceinline__ void load8_any(const void* p, int dtype, int i, float* v) {
-    if (dtype == SQ_F32) { Chunk<SQ_F32> c; load8(c, p, i); widen(c, v); }
-    else if (dtype == SQ_F16) { Chunk<SQ_F16> c; load8(c, p, i); widen(c, v); }
-    else { Chunk<SQ_BF16> c; load8(c, p, i); widen(c, v); }
-}
-
 // Sum over groups of 2^log2n neighbouring lanes, the same in all of them
-__device__ __forceinline__ float lanes_sum(float v, int log2n) {
+__device__ __forceinline__ float lanes_sum(float v, int log2n) {        // (of lanes that all are active)
     auto other = [](float x, auto ctrl) {
         const int b = __builtin_bit_cast(int, x);
         return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(b, b, decltype(ctrl)::value, 0xF, 0xF, false));
@@ -133,62 +127,74 @@ __device__ __forceinline__ float lanes_sum(float v, int log2n) {
 // One workgroup per token (and part of its heads, blockIdx.y).  A thread takes 16 elements of a head, whichever the layout: the 8 pairs
 // whose angles are 8c .. 8c + 7, or 16 neighbours behind the rotated part, so that a head is dim / 16 lanes (rounded up to a power
 // of two for the sum of its squares) with two 16-byte loads each, in flight while the token's angles are worked out, once for all heads.
-template <int DT>
+// WT: the type of the norm weights, or none; they are fetched with the elements (behind the sum of squares they cost 2048 tokens of 28 + 4 + 4 heads of
+// 128 another 4 us), and layout and type are chosen at compile time (chosen here they take a fifth of the waves' registers and more than that was worth).
+constexpr int NO_NORM = -1;
+template <int DT, int WT, bool INTERLEAVED>
 __global__ __launch_bounds__(HEADS_MAX_THREADS) void heads_kernel(HeadsArgs a) {
     extern __shared__ __attribute__((aligned(16))) float2v angles[];
+    constexpr bool NORM = WT != NO_NORM;
+    constexpr int WD = NORM ? WT : DT;
     const int tid = threadIdx.x, lanes = 1 << a.lanes_log2, items = a.heads << a.lanes_log2, c = tid & (lanes - 1);
     const bool live = c < a.dim / 16, turned = c < a.pairs / 8;
-    const int e0 = turned && !a.interleaved ? 8 * c : 16 * c, e1 = turned && !a.interleaved ? a.pairs + 8 * c : 16 * c + 8;
+    const int e0 = turned && !INTERLEAVED ? 8 * c : 16 * c, e1 = turned && !INTERLEAVED ? a.pairs + 8 * c : 16 * c + 8;
     for (int n = blockIdx.x; n < a.tokens; n += gridDim.x) {
         const int64_t pos = a.pairs ? load_index(a.positions, a.wide_positions, n) : 0;
         int64_t slot = -1;
         if (a.slots) slot = load_index(a.slots, a.wide_slots, n);
+        const double f = tid < a.pairs ? a.freqs[tid] : 0.0;
         bool first = true;
         for (int item = blockIdx.y * blockDim.x + tid; first || item < items; item += gridDim.y * blockDim.x) {
             int h = item >> a.lanes_log2;
             const HeadsPart p = part_of(a, h);
-            const bool mine = live && item < items;
+            const bool mine = live && item < items, normed = NORM && mine && p.w;
             Chunk<DT> x0, x1;
+            Chunk<WD> w0, w1;
             if (mine) {
                 load8(x0, p.in, n * p.in_t + h * p.in_h + e0);
                 load8(x1, p.in, n * p.in_t + h * p.in_h + e1);
             }
+            if (NORM && normed) {
+                load8(w0, p.w, e0);
+                load8(w1, p.w, e1);
+            }
             if (first) {
-                for (int i = tid; i < a.pairs; i += blockDim.x) angles[i] = angle_of(pos, a.freqs[i], a.scale, a.sign);
+                if (tid < a.pairs) angles[tid] = angle_of(pos, f, a.scale, a.sign);
+                for (int i = tid + blockDim.x; i < a.pairs; i += blockDim.x) angles[i] = angle_of(pos, a.freqs[i], a.scale, a.sign);
                 __syncthreads();
                 first = false;
             }
-            float v[16];
-            if (mine && (p.w || (p.turn && turned))) {
+            float v[16], rstd = 0.f;
+            if (mine) {
                 widen(x0, v);
                 widen(x1, v + 8);
             }
-            if (__any(mine && p.w)) {                     // (lanes of one head take the same way)
+            if (NORM) {                                   // (by all lanes: those behind a narrow head's elements add zeros)
                 float ss = 0.f;
-                if (mine && p.w)
+                if (mine)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) ss = __builtin_fmaf(v[e], v[e], ss);
-                ss = lanes_sum(ss, a.lanes_log2);
-                if (mine && p.w) {
-                    const float rstd = rsqrtf(ss / (float)a.dim + a.eps);
-                    float w[16];
-                    load8_any(p.w, a.w_dtype, e0, w);
-                    load8_any(p.w, a.w_dtype, e1, w + 8);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) v[e] = v[e] * rstd * (w[e] + a.w_offset);
-                }
+                rstd = rsqrtf(lanes_sum(ss, a.lanes_log2) * a.inv_dim + a.eps);
             }
             if (!mine) continue;
+            if (NORM && normed) {
+                float w[16];
+                widen(w0, w);
+                widen(w1, w + 8);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = v[e] * rstd * (w[e] + a.w_offset);
+            }
             if (p.turn && turned) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float2v t = angles[8 * c + i];
-                    const float x = a.interleaved ? v[2 * i] : v[i], y = a.interleaved ? v[2 * i + 1] : v[i + 8];
+                    float &x = v[INTERLEAVED ? 2 * i : i], &y = v[INTERLEAVED ? 2 * i + 1 : i + 8];
                     const float xx = __builtin_fmaf(x, t[0], -y * t[1]), yy = __builtin_fmaf(y, t[0], x * t[1]);
-                    if (a.interleaved) { v[2 * i] = xx; v[2 * i + 1] = yy; } else { v[i] = xx; v[i + 8] = yy; }
+                    x = xx;
+                    y = yy;
                 }
             }
-            if (p.w || (p.turn && turned)) {
+            if ((NORM && normed) || (p.turn && turned)) {    // (else the bits as they are: NaN payloads, signs)
                 narrow(x0, v);
                 narrow(x1, v + 8);
             }
@@ -240,7 +246,7 @@ __global__ __launch_bounds__(256) void heads_any_kernel(HeadsArgs a) {
         if (p.w) {
             float ss = 0.f;
             for (int e = lane; e < a.dim; e += 64) { const float v = load_one<DT>(p.in, from + e); ss = __builtin_fmaf(v, v, ss); }
-            rstd = rsqrtf(wave_sum(ss) / (float)a.dim + a.eps);
+            rstd = rsqrtf(wave_sum(ss) * a.inv_dim + a.eps);
         }
         auto normed = [&](int e) {
             const float v = load_one<DT>(p.in, from + e);
@@ -268,6 +274,7 @@ __global__ __launch_bounds__(256) void heads_any_kernel(HeadsArgs a) {
 static bool wide_ok(const HeadsArgs& a, int dtype) {
     const int unit = dtype == SQ_F32 ? 4 : 8;                               // elements of 16 bytes
     if (a.dim % 16 || a.dim > 512 || a.pairs % 8) return false;
+    if ((a.p[0].w || a.p[1].w) && a.w_dtype != dtype && a.w_dtype != SQ_F32) return false;
     uintptr_t at = 0;
     int64_t strides = 0;
     for (const HeadsPart& p : a.p) {
@@ -282,6 +289,7 @@ int launch_heads(const HeadsArgs& args, int dtype, const char* who, hipStream_t 
     HeadsArgs a = args;
     a.heads = a.p[0].heads + a.p[1].heads + a.p[2].heads;
     if (a.tokens == 0 || a.heads == 0) return SQ_OK;
+    a.inv_dim = 1.f / (float)a.dim;
     if (wide_ok(a, dtype)) {
         a.lanes_log2 = 0;
         while ((16 << a.lanes_log2) < a.dim) ++a.lanes_log2;
@@ -292,9 +300,20 @@ int launch_heads(const HeadsArgs& args, int dtype, const char* who, hipStream_t 
         const int parts = a.tokens >= 2 * device_cus() ? 1 : rounds;
         const dim3 grid((unsigned)(a.tokens < (1 << 20) ? a.tokens : 1 << 20), (unsigned)(parts < 65535 ? parts : 65535));
         const size_t lds = (size_t)(a.pairs ? a.pairs : 1) * sizeof(float2v);
-        if (dtype == SQ_F32) hipLaunchKernelGGL(heads_kernel<SQ_F32>, grid, dim3(threads), lds, s, a);
-        else if (dtype == SQ_F16) hipLaunchKernelGGL(heads_kernel<SQ_F16>, grid, dim3(threads), lds, s, a);
-        else hipLaunchKernelGGL(heads_kernel<SQ_BF16>, grid, dim3(threads), lds, s, a);
+        const int wt = !(a.p[0].w || a.p[1].w) ? NO_NORM : a.w_dtype;
+        auto go = [&](auto dt, auto w) {
+            constexpr int DT = decltype(dt)::value, WT = decltype(w)::value;
+            if (a.interleaved) hipLaunchKernelGGL((heads_kernel<DT, WT, true>), grid, dim3(threads), lds, s, a);
+            else hipLaunchKernelGGL((heads_kernel<DT, WT, false>), grid, dim3(threads), lds, s, a);
+        };
+        auto of = [&](auto dt) {
+            if (wt == NO_NORM) go(dt, std::integral_constant<int, NO_NORM>());
+            else if (wt == SQ_F32) go(dt, std::integral_constant<int, SQ_F32>());
+            else go(dt, dt);
+        };
+        if (dtype == SQ_F32) of(std::integral_constant<int, SQ_F32>());
+        else if (dtype == SQ_F16) of(std::integral_constant<int, SQ_F16>());
+        else of(std::integral_constant<int, SQ_BF16>());
         return check_launch(who);
     }
     const int64_t blocks = ((int64_t)a.tokens * a.heads + 3) / 4;
