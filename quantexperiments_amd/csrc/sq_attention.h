@@ -662,12 +662,19 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     attn_rows_ready(r);
 
     if constexpr (PIPELINE) if (begin < clear) {
-        // where this lane reads: piece c of key l % 16 (the step's other half 16 keys behind), elements 16 d .. of 4 keys (likewise)
-        int kat[KC], vat[VD];
-#pragma unroll
-        for (int c = 0; c < KC; ++c) kat[c] = i16 * T::PITCH + ((c * 4 + g) ^ T::k_xor(i16)) * 16;
-#pragma unroll
-        for (int d = 0; d < VD; ++d) vat[d] = (4 * g + (i16 >> 2)) * T::PITCH + ((d * 2 + ((i16 & 3) >> 1)) ^ T::v_xor(4 * g + (i16 >> 2))) * 16 + (i16 & 1) * 8;
+        // Where this lane reads in a step: of key l % 16 (the step's other half 16 keys behind) its first piece, of 4 keys their first elements (likewise).
+        // A step begins at a multiple of a key's bytes, so the others are an XOR away from the step's own address: no registers for each.
+        const uint32_t kat = i16 * T::PITCH + (g ^ T::k_xor(i16)) * 16;
+        const uint32_t vat = (4 * g + (i16 >> 2)) * T::PITCH + (((i16 & 3) >> 1) ^ T::v_xor(4 * g + (i16 >> 2))) * 16 + (i16 & 1) * 8;
+        typedef const __attribute__((address_space(3))) u32x4* k_ptr;
+        auto lds = [](const char* at) __attribute__((always_inline)) { return (uint32_t)(uintptr_t)(lds_ptr)at; };
+        auto read_k = [&](uint32_t step, int c, int h) __attribute__((always_inline)) { return *(k_ptr)(uintptr_t)(((step + kat) ^ (c * 64)) + h * 16 * T::PITCH); };
+        auto read_v = [&](uint32_t step, int d) __attribute__((always_inline)) {
+            const uint32_t at = (step + vat) ^ (d * 32);
+            const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(uintptr_t)at));
+            const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(uintptr_t)(at + 16 * T::PITCH)));
+            return u32x4{x[0], x[1], y[0], y[1]};
+        };
         u32x4 kf[KC][2], vf[VD], p = {0u, 0u, 0u, 0u};
         float4v now[2], was[2], old[2];                      // scores of a slot's tile, of the tile before and the one two before
         float e[8], by1 = a.scale2, less1 = 0.f, by2 = a.scale2, less2 = 0.f;         // exponents of the latter two: by * score - less
@@ -679,14 +686,14 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
         for (int d = 0; d < VD; ++d) vf[d] = u32x4{0u, 0u, 0u, 0u};
         uint64_t far = ~0ull;                                // lanes with a maximum that is none yet, or beyond 2^20
         constexpr int HALF = 6;                              // exponentials of a tile beside the sums, the others beside the scores
-        auto scores = [&](int t, auto last, const char* next) __attribute__((always_inline)) {    // last use of these keys: the next ones read behind it
+        auto scores = [&](int t, auto last, uint32_t next) __attribute__((always_inline)) {    // last use of these keys: the next ones read behind it
             now[0] = now[1] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < KC; ++c)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     now[h] = E::mfma(kf[c][h], r.q[t][c], now[h]);
-                    if constexpr (decltype(last)::value) kf[c][h] = *reinterpret_cast<const u32x4*>(next + kat[c] + h * 16 * T::PITCH);
+                    if constexpr (decltype(last)::value) kf[c][h] = read_k(next, c, h);
                 }
         };
         auto finish = [&](int t) __attribute__((always_inline)) {       // of the tile two before: the rest of its exponentials, its total and its weights
@@ -721,15 +728,11 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
                 }
             }
         };
-        auto sums = [&](int t, auto last, const char* next) __attribute__((always_inline)) {      // likewise
+        auto sums = [&](int t, auto last, uint32_t next) __attribute__((always_inline)) {      // likewise
 #pragma unroll
             for (int d = 0; d < VD; ++d) {
                 r.o[t][d] = E::mfma(vf[d], p, r.o[t][d]);
-                if constexpr (decltype(last)::value) {
-                    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(lds_ptr)(next + vat[d])));
-                    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(lds_ptr)(next + vat[d] + 16 * T::PITCH)));
-                    vf[d] = u32x4{x[0], x[1], y[0], y[1]};
-                }
+                if constexpr (decltype(last)::value) vf[d] = read_v(next, d);
             }
         };
         auto half = [&]() __attribute__((always_inline)) {
@@ -747,9 +750,9 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) kf[c][h] = *reinterpret_cast<const u32x4*>(place(begin) + kat[c] + h * 16 * T::PITCH);
+            for (int h = 0; h < 2; ++h) kf[c][h] = read_k(lds(place(begin)), c, h);
         for (int i = begin; i < clear; ++i) {
-            const char *cur = place(i), *nxt = place(i + 1);
+            const uint32_t cur = lds(place(i)), nxt = lds(place(i + 1));
             auto slot = [&](auto number) __attribute__((always_inline)) {
                 constexpr int n = decltype(number)::value, h = n / MT, t = n % MT, t1 = (t + MT - 1) % MT, t2 = (t + MT - 2) % MT;
                 if (n == SK * MT - 1 && i + 1 < clear) arrive(i + 1);
@@ -774,11 +777,11 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
         // the two tiles that are still on their way
         finish(MT - 2);
         raise(MT - 1, most());
-        sums(MT - 2, std::false_type(), nullptr);
+        sums(MT - 2, std::false_type(), 0);
         half();
         slot_end();
         finish(MT - 1);
-        sums(MT - 1, std::false_type(), nullptr);
+        sums(MT - 1, std::false_type(), 0);
     }
     for (int i = clear; i < end; ++i) {
         arrive(i);

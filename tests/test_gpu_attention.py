@@ -413,3 +413,23 @@ def test_a_drafted_step_equals_the_tokens_decoded_one_by_one():
         rows = torch.tensor([slot(b, s) for s in range(total)]).cuda()
         for c, o in zip(caches, one_by_one):
             assert torch.equal(c.view(layers, -1, hk, d)[:, rows], o.view(layers, -1, hk, d)[:, rows])
+
+
+@pytest.mark.parametrize("seqs,hq,hk,new,page", [(70, 2, 1, 1, 16), (130, 3, 1, 2, 5), (3, 7, 1, 20, 16), (9, 4, 2, 1, 64), (2, 2, 2, 40, 16), (66, 1, 1, 33, 16)])
+def test_sequences_of_unlike_lengths_cut_into_parts_of_one(seqs, hq, hk, new, page):
+    g = torch.Generator().manual_seed(seqs)
+    lens = [int(x) for x in torch.randint(0, 60, (seqs,), generator=g)]
+    lens[seqs // 2], lens[0], lens[-1] = 3100, 0, 700        # one takes most of the parts, others none of their own
+    news = [max(0, new - b % 3) if b != seqs // 2 else new for b in range(seqs)]
+    s = Setup(lens, news, hq, hk, 64, page, tree=new > 1, seed=seqs)
+    s.check(*attend(s))
+
+
+def test_queries_that_barely_differ_and_rows_that_see_the_same_agree_in_every_part():
+    # rows of one token with equal queries are equal bit for bit, wherever their key head's keys are cut
+    s = Setup([4000, 77], [5, 1], 16, 2, 128, 16, seed=12)
+    s.q[:, 1:8] = s.q[:, :1]
+    s.q[:, 9:] = s.q[:, 8:9]
+    out, lse = attend(s)
+    assert torch.equal(out[:, 1:8], out[:, :1].expand(-1, 7, -1)) and torch.equal(lse[:, 9:], lse[:, 8:9].expand(-1, 7))
+    s.check(out, lse)
