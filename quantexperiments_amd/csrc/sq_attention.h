@@ -809,7 +809,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
         finish(MT - 1);
         sums(MT - 1, std::false_type(), 0);
     }
-    for (int i = clear; i < end; ++i) {
+    auto plain = [&](int i, auto masked) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked)::value;
         arrive(i);
 #pragma unroll 1
         for (int h = 0; h < SK; ++h) {
@@ -821,14 +822,19 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
                 AttnRows<DP, 1> one = r.tile(t);
                 float4v st[1][2];
                 u32x4 p[1];
-                uint32_t sees[1] = {attn_sees(a, s, step, r.tok[t])};
+                uint32_t sees[1] = {};
+                if constexpr (MASKED) sees[0] = attn_sees(a, s, step, r.tok[t]);
                 attn_scores<DT, DP, 1>(one, at, lane, st);
-                attn_weights<DT, DP, 1, true>(a, one, st, sees, lane, p);
-                attn_sums<DT, DP, 1, true>(one, at + SK * T::BYTES, lane, p, sees);
+                attn_weights<DT, DP, 1, MASKED>(a, one, st, sees, lane, p);
+                attn_sums<DT, DP, 1, MASKED>(one, at + SK * T::BYTES, lane, p, sees);
                 r.put(t, one);
             }
         }
-    }
+    };
+    int next = clear;
+    if constexpr (!PIPELINE)
+        for (const int all = mine >= rows ? begin : min(max(whole / KEYS, begin), end); next < all; ++next) plain(next, std::false_type());
+    for (; next < end; ++next) plain(next, std::true_type());
     int* flags = reinterpret_cast<int*>(smem + NB * STAGE);
     if (lane == 0) flags[wave] = __any(pages.bad) || s.over;
     __syncthreads();
