@@ -981,6 +981,7 @@ int attn_launch(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
     if (p.dp == 128) return attn_launch_dim<DT, 128>(a, p, s);
     return attn_launch_dim<DT, 256>(a, p, s);
 }
+bool rows_apart(int tokens, int heads, int64_t t, int64_t h, int dim);      // sq_heads.hip
 int attn_launch_f16(const AttnArgs& a, const AttnPlan& p, hipStream_t s);
 int attn_launch_bf16(const AttnArgs& a, const AttnPlan& p, hipStream_t s);
 

@@ -45,6 +45,8 @@ static int check_attention(const char* who, const sq_attention* a, const sq_cach
         a->ld_table < a->max_pages)
         return fail(SQ_EINVAL, "%s: %d tokens, %d sequences, at most %d new, tables of %d (ld %lld), %d pages of %d", who, a->tokens, a->seqs, a->most_new, a->max_pages,
                     (long long)a->ld_table, c->pages, c->page);
+    if ((int64_t)a->seqs * a->most_new > INT32_MAX / a->q_heads)          // (no more rows than 32 bits count: a plan of more would wrap)
+        return fail(SQ_EUNSUPPORTED, "%s: %d sequences of up to %d new tokens and %d heads at once", who, a->seqs, a->most_new, a->q_heads);
     if (!(a->scale > 0.f) || a->scale > 3e38f) return fail(SQ_EINVAL, "%s: scale %g", who, (double)a->scale);
     if (!a->starts && (int64_t)a->seqs * a->most_new != a->tokens)
         return fail(SQ_EINVAL, "%s: %d tokens are not %d for each of %d sequences", who, a->tokens, a->most_new, a->seqs);
@@ -75,8 +77,10 @@ int sq_tree_attention(const sq_attention* a, const sq_cache* cache, void* worksp
     const int64_t strides = a->q_token | a->q_head | a->out_token | a->out_head | cache->k_page | cache->k_slot | cache->k_head | cache->v_page | cache->v_slot | cache->v_head;
     if (strides % 8 || (((uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)cache->k | (uintptr_t)cache->v) & 15))
         return fail(SQ_EUNSUPPORTED, "%s: q, out, keys and values need 16-byte aligned heads", who);
+    const int64_t ot = a->out_token < 0 ? -a->out_token : a->out_token, oh = a->out_head < 0 ? -a->out_head : a->out_head;
+    if (!rows_apart(a->tokens, a->q_heads, ot, oh, cache->dim)) return fail(SQ_EINVAL, "%s: rows of the output overlap (strides %lld, %lld)", who, (long long)ot, (long long)oh);
     const AttnPlan p = attn_plan(*a, *cache);
-    if ((int64_t)a->seqs * cache->heads * p.row_blocks * p.splits > (1 << 23) || (int64_t)a->seqs * a->most_new * a->q_heads > (p.splits > 1 ? 1 << 23 : INT32_MAX))
+    if ((int64_t)a->seqs * cache->heads * p.row_blocks * p.splits > (1 << 23) || (p.splits > 1 && (int64_t)a->seqs * a->most_new * a->q_heads > (1 << 23)))
         return fail(SQ_EUNSUPPORTED, "%s: %d sequences of up to %d new tokens and %d heads at once", who, a->seqs, a->most_new, a->q_heads);
     const size_t need = p.splits == 1 ? 0 : (size_t)a->tokens * a->q_heads * p.splits * (p.dp * 4 + 8);
     if (ws_bytes < need || (need && (!workspace || ((uintptr_t)workspace & 255))))

@@ -324,15 +324,20 @@ int launch_heads(const HeadsArgs& args, int dtype, const char* who, hipStream_t 
     return check_launch(who);
 }
 
+// Whether heads of dim elements, t apart from token to token and h from head to head, share no element: heads lie within tokens or tokens within heads,
+// as far as there are several
+bool rows_apart(int tokens, int heads, int64_t t, int64_t h, int dim) {
+    if (heads <= 1) return tokens <= 1 || t >= dim;
+    if (tokens <= 1) return h >= dim;
+    return (h >= dim && t >= (heads - 1) * h + dim) || (t >= dim && h >= (tokens - 1) * t + dim);
+}
+
 static int check_heads(const char* who, const sq_heads* p, int tokens, int dim, bool needs_out) {
     if (p->heads < 0 || p->heads > (1 << 20)) return fail(SQ_EINVAL, "%s: %d heads", who, p->heads);
     if (tokens && p->heads && (!p->in || (needs_out && !p->out))) return fail(SQ_EINVAL, "%s: null in / out", who);
     if (p->out && tokens && p->heads) {
-        // rows of the output must not overlap: heads within tokens or tokens within heads, as far as there are several
         const int64_t t = p->out_token < 0 ? -p->out_token : p->out_token, h = p->out_head < 0 ? -p->out_head : p->out_head;
-        const bool ok = p->heads == 1 ? tokens == 1 || t >= dim
-                        : tokens == 1 ? h >= dim
-                                      : (h >= dim && t >= (p->heads - 1) * h + dim) || (t >= dim && h >= (tokens - 1) * t + dim);
+        const bool ok = rows_apart(tokens, p->heads, t, h, dim);
         if (!ok) return fail(SQ_EINVAL, "%s: rows of the output overlap (strides %lld, %lld)", who, (long long)p->out_token, (long long)p->out_head);
         if (p->out == p->in && ((tokens > 1 && p->out_token != p->in_token) || (p->heads > 1 && p->out_head != p->in_head)))
             return fail(SQ_EINVAL, "%s: in place with other strides", who);
@@ -475,8 +480,8 @@ int sq_keep_drafted(const sq_cache* cache, int32_t layers, int64_t k_layer, int6
     const char* who = "sq_keep_drafted";
     if (!cache) return fail(SQ_EINVAL, "%s: null cache", who);
     if (cache->dtype < SQ_F32 || cache->dtype > SQ_BF16) return fail(SQ_EINVAL, "%s: dtype %d", who, cache->dtype);
-    if (layers < 0 || seqs < 0 || seqs > 65535 || most < 0 || cache->pages < 0 || cache->page < 1 || cache->heads < 0 || cache->dim < 1 || max_pages < 0 ||
-        ld_table < max_pages || ld_path < most)
+    if (layers < 0 || seqs < 0 || seqs > 65535 || most < 0 || cache->pages < 0 || cache->page < 1 || cache->heads < 0 || cache->dim < 1 || cache->heads > (1 << 20) ||
+        cache->dim > 65536 || layers > (1 << 20) || max_pages < 0 || ld_table < max_pages || ld_path < most)
         return fail(SQ_EINVAL, "%s: %d layers, %d sequences, paths of %d (ld %lld), tables of %d (ld %lld), %d pages of %d, %d heads of %d", who, layers, seqs, most,
                     (long long)ld_path, max_pages, (long long)ld_table, cache->pages, cache->page, cache->heads, cache->dim);
     if (!layers || !seqs || !most || !max_pages || !cache->pages || !cache->heads) return SQ_OK;

@@ -10,6 +10,7 @@
 // also words the errors.  Nothing is kept between calls but what a matrix is (its tensors and sizes, dropped by PackedLinear
 // whenever one of its attributes is set).
 #include <Python.h>
+#include <algorithm>
 #include <cmath>
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
@@ -506,6 +507,14 @@ bool apart(const at::Tensor& a, const at::Tensor& b) {       // no byte between 
     ends(b, bl, bh);
     return ah <= bl || bh <= al;
 }
+// No element of heads a in heads b: apart, or in different columns of one stacked product's rows
+bool columns_apart(const at::Tensor& a, const at::Tensor& b) {
+    if (apart(a, b)) return true;
+    const int64_t row = a.stride(0); const int64_t size = a.element_size(); const int64_t bytes = (const char*)b.data_ptr() - (const char*)a.data_ptr();
+    if (b.element_size() != size || b.stride(0) != row || row <= 0 || a.stride(1) < 0 || b.stride(1) < 0 || bytes % size) return false;
+    const int64_t at = ((bytes / size) % row + row) % row;
+    return at >= (a.size(1) - 1) * a.stride(1) + a.size(2) && at + (b.size(1) - 1) * b.stride(1) + b.size(2) <= row;
+}
 // out is x, or apart from it, with x's shape and type
 bool out_ok(const at::Tensor& out, const at::Tensor& x, int dev) {
     return heads_on(out, dev) && out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type() &&
@@ -588,12 +597,11 @@ PyObject* qk_norm_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
             if (w && (dtype_of(*w) < 0 || !vector_on(*w, dev, d, w->scalar_type(), w->scalar_type()))) return answer(NOT_COVERED);
         if (qw && kw && qw->scalar_type() != kw->scalar_type()) return answer(NOT_COVERED);
         if (qw || kw) wd = dtype_of(qw ? *qw : *kw);
-        // (in place, or new: other outputs are told apart in Python)
+        if (v && (v->dim() != 3 || v->numel() == 0)) return answer(NOT_COVERED);
         for (int i = 0; i < 2; ++i) {
-            const at::Tensor* g = i ? kg : qg; const at::Tensor& x = i ? k : q;
-            if (!g || (heads_on(*g, dev) && g->data_ptr() == x.data_ptr() && g->strides() == x.strides() && g->sizes() == x.sizes() && g->scalar_type() == x.scalar_type()))
-                continue;
-            if (!out_ok(*g, x, dev) || !apart(*g, i ? q : k) || (v && !apart(*g, *v)) || (i && qg && !apart(*g, *qg))) return answer(NOT_COVERED);
+            const at::Tensor* g = i ? kg : qg;
+            if (g && (!out_ok(*g, i ? k : q, dev) || !columns_apart(*g, i ? q : k) || (v && !columns_apart(*g, *v)) || (i && qg && !columns_apart(*g, *qg))))
+                return answer(NOT_COVERED);                  // (Python says what is wrong)
         }
         if (cached) {
             if (!heads_on(*v, dev) || v->sizes() != k.sizes() || v->scalar_type() != q.scalar_type() || !vector_on(*slots, dev, rows, at::kLong, at::kInt) || kc->dim() != 4 ||
@@ -644,7 +652,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
             (lse && (lse->scalar_type() != at::kFloat || lse->dim() != 2 || lse->size(0) != rows || lse->size(1) != q.size(1) || !plain_on(*lse, dev) || !lse->is_contiguous())))
             return answer(NOT_COVERED);
         int64_t most = starts ? rows : rows / b;
-        if (a[6] != Py_None) most = PyLong_AsLongLong(a[6]);
+        if (a[6] != Py_None) most = starts ? std::min<int64_t>(PyLong_AsLongLong(a[6]), rows) : PyLong_AsLongLong(a[6]);
         const double scale = a[8] == Py_None ? std::pow((double)c.dim, -0.5) : PyFloat_AsDouble(a[8]);
         if (PyErr_Occurred()) return nullptr;
         if (most < 0 || most > INT32_MAX || (!starts && most * b != rows) || !(scale > 0 && scale < 3e38)) return answer(NOT_COVERED);

@@ -78,10 +78,16 @@ def _on_gpu(who: str, dev, **tensors) -> None:
             raise ValueError(f"{who}: {name} is on {t.device}, not on {dev}")
 
 
+def _fits(who: str, *sizes: int) -> None:
+    if max(sizes) > 2 ** 31 - 1:
+        raise ValueError(f"{who}: sizes beyond 32 bits: {sizes}")
+
+
 def _heads3(who: str, name: str, t: torch.Tensor, shape=None) -> None:
     if t.dim() != 3 or t.dtype not in _lib.DTYPES or (t.shape[2] > 1 and t.stride(2) != 1) or (shape is not None and tuple(t.shape) != tuple(shape)):
         want = "[tokens, heads, D]" if shape is None else str(tuple(shape))
         raise ValueError(f"{who}: {name} must be {want}, fp16 / bf16 / fp32, with neighbouring elements: got {tuple(t.shape)} {t.dtype}, strides {t.stride()}")
+    _fits(who, *t.shape)
 
 
 def _vector(who: str, name: str, t: torch.Tensor, n: int, *dtypes) -> None:
@@ -92,6 +98,7 @@ def _vector(who: str, name: str, t: torch.Tensor, n: int, *dtypes) -> None:
 def _rows2(who: str, name: str, t: torch.Tensor, n: int, dtype) -> None:
     if t.dim() != 2 or t.shape[0] != n or t.dtype != dtype or (t.shape[1] > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < t.shape[1]):
         raise ValueError(f"{who}: {name} must be {dtype} with {n} rows and unit column stride: got {tuple(t.shape)} {t.dtype}, strides {t.stride()}")
+    _fits(who, *t.shape)
 
 
 def _extent(t: torch.Tensor) -> tuple:
@@ -156,6 +163,7 @@ def _cache(who: str, k: torch.Tensor, v: torch.Tensor, written: bool = False) ->
             raise ValueError(f"{who}: the elements of a head must be neighbours in the caches (strides {t.stride()})")
         if written and any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
             raise ValueError(f"{who}: a cache that is written must not be expanded (strides {t.stride()})")
+    _fits(who, *k.shape)
     if k.shape[-3] < 1:
         raise ValueError(f"{who}: pages without slots")
     if written and k.numel() and _extent(k)[0] < _extent(v)[1] and _extent(v)[0] < _extent(k)[1] and _same(k, v):
@@ -291,6 +299,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         raise ValueError(f"{who}: {n} tokens are not as many for each of {b} sequences: pass starts")
     if most_new is None:
         most_new = n if starts is not None else n // b
+    elif starts is not None:
+        most_new = min(most_new, n)                          # (no sequence has more)
     if most_new < 0 or (starts is None and most_new * b != n):
         raise ValueError(f"{who}: most_new {most_new} for {n} tokens of {b} sequences")
     if mask is not None:

@@ -143,3 +143,21 @@ def test_frequencies():
         with pytest.raises(ValueError):
             rotary_freqs(device="cpu", **bad)
     assert rotary_freqs(0, device="cpu")[0].numel() == 0
+
+
+def test_sizes_whose_products_pass_64_bits_are_refused():
+    L = _lib.lib()
+    U, E = _lib.SQ_EUNSUPPORTED, _lib.SQ_EINVAL
+    for seqs, new, hq in ((1, 1 << 30, 1 << 10), ((1 << 31) - 1, (1 << 31) - 1, 1 << 16), (1 << 16, 1 << 15, 1)):
+        a, c = attention(tokens=2, seqs=seqs, most_new=new, q_heads=hq, starts=P), cache(heads=1)
+        assert L.sq_tree_attention(a, c, None, 0, None) == U and L.sq_tree_attention_workspace_bytes(a, c) == 0
+    keep = lambda layers, **kw: L.sq_keep_drafted(cache(**kw), layers, 0, 0, P, 8, 8, P, P, 4, 4, P, 1, None)
+    for layers, kw in (((1 << 31) - 1, dict(heads=(1 << 31) - 1, dim=1 << 16)), ((1 << 20) + 1, {}), (1, dict(heads=(1 << 20) + 1)), (1, dict(dim=65537))):
+        assert keep(layers, **kw) == E
+    assert keep(1 << 20, heads=1 << 20, dim=1 << 16) == U
+
+
+def test_outputs_of_attention_whose_rows_overlap_are_refused():
+    L = _lib.lib()
+    for kw in (dict(out_token=256), dict(out_head=56), dict(out_token=0), dict(out_token=64, out_head=64)):
+        assert L.sq_tree_attention(attention(**kw), cache(), None, 0, None) == _lib.SQ_EINVAL, kw

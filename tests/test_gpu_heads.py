@@ -268,3 +268,74 @@ def test_the_c_entry_points_refuse_on_a_gpu_box_too():
     h, r = _lib.SqHeads(heads=2), _lib.SqRotation(scale=1.0)
     assert L.sq_rotary(h, 1, 64, _lib.SQ_F16, r, None) == _lib.SQ_EINVAL
     assert math.isclose(r.scale, 1.0)
+
+
+def test_operands_that_alias_are_refused_and_columns_of_one_product_are_not():
+    from quantexperiments_amd.kernels import qk_norm_rotary, rotary
+    n, d = 5, 64
+    pos, f = torch.arange(n).cuda(), torch.rand(32, dtype=torch.float64).cuda()
+    x = torch.randn(n, 4, d, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    was = x.clone()
+    y = torch.empty_like(x)
+    big = torch.zeros(n, 6, d, dtype=torch.bfloat16).cuda()
+    for kw in (dict(q=x, k=x, q_out=x), dict(q=x, k=x, k_out=x), dict(q=x, k=x[:, :2], q_out=x), dict(q=x, k=y, q_out=y), dict(q=x, k=y, k_out=x), dict(q=x, k=y, q_out=big[:, :4], k_out=big[:, 2:]),
+               dict(q=big[:, :4], k=y, q_out=big[:, 1:5]), dict(q=x, k=y, q_out=x[:, :3])):
+        with pytest.raises(ValueError):
+            qk_norm_rotary(positions=pos, freqs=f, **kw)
+    caches = [torch.zeros(2, 8, 4, d, dtype=torch.bfloat16).cuda() for _ in range(2)]
+    slots = torch.arange(n).cuda()
+    cached = dict(positions=pos, freqs=f, v=y, k_cache=caches[0], v_cache=caches[1], slots=slots)
+    for kw in (dict(q=x, k=x, q_out=x), dict(q=x, k=big[:, :4], q_out=y), dict(q=x, k=big[:, :4], k_cache=caches[1]), dict(q=x, k=caches[0][0, :n]), dict(q=x, k=big[:, :4], slots=None),
+               dict(q=x, k=big[:, :4], v=None), dict(q=x, k=big[:, :4], k_cache=caches[0][:1].expand(2, -1, -1, -1))):
+        with pytest.raises(ValueError):
+            qk_norm_rotary(**{**cached, **kw})
+    for kw in (dict(out=big[:, 1:5], x=big[:, :4]), dict(x=x, out=x[:1].expand(n, -1, -1)), dict(x=x, out=x.half()), dict(x=x, out=y[:, :3])):
+        with pytest.raises(ValueError):
+            rotary(positions=pos, freqs=f, **kw)
+    assert torch.equal(x, was) and not bool(big.any()) and not bool(caches[0].any())
+    # columns of one stacked product, in place: what a decoder layer does
+    both = torch.cat((x, was[:, :2]), 1)
+    q, k = qk_norm_rotary(both[:, :4], both[:, 4:], pos, f, q_out=both[:, :4], k_out=both[:, 4:])
+    assert torch.equal(q, rotary(was, pos, f)) and torch.equal(k, rotary(was[:, :2], pos, f))
+
+
+def test_what_has_a_gradient_or_another_type_is_refused():
+    from quantexperiments_amd.kernels import keep_drafted, qk_norm_rotary, rotary, tree_attention
+    x = torch.randn(2, 4, 64).half().cuda()
+    pos, f = torch.arange(2).cuda(), torch.ones(32, dtype=torch.float64).cuda()
+    c = torch.zeros(3, 16, 2, 64, dtype=torch.float16).cuda()
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32).cuda()
+    g = x.clone().requires_grad_()
+    for call in (lambda: rotary(g, pos, f), lambda: qk_norm_rotary(g, x, pos, f), lambda: qk_norm_rotary(x, x, pos, f, g[0, 0]), lambda: tree_attention(g, c, c, i32(2, 1), i32(2)),
+                 lambda: keep_drafted(c.clone().requires_grad_(), c, i32(2, 1), i32(2), i32(2, 2), i32(2))):
+        with pytest.raises(NotImplementedError):
+            call()
+    with torch.no_grad():
+        assert torch.equal(rotary(g, pos, f), rotary(x, pos, f))
+    for call in (lambda: rotary(x.double(), pos, f), lambda: rotary(x, pos.float(), f), lambda: rotary(x, pos, f.float()), lambda: rotary(x, pos[:1], f), lambda: rotary(x, pos, torch.ones(33).double().cuda()),
+                 lambda: rotary(x, pos.cpu(), f), lambda: rotary(x.transpose(1, 2), pos, f), lambda: qk_norm_rotary(x, x.bfloat16(), pos, f), lambda: qk_norm_rotary(x, x[:1], pos, f),
+                 lambda: qk_norm_rotary(x, x, pos, f, torch.ones(32).cuda()), lambda: qk_norm_rotary(x, x, pos, f, torch.ones(64).cuda(), torch.ones(64).half().cuda()),
+                 lambda: tree_attention(x.float(), c.float(), c.float(), i32(2, 1), i32(2)), lambda: tree_attention(x, c, c[:2], i32(2, 1), i32(2)), lambda: tree_attention(x, c, c, i32(2, 1), i32(1)),
+                 lambda: tree_attention(x[:, :3], c, c, i32(2, 1), i32(2)), lambda: tree_attention(x, c, c, i32(2, 1), i32(2).long()), lambda: tree_attention(x, c, c, i32(2, 1), i32(2), i32(2)),
+                 lambda: tree_attention(x, c, c, i32(2, 1), i32(2), most_new=2), lambda: tree_attention(x, c, c, i32(2, 1), i32(2), i32(3), most_new=-1),
+                 lambda: tree_attention(x, c, c, i32(2, 1), i32(2), scale=0.0), lambda: tree_attention(x, c, c, i32(2, 1), i32(2), out=x), lambda: tree_attention(x, c, c, i32(2, 1), i32(2), out=c[0, :2].repeat(1, 1, 1)[:, :1]),
+                 lambda: tree_attention(x, c, c, i32(2, 1), i32(2), mask=i32(2, 1)), lambda: tree_attention(x, c, c, i32(2, 1), i32(2), lse=torch.zeros(2, 3).cuda()),
+                 lambda: tree_attention(x, c, c, i32(2, 1).expand(2, 1)[:1].expand(2, 1), i32(2)), lambda: keep_drafted(c, c, i32(2, 1), i32(2), i32(2, 2), i32(2)),
+                 lambda: keep_drafted(c, c.clone(), i32(2, 1), i32(2), i32(1, 2), i32(2)), lambda: keep_drafted(c, c.clone(), i32(2, 1), i32(2), i32(2, 2).long(), i32(2))):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_sizes_beyond_32_bits_are_refused_not_wrapped():
+    from quantexperiments_amd.kernels import rotary, tree_attention
+    one = torch.ones(1, 1, 8).half().cuda()
+    f = torch.ones(4, dtype=torch.float64).cuda()
+    with pytest.raises(ValueError, match="32 bits"):
+        rotary(one.expand(1, 2 ** 32 + 1, 8), torch.zeros(1, dtype=torch.int64).cuda(), f, one.expand(1, 2 ** 32 + 1, 8))
+    c = torch.ones(1, 16, 1, 8).half().cuda()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32).cuda()
+    # bounds on new tokens far above what there is
+    for most in (2, 2 ** 32, 2 ** 40):
+        assert torch.equal(tree_attention(one, c, c, i32(0)[None], i32(3), i32(0, 1), most_new=most), one)
+    with pytest.raises(ValueError):
+        tree_attention(one, c, c, i32(0)[None], i32(3), most_new=2 ** 32 + 1)
