@@ -96,7 +96,7 @@ __device__ __forceinline__ void attn_copy16(uint32_t to, const char* at, uint32_
 __device__ __forceinline__ void attn_copy16(uint32_t to, const char* at) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(at) : "memory");
 }
-__device__ __forceinline__ void attn_reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }      // before copies to where was read
+__device__ __forceinline__ void attn_reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }      // before copies to where was read (or written)
 template <int N> __device__ __forceinline__ void attn_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 // value of every lane 16, 32 and 48 lanes away combined: the four groups of lanes that hold one row
@@ -118,6 +118,13 @@ template <int DP> struct AttnTile {
     static __device__ __forceinline__ constexpr int k_xor(int key) { return PIECES == 8 ? (key >> 1) & 7 : key & 15; }
     static __device__ __forceinline__ constexpr int v_xor(int key) { return PIECES == 8 ? 2 * ((key >> 1) & 3) : 2 * (key & 7); }
 };
+
+// Heads narrower than DP: what lies in LDS behind their pieces, which no copy writes, is zero, as the rows' elements there are (a piece of the key again would make
+// NaN of an infinity in it).  Such heads have kernels of their own (FULL: none of a key's pieces is missing): lanes told apart in each copy cost 500 slots 2 of
+// 11 us, a branch between two kinds of copies 1.  By `threads` of them, before the first copies; the caller waits.
+__device__ __forceinline__ void attn_clear(char* to, int bytes, int tid, int threads) {
+    for (int i = tid * 16; i < bytes; i += threads * 16) *reinterpret_cast<u32x4*>(to + i) = u32x4{0u, 0u, 0u, 0u};
+}
 
 // The pages of a wave's keys: 64 table entries at a time in a register, and the place of each of up to 32 keys
 struct AttnPages {
@@ -144,28 +151,25 @@ __device__ __forceinline__ void attn_lookup(const AttnArgs& a, const AttnSeq& s,
 
 // Copies the N keys (or values) looked up, from `first` on, of one head to `to`: `base` is the head's first byte of the pool.  at: the first one's
 // place in its step
-template <int DP, bool VALUES, int N>
+template <int DP, bool FULL, bool VALUES, int N>
 __device__ __forceinline__ void attn_copy(const AttnArgs& a, const AttnSeq& s, int first, int place, int lane, const AttnPages& p, const char* base, const char* to) {
     typedef AttnTile<DP> T;
     static_assert(N % T::ROWS == 0, "whole copies");
     const int64_t page_b = VALUES ? a.v_page : a.k_page, slot_b = VALUES ? a.v_slot : a.k_slot;
     const int row = lane / T::PIECES, pos = lane % T::PIECES, pieces = a.dim >> 3;
     const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr)to);
-    auto piece = [&](int j) {                                // heads narrower than DP: their first piece again
-        const int key = place + j * T::ROWS + row, c = pos ^ (VALUES ? T::v_xor(key) : T::k_xor(key));
-        return (c < pieces ? c : 0) * 16;
-    };
+    auto piece = [&](int j) { const int key = place + j * T::ROWS + row; return pos ^ (VALUES ? T::v_xor(key) : T::k_xor(key)); };
     if (a.near && a.page % T::ROWS == 0 && first + N <= s.total) {          // the keys of a copy lie in one page
 #pragma unroll
         for (int j = 0; j < N / T::ROWS; ++j) {
-            const int id = __builtin_amdgcn_readlane(p.id, j * T::ROWS), off = __builtin_amdgcn_readlane(p.off, j * T::ROWS);
-            attn_copy16(lds + j * 1024, base + id * page_b + off * slot_b, (uint32_t)(row * (int)slot_b + piece(j)));
+            const int id = __builtin_amdgcn_readlane(p.id, j * T::ROWS), off = __builtin_amdgcn_readlane(p.off, j * T::ROWS), c = piece(j);
+            if (FULL || c < pieces) attn_copy16(lds + j * 1024, base + id * page_b + off * slot_b, (uint32_t)(row * (int)slot_b + c * 16));
         }
     } else {
 #pragma unroll
         for (int j = 0; j < N / T::ROWS; ++j) {
-            const int id = __shfl(p.id, j * T::ROWS + row), off = __shfl(p.off, j * T::ROWS + row);
-            attn_copy16(lds + j * 1024, base + id * page_b + off * slot_b + piece(j));
+            const int id = __shfl(p.id, j * T::ROWS + row), off = __shfl(p.off, j * T::ROWS + row), c = piece(j);
+            if (FULL || c < pieces) attn_copy16(lds + j * 1024, base + id * page_b + off * slot_b + c * 16);
         }
     }
 }
@@ -194,7 +198,7 @@ struct AttnWalk {
 };
 
 // Copies N keys (values) of one group; where: the first one's place in its step
-template <int DP, bool VALUES, int N>
+template <int DP, bool FULL, bool VALUES, int N>
 __device__ __forceinline__ void attn_copy_group(const AttnArgs& a, int where, int lane, const char* from, const char* to) {
     typedef AttnTile<DP> T;
     static_assert(N % T::ROWS == 0, "whole copies");
@@ -203,7 +207,7 @@ __device__ __forceinline__ void attn_copy_group(const AttnArgs& a, int where, in
 #pragma unroll
     for (int j = 0; j < N / T::ROWS; ++j) {
         const int key = where + j * T::ROWS + row, c = pos ^ (VALUES ? T::v_xor(key) : T::k_xor(key));
-        attn_copy16(lds + j * 1024, from, (uint32_t)((j * T::ROWS + row) * slot_b + (c < pieces ? c : 0) * 16));
+        if (FULL || c < pieces) attn_copy16(lds + j * 1024, from, (uint32_t)((j * T::ROWS + row) * slot_b + c * 16));
     }
 }
 
@@ -486,7 +490,7 @@ template <int DP, int MT, int NW> constexpr int attn_lds() {
 
 // Few rows (MT * 16 at a time): the waves of a workgroup share the rows and split its keys, each with two steps of keys and values of its
 // own in LDS, no barrier until the end, where their sums are joined.  Sequences are cut into `splits` workgroups too.
-template <int DT, int DP, int MT, int NW>
+template <int DT, int DP, int MT, int NW, bool FULL>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(1, 1))) void attn_kernel(AttnArgs a) {
     typedef AttnTile<DP> T;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -523,21 +527,25 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 at[x] = walk.find(a, b, lane, pages);
-                attn_copy_group<DP, false, 16>(a, 16 * x, lane, kb + at[x].k, slot_k(i) + x * 16 * T::PITCH);
+                attn_copy_group<DP, FULL, false, 16>(a, 16 * x, lane, kb + at[x].k, slot_k(i) + x * 16 * T::PITCH);
                 walk.go(a, 16 / a.page, 16 % a.page);
             }
             return;
         }
         attn_lookup<ATTN_STEP>(a, s, b, i * ATTN_STEP, lane, pages);
-        attn_copy<DP, false, ATTN_STEP>(a, s, i * ATTN_STEP, 0, lane, pages, kb, slot_k(i));
+        attn_copy<DP, FULL, false, ATTN_STEP>(a, s, i * ATTN_STEP, 0, lane, pages, kb, slot_k(i));
     };
     auto get_v = [&](int i) __attribute__((always_inline)) {
         if (easy && (i + 1) * ATTN_STEP <= s.total) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x) attn_copy_group<DP, true, 16>(a, 16 * x, lane, vb + at[x].v, slot_v(i) + x * 16 * T::PITCH);
+            for (int x = 0; x < 2; ++x) attn_copy_group<DP, FULL, true, 16>(a, 16 * x, lane, vb + at[x].v, slot_v(i) + x * 16 * T::PITCH);
             return;
         }
-        attn_copy<DP, true, ATTN_STEP>(a, s, i * ATTN_STEP, 0, lane, pages, vb, slot_v(i)); };
+        attn_copy<DP, FULL, true, ATTN_STEP>(a, s, i * ATTN_STEP, 0, lane, pages, vb, slot_v(i)); };
+    if constexpr (!FULL) {
+        attn_clear(ring, 4 * T::BYTES, lane, 64);
+        attn_reads_done();
+    }
     if (w0 < w1) { get_k(w0); get_v(w0); }
     if (w0 + 1 < w1) { get_k(w0 + 1); get_v(w0 + 1); }
     attn_rows_ready(r);
@@ -625,7 +633,7 @@ __device__ __forceinline__ float attn_most(float4v x, float4v y) {
 // registers and moves them around the branch that scales them, 1300 cycles a slot instead of 500.
 // The stages at a sequence's end that some row does not see whole go step by step, behind the pipeline, and all of them for heads wider than 128
 // elements, whose keys and values would take the registers of four tiles.
-template <int DT, int DP, int NW>
+template <int DT, int DP, int NW, bool FULL>
 __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     typedef AttnTile<DP> T;
     typedef AttnType<DT> E;
@@ -666,14 +674,14 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
         const int first = i * KEYS + wave * MINE, in_step = wave * MINE % ATTN_STEP;
         if (easy && first + MINE <= s.total) {
             const AttnPlace from = walk.find(a, b, lane, pages);
-            attn_copy_group<DP, false, MINE>(a, in_step, lane, kb + from.k, at);
-            attn_copy_group<DP, true, MINE>(a, in_step, lane, vb + from.v, at + SK * T::BYTES);
+            attn_copy_group<DP, FULL, false, MINE>(a, in_step, lane, kb + from.k, at);
+            attn_copy_group<DP, FULL, true, MINE>(a, in_step, lane, vb + from.v, at + SK * T::BYTES);
             walk.go(a, KEYS / a.page, KEYS % a.page);
             return;
         }
         attn_lookup<MINE>(a, s, b, first, lane, pages);
-        attn_copy<DP, false, MINE>(a, s, first, in_step, lane, pages, kb, at);
-        attn_copy<DP, true, MINE>(a, s, first, in_step, lane, pages, vb, at + SK * T::BYTES);
+        attn_copy<DP, FULL, false, MINE>(a, s, first, in_step, lane, pages, kb, at);
+        attn_copy<DP, FULL, true, MINE>(a, s, first, in_step, lane, pages, vb, at + SK * T::BYTES);
     };
     auto arrive = [&](int i) __attribute__((always_inline)) {        // stage i is there
         if (i + NB - 2 <= end) attn_wait<2 * C * (NB - 3)>(); else attn_wait<0>();
@@ -682,6 +690,10 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
         asm volatile("" ::: "memory");
         if (i + NB - 2 < end) get(i + NB - 2);
     };
+    if constexpr (!FULL) {
+        attn_clear(smem, NB * STAGE, tid, NW * 64);
+        __syncthreads();
+    }
 #pragma unroll
     for (int i = 0; i < NB - 2; ++i)
         if (begin + i < end) get(begin + i);
@@ -944,29 +956,29 @@ inline void attn_raise(const void* kernel, int lds, bool (&raised)[64]) {
     if (!raised[dev]) (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     raised[dev] = true;
 }
-template <int DT, int DP, int MT>
+template <int DT, int DP, int MT, bool FULL>
 int attn_launch_few(const AttnArgs& a, unsigned grid, hipStream_t s) {
     constexpr int NW = attn_waves(DP), LDS = attn_lds<DP, MT, NW>();
     static bool raised[64];
-    attn_raise((const void*)attn_kernel<DT, DP, MT, NW>, LDS, raised);
-    hipLaunchKernelGGL((attn_kernel<DT, DP, MT, NW>), dim3(grid), dim3(NW * 64), LDS, s, a);
+    attn_raise((const void*)attn_kernel<DT, DP, MT, NW, FULL>, LDS, raised);
+    hipLaunchKernelGGL((attn_kernel<DT, DP, MT, NW, FULL>), dim3(grid), dim3(NW * 64), LDS, s, a);
     return check_launch("sq_tree_attention");
 }
-template <int DT, int DP, int NW>
+template <int DT, int DP, int NW, bool FULL>
 int attn_launch_many(const AttnArgs& a, unsigned grid, hipStream_t s) {
     constexpr int LDS = attn_tile_lds<DP, NW>();
     static bool raised[64];
-    attn_raise((const void*)attn_tile_kernel<DT, DP, NW>, LDS, raised);
-    hipLaunchKernelGGL((attn_tile_kernel<DT, DP, NW>), dim3(grid), dim3(NW * 64), LDS, s, a);
+    attn_raise((const void*)attn_tile_kernel<DT, DP, NW, FULL>, LDS, raised);
+    hipLaunchKernelGGL((attn_tile_kernel<DT, DP, NW, FULL>), dim3(grid), dim3(NW * 64), LDS, s, a);
     return check_launch("sq_tree_attention");
 }
 
-template <int DT, int DP>
+template <int DT, int DP, bool FULL>
 int attn_launch_dim(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
     const unsigned grid = (unsigned)((int64_t)a.seqs * a.kv_heads * p.row_blocks * p.splits);
     int rc;
-    if (p.nw) rc = p.nw == 4 ? attn_launch_many<DT, DP, 4>(a, grid, s) : attn_launch_many<DT, DP, 8>(a, grid, s);
-    else rc = p.mt == 1 ? attn_launch_few<DT, DP, 1>(a, grid, s) : attn_launch_few<DT, DP, DP == 256 ? 1 : 2>(a, grid, s);
+    if (p.nw) rc = p.nw == 4 ? attn_launch_many<DT, DP, 4, FULL>(a, grid, s) : attn_launch_many<DT, DP, 8, FULL>(a, grid, s);
+    else rc = p.mt == 1 ? attn_launch_few<DT, DP, 1, FULL>(a, grid, s) : attn_launch_few<DT, DP, DP == 256 ? 1 : 2, FULL>(a, grid, s);
     if (rc || p.splits == 1) return rc;
     const int64_t all = (int64_t)a.seqs * a.most_new * a.q_heads;
     constexpr int MOST = 1024 / DP;                          // parts of a row that fill a workgroup
@@ -977,9 +989,11 @@ int attn_launch_dim(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
 
 template <int DT>
 int attn_launch(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
-    if (p.dp == 64) return attn_launch_dim<DT, 64>(a, p, s);
-    if (p.dp == 128) return attn_launch_dim<DT, 128>(a, p, s);
-    return attn_launch_dim<DT, 256>(a, p, s);
+    auto go = [&](auto dp) {
+        constexpr int DP = decltype(dp)::value;
+        return a.dim == DP ? attn_launch_dim<DT, DP, true>(a, p, s) : attn_launch_dim<DT, DP, false>(a, p, s);
+    };
+    return p.dp == 64 ? go(std::integral_constant<int, 64>()) : p.dp == 128 ? go(std::integral_constant<int, 128>()) : go(std::integral_constant<int, 256>());
 }
 bool rows_apart(int tokens, int heads, int64_t t, int64_t h, int dim);      // sq_heads.hip
 int attn_launch_f16(const AttnArgs& a, const AttnPlan& p, hipStream_t s);

@@ -433,3 +433,19 @@ def test_queries_that_barely_differ_and_rows_that_see_the_same_agree_in_every_pa
     out, lse = attend(s)
     assert torch.equal(out[:, 1:8], out[:, :1].expand(-1, 7, -1)) and torch.equal(lse[:, 9:], lse[:, 8:9].expand(-1, 7))
     s.check(out, lse)
+
+
+@pytest.mark.parametrize("d", [8, 40, 64, 72, 80, 128, 144, 256])
+@pytest.mark.parametrize("new,length", [(1, 70), (40, 33)])
+def test_a_key_with_an_infinite_score_of_minus_infinity_weighs_nothing(d, new, length):
+    # (a key's -inf against an element of q that is above zero, all others finite: the score is -inf and the weight zero, in heads of any width)
+    s = Setup([length], [new], 2, 1, d, 16, seed=d)
+    s.q = s.q.abs() + 0.0625
+    for j in (0, 5, 31, 32, length - 1):
+        s.k[0][j, 0, 0 if j % 2 else d - 1] = -math.inf
+    s.put()
+    got, lse = attend(s)
+    keep = torch.tensor([j for j in range(length + new) if j not in (0, 5, 31, 32, length - 1)])
+    s.k[0], s.v[0] = s.k[0][keep], s.v[0][keep]
+    s.lens, s.sees = [len(keep) - new], s.sees
+    s.check(got, lse)
