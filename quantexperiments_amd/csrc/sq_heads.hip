@@ -224,7 +224,8 @@ template <int DT> __device__ __forceinline__ void store_one(void* p, int64_t i, 
     reinterpret_cast<typename store_as<DT>::type*>(p)[i] = store_as<DT>::cvt(v);
 }
 
-// Any width, part, stride and alignment: a wave per head, a lane per pair.  (Where 16-byte pieces fit, heads_kernel is 1.5 to 4 times as fast.)
+// Any width, part, stride and alignment: a wave per head, a lane per pair.  (Where 16-byte pieces fit, heads_kernel takes as long for up to 64 tokens of 32 heads
+// of 128 and is two to five times as fast for more: 2048 tokens 11.1 against 40.5 us with norms, 7.7 against 32.1 without.)
 template <int DT>
 __global__ __launch_bounds__(256) void heads_any_kernel(HeadsArgs a) {
     const int lane = threadIdx.x & 63;
