@@ -33,7 +33,8 @@ struct AttnArgs {
     float2v* pml;
     int64_t q_t, q_h, o_t, o_h, k_page, k_slot, k_head, v_page, v_slot, v_head;      // bytes
     int64_t ld_table, ld_mask;
-    int tokens, seqs, most_new, q_heads, kv_heads, group, dim, pages, page, max_pages, mask_words, row_blocks, splits;
+    int tokens, seqs, most_new, q_heads, kv_heads, group, dim, pages, page, max_pages, mask_words, row_blocks, splits, last_splits, last_row;
+    // (splits: of the row blocks before the last one, whose first row is last_row and which has last_splits)
     int near;                    // the slots of a page lie within 2^31 bytes, in order
     float scale2;                // scale * log2(e): weights are powers of two
 };
@@ -648,13 +649,16 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     int id = blockIdx.x;
     const int groups = a.seqs * a.kv_heads, b = id % groups / a.kv_heads, head = id % groups % a.kv_heads;
     id /= groups;
-    const int split = id % a.splits, row0 = (a.row_blocks - 1 - id / a.splits) * ROWS;
+    const bool end_block = id < a.last_splits;
+    const int splits = end_block ? a.last_splits : a.splits;
+    if (!end_block) id -= a.last_splits;
+    const int split = id % splits, row0 = (a.row_blocks - (end_block ? 1 : 2) - id / splits) * ROWS;
     const AttnSeq s = attn_seq(a, b);
     const int rows = s.n * a.group;
     if (row0 >= rows) return;
     const int last = min(row0 + ROWS, rows) - 1;
     const int seen = a.mask ? s.total : min(s.total, s.len + last / a.group + 1);
-    const int stages = (seen + KEYS - 1) / KEYS, per = (stages + a.splits - 1) / a.splits, begin = min(split * per, stages), end = min(begin + per, stages);
+    const int stages = (seen + KEYS - 1) / KEYS, per = (stages + splits - 1) / splits, begin = min(split * per, stages), end = min(begin + per, stages);
 
     AttnRows<DP, MT> r;
     const int mine = row0 + wave * MT * 16;
@@ -862,7 +866,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
         if (bad) l = NAN;
         if (row >= rows) continue;
         const int64_t tok_all = s.first + tok;
-        if (a.splits > 1) {
+        if (splits > 1) {
             const int64_t to_row = (tok_all * a.q_heads + hq) * a.splits + split;
 #pragma unroll
             for (int d = 0; d < VD; ++d) *reinterpret_cast<float4v*>(a.po + to_row * DP + d * 16 + e) = r.o[t][d];
@@ -893,40 +897,70 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     const int tid = threadIdx.x, q = tid % Q, g = tid / Q % G, rr = tid / (Q * G);
     const uint32_t per = (uint32_t)a.most_new * a.q_heads, i = blockIdx.x * R + rr, b = i / per, r = i - b * per, tok = r / a.q_heads, hq = r - tok * a.q_heads;
     const AttnSeq s = attn_seq(a, min((int)b, a.seqs - 1));
-    const bool live = (int)b < a.seqs && (int)tok < s.n;
+    const int splits = (int)tok * a.group + (int)hq % a.group < a.last_row ? a.splits : a.last_splits;
+    const bool live = (int)b < a.seqs && (int)tok < s.n && splits > 1;       // (a row of one part is written already)
     const int64_t row = (int64_t)(s.first + tok) * a.q_heads + hq, at = row * a.splits;
     float m = ATTN_NOTHING, l = 0.f;
     float4v v = float4v{0.f, 0.f, 0.f, 0.f};
     const float4v* po = reinterpret_cast<const float4v*>(a.po + at * DP) + q;
     if constexpr (G == 1) {
-        if (live) {
-            for (int x = 0; x < a.splits; ++x) m = fmaxf(m, a.pml[at + x][0]);
-            for (int x = 0; x < a.splits; ++x) {
-                const float2v one = a.pml[at + x];
-                const float by = __builtin_amdgcn_exp2f(one[0] - m);
-                l += one[1] * by;
-                if (by != 0.f) v += po[(size_t)x * Q] * by;
+        // (all of a row's parts in flight at once: one by one eight parts of 2240 rows took 10 us)
+        auto join = [&](auto most) __attribute__((always_inline)) {
+            constexpr int N = decltype(most)::value;
+            float2v ml[N];
+            float4v y[N];
+#pragma unroll
+            for (int x = 0; x < N; ++x) ml[x] = a.pml[at + min(x, splits - 1)];
+#pragma unroll
+            for (int x = 0; x < N; ++x) y[x] = po[(size_t)min(x, splits - 1) * Q];
+#pragma unroll
+            for (int x = 0; x < N; ++x) m = fmaxf(m, ml[x][0]);
+#pragma unroll
+            for (int x = 0; x < N; ++x) {
+                const float by = x < splits ? __builtin_amdgcn_exp2f(ml[x][0] - m) : 0.f;
+                if (x < splits) l += ml[x][1] * by;
+                v += by != 0.f ? y[x] * by : float4v{0.f, 0.f, 0.f, 0.f};
             }
+        };
+        if (live) {
+            if (a.splits <= 2) join(std::integral_constant<int, 2>());
+            else if (a.splits <= 4) join(std::integral_constant<int, 4>());
+            else join(std::integral_constant<int, 8>());
         }
     } else {
-        // (one row: its maxima and totals fetched at once, a split per thread)
-        __shared__ float2v ml[ATTN_SPLITS_MAX];
-        if (live && tid < a.splits) ml[tid] = a.pml[at + tid];
-        __syncthreads();
+        // (one row: its maxima and totals fetched at once, a part per lane, by every wave; the first parts' sums beside them)
+        __shared__ float weight[ATTN_SPLITS_MAX];
+        const int lane = tid & 63;
         if (live) {
-            for (int x = 0; x < a.splits; ++x) m = fmaxf(m, ml[x][0]);
-            for (int x = 0; x < a.splits; ++x) l += ml[x][1] * __builtin_amdgcn_exp2f(ml[x][0] - m);
-            for (int x = g; x < a.splits; x += 4 * G) {
-                float4v y[4];
-                float by[4];
+            float4v y[4];
+            auto fetch = [&](int x) __attribute__((always_inline)) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) y[k] = po[(size_t)min(x + k * G, splits - 1) * Q];
+            };
+            float2v one[ATTN_SPLITS_MAX / 64];
+#pragma unroll
+            for (int k = 0; k < ATTN_SPLITS_MAX / 64; ++k) one[k] = a.pml[at + min(lane + 64 * k, splits - 1)];
+            fetch(g);
+#pragma unroll
+            for (int k = 0; k < ATTN_SPLITS_MAX / 64; ++k) m = fmaxf(m, one[k][0]);
+#pragma unroll
+            for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+#pragma unroll
+            for (int k = 0; k < ATTN_SPLITS_MAX / 64; ++k) {
+                const float by = lane + 64 * k < splits ? __builtin_amdgcn_exp2f(one[k][0] - m) : 0.f;
+                if (lane + 64 * k < splits) l += one[k][1] * by;
+                if (tid < 64) weight[lane + 64 * k] = by;
+            }
+#pragma unroll
+            for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
+            __syncthreads();
+            for (int x = g; x < splits; x += 4 * G) {
+                if (x != g) fetch(x);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int z = x + k * G;
-                    by[k] = z < a.splits ? __builtin_amdgcn_exp2f(ml[min(z, a.splits - 1)][0] - m) : 0.f;
-                    y[k] = po[(size_t)min(z, a.splits - 1) * Q];
+                    const float by = x + k * G < splits ? weight[min(x + k * G, splits - 1)] : 0.f;
+                    v += by != 0.f ? y[k] * by : float4v{0.f, 0.f, 0.f, 0.f};
                 }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v += by[k] != 0.f ? y[k] * by[k] : float4v{0.f, 0.f, 0.f, 0.f};
             }
         }
     }
@@ -949,7 +983,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 
 // ------------------------------------------------------------------------------------------ host
 
-struct AttnPlan { int dp, mt, nw, row_blocks, splits; };       // nw: waves of the many-row kernel; 0: the few-row one, mt tiles of rows
+struct AttnPlan { int dp, mt, nw, row_blocks, splits, last_splits, last_row; };       // nw: waves of the many-row kernel; 0: the few-row one, mt tiles of rows
 constexpr int attn_waves(int dp) { return dp == 256 ? 2 : 4; }
 
 inline void attn_raise(const void* kernel, int lds, bool (&raised)[64]) {
@@ -977,7 +1011,7 @@ int attn_launch_many(const AttnArgs& a, unsigned grid, hipStream_t s) {
 
 template <int DT, int DP, bool FULL>
 int attn_launch_dim(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
-    const unsigned grid = (unsigned)((int64_t)a.seqs * a.kv_heads * p.row_blocks * p.splits);
+    const unsigned grid = (unsigned)((int64_t)a.seqs * a.kv_heads * ((p.row_blocks - 1) * p.splits + p.last_splits));
     int rc;
     if (p.nw) rc = p.nw == 4 ? attn_launch_many<DT, DP, 4, FULL>(a, grid, s) : attn_launch_many<DT, DP, 8, FULL>(a, grid, s);
     else rc = p.mt == 1 ? attn_launch_few<DT, DP, 1, FULL>(a, grid, s) : attn_launch_few<DT, DP, DP == 256 ? 1 : 2, FULL>(a, grid, s);

@@ -33,6 +33,18 @@ static AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
     p.splits = (int)(want < most ? want : most);
     if (p.splits < 1) p.splits = 1;
     if (p.splits > ATTN_SPLITS_MAX) p.splits = ATTN_SPLITS_MAX;
+    p.last_splits = p.splits;
+    p.last_row = (int)((p.row_blocks - 1) * per);
+    const int64_t waves_last = (rows - p.last_row + p.mt * 16 - 1) / (p.mt * 16);
+    if (p.nw == 8 && p.row_blocks > 1 && waves_last <= 4) {
+        const int64_t room = cus / ((int64_t)a.seqs * c.heads);
+        for (int s = (int)(room < most ? room : most); s > 1; --s) {
+            const int last = (s * 60 + 99) / 100;
+            if ((p.row_blocks - 1) * (int64_t)s + last > room) continue;
+            if (s <= ATTN_SPLITS_MAX) p.splits = s, p.last_splits = last;
+            break;
+        }
+    }
     return p;
 }
 
@@ -96,7 +108,7 @@ int sq_tree_attention(const sq_attention* a, const sq_cache* cache, void* worksp
     k.ld_table = a->ld_table; k.ld_mask = a->ld_mask;
     k.tokens = a->tokens; k.seqs = a->seqs; k.most_new = a->most_new; k.q_heads = a->q_heads; k.kv_heads = cache->heads; k.group = a->q_heads / cache->heads;
     k.dim = cache->dim; k.pages = cache->pages; k.page = cache->page; k.max_pages = a->max_pages; k.mask_words = a->mask_words;
-    k.row_blocks = p.row_blocks; k.splits = p.splits;
+    k.row_blocks = p.row_blocks; k.splits = p.splits; k.last_splits = p.last_splits; k.last_row = p.last_row;
     auto near = [&](int64_t b) { return b >= 0 && b < (1 << 24) && b * (cache->page + 32) < INT32_MAX; };
     k.near = near(k.k_slot) && near(k.v_slot);
     k.scale2 = a->scale * 1.4426950408889634f;
