@@ -898,7 +898,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     const uint32_t per = (uint32_t)a.most_new * a.q_heads, i = blockIdx.x * R + rr, b = i / per, r = i - b * per, tok = r / a.q_heads, hq = r - tok * a.q_heads;
     const AttnSeq s = attn_seq(a, min((int)b, a.seqs - 1));
     const int splits = (int)tok * a.group + (int)hq % a.group < a.last_row ? a.splits : a.last_splits;
-    const bool live = (int)b < a.seqs && (int)tok < s.n && splits > 1;       // (a row of one part is written already)
+    const bool live = (int)b < a.seqs && (int)tok < s.n;
     const int64_t row = (int64_t)(s.first + tok) * a.q_heads + hq, at = row * a.splits;
     float m = ATTN_NOTHING, l = 0.f;
     float4v v = float4v{0.f, 0.f, 0.f, 0.f};

@@ -4,10 +4,13 @@
 namespace sq {
 
 // Up to 32 rows (16 of wide heads): one workgroup for all of them, its waves splitting the keys; more: four or eight waves with 32 rows each (16).
-// Sequences are cut until the chip has a workgroup per compute unit, but not into less than two steps per wave, nor into two such parts (the joining
-// launch takes 3 us, as a step of 1 us does per wave: 500 slots whole 12.1, in two 12.9 us; 4000 in 15 parts 14.5, in 7 17.0 us).  Sequences of several lengths
-// are cut for two rounds of workgroups where a wave then still has 16 steps: 32 of 2,240 to 8,192 slots x 8 key heads 136 us, 163 in one round; but
-// 8 of 4000 x 4 heads 27 us in 480 parts, 23 in 224, and 64 of 500 27 us in 512, 18 in 256.
+// Sequences are cut until the chip has a workgroup per compute unit, few rows not into less than a step per wave nor into two such parts, many rows not into
+// less than four steps, or two in up to eight parts.  (The joining launch takes 2 to 3 us, a step of a wave 1: one token behind 300 slots whole 8.0, in two parts 8.9 us;
+// behind 500 whole 10.5, in four 9.1; behind 4000 in 15 parts of two steps a wave 12.3, in 31 of one 10.0.  40 tokens behind 1000 in 8 parts 22.5, in 16 28.9; behind
+// 256 in two parts 18.7, in four 18.2.)  Sequences of several lengths are cut for two rounds of workgroups where a wave then still has 16 steps: 32 of 2,240 to
+// 8,192 slots x 8 key heads 136 us, 163 in one round; but 8 of 4000 x 4 heads 27 us in 480 parts, 23 in 224, and 64 of 500 27 us in 512, 18 in 256.
+// A last block of rows that fills at most half of its waves takes 0.6 of the time, and gets as many fewer parts: 8 trees of 32 rows x 10 with heads of 256
+// 42.3 us evenly, 39.3 so; with 0.75 42.1.
 static AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
     AttnPlan p;
     p.dp = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
@@ -18,13 +21,13 @@ static AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
         p.nw = 0;
         p.mt = rows <= 16 ? 1 : 2;
         per = p.mt * 16;
-        most = steps / (2 * waves);
+        most = steps / waves;
         if (most <= 2) most = 1;
     } else {
         p.mt = attn_tiles(p.dp);
         p.nw = rows <= 4 * 16 * p.mt ? 4 : 8;
         per = p.mt * 16 * p.nw;
-        most = steps / 4;
+        most = steps / 4 > 8 ? steps / 4 : steps / 2 < 8 ? steps / 2 : 8;
     }
     p.row_blocks = (int)((rows + per - 1) / per);
     const int64_t base = (int64_t)a.seqs * c.heads * p.row_blocks, cus = device_cus();
@@ -39,7 +42,7 @@ static AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
     if (p.nw == 8 && p.row_blocks > 1 && waves_last <= 4) {
         const int64_t room = cus / ((int64_t)a.seqs * c.heads);
         for (int s = (int)(room < most ? room : most); s > 1; --s) {
-            const int last = (s * 60 + 99) / 100;
+            const int last = (s * 60 + 99) / 100;            // (two or more)
             if ((p.row_blocks - 1) * (int64_t)s + last > room) continue;
             if (s <= ATTN_SPLITS_MAX) p.splits = s, p.last_splits = last;
             break;
