@@ -339,3 +339,9 @@ def test_sizes_beyond_32_bits_are_refused_not_wrapped():
         assert torch.equal(tree_attention(one, c, c, i32(0)[None], i32(3), i32(0, 1), most_new=most), one)
     with pytest.raises(ValueError):
         tree_attention(one, c, c, i32(0)[None], i32(3), most_new=2 ** 32 + 1)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("n,hq,hk,d,rot,interleaved", [(1100, 19, 2, 128, 128, False), (2500, 5, 3, 256, 64, True), (1030, 33, 1, 16, 16, False), (1200, 3, 1, 512, 512, True)])
+def test_many_tokens_whose_heads_take_several_rounds(n, hq, hk, d, rot, interleaved, dtype):
+    test_norm_rotation_and_cache_slots(n, hq, hk, d, rot, 16, interleaved, 0.0, True, dtype)
