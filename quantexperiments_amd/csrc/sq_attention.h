@@ -635,7 +635,7 @@ __device__ __forceinline__ float attn_most(float4v x, float4v y) {
 // registers and moves them around the branch that scales them, 1300 cycles a slot instead of 500.  Bound by what a SIMD's two waves issue: matrix and other vector
 // instructions hardly overlap (1900 tokens of 28 heads of 128 behind 2100, 4 key heads: 121 us, 686 TFLOP/s, matrix cores busy 44 % of the time).
 // The stages at a sequence's end that some row does not see whole go step by step, behind the pipeline, and all of them (those that every row sees without masks) for
-// heads wider than 128 elements, whose keys and values would take the registers of four tiles (1000 tokens of 20 heads of 256 behind 2100: 140 us).
+// heads wider than 128 elements, whose keys and values would take the registers of four tiles (1000 tokens of 20 heads of 256 behind 2100: 136 us).
 template <int DT, int DP, int NW, bool FULL>
 __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     typedef AttnTile<DP> T;

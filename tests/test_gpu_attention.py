@@ -449,3 +449,59 @@ def test_a_key_with_an_infinite_score_of_minus_infinity_weighs_nothing(d, new, l
     s.k[0], s.v[0] = s.k[0][keep], s.v[0][keep]
     s.lens, s.sees = [len(keep) - new], s.sees
     s.check(got, lse)
+
+
+def test_threads_with_streams_of_their_own_get_what_one_gets():
+    import threading
+    from quantexperiments_amd.kernels import tree_attention
+    setups = [Setup([700, 30], [1, 3], 7, 1, 128, 16, seed=3), Setup([900], [40], 6, 2, 64, 16, tree=True, seed=4), Setup([400], [2], 4, 2, 256, 16, seed=5)]
+    args = [s.device() for s in setups]
+    alone = [tree_attention(**a) for a in args]
+    torch.cuda.synchronize()
+    got = [[] for _ in args]
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got[i].append(tree_attention(**args[i]))
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(args))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for outs, one in zip(got, alone):
+        assert len(outs) == 20 and all(torch.equal(o, one) for o in outs)
+
+
+FIRST = """
+import torch
+from quantexperiments_amd.kernels import qk_norm_rotary, tree_attention
+g = torch.Generator().manual_seed(0)
+q = torch.randn(40, 4, 128, generator=g).half().cuda()
+kc, vc = (torch.randn(64, 16, 2, 128, generator=g).half().cuda() for _ in range(2))
+i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+table, lens = torch.arange(64, dtype=torch.int32)[None].cuda(), i32([900])
+pos, f = torch.arange(40).cuda(), torch.rand(64, dtype=torch.float64, generator=g).cuda()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    turned, _ = qk_norm_rotary(q, q[:, :2], pos, f)
+    out = tree_attention(turned, kc, vc, table, lens)
+for n in (900, 17):
+    lens.fill_(n)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, tree_attention(qk_norm_rotary(q, q[:, :2], pos, f)[0], kc, vc, table, lens))
+print("captured first")
+"""
+
+
+def test_a_process_whose_first_calls_are_captured():
+    import pathlib
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", FIRST], cwd=pathlib.Path(__file__).parents[1], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]
