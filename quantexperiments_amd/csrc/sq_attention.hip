@@ -7,8 +7,9 @@ namespace sq {
 // Sequences are cut until the chip has a workgroup per compute unit, few rows not into less than a step per wave nor into two such parts, many rows not into
 // less than four steps, or two in up to eight parts.  (The joining launch takes 2 to 3 us, a step of a wave 1: one token behind 300 slots whole 8.0, in two parts 8.9 us;
 // behind 500 whole 10.5, in four 9.1; behind 4000 in 15 parts of two steps a wave 12.3, in 31 of one 10.0.  40 tokens behind 1000 in 8 parts 22.5, in 16 28.9; behind
-// 256 in two parts 18.7, in four 18.2.)  Sequences of several lengths are cut for two rounds of workgroups where a wave then still has 16 steps: 32 of 2,240 to
-// 8,192 slots x 8 key heads 136 us, 163 in one round; but 8 of 4000 x 4 heads 27 us in 480 parts, 23 in 224, and 64 of 500 27 us in 512, 18 in 256.
+// 256 in two parts 18.7, in four 18.2.)  Sequences of several lengths are cut for two rounds of workgroups where a wave then still has eight steps: 32 of 2,240 to 8,192 slots x 8 key
+// heads 131 us, 154 in one round, 64 of up to 4000 x 4 heads 69 and 77; with fewer steps it costs more than it evens out: 64 of up to 500 14.1 us in one round, 19.5 in
+// two, 16 of 2000 x 8 heads 26.6 and 30.4.
 // A last block of rows that fills at most half of its waves takes 0.6 of the time, and gets as many fewer parts: 8 trees of 32 rows x 10 with heads of 256
 // 42.3 us evenly, 39.3 so; with 0.75 42.1.
 static AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
@@ -32,7 +33,7 @@ static AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
     p.row_blocks = (int)((rows + per - 1) / per);
     const int64_t base = (int64_t)a.seqs * c.heads * p.row_blocks, cus = device_cus();
     int64_t want = cus / base;
-    if (a.seqs > 1 && !p.nw && 2 * cus / base > 1 && steps / (2 * cus / base) >= 16 * waves) want = 2 * cus / base;
+    if (a.seqs > 1 && !p.nw && 2 * cus / base > 1 && steps / (2 * cus / base) >= 8 * waves) want = 2 * cus / base;
     p.splits = (int)(want < most ? want : most);
     if (p.splits < 1) p.splits = 1;
     if (p.splits > ATTN_SPLITS_MAX) p.splits = ATTN_SPLITS_MAX;
