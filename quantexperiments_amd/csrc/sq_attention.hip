@@ -10,8 +10,8 @@ namespace sq {
 // 256 in two parts 18.7, in four 18.2.)  Sequences of several lengths are cut for two rounds of workgroups where a wave then still has eight steps: 32 of 2,240 to 8,192 slots x 8 key
 // heads 131 us, 154 in one round, 64 of up to 4000 x 4 heads 69 and 77; with fewer steps it costs more than it evens out: 64 of up to 500 14.1 us in one round, 19.5 in
 // two, 16 of 2000 x 8 heads 26.6 and 30.4.
-// A last block of rows that fills at most half of its waves takes 0.6 of the time, and gets as many fewer parts: 8 trees of 32 rows x 10 with heads of 256
-// 42.3 us evenly, 39.3 so; with 0.75 42.1.
+// A last block of rows that fills at most half of its waves takes 0.6 of the time, and gets as many fewer parts: 8 trees of 32 tokens of 5 heads of 256 per
+// key head (160 rows in blocks of 128) 42.3 us evenly, 39.3 so; with 0.75 42.1.
 static AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
     AttnPlan p;
     p.dp = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
