@@ -86,6 +86,19 @@ template <> struct AttnType<SQ_BF16> {
     static __device__ __forceinline__ uint16_t one(float v) { return f2bf(v); }
 };
 
+// The product that exponents of large scores are made from (attn_weights), in fp16 rounded by itself whatever is done with it
+template <int DT> __device__ __forceinline__ float attn_rounded(float s, float scale2) {
+    float x = s * scale2;
+    if constexpr (DT == SQ_F16) asm("" : "+v"(x));
+    return x;
+}
+// Whether the score `top` is more than ATTN_SLACK above m, which is taken off the exponents.  In fp16 by the rounded product: from 2^24 on it can lie further
+// above m than the exact one does, and a weight of 2^16 would be an infinity.
+template <int DT> __device__ __forceinline__ bool attn_above(float top, float scale2, float m) {
+    if constexpr (DT == SQ_F16) return attn_rounded<DT>(top, scale2) - m > ATTN_SLACK;
+    return __builtin_fmaf(top, scale2, -ATTN_SLACK) > m;
+}
+
 typedef __attribute__((address_space(3))) char* lds_ptr;
 
 // Copies 16 bytes per lane to LDS, lane l's to `to` + 16 l, and waits for all but the newest N memory operations.  Written out, because the
@@ -315,7 +328,7 @@ __device__ __forceinline__ void attn_weights(const AttnArgs& a, AttnRows<DP, MT>
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         mx[t] = fmaxf(fmaxf(fmaxf(st[t][0][0], st[t][0][1]), fmaxf(st[t][0][2], st[t][0][3])), fmaxf(fmaxf(st[t][1][0], st[t][1][1]), fmaxf(st[t][1][2], st[t][1][3])));
-        up |= __builtin_fmaf(mx[t], a.scale2, -ATTN_SLACK) > r.m[t];
+        up |= attn_above<DT>(mx[t], a.scale2, r.m[t]);
     }
     if (__any(up)) {
         bool far = false;
@@ -323,7 +336,7 @@ __device__ __forceinline__ void attn_weights(const AttnArgs& a, AttnRows<DP, MT>
         for (int t = 0; t < MT; ++t) {
             // (row by row, so that no row's bits depend on what the wave's other rows see)
             const float top = groups_fold(mx[t], [](float x, float y) { return fmaxf(x, y); });
-            const float m = __builtin_fmaf(top, a.scale2, -ATTN_SLACK) > r.m[t] ? top * a.scale2 : r.m[t], by = __builtin_amdgcn_exp2f(r.m[t] - m);
+            const float m = attn_above<DT>(top, a.scale2, r.m[t]) ? attn_rounded<DT>(top, a.scale2) : r.m[t], by = __builtin_amdgcn_exp2f(r.m[t] - m);
             r.m[t] = m;
             r.l[t] *= by;
             far |= !(fabsf(m) <= 0x1p20f);
@@ -750,9 +763,12 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
         auto raise = [&](int t, float mx) __attribute__((always_inline)) {      // of the tile before: its maximum against what is taken off
             by1 = a.scale2;
             less1 = r.m[t];
-            if ((__ballot(__builtin_fmaf(mx, a.scale2, -ATTN_SLACK) > r.m[t]) | far) != 0) {
-                const float top = groups_fold(mx, [](float x, float y) { return fmaxf(x, y); });
-                const float m = __builtin_fmaf(top, a.scale2, -ATTN_SLACK) > r.m[t] ? top * a.scale2 : r.m[t], f = __builtin_amdgcn_exp2f(r.m[t] - m);
+            // (one operation less than attn_above in fp16.  Rows beyond 2^20, where that is not enough, always come here; for others the second condition says nothing more)
+            auto above = [&](float x) __attribute__((always_inline)) { return __builtin_fmaf(x, a.scale2, -ATTN_SLACK) > r.m[t]; };
+            if ((__ballot(above(mx)) | far) != 0) {
+                const float top = groups_fold(mx, [](float x, float y) { return fmaxf(x, y); }), x = attn_rounded<DT>(top, a.scale2);
+                const bool up = above(top) || (DT == SQ_F16 && x - r.m[t] >= 16.f);
+                const float m = up ? x : r.m[t], f = __builtin_amdgcn_exp2f(r.m[t] - m);
                 r.m[t] = less1 = m;
                 r.l[t] *= f;
 #pragma unroll

@@ -505,3 +505,36 @@ def test_a_process_whose_first_calls_are_captured():
     import sys
     r = subprocess.run([sys.executable, "-c", FIRST], cwd=pathlib.Path(__file__).parents[1], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("d,hq,new,length", [(64, 4, 1, 600), (64, 4, 20, 600), (128, 7, 40, 700), (256, 4, 20, 500)])
+def test_scores_a_rounding_step_apart_where_steps_are_large(d, hq, new, length, dtype):
+    """Scores of 2^27 and, behind them, of the next larger number of 32 bits, 16 above: weights of 2^16 beside the first ones', which fp16 cannot hold.
+
+    Scores and their product with scale * log2 e = 1 are exact, so the first ones' weights are 2^-16 of the others', exactly in either type: only the sums' additions and the
+    result's rounding are left (and the total's of rounded weights, which are exact)."""
+    s = Setup([length], [new], hq, 1, d, 16, dtype, seed=d + new)
+    s.q[:] = 0
+    s.q[..., 0], s.q[..., 1] = 2.0 ** 14, 4.0
+    k = s.k[0]
+    k[:] = 0
+    k[..., 0] = 2.0 ** 13
+    larger = torch.arange(len(k)) % 128 >= 64                # (in whole steps of keys, behind smaller ones in one walk over them)
+    k[larger, :, 1] = 4.0
+    s.v[0] = (s.v[0].abs() + 1).to(s.dt)
+    s.put()
+    a, many = s.device(), 300                                # (so many sequences with the same pages that none is cut into parts)
+    lse = torch.empty(many * new, hq, device="cuda")
+    from quantexperiments_amd.kernels import tree_attention
+    out = tree_attention(a["q"].repeat(many, 1, 1), a["k_cache"], a["v_cache"], a["table"].repeat(many, 1), a["lens"].repeat(many), scale=math.log(2.0), lse=lse)
+    out, lse = out.view(many, new, hq, d), lse.view(many, new, hq)
+    assert torch.equal(out, out[:1].expand_as(out)) and torch.equal(lse, lse[:1].expand_as(lse))
+    u = torch.finfo(s.dt).eps / 2
+    for t in range(new):
+        n = length + t + 1
+        w = torch.where(larger[:n], 1.0, 2.0 ** -16).double()
+        want = (w[:, None] * s.v[0][:n, 0].double()).sum(0) / w.sum()
+        assert bool(((out[0, t].cpu().double() - want).abs() <= (u + (n + 64) * H) * 1.01 * want).all())
+        top = (2.0 ** 27 + 16) * math.log(2.0)
+        assert bool(((lse[0, t].cpu().double() - top - math.log(float(w.sum()))).abs() <= 4 * H * top).all())
