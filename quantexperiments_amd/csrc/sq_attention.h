@@ -9,8 +9,13 @@
 // as its B operand (lane l: row l % 16), so lane l holds, of row l % 16, the scores of keys 4 * (l / 16) .. + 3 and 16 + 4 * (l / 16) .. + 3: eight keys
 // which, taken in that order, are the eight consecutive k of the second product's B operand.  Its A operand, values with the
 // keys in the same order, is two transposing LDS reads (ds_read_b64_tr_b16: 16 lanes read 4 keys x 16 elements, lane i gets the 4 keys of element i).
-// So weights go from one product to the other in registers, rounded to the type once (half a step: 2^-9 of a weight in bf16, 2^-12 in fp16), and the
-// running maximum of a row, which its lanes share, scales the sums of that row without a shuffle.
+// So weights go from one product to the other in registers, and the running maximum of a row, which its lanes share, scales the sums of that row without a shuffle.
+//
+// The matrix instructions take both operands in one type, so the weights are rounded to that of the values, once (in 32 bits, as a high and a low part, the second product
+// would be two): by up to half a step, 2^-8 of a weight in bf16, 2^-11 in fp16.  fp16 holds them so down to 2^-14 only, in steps of 2^-24 below, and a key that has nearly all of
+// the weight, as the first ones of a sequence often do, leaves the others there.  So in fp16 weights are 2^7 times what they are, at most 2^15: full precision down to 2^-21 of a
+// row's largest weight, below that off by up to 2^-32 of it.  (2000 keys 17 below one whose value is zero: off by 4 % without the factor, by 2^-17 with it.  A larger one leaves
+// less room for a maximum to rise, and sums are scaled more often: 2^11 and 2^4 of room, trees of 48 tokens 46.3 -> 49.5 us, 1900 tokens 134 -> 140.)
 //
 // Keys and values reach LDS with global_load_lds, whole rows at a time (16 bytes per lane, a key's elements by neighbouring lanes), their
 // 16-byte pieces placed by XOR with the key's number so that 16 keys' pieces (first product) and 8 keys' pairs of pieces (transposing reads) lie in
@@ -42,7 +47,7 @@ struct AttnArgs {
 constexpr int ATTN_STEP = 32;                // keys of a step
 constexpr int ATTN_KEYS_MAX = INT32_MAX - 4096;
 constexpr int ATTN_SPLITS_MAX = 128;         // parts of a sequence
-constexpr float ATTN_SLACK = 8.f;
+constexpr float ATTN_SLACK = 8.f;            // so far (log2) a row's scores may rise before what is taken off its exponents, and so its sums, follow
 constexpr float ATTN_NOTHING = -3e38f;       // maximum of no scores: weights of -inf are zero against it, and it is nothing beside any other
 
 // A sequence's rows and keys.  What its arguments say beyond the buffers is cut off here: no index below leaves them.
@@ -69,6 +74,7 @@ template <int DT> struct AttnType;
 template <> struct AttnType<SQ_F16> {
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     static constexpr uint32_t INF = 0x7C00, ONE = 0x3C00;
+    static constexpr float SHIFT = 7.f;      // log2 of the factor on weights.  (Not 8: with ATTN_SLACK they would reach 2^16, which is none; and where 32 bits go in steps of 16, x - 7 is x)
     static __device__ __forceinline__ float4v mfma(u32x4 x, u32x4 y, float4v c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, x), __builtin_bit_cast(v8, y), c, 0, 0, 0);
     }
@@ -79,6 +85,7 @@ template <> struct AttnType<SQ_F16> {
 template <> struct AttnType<SQ_BF16> {
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     static constexpr uint32_t INF = 0x7F80, ONE = 0x3F80;
+    static constexpr float SHIFT = 0.f;
     static __device__ __forceinline__ float4v mfma(u32x4 x, u32x4 y, float4v c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, x), __builtin_bit_cast(v8, y), c, 0, 0, 0);
     }
@@ -92,11 +99,18 @@ template <int DT> __device__ __forceinline__ float attn_rounded(float s, float s
     if constexpr (DT == SQ_F16) asm("" : "+v"(x));
     return x;
 }
-// Whether the score `top` is more than ATTN_SLACK above m, which is taken off the exponents.  In fp16 by the rounded product: from 2^24 on it can lie further
+// Whether the score `top` is more than SHIFT + ATTN_SLACK above m, which is taken off the exponents.  In fp16 by the rounded product: from 2^24 on it can lie further
 // above m than the exact one does, and a weight of 2^16 would be an infinity.
 template <int DT> __device__ __forceinline__ bool attn_above(float top, float scale2, float m) {
-    if constexpr (DT == SQ_F16) return attn_rounded<DT>(top, scale2) - m > ATTN_SLACK;
-    return __builtin_fmaf(top, scale2, -ATTN_SLACK) > m;
+    if constexpr (DT == SQ_F16) return attn_rounded<DT>(top, scale2) - m > AttnType<DT>::SHIFT + ATTN_SLACK;
+    return __builtin_fmaf(top, scale2, -(AttnType<DT>::SHIFT + ATTN_SLACK)) > m;
+}
+// log of the sum of exponentials, from what was taken off and the total
+template <int DT> __device__ __forceinline__ float attn_lse(float m, float l) {
+    constexpr float S = AttnType<DT>::SHIFT;
+    if (l == 0.f) return -INFINITY;
+    const float bits = fabsf(m) <= 0x1p20f ? (m + S) + __builtin_amdgcn_logf(l * __builtin_exp2f(-S)) : m + __builtin_amdgcn_logf(l);
+    return bits * 0.6931471805599453f;
 }
 
 typedef __attribute__((address_space(3))) char* lds_ptr;
@@ -229,7 +243,7 @@ __device__ __forceinline__ void attn_copy_group(const AttnArgs& a, int where, in
 template <int DP, int MT> struct AttnRows {
     u32x4 q[MT][DP / 32];
     float4v o[MT][DP / 16];      // lane l: row l % 16, elements 16 * i + 4 * (l / 16) .. + 3
-    float m[MT], l[MT];          // maximum (times scale2) of the row, this lane's part of the total
+    float m[MT], l[MT];          // what is taken off the row's exponents (some maximum times scale2, less SHIFT), this lane's part of the total
     int tok[MT];                 // new token of the row
     bool far;                    // some maximum is none yet, or beyond 2^20 (the same for the wave)
 
@@ -311,8 +325,8 @@ __device__ __forceinline__ void attn_scores(const AttnRows<DP, MT>& r, const cha
 }
 
 // softmax weights of a step from its scores; the rows' maxima, totals and sums brought up to date.  sees: where MASKED.
-// What is taken off the exponents need not be the maximum itself: it is raised when a score is more than 2^ATTN_SLACK above it, so that most steps
-// neither fold their maxima over lanes nor scale the sums; weights stay below 2^ATTN_SLACK, far inside fp16 too.
+// What is taken off the exponents need not be the maximum itself: it is raised when a weight would be more than 2^ATTN_SLACK times the one it stands for, so that most steps
+// neither fold their maxima over lanes nor scale the sums; weights stay below 2^(SHIFT + ATTN_SLACK), inside fp16 too.
 template <int DT, int DP, int MT, bool MASKED>
 __device__ __forceinline__ void attn_weights(const AttnArgs& a, AttnRows<DP, MT>& r, float4v (&st)[MT][2], const uint32_t (&sees)[MT], int lane, u32x4 (&p)[MT]) {
     const int g = lane >> 4;
@@ -336,7 +350,7 @@ __device__ __forceinline__ void attn_weights(const AttnArgs& a, AttnRows<DP, MT>
         for (int t = 0; t < MT; ++t) {
             // (row by row, so that no row's bits depend on what the wave's other rows see)
             const float top = groups_fold(mx[t], [](float x, float y) { return fmaxf(x, y); });
-            const float m = attn_above<DT>(top, a.scale2, r.m[t]) ? attn_rounded<DT>(top, a.scale2) : r.m[t], by = __builtin_amdgcn_exp2f(r.m[t] - m);
+            const float m = attn_above<DT>(top, a.scale2, r.m[t]) ? attn_rounded<DT>(top, a.scale2) - AttnType<DT>::SHIFT : r.m[t], by = __builtin_amdgcn_exp2f(r.m[t] - m);
             r.m[t] = m;
             r.l[t] *= by;
             far |= !(fabsf(m) <= 0x1p20f);
@@ -493,7 +507,7 @@ __device__ __forceinline__ void attn_write(const AttnArgs& a, const AttnSeq& s, 
             for (int x = 0; x < 4; ++x) o[x] = (uint32_t)AttnType<DT>::one(v[2 * x] * inv) | ((uint32_t)AttnType<DT>::one(v[2 * x + 1] * inv) << 16);
             *reinterpret_cast<u32x4*>(a.out + tok_all * a.o_t + (int64_t)hq * a.o_h + e * 2) = o;
         }
-        if (e == 0 && a.lse) a.lse[tok_all * a.q_heads + hq] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+        if (e == 0 && a.lse) a.lse[tok_all * a.q_heads + hq] = attn_lse<DT>(m, l);
     }
 }
 
@@ -764,11 +778,11 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
             by1 = a.scale2;
             less1 = r.m[t];
             // (one operation less than attn_above in fp16.  Rows beyond 2^20, where that is not enough, always come here; for others the second condition says nothing more)
-            auto above = [&](float x) __attribute__((always_inline)) { return __builtin_fmaf(x, a.scale2, -ATTN_SLACK) > r.m[t]; };
+            auto above = [&](float x) __attribute__((always_inline)) { return __builtin_fmaf(x, a.scale2, -(E::SHIFT + ATTN_SLACK)) > r.m[t]; };
             if ((__ballot(above(mx)) | far) != 0) {
                 const float top = groups_fold(mx, [](float x, float y) { return fmaxf(x, y); }), x = attn_rounded<DT>(top, a.scale2);
                 const bool up = above(top) || (DT == SQ_F16 && x - r.m[t] >= 16.f);
-                const float m = up ? x : r.m[t], f = __builtin_amdgcn_exp2f(r.m[t] - m);
+                const float m = up ? x - E::SHIFT : r.m[t], f = __builtin_amdgcn_exp2f(r.m[t] - m);
                 r.m[t] = less1 = m;
                 r.l[t] *= f;
 #pragma unroll
@@ -901,7 +915,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
                 o[1] = (uint32_t)E::one(r.o[t][d][2] * inv) | ((uint32_t)E::one(r.o[t][d][3] * inv) << 16);
                 *reinterpret_cast<u32x2*>(out + d * 32) = o;
             }
-        if (lane < 16 && a.lse) a.lse[tok_all * a.q_heads + hq] = l == 0.f ? -INFINITY : (r.m[t] + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+        if (lane < 16 && a.lse) a.lse[tok_all * a.q_heads + hq] = attn_lse<DT>(r.m[t], l);
     }
 }
 
@@ -996,7 +1010,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
         o[1] = (uint32_t)AttnType<DT>::one(v[2] * inv) | ((uint32_t)AttnType<DT>::one(v[3] * inv) << 16);
         *reinterpret_cast<u32x2*>(a.out + (int64_t)(s.first + tok) * a.o_t + (int64_t)hq * a.o_h + q * 8) = o;
     }
-    if (q == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+    if (q == 0 && a.lse) a.lse[row] = attn_lse<DT>(m, l);
 }
 
 // ------------------------------------------------------------------------------------------ host

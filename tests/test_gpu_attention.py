@@ -538,3 +538,31 @@ def test_scores_a_rounding_step_apart_where_steps_are_large(d, hq, new, length, 
         assert bool(((out[0, t].cpu().double() - want).abs() <= (u + (n + 64) * H) * 1.01 * want).all())
         top = (2.0 ** 27 + 16) * math.log(2.0)
         assert bool(((lse[0, t].cpu().double() - top - math.log(float(w.sum()))).abs() <= 4 * H * top).all())
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("above", [9, 14, 17, 20])
+@pytest.mark.parametrize("d,hq,hk,news,length", [(64, 4, 1, [1], 900), (128, 6, 2, [3, 1], 1000), (256, 4, 1, [2], 700), (64, 4, 1, [20], 900), (128, 7, 1, [40], 700), (256, 2, 1, [70], 500),
+                                                 (96, 7, 1, [40, 3], 400)])
+def test_weights_far_below_the_largest(d, hq, hk, news, length, above, dtype):
+    """Keys in every 64 slots whose scores are `above` higher than the others' mean and whose values are zero, so that the result is what the others' weights leave.
+
+    A weight of fp16 is held times 2^7 beside a reference that is at most the row's largest score: with u relative where that is 2^-14 or more, with half a step of 2^-24 below.
+    So it is off by u of itself or by 2^-25 / 2^7 of the largest weight, and a result by up to 2^-32 sum |v| / sum exp(s - max) more than by the others' bound."""
+    s = Setup([length] * len(news), news, hq, hk, d, 16, dtype, tree=news[0] > 1, seed=above + d, scale=1.0)
+    s.q[..., 0] = 8.0
+    for b in range(len(news)):
+        s.k[b][..., 0] = 0
+        s.k[b][::64] = 0
+        s.k[b][::64, :, 0] = above * d ** 0.5 / 8
+        s.v[b] = (4000 * (0.5 + torch.rand(s.v[b].shape, generator=s.g))).to(s.dt)
+        s.v[b][::64] = 0
+    s.put()
+    got, got_lse = attend(s)
+    out, tol, lse, ltol = s.reference()
+    if dtype == "f16":
+        for b, (k, v) in enumerate(zip(s.k, s.v)):
+            tol[s.starts[b]:s.starts[b + 1]] += 2.0 ** -32 * float(v.double().abs().sum(0).max()) / len(k[:length:64])
+    off, off_lse = (got.cpu().double() - out).abs(), (got_lse.cpu().double() - lse).abs()
+    assert bool((off <= tol).all()), float((off / tol).max())
+    assert bool((off_lse <= ltol).all()), float((off_lse / ltol).max())
