@@ -453,7 +453,7 @@ int sq_qk_norm_rotary(const sq_heads* q, const sq_heads* k, const sq_heads* v, i
  * New token t of a sequence (t = 0 ..) sees all cached tokens, and new token j of its sequence if
  *     mask NULL: j <= t (one token: a decode step; many: a chunk of a prompt)
  *     otherwise: bit j % 64 of mask[row * ld_mask + j / 64] is set, row = starts[b] + t (a tree of drafted tokens: itself and its
- *     ancestors); bits of j >= 64 * mask_words count as clear.
+ *     ancestors); bits of j >= 64 * mask_words count as clear (mask_words 0: no new token is seen, and mask is any address but NULL).
  * Head h of q reads head h / (q_heads / cache->heads) of the cache:
  *     s_j = scale * q . k_j,  out = sum_j softmax(s)_j v_j  over what the token sees,  lse = log(sum_j exp(s_j))  (lse NULL: not written)
  * A token that sees nothing gets zeros and -inf.  Keys and values that a token does not see do not touch its result, whatever they hold.

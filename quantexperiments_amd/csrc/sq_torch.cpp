@@ -663,6 +663,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         at::Tensor out = given ? *given : at::empty(q.sizes(), q.options());
         t.q = q.data_ptr(); t.out = out.data_ptr(); t.lse = lse ? (float*)lse->data_ptr() : nullptr; t.table = (const int32_t*)table.data_ptr();
         t.lens = (const int32_t*)lens.data_ptr(); t.starts = starts ? (const int32_t*)starts->data_ptr() : nullptr; t.mask = mask ? (const int64_t*)mask->data_ptr() : nullptr;
+        if (mask && !t.mask) t.mask = (const int64_t*)lens.data_ptr();       // (a mask without words has no address, and none would mean no mask; nothing is read there)
         t.q_token = q.stride(0); t.q_head = q.stride(1); t.out_token = out.stride(0); t.out_head = out.stride(1);
         t.ld_table = b > 1 ? table.stride(0) : table.size(1); t.ld_mask = mask ? rows > 1 ? mask->stride(0) : mask->size(1) : 0;
         t.tokens = (int32_t)rows; t.seqs = (int32_t)b; t.most_new = (int32_t)most; t.q_heads = (int32_t)q.size(1); t.max_pages = (int32_t)table.size(1);

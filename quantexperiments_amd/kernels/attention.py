@@ -324,8 +324,9 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
             raise ValueError(f"{who}: out must not be expanded")
     if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (n, hq) or not lse.is_contiguous()):
         raise ValueError(f"{who}: lse must be contiguous fp32 [{n}, {hq}]")
+    # (a mask without words has no address of its own, and none would mean no mask: any other does, nothing is read there)
     a = SqAttention(q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), table.data_ptr(), lens.data_ptr(),
-                    None if starts is None else starts.data_ptr(), None if mask is None else mask.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1),
+                    None if starts is None else starts.data_ptr(), None if mask is None else mask.data_ptr() or lens.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1),
                     table.stride(0) if b > 1 else table.shape[1], 0 if mask is None else mask.stride(0) if n > 1 else mask.shape[1], n, b, most_new, hq, table.shape[1],
                     0 if mask is None else mask.shape[1], scale)
     L = _lib.lib()

@@ -566,3 +566,26 @@ def test_weights_far_below_the_largest(d, hq, hk, news, length, above, dtype):
     off, off_lse = (got.cpu().double() - out).abs(), (got_lse.cpu().double() - lse).abs()
     assert bool((off <= tol).all()), float((off / tol).max())
     assert bool((off_lse <= ltol).all()), float((off_lse / ltol).max())
+
+
+def test_a_mask_without_words_shows_the_cached_tokens_alone():
+    s = Setup([40, 0, 5], [3, 1, 50], 4, 2, 64, 16, tree=True, seed=14)
+    s.sees = [torch.zeros_like(t) for t in s.sees]
+    zeros, zeros_lse = attend(s, mask=torch.zeros(s.n, 1, dtype=torch.int64, device="cuda"))
+    s.check(zeros, zeros_lse)
+    out, lse = attend(s, mask=torch.empty(s.n, 0, dtype=torch.int64, device="cuda"))
+    assert torch.equal(out, zeros) and torch.equal(lse, zeros_lse)
+    strided = torch.zeros(s.n, 4, dtype=torch.int64, device="cuda")[:, 2:2]
+    out, lse = attend(s, mask=strided)
+    assert torch.equal(out, zeros) and torch.equal(lse, zeros_lse)
+
+
+def test_a_mask_without_words_through_the_call_path_in_python(monkeypatch):
+    from quantexperiments_amd import _lib
+
+    class NotCovered:
+        def __getattr__(self, name):
+            return lambda *args: 1
+
+    monkeypatch.setattr(_lib, "native", lambda: NotCovered())
+    test_a_mask_without_words_shows_the_cached_tokens_alone()
