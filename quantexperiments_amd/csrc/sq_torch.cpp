@@ -475,10 +475,10 @@ PyObject* q4_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // ------------------------------------------------------------------------------------------ heads of q|k|v, attention
 
-// A tensor these calls take as it is: on `dev`, strided, nothing that Python dispatches or that a gradient would be recorded for
+// A tensor these calls take as it is: on `dev`, strided, nothing that Python dispatches, that a gradient would be recorded for or that has a tangent
 bool plain_on(const at::Tensor& t, int dev) {
     return t.is_cuda() && t.get_device() == dev && t.layout() == at::kStrided && !t.unsafeGetTensorImpl()->is_python_dispatch() &&
-           !(t.requires_grad() && at::GradMode::is_enabled());
+           !(t.requires_grad() && at::GradMode::is_enabled()) && !t._fw_grad(0).defined();
 }
 // An argument that may be None: NULL, or the tensor; false where it is neither
 bool maybe(PyObject* o, const at::Tensor*& t) {

@@ -8,7 +8,8 @@ sequence b is slot s % page of page table[b, s // page].
 
 Everything launches on torch's current stream, allocates from torch and reads no device value on the host, so calls can be captured into HIP graphs;
 what lengths, tables and masks hold may change between replays.  The kernels index with them and cut off what lies outside the
-buffers, as include/sqhip.h says call by call.  Inference only: tensors that require a gradient are refused where one would be recorded.
+buffers, as include/sqhip.h says call by call.  Inference only: tensors that require a gradient are refused where one would be recorded, and
+tensors with a tangent (forward mode).
 The reference's engine has these steps as rope_cache, attn_rope and attn (reference shapequant/kernels/decode_e2e.py:142-225) and
 attn_prep (shapequant/kernels/qwen35_kernels.py:50-190), for single tokens and a contiguous cache."""
 
@@ -18,6 +19,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from .._lib import SqAttention, SqCache, SqHeads, SqRotation
@@ -68,6 +70,8 @@ def rotary_freqs(rot: int, base: float = 10000.0, scaling: dict | None = None, d
 def _no_grad(who: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise NotImplementedError(f"{who} has no autograd formula: call it under torch.no_grad()")
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{who} has no formula for tangents (forward mode): pass the primal tensors")
 
 
 def _on_gpu(who: str, dev, **tensors) -> None:

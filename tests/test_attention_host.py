@@ -161,3 +161,17 @@ def test_outputs_of_attention_whose_rows_overlap_are_refused():
     L = _lib.lib()
     for kw in (dict(out_token=256), dict(out_head=56), dict(out_token=0), dict(out_token=64, out_head=64)):
         assert L.sq_tree_attention(attention(**kw), cache(), None, 0, None) == _lib.SQ_EINVAL, kw
+
+
+def test_python_calls_refuse_tangents():
+    from torch.autograd import forward_ad
+    x, pos, f = torch.zeros(2, 4, 64, dtype=torch.float16), torch.arange(2), torch.ones(32, dtype=torch.float64)
+    c, i32 = torch.zeros(3, 16, 2, 64, dtype=torch.float16), lambda *s: torch.zeros(*s, dtype=torch.int32)
+    with forward_ad.dual_level():
+        d, dc = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, c))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for call in (lambda: rotary(d, pos, f), lambda: qk_norm_rotary(x, d[:, :2], pos, f), lambda: tree_attention(d, c, c, i32(2, 1), i32(2)),
+                             lambda: keep_drafted(c, dc, i32(2, 1), i32(2), i32(2, 2), i32(2))):
+                    with pytest.raises(NotImplementedError, match="tangents"):
+                        call()

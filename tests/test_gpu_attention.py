@@ -589,3 +589,30 @@ def test_a_mask_without_words_through_the_call_path_in_python(monkeypatch):
 
     monkeypatch.setattr(_lib, "native", lambda: NotCovered())
     test_a_mask_without_words_shows_the_cached_tokens_alone()
+
+
+def test_tensors_with_a_tangent_are_refused():
+    """Forward mode: a dual tensor asks for no gradient, and what is computed from its values alone would have a derivative of zero."""
+    from torch.autograd import forward_ad
+    from quantexperiments_amd.kernels import keep_drafted, qk_norm_rotary, rotary, tree_attention
+    s = Setup([20], [2], 4, 2, 64, 16, seed=15)
+    a = {**s.device(), "mask": None}
+    pos, f = torch.arange(2).cuda(), torch.ones(32, dtype=torch.float64).cuda()
+    x, k, w = a["q"], a["q"][:, :2], torch.ones(64, dtype=s.dt).cuda()
+    cache, slots = dict(v=k, k_cache=a["k_cache"], v_cache=a["v_cache"]), torch.arange(2).cuda()
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        calls = [lambda: rotary(dual(x), pos, f), lambda: rotary(x, pos, dual(f)), lambda: rotary(x, pos, f, dual(torch.empty_like(x))),
+                 lambda: qk_norm_rotary(dual(x), k, pos, f), lambda: qk_norm_rotary(x, dual(k), pos, f), lambda: qk_norm_rotary(x, k, pos, dual(f)),
+                 lambda: qk_norm_rotary(x, k, pos, f, dual(w), w), lambda: qk_norm_rotary(x, k, pos, f, w, dual(w)), lambda: keep_drafted(dual(a["k_cache"]), a["v_cache"], a["table"], a["lens"], i32([[0]]), i32([1])),
+                 lambda: keep_drafted(a["k_cache"], dual(a["v_cache"]), a["table"], a["lens"], i32([[0]]), i32([1]))]
+        calls += [lambda n=n: qk_norm_rotary(x, k, pos, f, slots=slots, **{**cache, n: dual(cache[n])}) for n in cache]
+        calls += [lambda n=n: tree_attention(**{**a, n: dual(a[n])}) for n in ("q", "k_cache", "v_cache")]
+        calls += [lambda: tree_attention(**a, out=dual(torch.empty_like(x)))]
+        for grad in (True, False):                           # (tangents are carried under no_grad too)
+            for i, call in enumerate(calls):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                    call()
+                    print("not refused:", i)
+        s.check(tree_attention(**a))
