@@ -63,7 +63,7 @@ static int check_attention(const char* who, const sq_attention* a, const sq_cach
                     (long long)a->ld_table, c->pages, c->page);
     if ((int64_t)a->seqs * a->most_new > INT32_MAX / a->q_heads)          // (no more rows than 32 bits count: a plan of more would wrap)
         return fail(SQ_EUNSUPPORTED, "%s: %d sequences of up to %d new tokens and %d heads at once", who, a->seqs, a->most_new, a->q_heads);
-    if (!(a->scale > 0.f) || a->scale > 3e38f) return fail(SQ_EINVAL, "%s: scale %g", who, (double)a->scale);
+    if (!(a->scale > 0.f) || a->scale > 2.3e38f) return fail(SQ_EINVAL, "%s: scale %g", who, (double)a->scale);          // (times log2 e a number)
     if (!a->starts && (int64_t)a->seqs * a->most_new != a->tokens)
         return fail(SQ_EINVAL, "%s: %d tokens are not %d for each of %d sequences", who, a->tokens, a->most_new, a->seqs);
     return SQ_OK;

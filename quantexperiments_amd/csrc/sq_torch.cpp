@@ -655,7 +655,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (a[6] != Py_None) most = starts ? std::min<int64_t>(PyLong_AsLongLong(a[6]), rows) : PyLong_AsLongLong(a[6]);
         const double scale = a[8] == Py_None ? std::pow((double)c.dim, -0.5) : PyFloat_AsDouble(a[8]);
         if (PyErr_Occurred()) return nullptr;
-        if (most < 0 || most > INT32_MAX || (!starts && most * b != rows) || !(scale > 0 && scale < 3e38)) return answer(NOT_COVERED);
+        if (most < 0 || most > INT32_MAX || (!starts && most * b != rows) || !(scale > 0 && scale < 2.3e38)) return answer(NOT_COVERED);
         if (given && (!heads_on(*given, dev) || given->sizes() != q.sizes() || given->scalar_type() != q.scalar_type() || !apart(*given, q) || !apart(*given, kc) || !apart(*given, vc) ||
                       (given->stride(0) == 0 && rows > 1) || (given->stride(1) == 0 && q.size(1) > 1)))
             return answer(NOT_COVERED);

@@ -311,7 +311,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         _rows2(who, "mask", mask, n, torch.int64)
     if scale is None:
         scale = d ** -0.5
-    if not 0 < scale < 3e38:
+    if not 0 < scale < 2.3e38:                                # (times log2 e a number)
         raise ValueError(f"{who}: scale {scale}")
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)

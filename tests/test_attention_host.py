@@ -175,3 +175,11 @@ def test_python_calls_refuse_tangents():
                              lambda: keep_drafted(c, dc, i32(2, 1), i32(2), i32(2, 2), i32(2))):
                     with pytest.raises(NotImplementedError, match="tangents"):
                         call()
+
+
+def test_scales_whose_product_with_log2_e_is_no_number_are_refused():
+    L = _lib.lib()
+    for scale in (2.4e38, 2.9e38, 3.4e38):
+        assert L.sq_tree_attention(attention(scale=scale), cache(), None, 0, None) == _lib.SQ_EINVAL, scale
+        assert L.sq_tree_attention(attention(scale=scale, tokens=0, seqs=0), cache(), None, 0, None) == _lib.SQ_EINVAL, scale
+    assert L.sq_tree_attention(attention(scale=2.2e38, tokens=0, seqs=0), cache(), None, 0, None) == _lib.SQ_OK

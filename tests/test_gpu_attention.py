@@ -616,3 +616,14 @@ def test_tensors_with_a_tangent_are_refused():
                     call()
                     print("not refused:", i)
         s.check(tree_attention(**a))
+
+
+def test_scales_at_the_ends_of_the_range():
+    from quantexperiments_amd.kernels import tree_attention
+    s = Setup([40], [1], 2, 1, 64, 16, seed=16)
+    for scale in (2.4e38, 3.4e38, math.inf, 0.0, -1.0, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            tree_attention(**{**s.device(), "scale": scale})
+    s.q[:] = 0                                               # scores of zero, whatever the scale: the mean of all values
+    for s.scale in (2.2e38, 1e-30):
+        s.check(*attend(s))
