@@ -627,3 +627,39 @@ def test_scales_at_the_ends_of_the_range():
     s.q[:] = 0                                               # scores of zero, whatever the scale: the mean of all values
     for s.scale in (2.2e38, 1e-30):
         s.check(*attend(s))
+
+
+@pytest.mark.parametrize("d,hq,hk,new,seqs,length,page,tree,dtype", [
+    # eight waves of 32 rows (16 of heads of 256), a workgroup per sequence, key head and block of rows
+    (128, 9, 3, 80, 100, 700, 8, True, "f16"), (128, 9, 3, 80, 100, 640, 24, False, "bf16"), (64, 9, 3, 80, 100, 1100, 8, False, "bf16"), (64, 9, 3, 80, 100, 700, 7, True, "f16"),
+    (96, 9, 3, 80, 100, 700, 16, True, "bf16"), (256, 6, 3, 64, 100, 420, 16, True, "bf16"), (256, 6, 3, 64, 100, 420, 5, False, "f16"), (128, 6, 2, 90, 100, 640, 1, True, "bf16"),
+    # four waves
+    (128, 9, 3, 40, 100, 420, 16, True, "bf16"), (256, 6, 3, 32, 100, 420, 16, False, "f16"), (96, 9, 3, 40, 100, 420, 9, False, "f16"), (64, 9, 3, 40, 100, 420, 16, True, "bf16"),
+    # several blocks of rows, which see unlike numbers of keys; sequences cut into parts of several rounds each
+    (128, 7, 1, 300, 40, 900, 16, False, "bf16"), (128, 28, 4, 48, 8, 2500, 16, True, "f16")])
+def test_rings_that_are_filled_again_and_again(d, hq, hk, new, seqs, length, page, tree, dtype):
+    """Workgroups that walk through many stages of keys, so that every place in LDS is filled, read and filled again; lengths that differ by some keys, so that the last
+    stages do too; tables of more than 64 pages among them, so that a wave fetches entries again.  Checked: some rows of some sequences."""
+    g = torch.Generator().manual_seed(d + new + page)
+    lens = [length - int(x) for x in torch.randint(0, 40, (seqs,), generator=g)]
+    news = [new - b % 3 for b in range(seqs)]
+    s = Setup(lens, news, hq, hk, d, page, dtype, tree, seed=d + new)
+    got, lse = attend(s)
+    again, lse2 = attend(s)
+    assert torch.equal(got, again) and torch.equal(lse, lse2) and bool(got.isfinite().all())
+    u = torch.finfo(s.dt).eps / 2
+    for b in (0, 1, seqs // 2, seqs - 1):
+        l, n = lens[b], news[b]
+        k, v = s.k[b].double(), s.v[b].double()
+        for t in sorted({0, 1, n // 2, n - 2, n - 1}):
+            see = torch.cat((torch.ones(l, dtype=torch.bool), s.sees[b][t]))
+            r = s.starts[b] + t
+            for h in range(hq):
+                kk, vv, q = k[see, h // (hq // hk)], v[see, h // (hq // hk)], s.q[r, h].double()
+                sc = kk @ q * s.scale
+                ds = (d + 4) * H * s.scale * float((kk.abs() @ q.abs()).max())
+                p = torch.softmax(sc, 0)
+                out, big, top = p @ vv, p @ vv.abs(), torch.logsumexp(sc, 0)
+                tol = (u * 1.01 + 2 * ds + (len(sc) + 64) * H) * big + u * out.abs() + torch.finfo(s.dt).tiny * torch.finfo(s.dt).eps
+                assert bool(((got[r, h].cpu().double() - out).abs() <= tol).all()), (b, t, h)
+                assert abs(float(lse[r, h]) - float(top)) <= ds + (len(sc) + 64) * H + 4 * H * max(1.0, abs(float(top)), abs(float(sc.max()))), (b, t, h)
