@@ -460,7 +460,9 @@ int sq_qk_norm_rotary(const sq_heads* q, const sq_heads* k, const sq_heads* v, i
  * dtype = cache->dtype, SQ_F16 or SQ_BF16, is q's and out's type; lse is fp32 [tokens, q_heads].  dim: a multiple of 8 up to 256; q, k, v and out
  * 16-byte aligned with strides that are multiples of 8.  Scores, softmax and sums in 32 bits, its weights rounded to dtype for
  * the matrix instructions: by up to 2^-8 of a weight in bf16, 2^-11 in fp16 (there, of a weight below 2^-21 of the row's largest, by up to 2^-32 of the largest).  Rows of out outside starts[0] .. starts[seqs] - 1 and new tokens from the most_new-th of a sequence on are
- * not written.  A sequence whose tokens do not fit its table row, or whose table names a page outside the cache, gets NaN.
+ * not written.  A sequence whose tokens do not fit its table row gets NaN; where a table names a page outside the
+ * cache, the rows whose keys need that page do, and others of the sequence may.
+ * lens is on the device, so the launch and the workspace are sized for sequences that fill their table rows: max_pages near the truth makes short ones faster.
  * The workspace (sq_tree_attention_workspace_bytes, 256-byte aligned; may be 0) needs no preparation and is the call's own while it runs.
  * Results do not depend on its content or on what else runs: no atomics. */
 typedef struct sq_attention {

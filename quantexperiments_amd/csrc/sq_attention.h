@@ -117,7 +117,8 @@ typedef __attribute__((address_space(3))) char* lds_ptr;
 
 // Copies 16 bytes per lane to LDS, lane l's to `to` + 16 l, and waits for all but the newest N memory operations.  Written out, because the
 // compiler waits for every copy in flight before a transposing read; they write no register, and what reads LDS stays behind the waits (memory clobber).
-// (m0 is not the compiler's to keep anything in.)  What the compiler loads into registers itself it waits for as if these were not there, that is for more than it has to.
+// (m0 is reserved: the compiler keeps nothing in it, takes no clobber of that name, and its own code for these kernels does not use it.)
+// What the compiler loads into registers itself it waits for as if these were not there, that is for more than it has to.
 __device__ __forceinline__ void attn_copy16(uint32_t to, const char* at, uint32_t offset) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(at) : "memory");
 }
@@ -518,7 +519,7 @@ template <int DP, int MT, int NW> constexpr int attn_lds() {
 
 // Few rows (MT * 16 at a time): the waves of a workgroup share the rows and split its keys, each with two steps of keys and values of its
 // own in LDS, no barrier until the end, where their sums are joined.  Sequences are cut into `splits` workgroups too.  Bound by HBM on long caches (32 sequences of
-// 2,240 to 8,192 slots, 8 key heads of 128, 5 query heads each: 126 us, 5.4 TB/s), by its chain of loads on short ones (500 slots 7 us).
+// 2,240 to 8,192 slots, 8 key heads of 128, 5 query heads each: 123 us, 5.6 TB/s; 64 of 8192 364 us, 5.9 TB/s), by its chain of loads on short ones (500 slots 7 us).
 template <int DT, int DP, int MT, int NW, bool FULL>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(1, 1))) void attn_kernel(AttnArgs a) {
     typedef AttnTile<DP> T;
@@ -662,7 +663,8 @@ __device__ __forceinline__ float attn_most(float4v x, float4v y) {
 // registers and moves them around the branch that scales them, 1300 cycles a slot instead of 500.  Bound by what a SIMD's two waves issue: matrix and other vector
 // instructions hardly overlap (1900 tokens of 28 heads of 128 behind 2100, 4 key heads: 121 us, 686 TFLOP/s, matrix cores busy 44 % of the time).
 // The stages at a sequence's end that some row does not see whole go step by step, behind the pipeline, and all of them (those that every row sees without masks) for
-// heads wider than 128 elements, whose keys and values would take the registers of four tiles (1000 tokens of 20 heads of 256 behind 2100: 136 us).
+// heads wider than 128 elements, whose keys and values would take the registers of four tiles.  There a wave has one tile, so a key's pieces are read from LDS once per 16 rows: 256 KB a
+// stage for eight waves, 2048 cycles at 128 bytes each, beside 1024 of matrix instructions (1000 tokens of 20 heads of 256 behind 2100: 133 us, 97 stages of some 3000 cycles).
 template <int DT, int DP, int NW, bool FULL>
 __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     typedef AttnTile<DP> T;
@@ -832,7 +834,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
                 if (n == SK * MT - 1 && i + 1 < clear) arrive(i + 1);
                 __builtin_amdgcn_sched_barrier(0);
                 // (behind the last stage of the pipeline: whatever lies in the next one's place, for nothing)
-                __builtin_amdgcn_s_setprio(1);           // (a SIMD's other wave is then more often in another region: 1900 new tokens behind 2100 141 -> 136 us, 8 trees of 48 53 -> 52)
+                __builtin_amdgcn_s_setprio(1);           // (a SIMD's other wave is then more often in another region: 1900 new tokens behind 2100 127 -> 121 us, 8 trees of 48 49.4 -> 47.6)
                 scores(t, std::integral_constant<bool, t == MT - 1>(), h + 1 < SK ? cur + (h + 1) * T::BYTES : nxt);
                 finish(t2);
                 asm volatile("" : "+v"(p), "+v"(r.l[t2]));      // (here, not behind the branch)

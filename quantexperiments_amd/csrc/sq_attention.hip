@@ -12,6 +12,9 @@ namespace sq {
 // two, 16 of 2000 x 8 heads 26.6 and 30.4.
 // A last block of rows that fills at most half of its waves takes 0.6 of the time, and gets as many fewer parts: 8 trees of 32 tokens of 5 heads of 256 per
 // key head (160 rows in blocks of 128) 42.3 us evenly, 39.3 so; with 0.75 42.1.
+// (All times of captured calls, one behind the other; calls back to back take up to 4 % less.)
+// A sequence's length is its table's width here: lengths are on the device.  Under a table of 131,072 slots one token behind 500 takes 10.2 us instead of 8.8, 48 26.7 instead of 21.4,
+// 64 sequences of 500 27.9 instead of 18.6, 64 of 2000 59.8 instead of 53.1.
 static AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
     AttnPlan p;
     p.dp = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;

@@ -129,8 +129,8 @@ __device__ __forceinline__ float lanes_sum(float v, int log2n) {        // (of l
 // of two for the sum of its squares) with two 16-byte loads each, in flight while the token's angles are worked out, once for all heads.
 // WT: the type of the norm weights, or none; they are fetched with the elements (behind the sum of squares they cost 2048 tokens of 28 + 4 + 4 heads of
 // 128 another 4 us), and layout and type are chosen at compile time (chosen here they take a fifth of the waves' registers and more than that was worth).
-// Bound by HBM from about 1000 tokens on (norm, rotation and cache slots of 8192 tokens of 28 + 4 + 4 heads of 128 34 us, 151 MB, 4.4 TB/s; rotation of 28 heads of 2048
-// tokens 7.7 us, 3.8 TB/s), by its chain of loads, angles, sum and stores below (8 tokens 3.9 us).
+// Bound by HBM from about 1000 tokens on (norm, rotation and cache slots of 8192 tokens of 28 + 4 + 4 heads of 128 37 us, 151 MB, 4.1 TB/s; rotation of 32 heads of 2048
+// tokens 7.3 us, 4.6 TB/s), by its chain of loads, angles, sum and stores below (8 tokens 3.9 us).
 constexpr int NO_NORM = -1;
 template <int DT, int WT, bool INTERLEAVED>
 __global__ __launch_bounds__(HEADS_MAX_THREADS) void heads_kernel(HeadsArgs a) {
@@ -227,7 +227,8 @@ template <int DT> __device__ __forceinline__ void store_one(void* p, int64_t i, 
 }
 
 // Any width, part, stride and alignment: a wave per head, a lane per pair.  (Where 16-byte pieces fit, heads_kernel takes as long for up to 64 tokens of 32 heads
-// of 128 and is two to five times as fast for more: 2048 tokens 11.1 against 40.5 us with norms, 7.7 against 32.1 without.)
+// of 128 and is two to five times as fast for more: 2048 tokens 11.1 against 40.5 us with norms, 7.7 against 32.1 without.  Bound by the angles, in 64 bits for each head again, and by
+// single elements, read twice where there is a norm.)
 template <int DT>
 __global__ __launch_bounds__(256) void heads_any_kernel(HeadsArgs a) {
     const int lane = threadIdx.x & 63;
@@ -298,7 +299,7 @@ int launch_heads(const HeadsArgs& args, int dtype, const char* who, hipStream_t 
         while ((16 << a.lanes_log2) < a.dim) ++a.lanes_log2;
         const int items = a.heads << a.lanes_log2;
         // Many tokens: two waves each, the heads in turn, so that fewer waves hold their places while one or two work the angles out (28 + 4 + 4 heads of 128 normed,
-        // 2048 tokens 15.1 us with a thread per item, 12.8 so, with one wave 13.7; 8192: 45.7, 34.0, 32.6; 1024: 8.2, 8.3, 9.9)
+        // 2048 tokens 15.1 us with a thread per item, 12.8 so, with one wave 13.7; 8192: 45.7, 34.0, 32.6; 1024: 8.2, 8.3, 9.9; over the same memory each time)
         const int most = a.tokens > 4 * device_cus() ? 128 : HEADS_MAX_THREADS, rounds = (items + most - 1) / most;
         const int threads = ((items + rounds - 1) / rounds + 63) / 64 * 64;
         // few tokens: their heads over several workgroups (each works the angles out again); enough of them: one workgroup takes a token whole

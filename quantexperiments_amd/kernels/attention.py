@@ -274,7 +274,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
                    lse: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of new tokens q [N, Hq, D] (fp16 / bf16) over a paged cache that holds lens[b] (int32 [B]) cached tokens of each sequence and, in the
     slots behind them, its new tokens' keys and values (sq_tree_attention).  The new tokens of sequence b are rows starts[b] .. starts[b + 1] - 1
-    (int32 [B + 1]; None: N / B each) of q, at most `most_new` of them (default: N; a bound near the truth makes the launch smaller).  A token sees all cached
+    (int32 [B + 1]; None: N / B each) of q, at most `most_new` of them (default: N; a bound near the truth makes the launch smaller, as a table that
+    is not much wider than the longest sequence does: table[:, :pages] may be passed).  A token sees all cached
     tokens, and of the new ones those in its row of mask (int64 [N, words], bit j % 64 of word j / 64: new token j of its sequence; a drafted tree's
     ancestors and the token itself), or, without a mask, those up to itself (single tokens, chunks of a prompt).  Query head h reads
     key head h / (Hq / Hk).  scale: default D ** -0.5.  out [N, Hq, D]: rows that belong to no sequence are left as they are (default: new, they
