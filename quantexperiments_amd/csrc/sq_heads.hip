@@ -403,7 +403,7 @@ __global__ __launch_bounds__(256) void keep_kernel(KeepArgs a) {
                 const int32_t* path = a.path + (int64_t)b * a.ld_path;
                 const int p = path[i];
                 const int64_t src = len + p, dst = len + i;
-                ok = p >= 0 && (i == 0 || p > path[i - 1]) && src < cap;
+                ok = p >= 0 && (i == 0 || p > path[i - 1]) && src < cap && dst < cap;          // (behind an entry that does not ascend, dst may lie behind src)
                 if (ok) {
                     const int sp = (int)(src / a.page), dp = (int)(dst / a.page);
                     const int32_t sid = a.table[(int64_t)b * a.ld_table + sp], did = a.table[(int64_t)b * a.ld_table + dp];
