@@ -487,6 +487,63 @@ size_t sq_tree_attention_workspace_bytes(const sq_attention* a, const sq_cache* 
 int sq_keep_drafted(const sq_cache* cache, int32_t layers, int64_t k_layer, int64_t v_layer, const int32_t* table, int64_t ld_table, int32_t max_pages,
                     const int32_t* lens, const int32_t* path, int64_t ld_path, int32_t most, const int32_t* counts, int32_t seqs, void* stream);
 
+/* ---- A cache held in 8 bits, and the pages of a cache ----
+ *
+ * sq_cache8: a layer's paged cache of keys and values as e4m3 codes (one sign, four exponent, three mantissa bits, largest 448, no infinities) and
+ * one e8m0 scale (a byte, 2^(byte - 127)) for each block of tokens and head: slot s of page p, head h, element i stands for
+ *     code(k + p * k_page + s * k_slot + h * k_head + i) * scale(k_scale + p * ks_page + s / (page / blocks) * ks_block + h * ks_head)
+ * and values likewise.  page / blocks, the tokens of a block, is a multiple of 16; dim a multiple of 16 up to 256, heads 16-byte aligned; the
+ * slots of a page ascend in memory, less than 2^27 bytes from one to the next. */
+typedef struct sq_cache8 {
+    void* k;
+    void* v;
+    uint8_t* k_scale;
+    uint8_t* v_scale;
+    int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
+    int64_t ks_page, ks_block, ks_head, vs_page, vs_block, vs_head;
+    int32_t pages, page, blocks, heads, dim;
+} sq_cache8;
+
+/* Keys and values of new tokens (k->in, v->in, strides multiples of 8, 16-byte aligned; dtype SQ_F16 or SQ_BF16) put into the cache.  Sequence b has
+ * lens[b] cached tokens; its new token t (row starts[b] + t; starts NULL: most_new tokens each) goes to slot lens[b] + t.  For each block that gets new
+ * tokens, and head:  a = the largest finite magnitude of its new tokens,  e = the smallest integer, -100 or more, with a <= 448 * 2^e, and
+ * where the block holds tokens before lens[b], not less than its e; those are scaled to it where it grows (exact, but for codes
+ * that fall below 2^-6: rounded to nearest even).  A code is x * 2^-e rounded to nearest even.  Elements that are not finite are held as NaN; |x| above 1.875 * 2^15 (fp16),
+ * 1.875 * 2^127 (bf16) as that, so that what is read is finite in dtype.  New tokens from the most_new-th of a sequence on, whose slot lies behind the
+ * table row, or whose page is not in the cache are not put anywhere.  Sequences must not share pages that are written. */
+int sq_put_tokens8(const sq_heads* k, const sq_heads* v, int32_t tokens, int dtype, const sq_cache8* cache, const int32_t* table, int64_t ld_table, int32_t max_pages,
+                   const int32_t* lens, const int32_t* starts, int32_t seqs, int32_t most_new, void* stream);
+
+/* sq_keep_drafted on such caches (k_layer, v_layer, ks_layer, vs_layer bytes from layer to layer).  A block that rows move to has the largest scale of those rows
+ * and, where it holds cached tokens, its own; codes are scaled to it as by sq_put_tokens8. */
+int sq_keep_drafted8(const sq_cache8* cache, int32_t layers, int64_t k_layer, int64_t v_layer, int64_t ks_layer, int64_t vs_layer, const int32_t* table, int64_t ld_table,
+                     int32_t max_pages, const int32_t* lens, const int32_t* path, int64_t ld_path, int32_t most, const int32_t* counts, int32_t seqs, void* stream);
+
+/* sq_plane: one array of a cache of any type, in bytes: row r of page p, head h, layer l at `at` + l * layer + p * page + r * row + h * head, `bytes` long.
+ * rows: the slots of a page, or its blocks of tokens (a divisor of the slots), of which row r holds slots r * slots / rows on.  Planes do not overlap.
+ *
+ * sq_fork_pages: a new batch of `rows` sequences whose i-th goes on where sequence parent[i] of the old one is (any number of them where one is):
+ * out_lens[i] = lens[parent[i]], and row i of out_table is the parent's row, where fresh[i] < 0; otherwise its whole pages, then fresh[i] in place of the page that slot
+ * lens[parent[i]] is in, whose slots in use are copied to page fresh[i] in all planes and layers, then -1.  A parent outside the old
+ * batch: a row of -1, length 0.  Pages outside the cache are neither read nor written.  The pages fresh[i] >= 0 are distinct and no old sequence's.  out_table and out_lens do not
+ * overlap table and lens. */
+typedef struct sq_plane {
+    void* at;
+    int64_t layer, page, row, head;
+    int32_t rows, heads, bytes;
+} sq_plane;
+int sq_fork_pages(const sq_plane* planes, int32_t n_planes, int32_t layers, int32_t pages, int32_t page, const int32_t* table, int64_t ld_table, int32_t max_pages,
+                  const int32_t* lens, int32_t seqs, const int32_t* parent, const int32_t* fresh, int32_t rows, int32_t* out_table, int64_t ld_out, int32_t* out_lens,
+                  void* stream);
+
+/* Pages freed: those that hold none of the first lens[b] slots of any sequence.  With n pages in use, those from n on move to the free ones before n, in
+ * ascending order, in all planes and layers; out_table names the new places, -1 behind a sequence's pages; used[0] = n: pages n .. are free.  Sequences may
+ * share pages.  Entries outside the cache stay as they are.  Pages: up to 2^20.  The workspace (256-byte aligned) needs no
+ * preparation and is the call's own while it runs.  out_table does not overlap table. */
+int sq_compact_pages(const sq_plane* planes, int32_t n_planes, int32_t layers, int32_t pages, int32_t page, const int32_t* table, int64_t ld_table, int32_t max_pages,
+                     const int32_t* lens, int32_t seqs, int32_t* out_table, int64_t ld_out, int32_t* used, void* workspace, size_t ws_bytes, void* stream);
+size_t sq_compact_pages_workspace_bytes(int32_t pages);
+
 #ifdef __cplusplus
 }
 #endif

@@ -66,6 +66,19 @@ class SqAttention(ctypes.Structure):
                [(n, ctypes.c_int32) for n in ("tokens", "seqs", "most_new", "q_heads", "max_pages", "mask_words")] + [("scale", ctypes.c_float)]
 
 
+class SqCache8(ctypes.Structure):
+    """struct sq_cache8 of include/sqhip.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + \
+               [(n, ctypes.c_int64) for n in ("k_page", "k_slot", "k_head", "v_page", "v_slot", "v_head",
+                                              "ks_page", "ks_block", "ks_head", "vs_page", "vs_block", "vs_head")] + \
+               [(n, ctypes.c_int32) for n in ("pages", "page", "blocks", "heads", "dim")]
+
+
+class SqPlane(ctypes.Structure):
+    """struct sq_plane of include/sqhip.h."""
+    _fields_ = [("at", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("layer", "page", "row", "head")] + [(n, ctypes.c_int32) for n in ("rows", "heads", "bytes")]
+
+
 class SqError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"sqhip error {code}: {msg}")
@@ -159,7 +172,14 @@ def lib() -> ctypes.CDLL:
         L.sq_tree_attention_workspace_bytes.argtypes = [ctypes.POINTER(SqAttention), cp]
         L.sq_tree_attention_workspace_bytes.restype = sz
         L.sq_keep_drafted.argtypes = [cp, i32, i64, i64, vp, i64, i32, vp, vp, i64, i32, vp, i32, vp]
-        for f in (L.sq_rotary, L.sq_qk_norm_rotary, L.sq_tree_attention, L.sq_keep_drafted):
+        c8 = ctypes.POINTER(SqCache8)
+        L.sq_put_tokens8.argtypes = [hp, hp, i32, ctypes.c_int, c8, vp, i64, i32, vp, vp, i32, i32, vp]
+        L.sq_keep_drafted8.argtypes = [c8, i32, i64, i64, i64, i64, vp, i64, i32, vp, vp, i64, i32, vp, i32, vp]
+        L.sq_fork_pages.argtypes = [ctypes.POINTER(SqPlane), i32, i32, i32, i32, vp, i64, i32, vp, i32, vp, vp, i32, vp, i64, vp, vp]
+        L.sq_compact_pages.argtypes = [ctypes.POINTER(SqPlane), i32, i32, i32, i32, vp, i64, i32, vp, i32, vp, i64, vp, vp, sz, vp]
+        L.sq_compact_pages_workspace_bytes.argtypes = [i32]
+        L.sq_compact_pages_workspace_bytes.restype = sz
+        for f in (L.sq_rotary, L.sq_qk_norm_rotary, L.sq_tree_attention, L.sq_keep_drafted, L.sq_put_tokens8, L.sq_keep_drafted8, L.sq_fork_pages, L.sq_compact_pages):
             f.restype = ctypes.c_int
         for f in (L.sq_dequant, L.sq_dequant_stack, L.sq_linear_small, L.sq_linear_gemm, L.sq_gemm_dense, L.sq_q8_linear, L.sq_q8_dequant,
                   L.sq_q4_embed, L.sq_addnorm, L.sq_silu_mul, L.sq_linear_small_from, L.sq_linear_small_silu, L.sq_workspace_status,
@@ -177,7 +197,8 @@ EXPORTS = ("sq_version", "sq_last_error", "sq_dequant", "sq_dequant_stack", "sq_
            "sq_stream_bytes_books", "sq_stream_build_books", "sq_codebook_balance_books", "sq_stream_counts_bytes", "sq_stream_plan_device",
            "sq_stream_fill_device", "sq_stream_fill_stack_device", "sq_stream_plan_free", "sq_codebook_balance_device", "sq_codebook_relabel_device",
            "sq_codebook_rebalance_bytes", "sq_codebook_rebalance_device", "sq_rotary", "sq_qk_norm_rotary", "sq_tree_attention",
-           "sq_tree_attention_workspace_bytes", "sq_keep_drafted")
+           "sq_tree_attention_workspace_bytes", "sq_keep_drafted", "sq_put_tokens8", "sq_keep_drafted8", "sq_fork_pages", "sq_compact_pages",
+           "sq_compact_pages_workspace_bytes")
 
 
 _native = None

@@ -709,6 +709,183 @@ PyObject* keep_drafted(PyObject*, PyObject* const* a, Py_ssize_t n) {
     )
 }
 
+// ------------------------------------------------------------------------------------------ 8-bit caches, pages
+
+// the last dimensions of an 8-bit cache's four tensors, for a call that takes these numbers of dimensions; not where they are written and expanded
+bool cache8_of(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs, int dev, bool stacked, bool written, sq_cache8& c) {
+    const int d = (int)k.dim(); const int e = d - 1;
+    if ((d != 4 && !(stacked && d == 5)) || k.sizes() != v.sizes() || ks.dim() != e || ks.sizes() != vs.sizes() || k.numel() == 0 || ks.numel() == 0) return false;
+    const at::Tensor* every[4] = {&k, &v, &ks, &vs};         // (one tensor given twice is one address twice)
+    for (int j = 0; j < 4; ++j) {
+        const at::Tensor& t = *every[j];
+        if (t.scalar_type() != (j < 2 ? at::kFloat8_e4m3fn : at::kFloat8_e8m0fnu) || !plain_on(t, dev)) return false;
+        for (int i = 0; written && i < t.dim(); ++i) if (t.stride(i) == 0 && t.size(i) > 1) return false;
+        for (int i = 0; written && i < j; ++i) if (every[i]->data_ptr() == t.data_ptr()) return false;
+    }
+    if ((k.stride(d - 1) != 1 && k.size(d - 1) > 1) || (v.stride(d - 1) != 1 && v.size(d - 1) > 1)) return false;
+    for (int i = 0; i < d - 3; ++i) if (ks.size(i) != k.size(i)) return false;
+    for (int i = 0; i < d; ++i) if (k.size(i) > INT32_MAX) return false;
+    if (ks.size(e - 1) != k.size(d - 2) || k.size(d - 3) % ks.size(e - 2)) return false;
+    c = {k.data_ptr(), v.data_ptr(), (uint8_t*)ks.data_ptr(), (uint8_t*)vs.data_ptr(), k.stride(d - 4), k.stride(d - 3), k.stride(d - 2), v.stride(d - 4), v.stride(d - 3), v.stride(d - 2),
+         ks.stride(e - 3), ks.stride(e - 2), ks.stride(e - 1), vs.stride(e - 3), vs.stride(e - 2), vs.stride(e - 1),
+         (int32_t)k.size(d - 4), (int32_t)k.size(d - 3), (int32_t)ks.size(e - 2), (int32_t)k.size(d - 2), (int32_t)k.size(d - 1)};
+    return true;
+}
+// a batch of sequences: lens, table and, or NULL, starts
+bool batch_on(const at::Tensor& table, const at::Tensor& lens, const at::Tensor* starts, int dev) {
+    if (lens.dim() != 1 || lens.size(0) < 1 || lens.size(0) > INT32_MAX) return false;
+    const int64_t b = lens.size(0);
+    return vector_on(lens, dev, b, at::kInt, at::kInt) && rows_on(table, dev, b, at::kInt) && table.size(1) <= INT32_MAX && (!starts || vector_on(*starts, dev, b + 1, at::kInt, at::kInt));
+}
+int64_t table_ld(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+// the most new tokens of a sequence, of `rows` in all; -1: not covered
+int64_t most_of(PyObject* o, const at::Tensor* starts, int64_t rows, int64_t b) {
+    if (!starts && rows % b) return -1;
+    int64_t most = starts ? rows : rows / b;
+    if (o != Py_None) most = starts ? std::min<int64_t>(PyLong_AsLongLong(o), rows) : PyLong_AsLongLong(o);
+    return most < 0 || most > INT32_MAX || (!starts && most * b != rows) ? -1 : most;
+}
+
+// put_tokens8(k, v, k_cache, v_cache, k_scale, v_scale, table, lens, starts, most_new)
+PyObject* put_tokens8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const at::Tensor* starts;
+    if (n != 10 || !tensors(a, 8) || !maybe(a[8], starts)) return answer(NOT_COVERED);
+    SQ_GUARD(
+        const at::Tensor& k = THPVariable_Unpack(a[0]);
+        const at::Tensor& v = THPVariable_Unpack(a[1]);
+        const at::Tensor& table = THPVariable_Unpack(a[6]);
+        const at::Tensor& lens = THPVariable_Unpack(a[7]);
+        if (k.dim() != 3 || !k.is_cuda() || k.numel() == 0 || k.numel() > INT32_MAX || v.dim() != 3) return answer(NOT_COVERED);
+        const int dev = k.get_device(); const int dt = dtype_of(k);
+        sq_cache8 c;
+        if (!heads_on(k, dev) || !heads_on(v, dev) || !is16(dt) || v.scalar_type() != k.scalar_type() || v.sizes() != k.sizes() || !batch_on(table, lens, starts, dev) ||
+            !cache8_of(THPVariable_Unpack(a[2]), THPVariable_Unpack(a[3]), THPVariable_Unpack(a[4]), THPVariable_Unpack(a[5]), dev, false, true, c) ||
+            c.heads != k.size(1) || c.dim != k.size(2))
+            return answer(NOT_COVERED);
+        for (int i = 2; i < 6; ++i)
+            if (!apart(THPVariable_Unpack(a[i]), k) || !apart(THPVariable_Unpack(a[i]), v)) return answer(NOT_COVERED);
+        const int64_t most = most_of(a[9], starts, k.size(0), lens.size(0));
+        if (PyErr_Occurred()) return nullptr;
+        if (most < 0) return answer(NOT_COVERED);
+        OnDevice on(dev);
+        const sq_heads hk = part_of(k, nullptr, nullptr); const sq_heads hv = part_of(v, nullptr, nullptr);
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = sq_put_tokens8(&hk, &hv, (int)k.size(0), dt, &c, (const int32_t*)table.data_ptr(), table_ld(table), (int)table.size(1), (const int32_t*)lens.data_ptr(),
+                            starts ? (const int32_t*)starts->data_ptr() : nullptr, (int)lens.size(0), (int)most, on.stream);
+        Py_END_ALLOW_THREADS
+        return answer(rc);
+    )
+}
+
+// keep_drafted8(k_cache, v_cache, k_scale, v_scale, table, lens, path, counts)
+PyObject* keep_drafted8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 8 || !tensors(a, 8)) return answer(NOT_COVERED);
+    SQ_GUARD(
+        const at::Tensor& kc = THPVariable_Unpack(a[0]);
+        const at::Tensor& table = THPVariable_Unpack(a[4]);
+        const at::Tensor& lens = THPVariable_Unpack(a[5]);
+        const at::Tensor& path = THPVariable_Unpack(a[6]);
+        const at::Tensor& counts = THPVariable_Unpack(a[7]);
+        if (!kc.is_cuda()) return answer(NOT_COVERED);
+        const int dev = kc.get_device();
+        sq_cache8 c;
+        if (!batch_on(table, lens, nullptr, dev) || !vector_on(counts, dev, lens.size(0), at::kInt, at::kInt) || !rows_on(path, dev, lens.size(0), at::kInt) || path.size(1) > INT32_MAX ||
+            !cache8_of(kc, THPVariable_Unpack(a[1]), THPVariable_Unpack(a[2]), THPVariable_Unpack(a[3]), dev, true, true, c))
+            return answer(NOT_COVERED);
+        const bool stacked = kc.dim() == 5;
+        auto step = [&](int i) { return stacked ? THPVariable_Unpack(a[i]).stride(0) : 0; };
+        OnDevice on(dev);
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = sq_keep_drafted8(&c, stacked ? (int)kc.size(0) : 1, step(0), step(1), step(2), step(3), (const int32_t*)table.data_ptr(), table_ld(table), (int)table.size(1),
+                              (const int32_t*)lens.data_ptr(), (const int32_t*)path.data_ptr(), table_ld(path), (int)path.size(1), (const int32_t*)counts.data_ptr(), (int)lens.size(0),
+                              on.stream);
+        Py_END_ALLOW_THREADS
+        return answer(rc);
+    )
+}
+
+// caches and, or NULL, scales as planes
+struct Planes { sq_plane p[4]; int n = 0, layers, pages, page; };
+bool planes_of(const at::Tensor& k, const at::Tensor& v, const at::Tensor* ks, const at::Tensor* vs, int dev, Planes& o) {
+    const int d = (int)k.dim();
+    if ((d != 4 && d != 5) || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type() || k.numel() == 0 || (ks != nullptr) != (vs != nullptr)) return false;
+    if (ks && (ks->dim() != d - 1 || ks->sizes() != vs->sizes() || ks->scalar_type() != vs->scalar_type() || ks->numel() == 0)) return false;
+    for (int i = 0; i < d; ++i) if (k.size(i) > INT32_MAX) return false;
+    for (int i = 0; ks && i < d - 3; ++i) if (ks->size(i) != k.size(i)) return false;
+    o.layers = d == 5 ? (int)k.size(0) : 1; o.pages = (int)k.size(d - 4); o.page = (int)k.size(d - 3);
+    const at::Tensor* every[4] = {&k, &v, ks, vs};
+    for (int j = 0; j < 4 && every[j]; ++j) {
+        const at::Tensor* t = every[j];
+        const bool code = j < 2; const int64_t size = t->element_size(); const int e = (int)t->dim() - (code ? 4 : 3);
+        if (!plain_on(*t, dev) || (code && t->stride(e + 3) != 1 && t->size(e + 3) > 1) || t->size(e + 2) > INT32_MAX) return false;
+        for (int i = 0; i < t->dim(); ++i) if (t->stride(i) == 0 && t->size(i) > 1) return false;
+        for (int i = 0; i < o.n; ++i) if (o.p[i].at == t->data_ptr()) return false;
+        if (o.page % t->size(e + 1)) return false;
+        o.p[o.n++] = {t->data_ptr(), e ? t->stride(0) * size : 0, t->stride(e) * size, t->stride(e + 1) * size, t->stride(e + 2) * size, (int32_t)t->size(e + 1),
+                      (int32_t)t->size(e + 2), (int32_t)((code ? t->size(e + 3) : 1) * size)};
+    }
+    return true;
+}
+
+// fork_pages(k_cache, v_cache, table, lens, parent, pages, k_scale, v_scale, out_table, out_lens) -> (table, lens), or a code
+PyObject* fork_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const at::Tensor *ks, *vs, *given, *given_lens;
+    if (n != 10 || !tensors(a, 6) || !maybe(a[6], ks) || !maybe(a[7], vs) || !maybe(a[8], given) || !maybe(a[9], given_lens)) return answer(NOT_COVERED);
+    SQ_GUARD(
+        const at::Tensor& kc = THPVariable_Unpack(a[0]);
+        const at::Tensor& table = THPVariable_Unpack(a[2]);
+        const at::Tensor& lens = THPVariable_Unpack(a[3]);
+        const at::Tensor& parent = THPVariable_Unpack(a[4]);
+        const at::Tensor& pages = THPVariable_Unpack(a[5]);
+        if (!kc.is_cuda() || parent.dim() != 1 || parent.size(0) < 1 || parent.size(0) > INT32_MAX || given || given_lens) return answer(NOT_COVERED);
+        const int dev = kc.get_device(); const int64_t r = parent.size(0);
+        Planes p;
+        if (!batch_on(table, lens, nullptr, dev) || !vector_on(parent, dev, r, at::kInt, at::kInt) || !vector_on(pages, dev, r, at::kInt, at::kInt) ||
+            !planes_of(kc, THPVariable_Unpack(a[1]), ks, vs, dev, p))
+            return answer(NOT_COVERED);
+        OnDevice on(dev);
+        at::Tensor out = at::empty({r, table.size(1)}, lens.options()); at::Tensor out_lens = at::empty({r}, lens.options());
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = sq_fork_pages(p.p, p.n, p.layers, p.pages, p.page, (const int32_t*)table.data_ptr(), table_ld(table), (int)table.size(1), (const int32_t*)lens.data_ptr(), (int)lens.size(0),
+                           (const int32_t*)parent.data_ptr(), (const int32_t*)pages.data_ptr(), (int)r, (int32_t*)out.data_ptr(), table.size(1), (int32_t*)out_lens.data_ptr(), on.stream);
+        Py_END_ALLOW_THREADS
+        if (rc) return answer(rc);
+        return pybind11::make_tuple(pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::move(out))),
+                                    pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::move(out_lens)))).release().ptr();
+    )
+}
+
+// compact_pages(k_cache, v_cache, table, lens, k_scale, v_scale, out_table) -> (table, used), or a code
+PyObject* compact_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const at::Tensor *ks, *vs, *given;
+    if (n != 7 || !tensors(a, 4) || !maybe(a[4], ks) || !maybe(a[5], vs) || !maybe(a[6], given)) return answer(NOT_COVERED);
+    SQ_GUARD(
+        const at::Tensor& kc = THPVariable_Unpack(a[0]);
+        const at::Tensor& table = THPVariable_Unpack(a[2]);
+        const at::Tensor& lens = THPVariable_Unpack(a[3]);
+        if (!kc.is_cuda() || given) return answer(NOT_COVERED);
+        const int dev = kc.get_device();
+        Planes p;
+        if (!batch_on(table, lens, nullptr, dev) || !planes_of(kc, THPVariable_Unpack(a[1]), ks, vs, dev, p)) return answer(NOT_COVERED);
+        OnDevice on(dev);
+        // (a workspace of the call's own: streams and captured graphs run side by side)
+        const size_t need = sq_compact_pages_workspace_bytes(p.pages);
+        at::Tensor out = at::empty({lens.size(0), table.size(1)}, lens.options()); at::Tensor used = at::empty({1}, lens.options());
+        at::Tensor ws = at::empty({(int64_t)need}, lens.options().dtype(at::kByte));
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = sq_compact_pages(p.p, p.n, p.layers, p.pages, p.page, (const int32_t*)table.data_ptr(), table_ld(table), (int)table.size(1), (const int32_t*)lens.data_ptr(),
+                              (int)lens.size(0), (int32_t*)out.data_ptr(), table.size(1), (int32_t*)used.data_ptr(), ws.data_ptr(), need, on.stream);
+        Py_END_ALLOW_THREADS
+        if (rc) return answer(rc);
+        return pybind11::make_tuple(pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::move(out))),
+                                    pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::move(used)))).release().ptr();
+    )
+}
+
 // ------------------------------------------------------------------------------------------ torch.ops.shapequant.linear
 
 at::Tensor linear_op(const at::Tensor& x, int64_t handle) {
@@ -771,6 +948,7 @@ PyObject* install_op(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {{"native", (PyCFunction)(void (*)(void))make_native, METH_FASTCALL, nullptr}, {"install", install, METH_O, nullptr}, SQ_FAST(install_op),
                          SQ_FAST(linear), SQ_FAST(forward), SQ_FAST(linear_from), SQ_FAST(linear_silu), SQ_FAST(addnorm), SQ_FAST(silu_mul), SQ_FAST(q8_linear), SQ_FAST(q4_rows),
                          SQ_FAST(rotary), SQ_FAST(qk_norm_rotary), SQ_FAST(tree_attention), SQ_FAST(keep_drafted),
+                         SQ_FAST(put_tokens8), SQ_FAST(keep_drafted8), SQ_FAST(fork_pages), SQ_FAST(compact_pages),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods};
 
