@@ -888,7 +888,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
         for (const int all = mine >= rows ? begin : min(max(whole / KEYS, begin), end); next < all; ++next) plain(next, std::false_type());
     for (; next < end; ++next) plain(next, std::true_type());
     int* flags = reinterpret_cast<int*>(smem + NB * STAGE);
-    if (lane == 0) flags[wave] = __any(pages.bad) || s.over;
+    const bool wrong = __any(pages.bad) || s.over;           // (of all lanes: each looks up a key of its own)
+    if (lane == 0) flags[wave] = wrong;
     __syncthreads();
     bool bad = false;
 #pragma unroll
