@@ -514,6 +514,11 @@ typedef struct sq_cache8 {
 int sq_put_tokens8(const sq_heads* k, const sq_heads* v, int32_t tokens, int dtype, const sq_cache8* cache, const int32_t* table, int64_t ld_table, int32_t max_pages,
                    const int32_t* lens, const int32_t* starts, int32_t seqs, int32_t most_new, void* stream);
 
+/* sq_tree_attention over such a cache: the same rows, masks, results, rounding and workspace rules, q and out of `dtype`.  Keys and values are code * scale as numbers
+ * of dtype: exact in bf16, and in fp16 for what sq_put_tokens8 made of fp16 tokens (others: rounded to its steps of 2^-24, infinite beyond its range). */
+int sq_tree_attention8(const sq_attention* a, const sq_cache8* cache, int dtype, void* workspace, size_t ws_bytes, void* stream);
+size_t sq_tree_attention8_workspace_bytes(const sq_attention* a, const sq_cache8* cache, int dtype);
+
 /* sq_keep_drafted on such caches (k_layer, v_layer, ks_layer, vs_layer bytes from layer to layer).  A block that rows move to has the largest scale of those rows
  * and, where it holds cached tokens, its own; codes are scaled to it as by sq_put_tokens8. */
 int sq_keep_drafted8(const sq_cache8* cache, int32_t layers, int64_t k_layer, int64_t v_layer, int64_t ks_layer, int64_t vs_layer, const int32_t* table, int64_t ld_table,

@@ -179,7 +179,10 @@ def lib() -> ctypes.CDLL:
         L.sq_compact_pages.argtypes = [ctypes.POINTER(SqPlane), i32, i32, i32, i32, vp, i64, i32, vp, i32, vp, i64, vp, vp, sz, vp]
         L.sq_compact_pages_workspace_bytes.argtypes = [i32]
         L.sq_compact_pages_workspace_bytes.restype = sz
-        for f in (L.sq_rotary, L.sq_qk_norm_rotary, L.sq_tree_attention, L.sq_keep_drafted, L.sq_put_tokens8, L.sq_keep_drafted8, L.sq_fork_pages, L.sq_compact_pages):
+        L.sq_tree_attention8.argtypes = [ctypes.POINTER(SqAttention), c8, ctypes.c_int, vp, sz, vp]
+        L.sq_tree_attention8_workspace_bytes.argtypes = [ctypes.POINTER(SqAttention), c8, ctypes.c_int]
+        L.sq_tree_attention8_workspace_bytes.restype = sz
+        for f in (L.sq_rotary, L.sq_qk_norm_rotary, L.sq_tree_attention, L.sq_keep_drafted, L.sq_tree_attention8, L.sq_put_tokens8, L.sq_keep_drafted8, L.sq_fork_pages, L.sq_compact_pages):
             f.restype = ctypes.c_int
         for f in (L.sq_dequant, L.sq_dequant_stack, L.sq_linear_small, L.sq_linear_gemm, L.sq_gemm_dense, L.sq_q8_linear, L.sq_q8_dequant,
                   L.sq_q4_embed, L.sq_addnorm, L.sq_silu_mul, L.sq_linear_small_from, L.sq_linear_small_silu, L.sq_workspace_status,
@@ -197,7 +200,8 @@ EXPORTS = ("sq_version", "sq_last_error", "sq_dequant", "sq_dequant_stack", "sq_
            "sq_stream_bytes_books", "sq_stream_build_books", "sq_codebook_balance_books", "sq_stream_counts_bytes", "sq_stream_plan_device",
            "sq_stream_fill_device", "sq_stream_fill_stack_device", "sq_stream_plan_free", "sq_codebook_balance_device", "sq_codebook_relabel_device",
            "sq_codebook_rebalance_bytes", "sq_codebook_rebalance_device", "sq_rotary", "sq_qk_norm_rotary", "sq_tree_attention",
-           "sq_tree_attention_workspace_bytes", "sq_keep_drafted", "sq_put_tokens8", "sq_keep_drafted8", "sq_fork_pages", "sq_compact_pages",
+           "sq_tree_attention_workspace_bytes", "sq_keep_drafted", "sq_put_tokens8", "sq_tree_attention8", "sq_tree_attention8_workspace_bytes",
+           "sq_keep_drafted8", "sq_fork_pages", "sq_compact_pages",
            "sq_compact_pages_workspace_bytes")
 
 

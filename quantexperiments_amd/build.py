@@ -15,7 +15,7 @@ SOURCES = ["sq_api.hip", "sq_dequant.hip", "sq_planes.hip", "sq_plane_product.hi
            "sq_gemv_b12d4.hip", "sq_gemv_b10d4.hip", "sq_gemv_b8d4.hip", "sq_gemm.hip", "sq_gemm256.hip", "sq_stream.hip", "sq_stream_build.hip", "sq_relabel.hip",
            "sq_q8.hip", "sq_neighbours.hip", "sq_segs.hip", "sq_sieve.hip", "sq_mid.hip", "sq_mid_b16d8.hip", "sq_mid_b12d4.hip", "sq_mid_b10d4.hip", "sq_mid_b8d4.hip",
            "sq_mid_dense.hip", "sq_fused.hip", "sq_fused_b16d8.hip", "sq_fused_b12d4.hip", "sq_fused_b10d4.hip", "sq_fused_b8d4.hip", "sq_heads.hip", "sq_attention.hip", "sq_attention_f16.hip", "sq_attention_bf16.hip",
-           "sq_cache8.hip", "sq_pages.hip"]
+           "sq_attention8.hip", "sq_attention8_f16.hip", "sq_attention8_bf16.hip", "sq_cache8.hip", "sq_pages.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 

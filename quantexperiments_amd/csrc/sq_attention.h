@@ -240,6 +240,58 @@ __device__ __forceinline__ void attn_copy_group(const AttnArgs& a, int where, in
     }
 }
 
+// ------------------------------------------------------------------------------------------ a cache held in 8 bits (sq_tree_attention8)
+
+// Keys and values as e4m3 codes with a power of two for each block of tokens and head.  Strides of the cache are its bytes.
+struct Attn8Args : AttnArgs {
+    const uint8_t *ks, *vs;
+    int64_t ks_page, ks_block, ks_head, vs_page, vs_block, vs_head;
+    int size;                    // tokens of a block, a multiple of 16
+};
+
+// 8 codes times a power of two as a matrix instruction's operand: v_cvt_scalef32_pk takes two at a time and the scale with them, exactly
+template <int DT> __device__ __forceinline__ u32x4 attn8_unpack(uint32_t x, uint32_t y, float sx, float sy) {
+    if constexpr (DT == SQ_F16)
+        return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, sx, false)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, sx, true)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, sy, false)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, sy, true))};
+    else
+        return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, sx, false)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, sx, true)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, sy, false)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, sy, true))};
+}
+__device__ __forceinline__ float attn8_scale(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
+
+// Where 64 groups of keys lie that a wave copies one after the other (lane l: the l-th, `step` keys after the one before), and their scales.  A group's keys are in
+// one block, so in one page.  Groups from key `limit` on: the first page, whose slots may be read as well, scale 1.
+struct Attn8Groups {
+    int window = 1 << 30;        // the first one's number
+    int64_t k, v;                // bytes from the head's first
+    uint32_t scales;             // of keys, of values in the second byte
+    bool bad = false;
+
+    __device__ __forceinline__ void find(const Attn8Args& a, int b, int head, int number, int key, int step, int limit, int lane) {
+        window = number;
+        const int64_t at = key + (int64_t)lane * step;
+        int id = 0, off = 0;
+        bool there = at < limit;
+        if (there) {
+            const int pg = (int)((uint32_t)at / (uint32_t)a.page);
+            off = (int)at - pg * a.page;
+            id = a.table[(int64_t)b * a.ld_table + pg];
+            if ((uint32_t)id >= (uint32_t)a.pages) there = false, bad = true, id = 0, off = 0;
+        }
+        k = id * a.k_page + off * a.k_slot;
+        v = id * a.v_page + off * a.v_slot;
+        const int block = off / a.size;
+        scales = there ? a.ks[id * a.ks_page + block * a.ks_block + head * a.ks_head] | (uint32_t)a.vs[id * a.vs_page + block * a.vs_block + head * a.vs_head] << 8 : 0x7F7Fu;
+    }
+    static __device__ __forceinline__ int64_t lane64(int64_t x, int l) {
+        return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, l) | (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32;
+    }
+    __device__ __forceinline__ int64_t key_at(int number) const { return lane64(k, number - window); }
+    __device__ __forceinline__ int64_t value_at(int number) const { return lane64(v, number - window); }
+    __device__ __forceinline__ uint32_t scales_at(int number) const { return __builtin_amdgcn_readlane((int)scales, number - window); }
+};
+
 // What a wave keeps of its MT * 16 rows
 template <int DP, int MT> struct AttnRows {
     u32x4 q[MT][DP / 32];
@@ -261,7 +313,8 @@ template <int DP, int MT> struct AttnRows {
     }
 };
 
-template <int DP, int MT>
+// (PAIRS: an operand of keys is 8 of the 16 elements that a lane reads of a key at once, the next one the others)
+template <int DP, int MT, bool PAIRS = false>
 __device__ __forceinline__ void attn_rows_begin(const AttnArgs& a, const AttnSeq& s, int head, int row0, int lane, AttnRows<DP, MT>& r) {
     const int rows = s.n * a.group;
     r.far = true;
@@ -274,7 +327,7 @@ __device__ __forceinline__ void attn_rows_begin(const AttnArgs& a, const AttnSeq
         r.l[t] = 0.f;
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
-            const int e = c * 32 + (lane >> 4) * 8;
+            const int e = PAIRS ? (c >> 1) * 64 + (lane >> 4) * 16 + (c & 1) * 8 : c * 32 + (lane >> 4) * 8;
             r.q[t][c] = e < a.dim ? *reinterpret_cast<const u32x4*>(q + e * 2) : u32x4{0u, 0u, 0u, 0u};
         }
 #pragma unroll
@@ -635,6 +688,10 @@ constexpr int attn_stage_steps(int dp, int nw) { return dp == 256 || nw == 4 ? 1
 constexpr int ATTN_STAGES = 4;
 template <int DP, int NW> constexpr int attn_stage_bytes() { return attn_stage_steps(DP, NW) * 2 * AttnTile<DP>::BYTES; }
 template <int DP, int NW> constexpr int attn_tile_lds() { return ATTN_STAGES * attn_stage_bytes<DP, NW>() + 64; }
+// Over a cache held in 8 bits: stages of 16 bits in LDS, stages of codes on their way to them (each wave's own part, half as many bytes)
+constexpr int ATTN8_STAGES = 3, ATTN8_RAW = 3;
+template <int DP, int NW> constexpr int attn8_copies() { return (attn_stage_steps(DP, NW) * ATTN_STEP / NW * DP + 1023) / 1024; }      // of a wave's keys of a stage
+template <int DP, int NW> constexpr int attn8_tile_lds() { return ATTN8_STAGES * attn_stage_bytes<DP, NW>() + ATTN8_RAW * NW * 2048 * attn8_copies<DP, NW>() + 64; }
 
 // In which order a region's instructions are issued: N times one matrix instruction, D LDS reads, V vector instructions, X exponentials
 template <int N, int V, int X, int D> __device__ __forceinline__ void attn_order() {
@@ -665,14 +722,17 @@ __device__ __forceinline__ float attn_most(float4v x, float4v y) {
 // The stages at a sequence's end that some row does not see whole go step by step, behind the pipeline, and all of them (those that every row sees without masks) for
 // heads wider than 128 elements, whose keys and values would take the registers of four tiles.  There a wave has one tile, so a key's pieces are read from LDS once per 16 rows: 256 KB a
 // stage for eight waves, 2048 cycles at 128 bytes each, beside 1024 of matrix instructions (1000 tokens of 20 heads of 256 behind 2100: 133 us, 97 stages of some 3000 cycles).
-template <int DT, int DP, int NW, bool FULL>
-__global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
+// Over a cache held in 8 bits (Attn8Args) each wave copies its part of a stage as codes to a place of its own, and unpacks it into the stage, scaled,
+// before the barrier that lets all waves read it; all that follows is the same.
+template <int DT, int DP, int NW, bool FULL, typename ARGS = AttnArgs>
+__global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(ARGS a) {
     typedef AttnTile<DP> T;
     typedef AttnType<DT> E;
     typedef short short4v __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) short4v* tr_ptr;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    constexpr int MT = attn_tiles(DP), SK = attn_stage_steps(DP, NW), KEYS = SK * ATTN_STEP, NB = ATTN_STAGES, STAGE = attn_stage_bytes<DP, NW>(), ROWS = NW * MT * 16;
+    constexpr bool C8 = !std::is_same_v<ARGS, AttnArgs>;
+    constexpr int MT = attn_tiles(DP), SK = attn_stage_steps(DP, NW), KEYS = SK * ATTN_STEP, NB = C8 ? ATTN8_STAGES : ATTN_STAGES, STAGE = attn_stage_bytes<DP, NW>(), ROWS = NW * MT * 16;
     constexpr int MINE = KEYS / NW, C = MINE / T::ROWS, KC = DP / 32, VD = DP / 16;
     constexpr bool PIPELINE = MT >= 2;                       // (a tile's maximum is raised while the sums of the tile before it are outstanding)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, i16 = lane & 15;
@@ -703,8 +763,28 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     const bool easy = a.near && a.page % MINE == 0;
     AttnWalk walk;
     walk.begin(a, begin * KEYS + wave * MINE);
+    Attn8Groups held;
+    uint64_t coming = 0;                                     // scales of the stages on their way, 16 bits each, the newest on top
+    constexpr int C8N = attn8_copies<DP, NW>(), RAW = 2048 * C8N, P8 = DP / 16, ROWS8 = 64 / P8;          // (16-byte pieces of a key's codes, keys per copy)
+    char* raw = smem + NB * STAGE + 64 + wave * (ATTN8_RAW * RAW);
     auto place = [&](int i) __attribute__((always_inline)) { return smem + (i - begin) % NB * STAGE; };      // keys of SK steps, values of SK steps
     auto get = [&](int i) __attribute__((always_inline)) {           // this wave copies keys wave * MINE .. of a stage
+        if constexpr (C8) {
+            const int piece = lane % P8;
+            if (i < held.window || i >= held.window + 64) held.find(a, b, head, i, i * KEYS + wave * MINE, KEYS, min(s.total, end * KEYS), lane);
+            const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr)(raw + (i - begin) % ATTN8_RAW * RAW));
+            const int64_t k_at = held.key_at(i), v_at = held.value_at(i);
+#pragma unroll
+            for (int j = 0; j < C8N; ++j) {
+                const int row = j * ROWS8 + lane / P8;
+                if (row < MINE && (FULL || piece < a.dim >> 4)) {
+                    attn_copy16(to + j * 1024, kb + k_at, (uint32_t)(row * (int)a.k_slot + piece * 16));
+                    attn_copy16(to + RAW / 2 + j * 1024, vb + v_at, (uint32_t)(row * (int)a.v_slot + piece * 16));
+                }
+            }
+            coming = coming >> 16 | (uint64_t)held.scales_at(i) << (16 * (ATTN8_RAW - 1));
+            return;
+        }
         char* at = place(i) + wave * MINE * T::PITCH;
         const int first = i * KEYS + wave * MINE, in_step = wave * MINE % ATTN_STEP;
         if (easy && first + MINE <= s.total) {
@@ -719,6 +799,33 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
         attn_copy<DP, FULL, true, MINE>(a, s, first, in_step, lane, pages, vb, at + SK * T::BYTES);
     };
     auto arrive = [&](int i) __attribute__((always_inline)) {        // stage i is there
+        if constexpr (C8) {
+            // (the stage's place is that of the one three before it, which no wave reads behind the barrier of the one before it)
+            const int piece = lane % P8, ahead = ATTN8_RAW - min(end - i, ATTN8_RAW);      // (its place in `coming`)
+            if (i + ATTN8_RAW <= end) attn_wait<2 * C8N * (ATTN8_RAW - 1)>(); else attn_wait<0>();
+            const uint32_t sc = (uint32_t)(coming >> (16 * ahead));
+#pragma unroll
+            for (int j = 0; j < C8N; ++j) {
+                const int row = j * ROWS8 + lane / P8, key = (wave * MINE + row) % ATTN_STEP;
+                if (row < MINE && (FULL || piece < a.dim >> 4)) {
+                    const char* from = raw + (i - begin) % ATTN8_RAW * RAW + j * 1024 + lane * 16;
+                    char* to = place(i) + (wave * MINE + row) * T::PITCH;
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+                        const u32x4 w = *reinterpret_cast<const u32x4*>(from + v * (RAW / 2));
+                        const float by = attn8_scale(v ? sc >> 8 & 0xFF : sc & 0xFF);
+                        const int x = v ? T::v_xor(key) : T::k_xor(key);
+                        *reinterpret_cast<u32x4*>(to + v * (SK * T::BYTES) + ((2 * piece) ^ x) * 16) = attn8_unpack<DT>(w[0], w[1], by, by);
+                        *reinterpret_cast<u32x4*>(to + v * (SK * T::BYTES) + ((2 * piece + 1) ^ x) * 16) = attn8_unpack<DT>(w[2], w[3], by, by);
+                    }
+                }
+            }
+            attn_reads_done();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (i + ATTN8_RAW < end) get(i + ATTN8_RAW);
+            return;
+        }
         if (i + NB - 2 <= end) attn_wait<2 * C * (NB - 3)>(); else attn_wait<0>();
         attn_reads_done();
         __builtin_amdgcn_s_barrier();
@@ -730,7 +837,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
         __syncthreads();
     }
 #pragma unroll
-    for (int i = 0; i < NB - 2; ++i)
+    for (int i = 0; i < (C8 ? ATTN8_RAW : NB - 2); ++i)
         if (begin + i < end) get(begin + i);
     attn_rows_ready(r);
 
@@ -888,7 +995,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
         for (const int all = mine >= rows ? begin : min(max(whole / KEYS, begin), end); next < all; ++next) plain(next, std::false_type());
     for (; next < end; ++next) plain(next, std::true_type());
     int* flags = reinterpret_cast<int*>(smem + NB * STAGE);
-    const bool wrong = __any(pages.bad) || s.over;           // (of all lanes: each looks up a key of its own)
+    const bool wrong = __any(C8 ? held.bad : pages.bad) || s.over;          // (of all lanes: each looks up a key of its own)
     if (lane == 0) flags[wave] = wrong;
     __syncthreads();
     bool bad = false;
@@ -1044,18 +1151,22 @@ int attn_launch_many(const AttnArgs& a, unsigned grid, hipStream_t s) {
     return check_launch("sq_tree_attention");
 }
 
+template <int DT, int DP>
+int attn_launch_join(const AttnArgs& a, hipStream_t s) {
+    const int64_t all = (int64_t)a.seqs * a.most_new * a.q_heads;
+    constexpr int MOST = 1024 / DP;                          // parts of a row that fill a workgroup
+    if (a.splits > 8) hipLaunchKernelGGL((attn_join_kernel<DT, DP, MOST>), dim3((unsigned)all), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_join_kernel<DT, DP, 1>), dim3((unsigned)((all + MOST - 1) / MOST)), dim3(256), 0, s, a);
+    return check_launch("sq_tree_attention: join");
+}
+
 template <int DT, int DP, bool FULL>
 int attn_launch_dim(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
     const unsigned grid = (unsigned)((int64_t)a.seqs * a.kv_heads * ((p.row_blocks - 1) * p.splits + p.last_splits));
     int rc;
     if (p.nw) rc = p.nw == 4 ? attn_launch_many<DT, DP, 4, FULL>(a, grid, s) : attn_launch_many<DT, DP, 8, FULL>(a, grid, s);
     else rc = p.mt == 1 ? attn_launch_few<DT, DP, 1, FULL>(a, grid, s) : attn_launch_few<DT, DP, DP == 256 ? 1 : 2, FULL>(a, grid, s);
-    if (rc || p.splits == 1) return rc;
-    const int64_t all = (int64_t)a.seqs * a.most_new * a.q_heads;
-    constexpr int MOST = 1024 / DP;                          // parts of a row that fill a workgroup
-    if (a.splits > 8) hipLaunchKernelGGL((attn_join_kernel<DT, DP, MOST>), dim3((unsigned)all), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attn_join_kernel<DT, DP, 1>), dim3((unsigned)((all + MOST - 1) / MOST)), dim3(256), 0, s, a);
-    return check_launch("sq_tree_attention: join");
+    return rc || p.splits == 1 ? rc : attn_launch_join<DT, DP>(a, s);
 }
 
 template <int DT>
@@ -1066,6 +1177,12 @@ int attn_launch(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
     };
     return p.dp == 64 ? go(std::integral_constant<int, 64>()) : p.dp == 128 ? go(std::integral_constant<int, 128>()) : go(std::integral_constant<int, 256>());
 }
+// sq_attention.hip: what a call must be like, how it is cut, and everything of it that the kernels are told but the cache's own arrays
+int check_attention(const char* who, const sq_attention* a, const sq_cache* c);
+bool attn_nothing(const sq_attention& a);
+AttnPlan attn_plan(const sq_attention& a, const sq_cache& c);
+size_t attn_workspace(const sq_attention& a, const AttnPlan& p);
+int attn_prepare(const char* who, const sq_attention& a, const sq_cache& c, const AttnPlan& p, void* workspace, size_t ws_bytes, AttnArgs& k);
 bool rows_apart(int tokens, int heads, int64_t t, int64_t h, int dim);      // sq_heads.hip
 int attn_launch_f16(const AttnArgs& a, const AttnPlan& p, hipStream_t s);
 int attn_launch_bf16(const AttnArgs& a, const AttnPlan& p, hipStream_t s);

@@ -15,7 +15,7 @@ namespace sq {
 // (All times of captured calls, one behind the other; calls back to back take up to 4 % less.)
 // A sequence's length is its table's width here: lengths are on the device.  Under a table of 131,072 slots one token behind 500 takes 10.2 us instead of 8.8, 48 26.7 instead of 21.4,
 // 64 sequences of 500 27.9 instead of 18.6, 64 of 2000 59.8 instead of 53.1.
-static AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
+AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
     AttnPlan p;
     p.dp = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
     const int64_t rows = (int64_t)a.most_new * (a.q_heads / c.heads), steps = ((int64_t)a.max_pages * c.page + ATTN_STEP - 1) / ATTN_STEP;
@@ -55,7 +55,7 @@ static AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
     return p;
 }
 
-static int check_attention(const char* who, const sq_attention* a, const sq_cache* c) {
+int check_attention(const char* who, const sq_attention* a, const sq_cache* c) {
     if (!a || !c) return fail(SQ_EINVAL, "%s: null argument", who);
     if (c->dtype != SQ_F16 && c->dtype != SQ_BF16) return fail(SQ_EINVAL, "%s: dtype %d (fp16 or bf16)", who, c->dtype);
     if (c->dim < 8 || c->dim > 256 || c->dim % 8) return fail(SQ_EUNSUPPORTED, "%s: heads of %d elements (a multiple of 8 up to 256)", who, c->dim);
@@ -72,7 +72,36 @@ static int check_attention(const char* who, const sq_attention* a, const sq_cach
     return SQ_OK;
 }
 
-static bool attn_nothing(const sq_attention& a) { return a.tokens == 0 || a.seqs == 0 || a.most_new == 0; }
+bool attn_nothing(const sq_attention& a) { return a.tokens == 0 || a.seqs == 0 || a.most_new == 0; }
+
+size_t attn_workspace(const sq_attention& a, const AttnPlan& p) { return p.splits == 1 ? 0 : (size_t)a.tokens * a.q_heads * p.splits * (p.dp * 4 + 8); }
+
+// Everything of a call that the kernels are told but the strides of its cache
+int attn_prepare(const char* who, const sq_attention& a, const sq_cache& c, const AttnPlan& p, void* workspace, size_t ws_bytes, AttnArgs& k) {
+    if (!a.max_pages || !c.pages) return fail(SQ_EINVAL, "%s: new tokens without a page", who);
+    if (!a.q || !a.out || !a.table || !a.lens || !c.k || !c.v) return fail(SQ_EINVAL, "%s: null argument", who);
+    const int64_t strides = a.q_token | a.q_head | a.out_token | a.out_head | c.k_page | c.k_slot | c.k_head | c.v_page | c.v_slot | c.v_head;
+    if (strides % 8 || (((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)c.k | (uintptr_t)c.v) & 15))
+        return fail(SQ_EUNSUPPORTED, "%s: q, out, keys and values need 16-byte aligned heads", who);
+    const int64_t ot = a.out_token < 0 ? -a.out_token : a.out_token, oh = a.out_head < 0 ? -a.out_head : a.out_head;
+    if (!rows_apart(a.tokens, a.q_heads, ot, oh, c.dim)) return fail(SQ_EINVAL, "%s: rows of the output overlap (strides %lld, %lld)", who, (long long)ot, (long long)oh);
+    if ((int64_t)a.seqs * c.heads * p.row_blocks * p.splits > (1 << 23) || (p.splits > 1 && (int64_t)a.seqs * a.most_new * a.q_heads > (1 << 23)))
+        return fail(SQ_EUNSUPPORTED, "%s: %d sequences of up to %d new tokens and %d heads at once", who, a.seqs, a.most_new, a.q_heads);
+    const size_t need = attn_workspace(a, p);
+    if (ws_bytes < need || (need && (!workspace || ((uintptr_t)workspace & 255))))
+        return fail(SQ_EWORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who, need, ws_bytes);
+    k.q = (const char*)a.q; k.out = (char*)a.out; k.lse = a.lse; k.kc = (const char*)c.k; k.vc = (const char*)c.v;
+    k.table = a.table; k.lens = a.lens; k.starts = a.starts; k.mask = a.mask;
+    k.po = (float*)workspace;
+    k.pml = (float2v*)((float*)workspace + (need ? (size_t)a.tokens * a.q_heads * p.splits * p.dp : 0));
+    k.q_t = a.q_token * 2; k.q_h = a.q_head * 2; k.o_t = a.out_token * 2; k.o_h = a.out_head * 2;
+    k.ld_table = a.ld_table; k.ld_mask = a.ld_mask;
+    k.tokens = a.tokens; k.seqs = a.seqs; k.most_new = a.most_new; k.q_heads = a.q_heads; k.kv_heads = c.heads; k.group = a.q_heads / c.heads;
+    k.dim = c.dim; k.pages = c.pages; k.page = c.page; k.max_pages = a.max_pages; k.mask_words = a.mask_words;
+    k.row_blocks = p.row_blocks; k.splits = p.splits; k.last_splits = p.last_splits; k.last_row = p.last_row;
+    k.scale2 = a.scale * 1.4426950408889634f;
+    return SQ_OK;
+}
 
 }  // namespace sq
 
@@ -82,43 +111,20 @@ extern "C" {
 
 size_t sq_tree_attention_workspace_bytes(const sq_attention* a, const sq_cache* cache) {
     if (check_attention("sq_tree_attention_workspace_bytes", a, cache) || attn_nothing(*a)) return 0;
-    const AttnPlan p = attn_plan(*a, *cache);
-    if (p.splits == 1) return 0;
-    return (size_t)a->tokens * a->q_heads * p.splits * (p.dp * 4 + 8);
+    return attn_workspace(*a, attn_plan(*a, *cache));
 }
 
 int sq_tree_attention(const sq_attention* a, const sq_cache* cache, void* workspace, size_t ws_bytes, void* stream) {
     const char* who = "sq_tree_attention";
     if (int rc = check_attention(who, a, cache)) return rc;
     if (attn_nothing(*a)) return SQ_OK;
-    if (!a->max_pages || !cache->pages) return fail(SQ_EINVAL, "%s: new tokens without a page", who);
-    if (!a->q || !a->out || !a->table || !a->lens || !cache->k || !cache->v) return fail(SQ_EINVAL, "%s: null argument", who);
-    const int64_t strides = a->q_token | a->q_head | a->out_token | a->out_head | cache->k_page | cache->k_slot | cache->k_head | cache->v_page | cache->v_slot | cache->v_head;
-    if (strides % 8 || (((uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)cache->k | (uintptr_t)cache->v) & 15))
-        return fail(SQ_EUNSUPPORTED, "%s: q, out, keys and values need 16-byte aligned heads", who);
-    const int64_t ot = a->out_token < 0 ? -a->out_token : a->out_token, oh = a->out_head < 0 ? -a->out_head : a->out_head;
-    if (!rows_apart(a->tokens, a->q_heads, ot, oh, cache->dim)) return fail(SQ_EINVAL, "%s: rows of the output overlap (strides %lld, %lld)", who, (long long)ot, (long long)oh);
     const AttnPlan p = attn_plan(*a, *cache);
-    if ((int64_t)a->seqs * cache->heads * p.row_blocks * p.splits > (1 << 23) || (p.splits > 1 && (int64_t)a->seqs * a->most_new * a->q_heads > (1 << 23)))
-        return fail(SQ_EUNSUPPORTED, "%s: %d sequences of up to %d new tokens and %d heads at once", who, a->seqs, a->most_new, a->q_heads);
-    const size_t need = p.splits == 1 ? 0 : (size_t)a->tokens * a->q_heads * p.splits * (p.dp * 4 + 8);
-    if (ws_bytes < need || (need && (!workspace || ((uintptr_t)workspace & 255))))
-        return fail(SQ_EWORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who, need, ws_bytes);
     AttnArgs k;
-    k.q = (const char*)a->q; k.out = (char*)a->out; k.lse = a->lse; k.kc = (const char*)cache->k; k.vc = (const char*)cache->v;
-    k.table = a->table; k.lens = a->lens; k.starts = a->starts; k.mask = a->mask;
-    k.po = (float*)workspace;
-    k.pml = (float2v*)((float*)workspace + (need ? (size_t)a->tokens * a->q_heads * p.splits * p.dp : 0));
-    k.q_t = a->q_token * 2; k.q_h = a->q_head * 2; k.o_t = a->out_token * 2; k.o_h = a->out_head * 2;
+    if (int rc = attn_prepare(who, *a, *cache, p, workspace, ws_bytes, k)) return rc;
     k.k_page = cache->k_page * 2; k.k_slot = cache->k_slot * 2; k.k_head = cache->k_head * 2;
     k.v_page = cache->v_page * 2; k.v_slot = cache->v_slot * 2; k.v_head = cache->v_head * 2;
-    k.ld_table = a->ld_table; k.ld_mask = a->ld_mask;
-    k.tokens = a->tokens; k.seqs = a->seqs; k.most_new = a->most_new; k.q_heads = a->q_heads; k.kv_heads = cache->heads; k.group = a->q_heads / cache->heads;
-    k.dim = cache->dim; k.pages = cache->pages; k.page = cache->page; k.max_pages = a->max_pages; k.mask_words = a->mask_words;
-    k.row_blocks = p.row_blocks; k.splits = p.splits; k.last_splits = p.last_splits; k.last_row = p.last_row;
     auto near = [&](int64_t b) { return b >= 0 && b < (1 << 24) && b * (cache->page + 32) < INT32_MAX; };
     k.near = near(k.k_slot) && near(k.v_slot);
-    k.scale2 = a->scale * 1.4426950408889634f;
     return cache->dtype == SQ_F16 ? attn_launch_f16(k, p, (hipStream_t)stream) : attn_launch_bf16(k, p, (hipStream_t)stream);
 }
 

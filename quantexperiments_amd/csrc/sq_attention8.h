@@ -1,0 +1,254 @@
+// Attention of few rows over a cache held in 8 bits (sq_tree_attention8), built once per 16-bit type of the rows; that of many rows is
+// attn_tile_kernel of sq_attention.h, and so is all that does not read the cache.
+//
+// A key's codes are half the bytes of 16-bit elements, and what holds the kernel up is reading them.  They reach LDS as they are, become the
+// matrix instructions' 16-bit operands in registers, scale included, and from there on all is as over a 16-bit cache: the products are of the very numbers that are held.
+// First operand, keys: lane l reads 16 elements of key l % 16 at once, two operands of 8 (the rows' elements are in the same order).
+// First operand, values: ds_read_b64_tr_b8 lets 16 lanes read 8 keys x 16 elements and gives lane i the 8 keys of element i; the keys are the
+// scores' (4 * (l / 16) .. + 3 and 16 + 4 * (l / 16) .. + 3), so each half of them has one scale.
+#pragma once
+#include "sq_attention.h"
+
+namespace sq {
+
+// Layout of a step's keys (or values) in LDS: rows of DP bytes, their 16-byte pieces placed by XOR with the key's number so that 16 keys' pieces (first product), and the
+// 16 keys that two groups of lanes read at once (transposing reads), lie in different banks
+template <int DP> struct Attn8Tile {
+    static constexpr int PIECES = DP / 16;                  // of a key
+    static constexpr int ROWS = 64 / PIECES;                // keys per copy
+    static constexpr int COPIES = ATTN_STEP / ROWS;
+    static constexpr int PITCH = DP, BYTES = ATTN_STEP * PITCH;
+    static __device__ __forceinline__ constexpr int k_xor(int key) { return PIECES == 4 ? (key >> 2) & 3 : PIECES == 8 ? (key >> 1) & 7 : key & 15; }
+    static __device__ __forceinline__ constexpr int v_xor(int key) {
+        const int half = (key >> 4) & 1;
+        return PIECES == 4 ? ((key >> 2) & 1) | half << 1 : PIECES == 8 ? ((key >> 1) & 3) | half << 2 : (key & 7) | half << 3;
+    }
+};
+
+// Copies 16 keys (or values), of half x of a step, to `to`; from: the first one's byte of the head
+template <int DP, bool FULL, bool VALUES>
+__device__ __forceinline__ void attn8_copy(const Attn8Args& a, int x, int lane, const char* from, const char* to) {
+    typedef Attn8Tile<DP> T;
+    const int row = lane / T::PIECES, pos = lane % T::PIECES, pieces = a.dim >> 4, slot = (int)(VALUES ? a.v_slot : a.k_slot);
+    const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr)to);
+#pragma unroll
+    for (int j = 0; j < 16 / T::ROWS; ++j) {
+        const int key = 16 * x + j * T::ROWS + row, c = pos ^ (VALUES ? T::v_xor(key) : T::k_xor(key));
+        if (FULL || c < pieces) attn_copy16(lds + j * 1024, from, (uint32_t)((j * T::ROWS + row) * slot + c * 16));
+    }
+}
+
+// scores of a step: codes of its keys at k, scales of its halves
+template <int DT, int DP, int MT>
+__device__ __forceinline__ void attn8_scores(const AttnRows<DP, MT>& r, const char* k, const float (&by)[2], int lane, float4v (&st)[MT][2]) {
+    typedef Attn8Tile<DP> T;
+    const int g = lane >> 4, i16 = lane & 15;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) st[t][0] = st[t][1] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < DP / 64; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(k + (h * 16 + i16) * T::PITCH + (((c * 4 + g) ^ T::k_xor(h * 16 + i16)) * 16));
+            const u32x4 f0 = attn8_unpack<DT>(w[0], w[1], by[h], by[h]), f1 = attn8_unpack<DT>(w[2], w[3], by[h], by[h]);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                st[t][h] = AttnType<DT>::mfma(f0, r.q[t][2 * c], st[t][h]);
+                st[t][h] = AttnType<DT>::mfma(f1, r.q[t][2 * c + 1], st[t][h]);
+            }
+        }
+}
+
+// sums of a step: codes of its values at v.  Where MASKED, values that are not finite (codes of NaN; in fp16 what a scale carries beyond its range) do not go
+// through the product, see attn_sums.
+template <int DT, int DP, int MT, bool MASKED>
+__device__ __forceinline__ void attn8_sums(AttnRows<DP, MT>& r, const char* v, const float (&by)[2], int lane, const u32x4 (&p)[MT], const uint32_t (&sees)[MT]) {
+    typedef Attn8Tile<DP> T;
+    typedef AttnType<DT> E;
+    typedef int int2v __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) int2v* tr_ptr;
+    const int g = lane >> 4, i16 = lane & 15, key = ((i16 & 8) << 1) + 4 * g + ((i16 >> 1) & 3);
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((tr_ptr)(lds_ptr)(v + key * T::PITCH + ((d ^ T::v_xor(key)) * 16) + (i16 & 1) * 8)));
+        u32x4 f = attn8_unpack<DT>(w[0], w[1], by[0], by[1]);
+        if constexpr (MASKED) {
+            uint32_t odd = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) odd |= (f[i] & 0x7FFF7FFFu) + (0x8000u - E::INF) * 0x10001u;
+            if (__any((odd & 0x80008000u) != 0)) {
+                u32x4 up, down;                              // ones where a value is not below +inf, not above -inf
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t clean = 0, u = 0, n = 0;
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const uint32_t bits = (f[i] >> (16 * y)) & 0xFFFF;
+                        const bool nan = (bits & 0x7FFF) > E::INF, inf = (bits & 0x7FFF) == E::INF;
+                        if (!nan && !inf) clean |= bits << (16 * y);
+                        if (nan || (inf && !(bits & 0x8000))) u |= E::ONE << (16 * y);
+                        if (nan || (inf && (bits & 0x8000))) n |= E::ONE << (16 * y);
+                    }
+                    f[i] = clean; up[i] = u; down[i] = n;
+                }
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    u32x4 vis;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t two = sees[t] >> ((i >> 1) * 16 + g * 4 + (i & 1) * 2);
+                        vis[i] = (two & 1 ? E::ONE : 0u) | (two & 2 ? E::ONE << 16 : 0u);
+                    }
+                    const float4v zero = float4v{0.f, 0.f, 0.f, 0.f};
+                    const float4v cu = E::mfma(up, vis, zero), cd = E::mfma(down, vis, zero);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (cu[i] > 0.f) r.o[t][d][i] += INFINITY;
+                        if (cd[i] > 0.f) r.o[t][d][i] -= INFINITY;
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) r.o[t][d] = E::mfma(f, p[t], r.o[t][d]);
+    }
+}
+
+// Steps of codes that a wave has in LDS
+constexpr int ATTN8_RING = 4;
+template <int DP, int MT, int NW> constexpr int attn8_lds() {
+    constexpr int ring = NW * ATTN8_RING * 2 * Attn8Tile<DP>::BYTES, join = NW * MT * 16 * ((DP + 4) * 4 + 8) + 64;
+    return ring > join ? ring : join;
+}
+
+// Few rows, as attn_kernel: the waves of a workgroup share the rows and split its keys, no barrier until their sums are joined.
+template <int DT, int DP, int MT, int NW, bool FULL>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(1, 1))) void attn8_kernel(Attn8Args a) {
+    typedef Attn8Tile<DP> T;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    constexpr int C = 2 * T::COPIES, ROWS = MT * 16, RING = ATTN8_RING;          // (C: of a step)
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int id = blockIdx.x;
+    const int split = id % a.splits; id /= a.splits;
+    const int head = id % a.kv_heads; id /= a.kv_heads;
+    const int row0 = id % a.row_blocks * ROWS, b = id / a.row_blocks;
+    const AttnSeq s = attn_seq(a, b);
+    const int rows = s.n * a.group;
+    if (row0 >= rows) return;
+    const int last = min(row0 + ROWS, rows) - 1;
+    const int seen = a.mask ? s.total : min(s.total, s.len + last / a.group + 1);            // keys that some row sees
+    const int whole = a.mask ? min(s.len, s.total) : min(s.total, s.len + row0 / a.group + 1);        // and that all do
+    const int steps = (seen + ATTN_STEP - 1) / ATTN_STEP;
+    const int per = max((steps + a.splits - 1) / a.splits, NW), begin = min(split * per, steps), end = min(begin + per, steps);
+    const int each = (end - begin + NW - 1) / NW, w0 = min(begin + wave * each, end), w1 = min(w0 + each, end);
+
+    AttnRows<DP, MT> r;
+    attn_rows_begin<DP, MT, true>(a, s, head, row0, lane, r);
+    const char *kb = a.kc + head * a.k_head, *vb = a.vc + head * a.v_head;
+    char* ring = smem + wave * (RING * 2 * T::BYTES);
+    Attn8Groups groups;
+    uint64_t older = 0, newer = 0;                           // scales of the four steps on their way, 32 bits each: of keys and values of both halves
+    auto get = [&](int i) __attribute__((always_inline)) {
+        char* to = ring + (i % RING) * (2 * T::BYTES);
+        // (32 steps at a time, counted from the wave's first)
+        if (2 * i < groups.window || 2 * i >= groups.window + 64) groups.find(a, b, head, 2 * i, i * ATTN_STEP, 16, min(s.total, w1 * ATTN_STEP), lane);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) attn8_copy<DP, FULL, false>(a, x, lane, kb + groups.key_at(2 * i + x), to + x * 16 * T::PITCH);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) attn8_copy<DP, FULL, true>(a, x, lane, vb + groups.value_at(2 * i + x), to + T::BYTES + x * 16 * T::PITCH);
+        older = older >> 32 | newer << 32;
+        newer = newer >> 32 | (uint64_t)(groups.scales_at(2 * i) | groups.scales_at(2 * i + 1) << 16) << 32;
+    };
+    if constexpr (!FULL) {
+        attn_clear(ring, RING * 2 * T::BYTES, lane, 64);
+        attn_reads_done();
+    }
+#pragma unroll
+    for (int i = 0; i < RING; ++i)
+        if (w0 + i < w1) get(w0 + i);
+    attn_rows_ready(r);
+    auto step = [&](int i, auto masked) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked)::value;
+        float4v st[MT][2];
+        u32x4 p[MT];
+        uint32_t sees[MT] = {};
+        const int behind = min(w1 - 1 - i, RING - 1);        // steps that follow on their way
+        const uint32_t sc = (uint32_t)((behind > 1 ? older : newer) >> (behind & 1 ? 0 : 32));
+        const float kby[2] = {attn8_scale(sc & 0xFF), attn8_scale(sc >> 16 & 0xFF)}, vby[2] = {attn8_scale(sc >> 8 & 0xFF), attn8_scale(sc >> 24)};
+        if (behind == 3) attn_wait<3 * C>(); else if (behind == 2) attn_wait<2 * C>(); else if (behind == 1) attn_wait<C>(); else attn_wait<0>();
+        const char* at = ring + (i % RING) * (2 * T::BYTES);
+        attn8_scores<DT, DP, MT>(r, at, kby, lane, st);
+        if constexpr (MASKED)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) sees[t] = attn_sees(a, s, i, r.tok[t]);
+        attn_weights<DT, DP, MT, MASKED>(a, r, st, sees, lane, p);
+        attn8_sums<DT, DP, MT, MASKED>(r, at + T::BYTES, vby, lane, p, sees);
+        __builtin_amdgcn_sched_barrier(0);
+        attn_reads_done();
+        if (i + RING < w1) get(i + RING);
+    };
+    const int clear = min(max(whole / ATTN_STEP, w0), w1);
+    for (int i = w0; i < clear; ++i) step(i, std::false_type());
+    for (int i = clear; i < w1; ++i) step(i, std::true_type());
+    // the waves' sums meet in LDS
+    __syncthreads();
+    constexpr int PITCH = DP + 4;
+    float* sums = reinterpret_cast<float*>(smem);
+    float2v* ml = reinterpret_cast<float2v*>(smem + NW * ROWS * PITCH * 4);
+    int* flags = reinterpret_cast<int*>(ml + NW * ROWS);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int row = t * 16 + (lane & 15);
+        const float l = groups_fold(r.l[t], [](float x, float y) { return x + y; });
+        if (lane < 16) ml[wave * ROWS + row] = float2v{r.m[t], l};
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+            *reinterpret_cast<float4v*>(sums + (size_t)(wave * ROWS + row) * PITCH + d * 16 + (lane >> 4) * 4) = r.o[t][d];
+    }
+    const bool bad = __any(groups.bad) || s.over;
+    if (lane == 0) flags[wave] = bad;
+    __syncthreads();
+    bool any = false;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) any |= flags[w] != 0;
+    attn_write<DT, DP>(a, s, head, row0, ROWS, split, sums, ml, NW, ROWS, any, tid, NW * 64);
+}
+
+// ------------------------------------------------------------------------------------------ host
+
+template <int DT, int DP, int MT, bool FULL>
+int attn8_launch_few(const Attn8Args& a, unsigned grid, hipStream_t s) {
+    constexpr int NW = attn_waves(DP), LDS = attn8_lds<DP, MT, NW>();
+    static bool raised[64];
+    attn_raise((const void*)attn8_kernel<DT, DP, MT, NW, FULL>, LDS, raised);
+    hipLaunchKernelGGL((attn8_kernel<DT, DP, MT, NW, FULL>), dim3(grid), dim3(NW * 64), LDS, s, a);
+    return check_launch("sq_tree_attention8");
+}
+template <int DT, int DP, int NW, bool FULL>
+int attn8_launch_many(const Attn8Args& a, unsigned grid, hipStream_t s) {
+    constexpr int LDS = attn8_tile_lds<DP, NW>();
+    static bool raised[64];
+    attn_raise((const void*)attn_tile_kernel<DT, DP, NW, FULL, Attn8Args>, LDS, raised);
+    hipLaunchKernelGGL((attn_tile_kernel<DT, DP, NW, FULL, Attn8Args>), dim3(grid), dim3(NW * 64), LDS, s, a);
+    return check_launch("sq_tree_attention8");
+}
+template <int DT, int DP, bool FULL>
+int attn8_launch_dim(const Attn8Args& a, const AttnPlan& p, hipStream_t s) {
+    const unsigned grid = (unsigned)((int64_t)a.seqs * a.kv_heads * ((p.row_blocks - 1) * p.splits + p.last_splits));
+    int rc;
+    if (p.nw) rc = p.nw == 4 ? attn8_launch_many<DT, DP, 4, FULL>(a, grid, s) : attn8_launch_many<DT, DP, 8, FULL>(a, grid, s);
+    else rc = p.mt == 1 ? attn8_launch_few<DT, DP, 1, FULL>(a, grid, s) : attn8_launch_few<DT, DP, DP == 256 ? 1 : 2, FULL>(a, grid, s);
+    return rc || p.splits == 1 ? rc : attn_launch_join<DT, DP>(a, s);
+}
+template <int DT>
+int attn8_launch(const Attn8Args& a, const AttnPlan& p, hipStream_t s) {
+    auto go = [&](auto dp) {
+        constexpr int DP = decltype(dp)::value;
+        return a.dim == DP ? attn8_launch_dim<DT, DP, true>(a, p, s) : attn8_launch_dim<DT, DP, false>(a, p, s);
+    };
+    return p.dp == 64 ? go(std::integral_constant<int, 64>()) : p.dp == 128 ? go(std::integral_constant<int, 128>()) : go(std::integral_constant<int, 256>());
+}
+int attn8_launch_f16(const Attn8Args& a, const AttnPlan& p, hipStream_t s);
+int attn8_launch_bf16(const Attn8Args& a, const AttnPlan& p, hipStream_t s);
+
+}  // namespace sq

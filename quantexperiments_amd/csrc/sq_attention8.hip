@@ -1,0 +1,47 @@
+// sq_tree_attention8: argument checks and launch.  Calls are cut into workgroups as over a 16-bit cache (attn_plan).
+#include "sq_attention8.h"
+
+namespace sq {
+
+// the cache as one of 16-bit elements, for what does not read it
+static sq_cache as_cache(const sq_cache8& c, int dtype) {
+    return {c.k, c.v, c.k_page, c.k_slot, c.k_head, c.v_page, c.v_slot, c.v_head, c.pages, c.page, c.heads, c.dim, dtype};
+}
+
+static int check_attention8(const char* who, const sq_attention* a, const sq_cache8* cache, int dtype, sq_cache& c) {
+    if (!a || !cache) return fail(SQ_EINVAL, "%s: null argument", who);
+    if (int rc = check_cache8(who, cache)) return rc;
+    c = as_cache(*cache, dtype);
+    return check_attention(who, a, &c);
+}
+
+}  // namespace sq
+
+using namespace sq;
+
+extern "C" {
+
+size_t sq_tree_attention8_workspace_bytes(const sq_attention* a, const sq_cache8* cache, int dtype) {
+    sq_cache c;
+    if (check_attention8("sq_tree_attention8_workspace_bytes", a, cache, dtype, c) || attn_nothing(*a)) return 0;
+    return attn_workspace(*a, attn_plan(*a, c));
+}
+
+int sq_tree_attention8(const sq_attention* a, const sq_cache8* cache, int dtype, void* workspace, size_t ws_bytes, void* stream) {
+    const char* who = "sq_tree_attention8";
+    sq_cache c;
+    if (int rc = check_attention8(who, a, cache, dtype, c)) return rc;
+    if (attn_nothing(*a)) return SQ_OK;
+    const AttnPlan p = attn_plan(*a, c);
+    Attn8Args k;
+    if (int rc = attn_prepare(who, *a, c, p, workspace, ws_bytes, k)) return rc;
+    k.k_page = cache->k_page; k.k_slot = cache->k_slot; k.k_head = cache->k_head; k.v_page = cache->v_page; k.v_slot = cache->v_slot; k.v_head = cache->v_head;
+    k.near = 1;
+    k.ks = cache->k_scale; k.vs = cache->v_scale;
+    k.ks_page = cache->ks_page; k.ks_block = cache->ks_block; k.ks_head = cache->ks_head;
+    k.vs_page = cache->vs_page; k.vs_block = cache->vs_block; k.vs_head = cache->vs_head;
+    k.size = cache->page / cache->blocks;
+    return dtype == SQ_F16 ? attn8_launch_f16(k, p, (hipStream_t)stream) : attn8_launch_bf16(k, p, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -141,6 +141,7 @@ constexpr size_t SQ_WS_ERR_OFF = SQ_WS_HEADER - 256;
 int fail(int code, const char* fmt, ...);
 int check_launch(const char* what);
 int device_cus();       // compute units of the current device (cached)
+int check_cache8(const char* who, const sq_cache8* c);      // (sq_cache8.hip)
 
 // launchers implemented in the kernel translation units
 int launch_dequant(const sq_matrix& m, void* out, int out_dtype, int64_t ld_out, int r0, int r1, hipStream_t s,

@@ -778,6 +778,54 @@ PyObject* put_tokens8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     )
 }
 
+// tree_attention8(q, k_cache, v_cache, k_scale, v_scale, table, lens, starts, most_new, mask, scale, out, lse) -> out, or a code
+PyObject* tree_attention8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const at::Tensor *starts, *mask, *given, *lse;
+    if (n != 13 || !tensors(a, 7) || !maybe(a[7], starts) || !maybe(a[9], mask) || !maybe(a[11], given) || !maybe(a[12], lse)) return answer(NOT_COVERED);
+    SQ_GUARD(
+        const at::Tensor& q = THPVariable_Unpack(a[0]);
+        const at::Tensor& table = THPVariable_Unpack(a[5]);
+        const at::Tensor& lens = THPVariable_Unpack(a[6]);
+        if (q.dim() != 3 || !q.is_cuda() || q.numel() == 0 || q.numel() > INT32_MAX) return answer(NOT_COVERED);
+        const int dev = q.get_device(); const int dt = dtype_of(q);
+        const int64_t rows = q.size(0);
+        sq_cache8 c; sq_attention t{};
+        if (!heads_on(q, dev) || !is16(dt) || !batch_on(table, lens, starts, dev) ||
+            !cache8_of(THPVariable_Unpack(a[1]), THPVariable_Unpack(a[2]), THPVariable_Unpack(a[3]), THPVariable_Unpack(a[4]), dev, false, false, c) || c.dim != q.size(2) ||
+            q.size(1) % c.heads || (mask && (!rows_on(*mask, dev, rows, at::kLong) || mask->size(1) > INT32_MAX)) ||
+            (lse && (lse->scalar_type() != at::kFloat || lse->dim() != 2 || lse->size(0) != rows || lse->size(1) != q.size(1) || !plain_on(*lse, dev) || !lse->is_contiguous())))
+            return answer(NOT_COVERED);
+        const int64_t b = lens.size(0); const int64_t most = most_of(a[8], starts, rows, b);
+        const double scale = a[10] == Py_None ? std::pow((double)c.dim, -0.5) : PyFloat_AsDouble(a[10]);
+        if (PyErr_Occurred()) return nullptr;
+        if (most < 0 || !(scale > 0 && scale < 2.3e38)) return answer(NOT_COVERED);
+        if (given) {
+            if (!heads_on(*given, dev) || given->sizes() != q.sizes() || given->scalar_type() != q.scalar_type() || !apart(*given, q) || (given->stride(0) == 0 && rows > 1) ||
+                (given->stride(1) == 0 && q.size(1) > 1))
+                return answer(NOT_COVERED);
+            for (int i = 1; i < 5; ++i) if (!apart(*given, THPVariable_Unpack(a[i]))) return answer(NOT_COVERED);
+        }
+        OnDevice on(dev);
+        at::Tensor out = given ? *given : at::empty(q.sizes(), q.options());
+        t.q = q.data_ptr(); t.out = out.data_ptr(); t.lse = lse ? (float*)lse->data_ptr() : nullptr; t.table = (const int32_t*)table.data_ptr();
+        t.lens = (const int32_t*)lens.data_ptr(); t.starts = starts ? (const int32_t*)starts->data_ptr() : nullptr; t.mask = mask ? (const int64_t*)mask->data_ptr() : nullptr;
+        if (mask && !t.mask) t.mask = (const int64_t*)lens.data_ptr();       // (a mask without words has no address, and none would mean no mask; nothing is read there)
+        t.q_token = q.stride(0); t.q_head = q.stride(1); t.out_token = out.stride(0); t.out_head = out.stride(1);
+        t.ld_table = table_ld(table); t.ld_mask = mask ? table_ld(*mask) : 0;
+        t.tokens = (int32_t)rows; t.seqs = (int32_t)b; t.most_new = (int32_t)most; t.q_heads = (int32_t)q.size(1); t.max_pages = (int32_t)table.size(1);
+        t.mask_words = mask ? (int32_t)mask->size(1) : 0; t.scale = (float)scale;
+        // (a buffer of the call's own: streams and captured graphs run side by side)
+        const size_t need = sq_tree_attention8_workspace_bytes(&t, &c, dt);
+        at::Tensor ws;
+        if (need) ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = sq_tree_attention8(&t, &c, dt, need ? ws.data_ptr() : nullptr, need, on.stream);
+        Py_END_ALLOW_THREADS
+        return rc ? answer(rc) : THPVariable_Wrap(std::move(out));
+    )
+}
+
 // keep_drafted8(k_cache, v_cache, k_scale, v_scale, table, lens, path, counts)
 PyObject* keep_drafted8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 8 || !tensors(a, 8)) return answer(NOT_COVERED);
@@ -948,7 +996,7 @@ PyObject* install_op(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {{"native", (PyCFunction)(void (*)(void))make_native, METH_FASTCALL, nullptr}, {"install", install, METH_O, nullptr}, SQ_FAST(install_op),
                          SQ_FAST(linear), SQ_FAST(forward), SQ_FAST(linear_from), SQ_FAST(linear_silu), SQ_FAST(addnorm), SQ_FAST(silu_mul), SQ_FAST(q8_linear), SQ_FAST(q4_rows),
                          SQ_FAST(rotary), SQ_FAST(qk_norm_rotary), SQ_FAST(tree_attention), SQ_FAST(keep_drafted),
-                         SQ_FAST(put_tokens8), SQ_FAST(keep_drafted8), SQ_FAST(fork_pages), SQ_FAST(compact_pages),
+                         SQ_FAST(put_tokens8), SQ_FAST(tree_attention8), SQ_FAST(keep_drafted8), SQ_FAST(fork_pages), SQ_FAST(compact_pages),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods};
 

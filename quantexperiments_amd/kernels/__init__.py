@@ -802,5 +802,5 @@ def linear_small_silu(pieces, x: torch.Tensor, out: torch.Tensor, *, x_out=None,
 
 
 from .attention import keep_drafted, qk_norm_rotary, rotary, rotary_freqs, tree_attention  # noqa: E402,F401
-from .cache8 import keep_drafted8, put_tokens8  # noqa: E402,F401
+from .cache8 import keep_drafted8, put_tokens8, tree_attention8  # noqa: E402,F401
 from .pages import compact_pages, fork_pages  # noqa: E402,F401

@@ -106,6 +106,60 @@ def put_tokens8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
                                              _ld(table), table.shape[1], lens.data_ptr(), None if starts is None else starts.data_ptr(), b, most_new, _lib.stream_ptr(dev)))
 
 
+def tree_attention8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                    starts: torch.Tensor | None = None, *, most_new: int | None = None, mask: torch.Tensor | None = None, scale: float | None = None,
+                    out: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
+    """`tree_attention` over an 8-bit cache: attention of new tokens q [N, Hq, D] (fp16 / bf16) over lens[b] cached tokens of each sequence and, in the slots behind them, its new
+    tokens' keys and values, as put_tokens8 puts them there (sq_tree_attention8).  Rows, starts, most_new, mask, scale, out, lse and what a token sees are as there.  Keys and
+    values are what the cache holds, code * scale, exactly in bf16; in fp16 as far as fp16 has them, which is all that put_tokens8 made of fp16 tokens."""
+    done = _lib.native().tree_attention8(q, k_cache, v_cache, k_scale, v_scale, table, lens, starts, most_new, mask, scale, out, lse)
+    if type(done) is not int:
+        return done
+    if done < 0:
+        _lib.check(done)
+    who = "tree_attention8"
+    _heads3(who, "q", q)
+    _no_grad(who, q, k_cache, v_cache, k_scale, v_scale, out, lse)
+    n, hq, d = q.shape
+    dev = q.device
+    _on_gpu(who, dev, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, table=table, lens=lens, starts=starts, mask=mask, out=out, lse=lse)
+    cache = _cache8(who, k_cache, v_cache, k_scale, v_scale)
+    if q.dtype not in DTYPES or k_cache.shape[3] != d or k_cache.shape[2] < 1 or hq < 1 or hq % k_cache.shape[2]:
+        raise ValueError(f"{who}: q {tuple(q.shape)} {q.dtype} (fp16 or bf16) and caches {tuple(k_cache.shape)}")
+    b, most_new = _sequences(who, n, table, lens, starts, most_new)
+    if mask is not None:
+        _rows2(who, "mask", mask, n, torch.int64)
+    if scale is None:
+        scale = d ** -0.5
+    if not 0 < scale < 2.3e38:                                # (times log2 e a number)
+        raise ValueError(f"{who}: scale {scale}")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    else:
+        _heads3(who, "out", out, q.shape)
+        if out.dtype != q.dtype:
+            raise ValueError(f"{who}: out is {out.dtype}, q {q.dtype}")
+        if _clash(out, q):
+            raise ValueError(f"{who}: out overlaps q")
+        if any(_near(c, out) for c in (k_cache, v_cache, k_scale, v_scale)):
+            raise ValueError(f"{who}: out overlaps a cache")
+        if any(s == 0 and m > 1 for m, s in zip(out.shape, out.stride())):
+            raise ValueError(f"{who}: out must not be expanded")
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (n, hq) or not lse.is_contiguous()):
+        raise ValueError(f"{who}: lse must be contiguous fp32 [{n}, {hq}]")
+    # (a mask without words has no address of its own, and none would mean no mask: any other does, nothing is read there)
+    a = SqAttention(q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), table.data_ptr(), lens.data_ptr(),
+                    None if starts is None else starts.data_ptr(), None if mask is None else mask.data_ptr() or lens.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1),
+                    _ld(table), 0 if mask is None else _ld(mask), n, b, most_new, hq, table.shape[1], 0 if mask is None else mask.shape[1], scale)
+    L, dt = _lib.lib(), _lib.DTYPES[q.dtype]
+    with torch.cuda.device(dev):
+        need = L.sq_tree_attention8_workspace_bytes(ctypes.byref(a), ctypes.byref(cache), dt)
+        # (a buffer of the call's own: streams and captured graphs run side by side)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _lib.check(L.sq_tree_attention8(ctypes.byref(a), ctypes.byref(cache), dt, None if ws is None else ws.data_ptr(), need, _lib.stream_ptr(dev)))
+    return out
+
+
 def keep_drafted8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, path: torch.Tensor,
                   counts: torch.Tensor) -> None:
     """`keep_drafted` in 8-bit caches [pages, slots, heads, D] of one layer or [layers, pages, slots, heads, D] of all: new token path[b, i] (int32 [B, m], ascending) of sequence
