@@ -247,6 +247,7 @@ struct Attn8Args : AttnArgs {
     const uint8_t *ks, *vs;
     int64_t ks_page, ks_block, ks_head, vs_page, vs_block, vs_head;
     int size;                    // tokens of a block, a multiple of 16
+    int together;                // few rows: the heads of the same keys are dealt to one die
 };
 
 // 8 codes times a power of two as a matrix instruction's operand: v_cvt_scalef32_pk takes two at a time and the scale with them, exactly
@@ -261,35 +262,30 @@ template <int DT> __device__ __forceinline__ u32x4 attn8_unpack(uint32_t x, uint
 __device__ __forceinline__ float attn8_scale(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
 
 // Where 64 groups of keys lie that a wave copies one after the other (lane l: the l-th, `step` keys after the one before), and their scales.  A group's keys are in
-// one block, so in one page.  Groups from key `limit` on: the first page, whose slots may be read as well, scale 1.
+// one block, so in one page.  Groups from key `limit` on: the first page, whose slots and scales may be read as well.
 struct Attn8Groups {
-    int window = 1 << 30;        // the first one's number
     int64_t k, v;                // bytes from the head's first
-    uint32_t scales;             // of keys, of values in the second byte
+    const uint8_t *ks, *vs;
     bool bad = false;
 
-    __device__ __forceinline__ void find(const Attn8Args& a, int b, int head, int number, int key, int step, int limit, int lane) {
-        window = number;
+    __device__ __forceinline__ void find(const Attn8Args& a, int b, int head, int key, int step, int limit, int lane) {
         const int64_t at = key + (int64_t)lane * step;
         int id = 0, off = 0;
-        bool there = at < limit;
-        if (there) {
+        if (at < limit) {
             const int pg = (int)((uint32_t)at / (uint32_t)a.page);
             off = (int)at - pg * a.page;
             id = a.table[(int64_t)b * a.ld_table + pg];
-            if ((uint32_t)id >= (uint32_t)a.pages) there = false, bad = true, id = 0, off = 0;
+            if ((uint32_t)id >= (uint32_t)a.pages) bad = true, id = 0, off = 0;
         }
+        const int block = off / a.size;
         k = id * a.k_page + off * a.k_slot;
         v = id * a.v_page + off * a.v_slot;
-        const int block = off / a.size;
-        scales = there ? a.ks[id * a.ks_page + block * a.ks_block + head * a.ks_head] | (uint32_t)a.vs[id * a.vs_page + block * a.vs_block + head * a.vs_head] << 8 : 0x7F7Fu;
+        ks = a.ks + id * a.ks_page + block * a.ks_block + head * a.ks_head;
+        vs = a.vs + id * a.vs_page + block * a.vs_block + head * a.vs_head;
     }
     static __device__ __forceinline__ int64_t lane64(int64_t x, int l) {
         return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, l) | (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32;
     }
-    __device__ __forceinline__ int64_t key_at(int number) const { return lane64(k, number - window); }
-    __device__ __forceinline__ int64_t value_at(int number) const { return lane64(v, number - window); }
-    __device__ __forceinline__ uint32_t scales_at(int number) const { return __builtin_amdgcn_readlane((int)scales, number - window); }
 };
 
 // What a wave keeps of its MT * 16 rows
@@ -763,17 +759,33 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(ARGS a) {
     const bool easy = a.near && a.page % MINE == 0;
     AttnWalk walk;
     walk.begin(a, begin * KEYS + wave * MINE);
-    Attn8Groups held;
+    Attn8Groups held;                                        // of stages `window` on, and their scales
+    int window = 1 << 30;
+    uint32_t scales = 0;
     uint64_t coming = 0;                                     // scales of the stages on their way, 16 bits each, the newest on top
     constexpr int C8N = attn8_copies<DP, NW>(), RAW = 2048 * C8N, P8 = DP / 16, ROWS8 = 64 / P8;          // (16-byte pieces of a key's codes, keys per copy)
     char* raw = smem + NB * STAGE + 64 + wave * (ATTN8_RAW * RAW);
+    // where a lane's codes go in a stage: their first 8 elements of keys, of values in the upper half (the other 8: 16 bytes on or back).  Held in one register each, because
+    // there are none to spare for what they are worked out from, which took more instructions than the unpacking.
+    uint32_t goes[C8N];
+    if constexpr (C8)
+#pragma unroll
+        for (int j = 0; j < C8N; ++j) {
+            const int row = wave * MINE + j * ROWS8 + lane / P8, key = row % ATTN_STEP, two = 2 * (lane % P8);
+            goes[j] = (row * T::PITCH + (two ^ T::k_xor(key)) * 16) | (SK * T::BYTES + row * T::PITCH + (two ^ T::v_xor(key)) * 16) << 16;
+            asm volatile("" : "+v"(goes[j]));
+        }
     auto place = [&](int i) __attribute__((always_inline)) { return smem + (i - begin) % NB * STAGE; };      // keys of SK steps, values of SK steps
     auto get = [&](int i) __attribute__((always_inline)) {           // this wave copies keys wave * MINE .. of a stage
         if constexpr (C8) {
             const int piece = lane % P8;
-            if (i < held.window || i >= held.window + 64) held.find(a, b, head, i, i * KEYS + wave * MINE, KEYS, min(s.total, end * KEYS), lane);
+            if (i < window || i >= window + 64) {
+                held.find(a, b, head, i * KEYS + wave * MINE, KEYS, min(s.total, end * KEYS), lane);
+                scales = *held.ks | (uint32_t)*held.vs << 8;
+                window = i;
+            }
             const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr)(raw + (i - begin) % ATTN8_RAW * RAW));
-            const int64_t k_at = held.key_at(i), v_at = held.value_at(i);
+            const int64_t k_at = held.lane64(held.k, i - window), v_at = held.lane64(held.v, i - window);
 #pragma unroll
             for (int j = 0; j < C8N; ++j) {
                 const int row = j * ROWS8 + lane / P8;
@@ -782,7 +794,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(ARGS a) {
                     attn_copy16(to + RAW / 2 + j * 1024, vb + v_at, (uint32_t)(row * (int)a.v_slot + piece * 16));
                 }
             }
-            coming = coming >> 16 | (uint64_t)held.scales_at(i) << (16 * (ATTN8_RAW - 1));
+            coming = coming >> 16 | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)scales, i - window) << (16 * (ATTN8_RAW - 1));
             return;
         }
         char* at = place(i) + wave * MINE * T::PITCH;
@@ -798,32 +810,38 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(ARGS a) {
         attn_copy<DP, FULL, false, MINE>(a, s, first, in_step, lane, pages, kb, at);
         attn_copy<DP, FULL, true, MINE>(a, s, first, in_step, lane, pages, vb, at + SK * T::BYTES);
     };
-    auto arrive = [&](int i) __attribute__((always_inline)) {        // stage i is there
+    // C8: this wave's part of stage i unpacked.  Once for each stage, in order, behind the barrier of the stage before it: the stage's place is that of the one three before it, which
+    // no wave reads from then on.
+    auto unpack = [&](int i) __attribute__((always_inline)) {
         if constexpr (C8) {
-            // (the stage's place is that of the one three before it, which no wave reads behind the barrier of the one before it)
-            const int piece = lane % P8, ahead = ATTN8_RAW - min(end - i, ATTN8_RAW);      // (its place in `coming`)
+            const int ahead = ATTN8_RAW - min(end - i, ATTN8_RAW);      // (its place in `coming`)
             if (i + ATTN8_RAW <= end) attn_wait<2 * C8N * (ATTN8_RAW - 1)>(); else attn_wait<0>();
             const uint32_t sc = (uint32_t)(coming >> (16 * ahead));
 #pragma unroll
-            for (int j = 0; j < C8N; ++j) {
-                const int row = j * ROWS8 + lane / P8, key = (wave * MINE + row) % ATTN_STEP;
-                if (row < MINE && (FULL || piece < a.dim >> 4)) {
+            for (int j = 0; j < C8N; ++j)
+                if (j * ROWS8 + lane / P8 < MINE && (FULL || lane % P8 < a.dim >> 4)) {
                     const char* from = raw + (i - begin) % ATTN8_RAW * RAW + j * 1024 + lane * 16;
-                    char* to = place(i) + (wave * MINE + row) * T::PITCH;
+                    char* stage = place(i);
+                    const u32x4 both[2] = {*reinterpret_cast<const u32x4*>(from), *reinterpret_cast<const u32x4*>(from + RAW / 2)};
 #pragma unroll
                     for (int v = 0; v < 2; ++v) {
-                        const u32x4 w = *reinterpret_cast<const u32x4*>(from + v * (RAW / 2));
+                        const u32x4 w = both[v];
                         const float by = attn8_scale(v ? sc >> 8 & 0xFF : sc & 0xFF);
-                        const int x = v ? T::v_xor(key) : T::k_xor(key);
-                        *reinterpret_cast<u32x4*>(to + v * (SK * T::BYTES) + ((2 * piece) ^ x) * 16) = attn8_unpack<DT>(w[0], w[1], by, by);
-                        *reinterpret_cast<u32x4*>(to + v * (SK * T::BYTES) + ((2 * piece + 1) ^ x) * 16) = attn8_unpack<DT>(w[2], w[3], by, by);
+                        const uint32_t to = v ? goes[j] >> 16 : goes[j] & 0xFFFF;
+                        *reinterpret_cast<u32x4*>(stage + to) = attn8_unpack<DT>(w[0], w[1], by, by);
+                        *reinterpret_cast<u32x4*>(stage + (to ^ 16)) = attn8_unpack<DT>(w[2], w[3], by, by);
                     }
                 }
-            }
+            // (its codes are read, all but the writes behind them done: the stage that comes three later takes their place)
+            asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(4 * C8N) : "memory");
+            if (i + ATTN8_RAW < end) get(i + ATTN8_RAW);
+        }
+    };
+    auto arrive = [&](int i) __attribute__((always_inline)) {        // stage i is there
+        if constexpr (C8) {
             attn_reads_done();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            if (i + ATTN8_RAW < end) get(i + ATTN8_RAW);
             return;
         }
         if (i + NB - 2 <= end) attn_wait<2 * C * (NB - 3)>(); else attn_wait<0>();
@@ -840,6 +858,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(ARGS a) {
     for (int i = 0; i < (C8 ? ATTN8_RAW : NB - 2); ++i)
         if (begin + i < end) get(begin + i);
     attn_rows_ready(r);
+    if constexpr (C8) if (begin < end) unpack(begin);
 
     if constexpr (PIPELINE) if (begin < clear) {
         // Where this lane reads in a step: of key l % 16 (the step's other half 16 keys behind) its first piece, of 4 keys their first elements (likewise).
@@ -938,6 +957,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(ARGS a) {
             const uint32_t cur = lds(place(i)), nxt = lds(place(i + 1));
             auto slot = [&](auto number) __attribute__((always_inline)) {
                 constexpr int n = decltype(number)::value, h = n / MT, t = n % MT, t1 = (t + MT - 1) % MT, t2 = (t + MT - 2) % MT;
+                // (a SIMD's two waves at different times: 1900 tokens behind 2100 142 -> 136 us)
+                if constexpr (C8) if (n == wave / 4 % 2 * (SK * MT / 2) && i + 1 < end) unpack(i + 1);
                 if (n == SK * MT - 1 && i + 1 < clear) arrive(i + 1);
                 __builtin_amdgcn_sched_barrier(0);
                 // (behind the last stage of the pipeline: whatever lies in the next one's place, for nothing)
@@ -971,6 +992,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(ARGS a) {
     auto plain = [&](int i, auto masked) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked)::value;
         arrive(i);
+        if constexpr (C8) if (i + 1 < end) unpack(i + 1);
 #pragma unroll 1
         for (int h = 0; h < SK; ++h) {
             const int step = SK * i + h;
@@ -1127,6 +1149,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 
 struct AttnPlan { int dp, mt, nw, row_blocks, splits, last_splits, last_row; };       // nw: waves of the many-row kernel; 0: the few-row one, mt tiles of rows
 constexpr int attn_waves(int dp) { return dp == 256 ? 2 : 4; }
+constexpr int ATTN8_WAVES = 4;
 
 inline void attn_raise(const void* kernel, int lds, bool (&raised)[64]) {
     int dev = 0;
@@ -1180,7 +1203,7 @@ int attn_launch(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
 // sq_attention.hip: what a call must be like, how it is cut, and everything of it that the kernels are told but the cache's own arrays
 int check_attention(const char* who, const sq_attention* a, const sq_cache* c);
 bool attn_nothing(const sq_attention& a);
-AttnPlan attn_plan(const sq_attention& a, const sq_cache& c);
+AttnPlan attn_plan(const sq_attention& a, const sq_cache& c, bool held8 = false);
 size_t attn_workspace(const sq_attention& a, const AttnPlan& p);
 int attn_prepare(const char* who, const sq_attention& a, const sq_cache& c, const AttnPlan& p, void* workspace, size_t ws_bytes, AttnArgs& k);
 bool rows_apart(int tokens, int heads, int64_t t, int64_t h, int dim);      // sq_heads.hip

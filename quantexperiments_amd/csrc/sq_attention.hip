@@ -13,13 +13,16 @@ namespace sq {
 // A last block of rows that fills at most half of its waves takes 0.6 of the time, and gets as many fewer parts: 8 trees of 32 tokens of 5 heads of 256 per
 // key head (160 rows in blocks of 128) 42.3 us evenly, 39.3 so; with 0.75 42.1.
 // (All times of captured calls, one behind the other; calls back to back take up to 4 % less.)
+// Over a cache held in 8 bits a compute unit holds two of the few-row workgroups (four of heads up to 64), and sequences are also cut into parts of 20 steps a wave, which ends
+// them closer together: 64 sequences of 8192 slots x 8 key heads in three parts 205 us, whole 218; of 2,240 to 8,192 131 and 152; 32 of those 72 and 91; 32 of 4000 x 2 key heads of 64 in
+// eight 12.9, in four 14.3.
 // A sequence's length is its table's width here: lengths are on the device.  Under a table of 131,072 slots one token behind 500 takes 10.2 us instead of 8.8, 48 26.7 instead of 21.4,
 // 64 sequences of 500 27.9 instead of 18.6, 64 of 2000 59.8 instead of 53.1.
-AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
+AttnPlan attn_plan(const sq_attention& a, const sq_cache& c, bool held8) {
     AttnPlan p;
     p.dp = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
     const int64_t rows = (int64_t)a.most_new * (a.q_heads / c.heads), steps = ((int64_t)a.max_pages * c.page + ATTN_STEP - 1) / ATTN_STEP;
-    const int waves = attn_waves(p.dp);
+    const int waves = held8 ? ATTN8_WAVES : attn_waves(p.dp);
     int64_t per, most;
     if (rows <= (p.dp == 256 ? 16 : 32)) {
         p.nw = 0;
@@ -36,7 +39,10 @@ AttnPlan attn_plan(const sq_attention& a, const sq_cache& c) {
     p.row_blocks = (int)((rows + per - 1) / per);
     const int64_t base = (int64_t)a.seqs * c.heads * p.row_blocks, cus = device_cus();
     int64_t want = cus / base;
-    if (a.seqs > 1 && !p.nw && 2 * cus / base > 1 && steps / (2 * cus / base) >= 8 * waves) want = 2 * cus / base;
+    if (held8 && !p.nw) {
+        if (p.dp == 64) want = 2 * cus / base;
+        if (want < steps / (20 * waves)) want = steps / (20 * waves);
+    } else if (a.seqs > 1 && !p.nw && 2 * cus / base > 1 && steps / (2 * cus / base) >= 8 * waves) want = 2 * cus / base;
     p.splits = (int)(want < most ? want : most);
     if (p.splits < 1) p.splits = 1;
     if (p.splits > ATTN_SPLITS_MAX) p.splits = ATTN_SPLITS_MAX;

@@ -114,23 +114,37 @@ __device__ __forceinline__ void attn8_sums(AttnRows<DP, MT>& r, const char* v, c
     }
 }
 
-// Steps of codes that a wave has in LDS
-constexpr int ATTN8_RING = 4;
+// Workgroups of ATTN8_WAVES that a compute unit holds, and steps of codes that each wave has in LDS (two or four), 128 KB of a unit in all.  A step is a chain (wait, read, unpack,
+// multiply, exponentials, read, unpack, multiply) of which a second wave of the SIMD fills the gaps: with all data in the caches, 32 sequences of 8192 x 8 key heads of 128 take 80 us
+// with one wave a SIMD, 55 with two; heads of 256 have no registers for it.
+constexpr int attn8_groups(int dp, int mt) { return dp == 256 ? 1 : dp == 64 && mt == 1 ? 4 : 2; }
+constexpr int attn8_ring(int dp, int mt) { return 131072 / attn8_groups(dp, mt) / (ATTN8_WAVES * 2 * ATTN_STEP * dp); }
+// and the scales of the groups they are of: of 64 groups of keys and 64 of values, twice
+constexpr int ATTN8_SCALES = 1024;
+// Copies a byte per lane to LDS, lane l's to `to` + 4 l, as 32 bits (see attn_copy16)
+__device__ __forceinline__ void attn8_copy_scale(uint32_t to, const uint8_t* at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" ::"s"(to), "v"(at) : "memory");
+}
 template <int DP, int MT, int NW> constexpr int attn8_lds() {
-    constexpr int ring = NW * ATTN8_RING * 2 * Attn8Tile<DP>::BYTES, join = NW * MT * 16 * ((DP + 4) * 4 + 8) + 64;
+    constexpr int ring = NW * (attn8_ring(DP, MT) * 2 * Attn8Tile<DP>::BYTES + ATTN8_SCALES), join = NW * MT * 16 * ((DP + 4) * 4 + 8) + 64;
     return ring > join ? ring : join;
 }
 
 // Few rows, as attn_kernel: the waves of a workgroup share the rows and split its keys, no barrier until their sums are joined.
 template <int DT, int DP, int MT, int NW, bool FULL>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(1, 1))) void attn8_kernel(Attn8Args a) {
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW * attn8_groups(DP, MT) / 4, NW * attn8_groups(DP, MT) / 4))) void attn8_kernel(Attn8Args a) {
     typedef Attn8Tile<DP> T;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    constexpr int C = 2 * T::COPIES, ROWS = MT * 16, RING = ATTN8_RING;          // (C: of a step)
+    constexpr int C = T::COPIES, ROWS = MT * 16, RING = attn8_ring(DP, MT);          // (C: of a step's keys, or values)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int id = blockIdx.x;
+    int id = blockIdx.x, head;
+    if (a.together) {                                        // as far as eights of parts go
+        const int parts = gridDim.x / a.kv_heads, eights = parts & ~7, over = id - eights * a.kv_heads;
+        head = over < 0 ? id / 8 % a.kv_heads : over % a.kv_heads;
+        id = over < 0 ? id / 8 / a.kv_heads * 8 + id % 8 : eights + over / a.kv_heads;
+    }
     const int split = id % a.splits; id /= a.splits;
-    const int head = id % a.kv_heads; id /= a.kv_heads;
+    if (!a.together) { head = id % a.kv_heads; id /= a.kv_heads; }
     const int row0 = id % a.row_blocks * ROWS, b = id / a.row_blocks;
     const AttnSeq s = attn_seq(a, b);
     const int rows = s.n * a.group;
@@ -147,17 +161,22 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
     const char *kb = a.kc + head * a.k_head, *vb = a.vc + head * a.v_head;
     char* ring = smem + wave * (RING * 2 * T::BYTES);
     Attn8Groups groups;
-    uint64_t older = 0, newer = 0;                           // scales of the four steps on their way, 32 bits each: of keys and values of both halves
-    auto get = [&](int i) __attribute__((always_inline)) {
-        char* to = ring + (i % RING) * (2 * T::BYTES);
-        // (32 steps at a time, counted from the wave's first)
-        if (2 * i < groups.window || 2 * i >= groups.window + 64) groups.find(a, b, head, 2 * i, i * ATTN_STEP, 16, min(s.total, w1 * ATTN_STEP), lane);
+    char* scales = smem + NW * (RING * 2 * T::BYTES) + wave * ATTN8_SCALES;
+    auto slot = [&](int i) __attribute__((always_inline)) { return ring + (i % RING) * (2 * T::BYTES); };
+    auto get_k = [&](int i) __attribute__((always_inline)) {
+        const int n = i - w0;
+        if (n % 32 == 0) {                                   // the groups of the next 32 steps, their scales ahead of the keys
+            groups.find(a, b, head, i * ATTN_STEP, 16, min(s.total, w1 * ATTN_STEP), lane);
+            const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr)(scales + n / 32 % 2 * 512));
+            attn8_copy_scale(to, groups.ks);
+            attn8_copy_scale(to + 256, groups.vs);
+        }
 #pragma unroll
-        for (int x = 0; x < 2; ++x) attn8_copy<DP, FULL, false>(a, x, lane, kb + groups.key_at(2 * i + x), to + x * 16 * T::PITCH);
+        for (int x = 0; x < 2; ++x) attn8_copy<DP, FULL, false>(a, x, lane, kb + groups.lane64(groups.k, 2 * (n % 32) + x), slot(i) + x * 16 * T::PITCH);
+    };
+    auto get_v = [&](int i) __attribute__((always_inline)) {         // (behind get_k of the same step)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) attn8_copy<DP, FULL, true>(a, x, lane, vb + groups.value_at(2 * i + x), to + T::BYTES + x * 16 * T::PITCH);
-        older = older >> 32 | newer << 32;
-        newer = newer >> 32 | (uint64_t)(groups.scales_at(2 * i) | groups.scales_at(2 * i + 1) << 16) << 32;
+        for (int x = 0; x < 2; ++x) attn8_copy<DP, FULL, true>(a, x, lane, vb + groups.lane64(groups.v, 2 * ((i - w0) % 32) + x), slot(i) + T::BYTES + x * 16 * T::PITCH);
     };
     if constexpr (!FULL) {
         attn_clear(ring, RING * 2 * T::BYTES, lane, 64);
@@ -165,7 +184,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
     }
 #pragma unroll
     for (int i = 0; i < RING; ++i)
-        if (w0 + i < w1) get(w0 + i);
+        if (w0 + i < w1) { get_k(w0 + i); get_v(w0 + i); }
     attn_rows_ready(r);
     auto step = [&](int i, auto masked) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked)::value;
@@ -173,19 +192,32 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
         u32x4 p[MT];
         uint32_t sees[MT] = {};
         const int behind = min(w1 - 1 - i, RING - 1);        // steps that follow on their way
-        const uint32_t sc = (uint32_t)((behind > 1 ? older : newer) >> (behind & 1 ? 0 : 32));
-        const float kby[2] = {attn8_scale(sc & 0xFF), attn8_scale(sc >> 16 & 0xFF)}, vby[2] = {attn8_scale(sc >> 8 & 0xFF), attn8_scale(sc >> 24)};
-        if (behind == 3) attn_wait<3 * C>(); else if (behind == 2) attn_wait<2 * C>(); else if (behind == 1) attn_wait<C>(); else attn_wait<0>();
-        const char* at = ring + (i % RING) * (2 * T::BYTES);
-        attn8_scores<DT, DP, MT>(r, at, kby, lane, st);
+        // (steps that follow are on their way: their keys and values, and of this one its values)
+        auto arrived = [&](auto extra) __attribute__((always_inline)) {
+            constexpr int X = decltype(extra)::value;
+            if (RING > 2 && behind == 3) attn_wait<(6 + X) * C>();
+            else if (RING > 2 && behind == 2) attn_wait<(4 + X) * C>();
+            else if (behind == 1) attn_wait<(2 + X) * C>();
+            else attn_wait<X * C>();
+        };
+        arrived(std::integral_constant<int, 1>());
+        const u32x2* sc = reinterpret_cast<const u32x2*>(scales + (i - w0) / 32 % 2 * 512 + (i - w0) % 32 * 8);
+        const u32x2 ksc = sc[0], vsc = sc[32];
+        const float kby[2] = {attn8_scale(ksc[0]), attn8_scale(ksc[1])}, vby[2] = {attn8_scale(vsc[0]), attn8_scale(vsc[1])};
+        attn8_scores<DT, DP, MT>(r, slot(i), kby, lane, st);
+        __builtin_amdgcn_sched_barrier(0);
+        attn_reads_done();
+        const bool more = i + RING < w1;
+        if (more) get_k(i + RING);
         if constexpr (MASKED)
 #pragma unroll
             for (int t = 0; t < MT; ++t) sees[t] = attn_sees(a, s, i, r.tok[t]);
         attn_weights<DT, DP, MT, MASKED>(a, r, st, sees, lane, p);
-        attn8_sums<DT, DP, MT, MASKED>(r, at + T::BYTES, vby, lane, p, sees);
+        if (more) arrived(std::integral_constant<int, 1>()); else arrived(std::integral_constant<int, 0>());
+        attn8_sums<DT, DP, MT, MASKED>(r, slot(i) + T::BYTES, vby, lane, p, sees);
         __builtin_amdgcn_sched_barrier(0);
         attn_reads_done();
-        if (i + RING < w1) get(i + RING);
+        if (more) get_v(i + RING);
     };
     const int clear = min(max(whole / ATTN_STEP, w0), w1);
     for (int i = w0; i < clear; ++i) step(i, std::false_type());
@@ -218,7 +250,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
 
 template <int DT, int DP, int MT, bool FULL>
 int attn8_launch_few(const Attn8Args& a, unsigned grid, hipStream_t s) {
-    constexpr int NW = attn_waves(DP), LDS = attn8_lds<DP, MT, NW>();
+    constexpr int NW = ATTN8_WAVES, LDS = attn8_lds<DP, MT, NW>();
     static bool raised[64];
     attn_raise((const void*)attn8_kernel<DT, DP, MT, NW, FULL>, LDS, raised);
     hipLaunchKernelGGL((attn8_kernel<DT, DP, MT, NW, FULL>), dim3(grid), dim3(NW * 64), LDS, s, a);
