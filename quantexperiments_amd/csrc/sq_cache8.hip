@@ -11,7 +11,8 @@ struct Cache8 {
     char *k, *v;
     uint8_t *ks, *vs;
     int64_t k_page, k_slot, k_head, v_page, v_slot, v_head, ks_page, ks_block, ks_head, vs_page, vs_block, vs_head;      // bytes
-    int pages, page, blocks, size, heads, dim;                     // size: tokens of a block
+    int pages, page, blocks, size, heads, dim, per;                // size: tokens of a block; per: 16-byte pieces of a head
+    uint32_t over_per;                                              // 2^32 / per, rounded up
 };
 struct Put8Args {
     Cache8 c;
@@ -49,39 +50,72 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     return max(v, row_rotated_bits<1>(v));
 }
 
-// 16 codes times 2^-down
+// the same of 16-bit halves
+__device__ __forceinline__ uint32_t wave_max2(uint32_t x) {
+    typedef unsigned short pair __attribute__((ext_vector_type(2)));
+    auto most = [](uint32_t a, uint32_t b) { return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pair, a), __builtin_bit_cast(pair, b))); };
+    const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = most((uint32_t)h[0], (uint32_t)h[1]);
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = most((uint32_t)r[0], (uint32_t)r[1]);
+    x = most(x, row_rotated_bits<8>(x));
+    x = most(x, row_rotated_bits<4>(x));
+    x = most(x, row_rotated_bits<2>(x));
+    return most(x, row_rotated_bits<1>(x));
+}
+
+// i / per, for i below 2^28
+__device__ __forceinline__ int row_of(const Cache8& c, int i) { return c.per == 1 ? i : (int)__umulhi((uint32_t)i, c.over_per); }
+
+// 16 codes times 2^-down.  (By way of fp16, which has every one of these numbers down to 2^-24, where the nearest code is zero.)
 __device__ __forceinline__ u32x4 scaled_codes(u32x4 x, int down) {
+    typedef short short2v __attribute__((ext_vector_type(2)));
     const float by = two_to(-down);
     u32x4 y;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float2v lo = __builtin_amdgcn_cvt_pk_f32_fp8(x[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(x[i], true);
-        y[i] = __builtin_amdgcn_cvt_pk_fp8_f32(lo[0] * by, lo[1] * by, 0, false);
-        y[i] = __builtin_amdgcn_cvt_pk_fp8_f32(hi[0] * by, hi[1] * by, y[i], true);
+        const half2v lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[i], by, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[i], by, true);
+        y[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(__builtin_amdgcn_cvt_scalef32_pk_fp8_f16(short2v{0, 0}, lo, 1.f, false), hi, 1.f, true));
     }
     return y;
 }
 
-// Scales slots of a page down, a piece of 16 elements per lane
-__device__ __forceinline__ void scale_slots(const Plane8& p, int page, int slot, int n, int per, int down, int lane) {
-    for (int x = lane; x < n * per; x += 64) {
-        u32x4* at = reinterpret_cast<u32x4*>(p.at + page * p.page + (slot + x / per) * p.slot + x % per * 16);
+// Scales n slots from `first` on down, a piece of 16 elements per lane of G
+template <int G>
+__device__ __forceinline__ void scale_slots(const Cache8& c, char* first, int64_t slot, int n, int down, int lane) {
+    for (int x = lane; x < n * c.per; x += G) {
+        const int row = row_of(c, x);
+        u32x4* at = reinterpret_cast<u32x4*>(first + row * slot + (x - row * c.per) * 16);
         *at = scaled_codes(*at, down);
     }
 }
 
+// MOST: the largest magnitude that is held, 1.875 * 2^15 and 1.875 * 2^127
 template <int DT> struct Put8Type;
-template <> struct Put8Type<SQ_F16> { static constexpr float MOST = 0x1.Ep15f; static __device__ __forceinline__ float get(uint32_t b) { return h2f((uint16_t)b); } };
-template <> struct Put8Type<SQ_BF16> { static constexpr float MOST = 0x1.Ep127f; static __device__ __forceinline__ float get(uint32_t b) { return bf2f((uint16_t)b); } };
+template <> struct Put8Type<SQ_F16> {
+    static constexpr uint32_t MOST = 0x7B80;
+    typedef half2v two;
+    static __device__ __forceinline__ float get(uint32_t b) { return h2f((uint16_t)b); }
+    template <bool HI, typename V> static __device__ __forceinline__ V codes(V old, uint32_t x, float scale) { return __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(old, __builtin_bit_cast(two, x), scale, HI); }
+};
+template <> struct Put8Type<SQ_BF16> {
+    static constexpr uint32_t MOST = 0x7F70;
+    typedef __bf16 two __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ float get(uint32_t b) { return bf2f((uint16_t)b); }
+    template <bool HI, typename V> static __device__ __forceinline__ V codes(V old, uint32_t x, float scale) { return __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(old, __builtin_bit_cast(two, x), scale, HI); }
+};
 
-// One wave per block that gets new tokens, head, and keys or values: the largest magnitude over its tokens, then the codes.  Up to 8 pieces of
-// 16 elements a lane stay in registers between the two (64 tokens of 128), larger blocks are read again.
+// One wave per block that gets new tokens, head, and keys or values: the largest magnitude over its tokens, then the codes.  Magnitudes order as their bits, so the largest is
+// looked for two elements at a time, and v_cvt_scalef32_pk_fp8 makes two codes of the elements as they are (one by one, as where some element is beyond what is
+// held, 8000 tokens of 8 heads of 128 took 15.0 us, not 12.1).  Up to 8 pieces of 16 elements a lane stay in registers between the two: 64 tokens of 128 a wave.  WAVES: four waves share
+// a block of more than that (8000 tokens of 4 heads of 256 in blocks of 64: 12.1 us, read twice by one wave 18.0); of more than four hold, the elements are read again.
 constexpr int PUT8_KEEP = 8;
-template <int DT>
+template <int DT, int WAVES>
 __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
     typedef Put8Type<DT> T;
-    const int lane = threadIdx.x & 63;
-    const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    constexpr int G = 64 * WAVES;                            // lanes of a block
+    const int lane = threadIdx.x % G;
+    const uint32_t unit = blockIdx.x * (4 / WAVES) + (WAVES == 1 ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) : 0);
     const bool v = unit & 1;
     const uint32_t run_of = (unit >> 1) / (uint32_t)a.c.heads;
     const int head = (int)((unit >> 1) - run_of * a.c.heads), b = (int)(run_of / (uint32_t)a.runs), run = (int)(run_of - (uint32_t)b * a.runs);
@@ -102,7 +136,7 @@ __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
     const int32_t id = a.table[b * a.ld_table + pg];
     if ((uint32_t)id >= (uint32_t)a.c.pages) return;
     const Plane8 p = plane_of(a.c, v, head);
-    const int off = (int)(from - pg * a.c.page), in_block = off % a.c.size, n = (int)(to - from), per = a.c.dim / 16, pieces = n * per;
+    const int off = (int)(from - pg * a.c.page), in_block = off % a.c.size, n = (int)(to - from), per = a.c.per, pieces = n * per;
     const int64_t t_b = v ? a.v_t : a.k_t;
     const char* in = (v ? a.v + head * a.v_h : a.k + head * a.k_h) + (first + (from - len)) * t_b;
     uint8_t* scale = p.scale + id * p.s_page + off / a.c.size * p.s_block;
@@ -112,47 +146,77 @@ __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
     auto load = [&](int j0) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < PUT8_KEEP; ++j)
-            if ((j0 + j) * 64 < pieces) {
-                const int i = min((j0 + j) * 64 + lane, pieces - 1), t = i / per;
+            if ((j0 + j) * G < pieces) {
+                const int i = min((j0 + j) * G + lane, pieces - 1), t = row_of(a.c, i);
                 const u32x4* at = reinterpret_cast<const u32x4*>(in + t * t_b + (i - t * per) * 32);
                 x[j][0] = at[0];
                 x[j][1] = at[1];
             }
     };
-    auto value = [&](int j, int i) __attribute__((always_inline)) { return T::get(x[j][i >> 3][(i & 7) >> 1] >> (16 * (i & 1)) & 0xFFFF); };
-    float top = 0.f;
-    for (int j0 = 0; j0 * 64 < pieces; j0 += PUT8_KEEP) {
+    typedef unsigned short pair __attribute__((ext_vector_type(2)));
+    pair both = {0, 0};
+    for (int j0 = 0; j0 * G < pieces; j0 += PUT8_KEEP) {
         load(j0);
 #pragma unroll
         for (int j = 0; j < PUT8_KEEP; ++j)
-            if ((j0 + j) * 64 < pieces)
+            if ((j0 + j) * G < pieces)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float m = fabsf(value(j, i));
-                    top = m < INFINITY ? fmaxf(top, m) : top;
-                }
+                for (int i = 0; i < 8; ++i) both = __builtin_elementwise_max(both, __builtin_bit_cast(pair, x[j][i >> 2][i & 3] & 0x7FFF7FFFu));
     }
-    // (magnitudes order as their bits)
-    const uint32_t bits = wave_max(__builtin_bit_cast(uint32_t, fminf(top, T::MOST)));
+    __shared__ uint32_t tops[2][WAVES];
+    auto most_of = [&](uint32_t v, int which) __attribute__((always_inline)) {
+        v = wave_max(v);
+        if constexpr (WAVES > 1) {
+            if (lane % 64 == 0) tops[which][lane / 64] = v;
+            __syncthreads();                                 // (which all waves pass behind having read the block's scale)
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) v = max(v, tops[which][w]);
+        }
+        return v;
+    };
+    uint32_t top = most_of(max((uint32_t)both[0], (uint32_t)both[1]), 0);
+    const bool plain = top <= T::MOST;
+    if (!plain) {                                            // the largest that is finite, or MOST
+        top = 0;
+        for (int j0 = 0; j0 * G < pieces; j0 += PUT8_KEEP) {
+            if (pieces > PUT8_KEEP * G) load(j0);
+#pragma unroll
+            for (int j = 0; j < PUT8_KEEP; ++j)
+                if ((j0 + j) * G < pieces)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const uint32_t m = x[j][i >> 3][(i & 7) >> 1] >> (16 * (i & 1)) & 0x7FFF;
+                        if (fabsf(T::get(m)) < INFINITY) top = max(top, m);
+                    }
+        }
+        top = most_of(min(top, T::MOST), 1);
+    }
+    const uint32_t bits = __builtin_bit_cast(uint32_t, T::get(top));
     int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFF) > 0x600000);
     e = max(max(e, -100), was - 127);
-    if (in_block && e > was - 127) scale_slots(p, id, off - in_block, in_block, per, e + 127 - was, lane);
+    if (in_block && e > was - 127) scale_slots<G>(a.c, p.at + id * p.page + (off - in_block) * p.slot, p.slot, in_block, e + 127 - was, lane);
     if (lane == 0) *scale = (uint8_t)(e + 127);
-    const float by = two_to(-e);
-    for (int j0 = 0; j0 * 64 < pieces; j0 += PUT8_KEEP) {
-        if (pieces > PUT8_KEEP * 64) load(j0);
+    const float by = two_to(-e), unit_of = two_to(e), most = T::get(T::MOST);
+    for (int j0 = 0; j0 * G < pieces; j0 += PUT8_KEEP) {
+        if (pieces > PUT8_KEEP * G) load(j0);
 #pragma unroll
         for (int j = 0; j < PUT8_KEEP; ++j)
-            if ((j0 + j) * 64 + lane < pieces) {
-                const int i = (j0 + j) * 64 + lane, t = i / per;
+            if ((j0 + j) * G + lane < pieces) {
+                const int i = (j0 + j) * G + lane, t = row_of(a.c, i);
                 u32x4 y;
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
+                    const uint32_t lo = x[j][d >> 1][2 * (d & 1)], hi = x[j][d >> 1][2 * (d & 1) + 1];
+                    if (plain) {
+                        typedef short short2v __attribute__((ext_vector_type(2)));
+                        y[d] = __builtin_bit_cast(uint32_t, T::template codes<true>(T::template codes<false>(short2v{0, 0}, lo, unit_of), hi, unit_of));
+                        continue;
+                    }
                     float f[4];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const float one = value(j, 4 * d + q);
-                        f[q] = fabsf(one) < INFINITY ? fminf(fmaxf(one, -T::MOST), T::MOST) * by : NAN;
+                        const float one = T::get((q & 2 ? hi : lo) >> (16 * (q & 1)) & 0xFFFF);
+                        f[q] = fabsf(one) < INFINITY ? fminf(fmaxf(one, -most), most) * by : NAN;
                     }
                     y[d] = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
                     y[d] = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], y[d], true);
@@ -162,83 +226,126 @@ __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
     }
 }
 
-// One wave per sequence, layer, head, and keys or values, a block that rows move to at a time.  The path ascends, so row i comes from a slot at or behind lens + i:
-// no row is read after its slot was written, and what goes to a block comes from it or from blocks behind it, whose scales have not changed yet.
-constexpr int KEEP8_FLY = 4;
+// One wave per sequence and U units (heads of a layer's keys or values), a block that rows move to at a time.  The path ascends, so row i comes from a slot at or
+// behind lens + i: no row is read after its slot was written, and what goes to a block comes from it or from blocks behind it, whose scales have not changed yet.
+// The path and the pages are looked up once for the units; then the scales and the first rows of all of them are in flight together, whatever blocks they go to, and further rows are
+// fetched as they come.  Bound by that chain of loads (lengths, path, pages, rows) and by what is worked out along it: 64 sequences, 28 layers of 4 heads, 8 rows of 128, 11.1 us for 14.7 MB
+// read and written, with a wave per unit 17.5; 256 sequences 29.7 and 52; one sequence 4.2.
+template <int U>
 __global__ __launch_bounds__(256) void keep8_kernel(Keep8Args a) {
     const int lane = threadIdx.x & 63, b = blockIdx.y;
-    const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    if (unit >= 2 * (uint32_t)a.layers * a.c.heads) return;
-    const uint32_t lk = unit / (uint32_t)a.c.heads, layer = lk >> 1;
-    const bool v = lk & 1;
-    const int head = (int)(unit - lk * a.c.heads);
-    Plane8 p = plane_of(a.c, v, head);
-    p.at += (int64_t)layer * (v ? a.v_layer : a.k_layer);
-    p.scale += (int64_t)layer * (v ? a.vs_layer : a.ks_layer);
-    const int count = min(a.counts[b], a.most), size = a.c.size, page = a.c.page, per = a.c.dim / 16, rows = 64 / per;
-    const int64_t len = max(a.lens[b], 0), cap = (int64_t)a.max_pages * page;
+    const bool v = blockIdx.z;
+    const uint32_t units = (uint32_t)a.layers * a.c.heads, first = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))) * U;
+    if (first >= units) return;
+    const Plane8 p = plane_of(a.c, v, 0);
+    char* at[U];
+    uint8_t* scale_at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {                            // (units behind the last one: the last one again, not written)
+        const uint32_t unit = min(first + u, units - 1), layer = unit / (uint32_t)a.c.heads;
+        const int64_t head = unit - layer * a.c.heads;
+        at[u] = p.at + layer * (v ? a.v_layer : a.k_layer) + head * (v ? a.c.v_head : a.c.k_head);
+        scale_at[u] = p.scale + layer * (v ? a.vs_layer : a.ks_layer) + head * (v ? a.c.vs_head : a.c.ks_head);
+    }
+    const int count = min(a.counts[b], a.most), per = a.c.per, rows = 64 / per, entries = 64 / rows * rows;         // rows of a wave's load, path entries looked up at once
+    const int64_t len = max(a.lens[b], 0), cap = (int64_t)a.max_pages * a.c.page;
+    const uint32_t size = a.c.size, page = a.c.page;
     const int32_t *path = a.path + b * a.ld_path, *table = a.table + b * a.ld_table;
-    // a lane's path entry: where it comes from and goes to, and the scale there
-    struct Entry { int src, src_off, dst, dst_off, scale, ok; };
-    auto look = [&](int w) __attribute__((always_inline)) {
-        Entry r = {0, 0, 0, 0, 0, 0};
-        const int i = w * 64 + lane, x = i < count ? path[i] : -1, before = i < count && i ? path[i - 1] : -1;
+    // a lane's path entry: where it comes from and goes to (bytes of a unit), its target's block, and the units' scales where it comes from
+    struct Entry { int64_t src, dst, block; int ok; };
+    Entry r;
+    uint32_t scale[U];
+    int window = -1;
+    auto at_window = [&](int w) __attribute__((always_inline)) {
+        if (w == window) return;
+        window = w;
+        r = {0, 0, 0, 0};
+        const int i = w * entries + lane, x = lane < entries && i < count ? path[i] : -1, before = x >= 0 && i ? path[i - 1] : -1;
         const int64_t s = len + x, d = len + i;
+        int64_t from = 0;
         if (x > max(before, -1) && s < cap && d < cap) {
-            const int sp = (int)(s / page), dp = (int)(d / page), src = table[sp], dst = table[dp];
+            const uint32_t sp = (uint32_t)s / page, dp = (uint32_t)d / page, so = (uint32_t)s - sp * page, to = (uint32_t)d - dp * page;
+            const int src = table[sp], dst = table[dp];
             if ((uint32_t)src < (uint32_t)a.c.pages && (uint32_t)dst < (uint32_t)a.c.pages) {
-                const int src_off = (int)(s - (int64_t)sp * page);
-                r = {src, src_off, dst, (int)(d - (int64_t)dp * page), p.scale[src * p.s_page + src_off / size * p.s_block], 1};
+                r = {src * p.page + so * p.slot, dst * p.page + to * p.slot, dst * p.s_page + to / size * p.s_block, 1};
+                from = src * p.s_page + so / size * p.s_block;
             }
         }
-        return r;
+#pragma unroll
+        for (int u = 0; u < U; ++u) scale[u] = scale_at[u][from];
     };
-    Entry r = {};
-    int window = -1;
-    auto at_window = [&](int w) __attribute__((always_inline)) { if (w != window) { r = look(w); window = w; } };
+    auto of_lane = [](int64_t x, int l) __attribute__((always_inline)) {
+        return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, l) | (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32;
+    };
+    // a load's rows: from rows * chunk on
+    const int row = min(row_of(a.c, lane), rows - 1), piece = lane - row * per;
+    const bool whole = piece < per;                          // (a last lane may have no row)
+    u32x4 x[U];
+    int chunk = -1;
+    auto fetch = [&](int c) __attribute__((always_inline)) {
+        if (c == chunk) return;
+        chunk = c;
+        const int64_t src = __shfl(r.src, (c * rows + row) % entries) + min(piece, per - 1) * 16;
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const u32x4*>(at[u] + src);
+    };
+    at_window(0);
+    fetch(0);
+    uint32_t was[U];                                         // the scales of the block that the first row goes to
+    const int64_t block0 = of_lane(r.block, 0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) was[u] = scale_at[u][block0];
     int m = 0;
-    for (int w = 0; w * 64 < count; ++w) {
+    for (int w = 0; w * entries < count; ++w) {
         at_window(w);
-        const uint64_t all = __ballot(r.ok);
-        m = all == ~0ull ? (w + 1) * 64 : w * 64 + __builtin_ctzll(~all);
+        const uint64_t all = __ballot(r.ok) | (entries < 64 ? ~0ull << entries : 0);
+        m = w * entries + (all == ~0ull ? entries : __builtin_ctzll(~all));
         if (all != ~0ull) break;
     }
-    if (m == 0) return;
-    for (int64_t block = len / size; block * size < len + m; ++block) {
-        const int lo = (int)max((int64_t)0, block * size - len), hi = (int)min((int64_t)m, (block + 1) * size - len), w0 = lo / 64, w1 = (hi - 1) / 64;
+    const int in_first = (int)(len % size);                  // cached tokens in that block
+    for (int lo = 0, hi; lo < m; lo = hi) {
+        const int held = lo ? 0 : in_first, w0 = lo / entries;
+        hi = min(m, lo + (int)size - held);
+        const int w1 = (hi - 1) / entries;
         at_window(w0);
-        const int to = __builtin_amdgcn_readlane(r.dst, lo & 63), to_off = __builtin_amdgcn_readlane(r.dst_off, lo & 63), in_block = to_off % size;
-        uint8_t* to_scale = p.scale + to * p.s_page + to_off / size * p.s_block;
-        const int was = in_block ? *to_scale : 0;
-        uint32_t e = was;
+        const int64_t to = of_lane(r.dst, lo - w0 * entries), block = of_lane(r.block, lo - w0 * entries);
+        uint32_t e[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) e[u] = 0;
         for (int w = w0; w <= w1; ++w) {
             at_window(w);
-            const int i = w * 64 + lane;
-            e = max(e, wave_max(i >= lo && i < hi ? (uint32_t)r.scale : 0u));
-        }
-        if (in_block && (int)e > was) scale_slots(p, to, to_off - in_block, in_block, per, (int)e - was, lane);
-        for (int w = w0; w <= w1; ++w) {
-            at_window(w);
-            const int end = min(hi, (w + 1) * 64);
-            for (int i0 = max(lo, w * 64); i0 < end; i0 += rows * KEEP8_FLY) {
-                u32x4 x[KEEP8_FLY];
-                int down[KEEP8_FLY];
-                char* at[KEEP8_FLY];
-                const int row = lane / per, piece = lane - row * per;
+            const int i = w * entries + lane;
+            const bool mine = lane < entries && i >= lo && i < hi;
 #pragma unroll
-                for (int j = 0; j < KEEP8_FLY; ++j) {
-                    const int i = i0 + j * rows + row, l = min(i, end - 1) & 63;
-                    const int from = __shfl(r.src, l), from_off = __shfl(r.src_off, l), goes = __shfl(r.dst, l), goes_off = __shfl(r.dst_off, l);
-                    down[j] = (int)e - __shfl(r.scale, l);
-                    at[j] = i < end && row < rows ? p.at + goes * p.page + goes_off * p.slot + piece * 16 : nullptr;
-                    if (at[j]) x[j] = *reinterpret_cast<const u32x4*>(p.at + from * p.page + from_off * p.slot + piece * 16);
-                }
-#pragma unroll
-                for (int j = 0; j < KEEP8_FLY; ++j)
-                    if (at[j]) *reinterpret_cast<u32x4*>(at[j]) = down[j] ? scaled_codes(x[j], down[j]) : x[j];
+            for (int u = 0; u < U; u += 2) {                 // (two units' at a time)
+                const uint32_t two = mine ? scale[u] | (u + 1 < U ? scale[min(u + 1, U - 1)] << 16 : 0u) : 0u, most = wave_max2(two);
+                e[u] = max(e[u], most & 0xFFFF);
+                if (u + 1 < U) e[min(u + 1, U - 1)] = max(e[min(u + 1, U - 1)], most >> 16);
             }
         }
-        if (lane == 0) *to_scale = (uint8_t)e;
+        if (held)
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int down = (int)e[u] - (int)was[u];
+                e[u] = max(e[u], was[u]);
+                if (first + u < units && down > 0) scale_slots<64>(a.c, at[u] + to - held * p.slot, p.slot, held, down, lane);
+            }
+        for (int c = lo / rows; c * rows < hi; ++c) {
+            at_window(c * rows / entries);
+            fetch(c);
+            const int i = c * rows + row, l = i % entries;
+            const int64_t dst = __shfl(r.dst, l) + piece * 16;
+            const bool mine = whole && i >= lo && i < hi;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int down = (int)e[u] - __shfl((int)scale[u], l);
+                if (mine && first + u < units) *reinterpret_cast<u32x4*>(at[u] + dst) = down ? scaled_codes(x[u], down) : x[u];
+            }
+        }
+        if (lane == 0)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (first + u < units) scale_at[u][block] = (uint8_t)e[u];
     }
 }
 
@@ -257,7 +364,7 @@ int check_cache8(const char* who, const sq_cache8* c) {
 
 static Cache8 cache8_of(const sq_cache8& c) {
     return {(char*)c.k, (char*)c.v, c.k_scale, c.v_scale, c.k_page, c.k_slot, c.k_head, c.v_page, c.v_slot, c.v_head, c.ks_page, c.ks_block, c.ks_head,
-            c.vs_page, c.vs_block, c.vs_head, c.pages, c.page, c.blocks, c.page / c.blocks, c.heads, c.dim};
+            c.vs_page, c.vs_block, c.vs_head, c.pages, c.page, c.blocks, c.page / c.blocks, c.heads, c.dim, c.dim / 16, (uint32_t)(((1ull << 32) + c.dim / 16 - 1) / (c.dim / 16))};
 }
 
 }  // namespace sq
@@ -288,10 +395,12 @@ int sq_put_tokens8(const sq_heads* k, const sq_heads* v, int32_t tokens, int dty
     a.table = table; a.ld_table = ld_table; a.max_pages = max_pages; a.lens = lens; a.starts = starts;
     a.tokens = tokens; a.seqs = seqs; a.most_new = most_new;
     a.runs = (int)(((int64_t)most_new + 2 * a.c.size - 2) / a.c.size);          // the first token may be its block's last
-    const int64_t units = 2 * (int64_t)seqs * a.runs * a.c.heads, groups = (units + 3) / 4;
+    const bool shared = (int64_t)(a.c.size < most_new ? a.c.size : most_new) * a.c.per > PUT8_KEEP * 64;
+    const int64_t units = 2 * (int64_t)seqs * a.runs * a.c.heads, groups = shared ? units : (units + 3) / 4;
     if (groups > (1 << 23)) return fail(SQ_EUNSUPPORTED, "%s: %d sequences of up to %d new tokens and %d heads at once", who, seqs, most_new, cache->heads);
-    if (dtype == SQ_F16) hipLaunchKernelGGL(put8_kernel<SQ_F16>, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(put8_kernel<SQ_BF16>, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, a);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, a); };
+    if (dtype == SQ_F16) go(shared ? put8_kernel<SQ_F16, 4> : put8_kernel<SQ_F16, 1>);
+    else go(shared ? put8_kernel<SQ_BF16, 4> : put8_kernel<SQ_BF16, 1>);
     return check_launch(who);
 }
 
@@ -311,9 +420,14 @@ int sq_keep_drafted8(const sq_cache8* cache, int32_t layers, int64_t k_layer, in
     a.k_layer = k_layer; a.v_layer = v_layer; a.ks_layer = ks_layer; a.vs_layer = vs_layer;
     a.table = table; a.ld_table = ld_table; a.max_pages = max_pages; a.lens = lens; a.path = path; a.ld_path = ld_path; a.counts = counts;
     a.layers = layers; a.most = most;
-    const int64_t groups = (2 * (int64_t)layers * a.c.heads + 3) / 4;
+    // (few units: a wave each, more of them at once)
+    const int64_t units = (int64_t)layers * a.c.heads;
+    const int each = 2 * units * seqs > 16 * device_cus() ? 4 : 1;
+    const int64_t groups = (units + 4 * each - 1) / (4 * each);
     if (groups > (1 << 23)) return fail(SQ_EUNSUPPORTED, "%s: %d layers of %d heads", who, layers, cache->heads);
-    hipLaunchKernelGGL(keep8_kernel, dim3((unsigned)groups, (unsigned)seqs), dim3(256), 0, (hipStream_t)stream, a);
+    const dim3 grid((unsigned)groups, (unsigned)seqs, 2);
+    if (each == 4) hipLaunchKernelGGL(keep8_kernel<4>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL(keep8_kernel<1>, grid, dim3(256), 0, (hipStream_t)stream, a);
     return check_launch(who);
 }
 
