@@ -16,6 +16,8 @@ namespace sq {
 // Over a cache held in 8 bits a compute unit holds two of the few-row workgroups (four of heads up to 64), and sequences are also cut into parts of 20 steps a wave, which ends
 // them closer together: 64 sequences of 8192 slots x 8 key heads in three parts 205 us, whole 218; of 2,240 to 8,192 131 and 152; 32 of those 72 and 91; 32 of 4000 x 2 key heads of 64 in
 // eight 12.9, in four 14.3.
+// One of up to four steps a wave is not cut (a step takes 0.6 us then: one token behind 500 slots 8.7 us call by call, in four parts 10.1; captured 8.5 and 8.1; of heads of 256 12.1 and 9.9,
+// which are).
 // A sequence's length is its table's width here: lengths are on the device.  Under a table of 131,072 slots one token behind 500 takes 10.2 us instead of 8.8, 48 26.7 instead of 21.4,
 // 64 sequences of 500 27.9 instead of 18.6, 64 of 2000 59.8 instead of 53.1.
 AttnPlan attn_plan(const sq_attention& a, const sq_cache& c, bool held8) {
@@ -29,7 +31,7 @@ AttnPlan attn_plan(const sq_attention& a, const sq_cache& c, bool held8) {
         p.mt = rows <= 16 ? 1 : 2;
         per = p.mt * 16;
         most = steps / waves;
-        if (most <= 2) most = 1;
+        if (most <= (held8 && p.dp < 256 ? 4 : 2)) most = 1;
     } else {
         p.mt = attn_tiles(p.dp);
         p.nw = rows <= 4 * 16 * p.mt ? 4 : 8;

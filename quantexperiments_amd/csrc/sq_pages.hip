@@ -18,7 +18,7 @@ struct PageArgs {
     PagePlane p[PLANES_MAX];
     int first[PLANES_MAX + 1];                 // chunk that a plane begins with; the last: how many there are
     const int32_t *table, *lens, *parent, *fresh;
-    int32_t *out_table, *out_lens, *used, *ws; // ws: pages that move, [16 ..] to where, [16 + pages ..] which, [16 + 2 pages ..] new place by page
+    int32_t *out_table, *out_lens, *used, *ws; // ws: pages that move, [16 ..] to where, [16 + pages ..] which
     int64_t ld_table, ld_out;
     int layers, pages, page, max_pages, seqs;
 };
@@ -85,83 +85,89 @@ __global__ __launch_bounds__(256) void fork_kernel(PageArgs a) {
 }
 
 // Which pages move where: one workgroup, a bit per page in LDS.  With n pages in use, the ones from n on move to the free ones before n, in
-// order; no page is both, so they move in any order, and a call made again on the same tables does the same again.
+// order; no page is both, so they move in any order, and a call made again on the same tables does the same again.  A page's place among those in use is the sum of the bits
+// before it: of whole groups of 256 pages added up beforehand, and of its own.  Bound by its chain (lengths, entries, sums, lists, entries again): 24 sequences
+// of 32 entries, 1024 pages 4.5 us, behind 460 MB of other traffic 8.3.
+constexpr int COMPACT_GROUP = 8;                   // words of 32 pages
 __global__ __launch_bounds__(1024) void compact_plan_kernel(PageArgs a) {
-    extern __shared__ uint32_t used[];
-    __shared__ int part[16], total, before_n;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, words = (a.pages + 31) / 32;
-    int32_t *holes = a.ws + 16, *movers = holes + a.pages, *place = movers + a.pages;
+    extern __shared__ uint32_t used[];             // bits, then sums before groups
+    __shared__ int part[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, groups = (a.pages + 32 * COMPACT_GROUP - 1) / (32 * COMPACT_GROUP), words = groups * COMPACT_GROUP;
+    int* before = reinterpret_cast<int*>(used + words);
+    int32_t *holes = a.ws + 16, *movers = holes + a.pages;
     for (int i = tid; i < words; i += 1024) used[i] = 0;
     __syncthreads();
     constexpr int FLY = 8;
     auto entries = [&](int b) { return (int)min(((int64_t)max(a.lens[b], 0) + a.page - 1) / a.page, (int64_t)a.max_pages); };
-    for (int b = wave; b < a.seqs; b += 16) {
-        const int n = entries(b);
-        const int32_t* row = a.table + b * a.ld_table;
-        for (int j0 = 0; j0 < n; j0 += 64 * FLY) {
-            int32_t id[FLY];
+    // the wave's sequences, 64 * FLY entries at a time
+    auto walk = [&](auto f) __attribute__((always_inline)) {
+        for (int b = wave; b < a.seqs; b += 16) {
+            const int n = entries(b);
+            const int32_t* row = a.table + b * a.ld_table;
+            for (int j0 = 0; j0 < a.max_pages; j0 += 64 * FLY) {
+                int32_t id[FLY];                   // (fetched beside the length, not behind it)
 #pragma unroll
-            for (int x = 0; x < FLY; ++x) id[x] = j0 + x * 64 + lane < n ? row[j0 + x * 64 + lane] : -1;
+                for (int x = 0; x < FLY; ++x)
+                    if (j0 + x * 64 < a.max_pages) id[x] = row[min(j0 + x * 64 + lane, a.max_pages - 1)];
 #pragma unroll
-            for (int x = 0; x < FLY; ++x)
-                if ((uint32_t)id[x] < (uint32_t)a.pages) atomicOr(&used[id[x] >> 5], 1u << (id[x] & 31));
+                for (int x = 0; x < FLY; ++x)
+                    if (j0 + x * 64 < a.max_pages) f(b, j0 + x * 64 + lane, j0 + x * 64 + lane < n ? id[x] : -1);
+            }
         }
-    }
+    };
+    walk([&](int, int, int32_t id) { if ((uint32_t)id < (uint32_t)a.pages) atomicOr(&used[id >> 5], 1u << (id & 31)); });
     __syncthreads();
-    const int per = (words + 1023) / 1024, w0 = min(tid * per, words), w1 = min(w0 + per, words);
-    int mine = 0;
-    for (int w = w0; w < w1; ++w) mine += __popc(used[w]);
-    int upto = mine;
+    // sums of groups, and before each of them
+    int n = 0;                                     // in use so far, of all at last
+    for (int g0 = 0; g0 < groups; g0 += 1024) {
+        int mine = 0, upto;
+        if (g0 + tid < groups)
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1) {
-        const int v = __shfl_up(upto, x);
-        if (lane >= x) upto += v;
-    }
-    if (lane == 63) part[wave] = upto;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) upto += part[w];
-    if (tid == 1023) {
-        total = upto;
-        before_n = upto;                           // (all pages in use: there is no page n)
-    }
-    __syncthreads();
-    const int n = total, first = upto - mine;
-    if ((n >> 5) >= w0 && (n >> 5) < w1) {
-        int v = first;
-        for (int w = w0; w < n >> 5; ++w) v += __popc(used[w]);
-        before_n = v + __popc(used[n >> 5] & ((1u << (n & 31)) - 1));
-    }
-    __syncthreads();
-    const int kept = before_n;                     // pages in use before n
-    int rank = first;
-    for (int w = w0; w < w1; ++w) {
-        const uint32_t bits = used[w], below = n - w * 32 >= 32 ? ~0u : n - w * 32 <= 0 ? 0u : (1u << (n - w * 32)) - 1;
-        for (uint32_t free = ~bits & below; free; free &= free - 1) {
-            const int x = __builtin_ctz(free);
-            holes[w * 32 + x - (rank + __popc(bits & ((1u << x) - 1)))] = w * 32 + x;
+            for (int w = 0; w < COMPACT_GROUP; ++w) mine += __popc(used[(g0 + tid) * COMPACT_GROUP + w]);
+        upto = mine;
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) {
+            const int v = __shfl_up(upto, x);
+            if (lane >= x) upto += v;
         }
-        for (uint32_t move = bits & ~below; move; move &= move - 1) {
-            const int x = __builtin_ctz(move);
-            movers[rank + __popc(bits & ((1u << x) - 1)) - kept] = w * 32 + x;
+        if (lane == 63) part[wave] = upto;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) upto += part[w];
+            all += part[w];
         }
-        rank += __popc(bits);
+        if (g0 + tid < groups) before[g0 + tid] = n + upto - mine;
+        n += all;
+        __syncthreads();
     }
-    __syncthreads();
-    for (int i = tid; i < n - kept; i += 1024) place[movers[i]] = holes[i];
+    auto rank = [&](int id) __attribute__((always_inline)) {         // pages in use before page id
+        const int g = id / (32 * COMPACT_GROUP), w = id >> 5;
+        int v = before[g] + __popc(used[w] & ((1u << (id & 31)) - 1));
+#pragma unroll
+        for (int x = 0; x < COMPACT_GROUP - 1; ++x)
+            if (g * COMPACT_GROUP + x < w) v += __popc(used[g * COMPACT_GROUP + x]);
+        return v;
+    };
+    const int kept = n < a.pages ? rank(n) : n;    // pages in use before page n
+    for (int id = tid; id < a.pages; id += 1024) {
+        const bool on = used[id >> 5] >> (id & 31) & 1;
+        if (on == (id < n)) continue;
+        const int v = rank(id);
+        if (on) movers[v - kept] = id;
+        else holes[id - v] = id;
+    }
     if (tid == 0) {
         a.ws[0] = n - kept;
         a.used[0] = n;
     }
     __syncthreads();
-    for (int b = wave; b < a.seqs; b += 16) {
-        const int m = entries(b);
-        for (int j = lane; j < a.max_pages; j += 64) {
-            int32_t id = a.table[b * a.ld_table + j];
-            if (j >= m) id = -1;
-            else if ((uint32_t)id < (uint32_t)a.pages && id >= n) id = place[id];
-            a.out_table[b * a.ld_out + j] = id;
-        }
-    }
+    walk([&](int b, int j, int32_t id) {
+        if (j >= a.max_pages) return;
+        if (id >= n && id < a.pages) id = holes[rank(id) - kept];
+        a.out_table[b * a.ld_out + j] = id;
+    });
 }
 
 __global__ __launch_bounds__(256) void compact_move_kernel(PageArgs a) {
@@ -234,7 +240,7 @@ int sq_fork_pages(const sq_plane* planes, int32_t n_planes, int32_t layers, int3
     return check_launch(who);
 }
 
-size_t sq_compact_pages_workspace_bytes(int32_t pages) { return pages < 0 || pages > PAGES_MAX ? 0 : (16 + 3 * (size_t)pages) * 4; }
+size_t sq_compact_pages_workspace_bytes(int32_t pages) { return pages < 0 || pages > PAGES_MAX ? 0 : (16 + 2 * (size_t)pages) * 4; }
 
 int sq_compact_pages(const sq_plane* planes, int32_t n_planes, int32_t layers, int32_t pages, int32_t page, const int32_t* table, int64_t ld_table, int32_t max_pages,
                      const int32_t* lens, int32_t seqs, int32_t* out_table, int64_t ld_out, int32_t* used, void* workspace, size_t ws_bytes, void* stream) {
@@ -248,11 +254,12 @@ int sq_compact_pages(const sq_plane* planes, int32_t n_planes, int32_t layers, i
     const size_t need = sq_compact_pages_workspace_bytes(pages);
     if (ws_bytes < need || !workspace || ((uintptr_t)workspace & 255)) return fail(SQ_EWORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who, need, ws_bytes);
     a.used = used; a.ws = (int32_t*)workspace;
-    const unsigned lds = (unsigned)((pages + 31) / 32 * 4);
+    const auto lds_of = [](int pages) { return (unsigned)((pages + 32 * COMPACT_GROUP - 1) / (32 * COMPACT_GROUP) * (4 * COMPACT_GROUP + 4)); };
+    const unsigned lds = lds_of(pages);
     static bool raised[64];
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
-    if (lds > 48 * 1024 && !raised[dev]) raised[dev] = hipFuncSetAttribute((const void*)compact_plan_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, PAGES_MAX / 8) == hipSuccess;
+    if (lds > 48 * 1024 && !raised[dev]) raised[dev] = hipFuncSetAttribute((const void*)compact_plan_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds_of(PAGES_MAX)) == hipSuccess;
     hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(1024), lds, (hipStream_t)stream, a);
     if (int rc = check_launch(who)) return rc;
     const int64_t most = (int64_t)seqs * max_pages < pages / 2 ? (int64_t)seqs * max_pages : pages / 2, all = most * a.first[PLANES_MAX];
