@@ -248,6 +248,7 @@ struct Attn8Args : AttnArgs {
     int64_t ks_page, ks_block, ks_head, vs_page, vs_block, vs_head;
     int size;                    // tokens of a block, a multiple of 16
     int together;                // few rows: the heads of the same keys are dealt to one die
+    int passing;                 // few rows: keys and values are read past the caches
 };
 
 // 8 codes times a power of two as a matrix instruction's operand: v_cvt_scalef32_pk takes two at a time and the scale with them, exactly

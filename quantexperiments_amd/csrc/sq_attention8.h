@@ -25,8 +25,11 @@ template <int DP> struct Attn8Tile {
     }
 };
 
-// Copies 16 keys (or values), of half x of a step, to `to`; from: the first one's byte of the head
-template <int DP, bool FULL, bool VALUES>
+// Copies 16 keys (or values), of half x of a step, to `to`; from: the first one's byte of the head.  PASSING: past the caches (see attn_copy16)
+__device__ __forceinline__ void attn8_copy16_passing(uint32_t to, const char* at, uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(to), "v"(offset), "s"(at) : "memory");
+}
+template <int DP, bool FULL, bool VALUES, bool PASSING>
 __device__ __forceinline__ void attn8_copy(const Attn8Args& a, int x, int lane, const char* from, const char* to) {
     typedef Attn8Tile<DP> T;
     const int row = lane / T::PIECES, pos = lane % T::PIECES, pieces = a.dim >> 4, slot = (int)(VALUES ? a.v_slot : a.k_slot);
@@ -34,7 +37,10 @@ __device__ __forceinline__ void attn8_copy(const Attn8Args& a, int x, int lane, 
 #pragma unroll
     for (int j = 0; j < 16 / T::ROWS; ++j) {
         const int key = 16 * x + j * T::ROWS + row, c = pos ^ (VALUES ? T::v_xor(key) : T::k_xor(key));
-        if (FULL || c < pieces) attn_copy16(lds + j * 1024, from, (uint32_t)((j * T::ROWS + row) * slot + c * 16));
+        if (FULL || c < pieces) {
+            if constexpr (PASSING) attn8_copy16_passing(lds + j * 1024, from, (uint32_t)((j * T::ROWS + row) * slot + c * 16));
+            else attn_copy16(lds + j * 1024, from, (uint32_t)((j * T::ROWS + row) * slot + c * 16));
+        }
     }
 }
 
@@ -131,7 +137,7 @@ template <int DP, int MT, int NW> constexpr int attn8_lds() {
 }
 
 // Few rows, as attn_kernel: the waves of a workgroup share the rows and split its keys, no barrier until their sums are joined.
-template <int DT, int DP, int MT, int NW, bool FULL>
+template <int DT, int DP, int MT, int NW, bool FULL, bool PASSING>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW * attn8_groups(DP, MT) / 4, NW * attn8_groups(DP, MT) / 4))) void attn8_kernel(Attn8Args a) {
     typedef Attn8Tile<DP> T;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -172,11 +178,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW * at
             attn8_copy_scale(to + 256, groups.vs);
         }
 #pragma unroll
-        for (int x = 0; x < 2; ++x) attn8_copy<DP, FULL, false>(a, x, lane, kb + groups.lane64(groups.k, 2 * (n % 32) + x), slot(i) + x * 16 * T::PITCH);
+        for (int x = 0; x < 2; ++x) attn8_copy<DP, FULL, false, PASSING>(a, x, lane, kb + groups.lane64(groups.k, 2 * (n % 32) + x), slot(i) + x * 16 * T::PITCH);
     };
     auto get_v = [&](int i) __attribute__((always_inline)) {         // (behind get_k of the same step)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) attn8_copy<DP, FULL, true>(a, x, lane, vb + groups.lane64(groups.v, 2 * ((i - w0) % 32) + x), slot(i) + T::BYTES + x * 16 * T::PITCH);
+        for (int x = 0; x < 2; ++x) attn8_copy<DP, FULL, true, PASSING>(a, x, lane, vb + groups.lane64(groups.v, 2 * ((i - w0) % 32) + x), slot(i) + T::BYTES + x * 16 * T::PITCH);
     };
     if constexpr (!FULL) {
         attn_clear(ring, RING * 2 * T::BYTES, lane, 64);
@@ -248,12 +254,12 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW * at
 
 // ------------------------------------------------------------------------------------------ host
 
-template <int DT, int DP, int MT, bool FULL>
+template <int DT, int DP, int MT, bool FULL, bool PASSING>
 int attn8_launch_few(const Attn8Args& a, unsigned grid, hipStream_t s) {
     constexpr int NW = ATTN8_WAVES, LDS = attn8_lds<DP, MT, NW>();
     static bool raised[64];
-    attn_raise((const void*)attn8_kernel<DT, DP, MT, NW, FULL>, LDS, raised);
-    hipLaunchKernelGGL((attn8_kernel<DT, DP, MT, NW, FULL>), dim3(grid), dim3(NW * 64), LDS, s, a);
+    attn_raise((const void*)attn8_kernel<DT, DP, MT, NW, FULL, PASSING>, LDS, raised);
+    hipLaunchKernelGGL((attn8_kernel<DT, DP, MT, NW, FULL, PASSING>), dim3(grid), dim3(NW * 64), LDS, s, a);
     return check_launch("sq_tree_attention8");
 }
 template <int DT, int DP, int NW, bool FULL>
@@ -269,7 +275,14 @@ int attn8_launch_dim(const Attn8Args& a, const AttnPlan& p, hipStream_t s) {
     const unsigned grid = (unsigned)((int64_t)a.seqs * a.kv_heads * ((p.row_blocks - 1) * p.splits + p.last_splits));
     int rc;
     if (p.nw) rc = p.nw == 4 ? attn8_launch_many<DT, DP, 4, FULL>(a, grid, s) : attn8_launch_many<DT, DP, 8, FULL>(a, grid, s);
-    else rc = p.mt == 1 ? attn8_launch_few<DT, DP, 1, FULL>(a, grid, s) : attn8_launch_few<DT, DP, DP == 256 ? 1 : 2, FULL>(a, grid, s);
+    else {
+        auto few = [&](auto passing) {
+            constexpr bool P = decltype(passing)::value;
+            return p.mt == 1 ? attn8_launch_few<DT, DP, 1, FULL, P>(a, grid, s) : attn8_launch_few<DT, DP, DP == 256 ? 1 : 2, FULL, P>(a, grid, s);
+        };
+        constexpr bool lines = FULL && DP >= 128;            // (heads that are lines of their own: nobody else reads them)
+        rc = lines && a.passing ? few(std::integral_constant<bool, lines>()) : few(std::false_type());
+    }
     return rc || p.splits == 1 ? rc : attn_launch_join<DT, DP>(a, s);
 }
 template <int DT>

@@ -3,6 +3,7 @@
 // A block of tokens of one head has one scale 2^e, and an element x the code rne_e4m3(x * 2^-e): three bits of mantissa whatever e is, down to 2^-6 of the scale, so a
 // scale that is a power of two loses nothing beside the exact a / 448 but, at worst, the last of the bits below that.  It buys that attention multiplies by the scale while it
 // unpacks codes, exactly, and that a block whose scale grows with later tokens is scaled to it without another rounding (below 2^-6: with one).
+#include <type_traits>
 #include "sq_common.h"
 
 namespace sq {
@@ -109,8 +110,9 @@ template <> struct Put8Type<SQ_BF16> {
 // looked for two elements at a time, and v_cvt_scalef32_pk_fp8 makes two codes of the elements as they are (one by one, as where some element is beyond what is
 // held, 8000 tokens of 8 heads of 128 took 15.0 us, not 12.1).  Up to 8 pieces of 16 elements a lane stay in registers between the two: 64 tokens of 128 a wave.  WAVES: four waves share
 // a block of more than that (8000 tokens of 4 heads of 256 in blocks of 64: 12.1 us, read twice by one wave 18.0); of more than four hold, the elements are read again.
+constexpr int64_t PUT8_CACHED = 4 << 20;         // bytes of codes up to which they stay in the caches for who reads them next (16 MB: 11.9 us, past them 10.3)
 constexpr int PUT8_KEEP = 8;
-template <int DT, int WAVES>
+template <int DT, int WAVES, bool PASSING>
 __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
     typedef Put8Type<DT> T;
     constexpr int G = 64 * WAVES;                            // lanes of a block
@@ -221,7 +223,8 @@ __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
                     y[d] = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
                     y[d] = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], y[d], true);
                 }
-                *reinterpret_cast<u32x4*>(p.at + id * p.page + (off + t) * p.slot + (i - t * per) * 16) = y;
+                u32x4* to = reinterpret_cast<u32x4*>(p.at + id * p.page + (off + t) * p.slot + (i - t * per) * 16);
+                if constexpr (PASSING) __builtin_nontemporal_store(y, to); else *to = y;
             }
     }
 }
@@ -399,8 +402,12 @@ int sq_put_tokens8(const sq_heads* k, const sq_heads* v, int32_t tokens, int dty
     const int64_t units = 2 * (int64_t)seqs * a.runs * a.c.heads, groups = shared ? units : (units + 3) / 4;
     if (groups > (1 << 23)) return fail(SQ_EUNSUPPORTED, "%s: %d sequences of up to %d new tokens and %d heads at once", who, seqs, most_new, cache->heads);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, a); };
-    if (dtype == SQ_F16) go(shared ? put8_kernel<SQ_F16, 4> : put8_kernel<SQ_F16, 1>);
-    else go(shared ? put8_kernel<SQ_BF16, 4> : put8_kernel<SQ_BF16, 1>);
+    auto of = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if ((int64_t)tokens * a.c.heads * a.c.dim * 2 > PUT8_CACHED) go(shared ? put8_kernel<DT, 4, true> : put8_kernel<DT, 1, true>);
+        else go(shared ? put8_kernel<DT, 4, false> : put8_kernel<DT, 1, false>);
+    };
+    if (dtype == SQ_F16) of(std::integral_constant<int, SQ_F16>()); else of(std::integral_constant<int, SQ_BF16>());
     return check_launch(who);
 }
 
