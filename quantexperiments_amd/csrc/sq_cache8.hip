@@ -181,7 +181,7 @@ __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
     if (!plain) {                                            // the largest that is finite, or MOST
         top = 0;
         for (int j0 = 0; j0 * G < pieces; j0 += PUT8_KEEP) {
-            if (pieces > PUT8_KEEP * G) load(j0);
+            if (WAVES > 1 && pieces > PUT8_KEEP * G) load(j0);          // (one wave has all of its pieces)
 #pragma unroll
             for (int j = 0; j < PUT8_KEEP; ++j)
                 if ((j0 + j) * G < pieces)
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
     if (lane == 0) *scale = (uint8_t)(e + 127);
     const float by = two_to(-e), unit_of = two_to(e), most = T::get(T::MOST);
     for (int j0 = 0; j0 * G < pieces; j0 += PUT8_KEEP) {
-        if (pieces > PUT8_KEEP * G) load(j0);
+        if (WAVES > 1 && pieces > PUT8_KEEP * G) load(j0);          // (one wave has all of its pieces)
 #pragma unroll
         for (int j = 0; j < PUT8_KEEP; ++j)
             if ((j0 + j) * G + lane < pieces) {

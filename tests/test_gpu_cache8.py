@@ -125,6 +125,42 @@ def test_put_layouts(permute):
     pool.assert_same(*dev)
 
 
+@pytest.mark.parametrize("dim,n,odd", [(128, 700, False), (128, 700, True), (16, 2100, True), (256, 60, True)])
+def test_put_of_large_blocks(dim, n, odd):
+    """More elements in a block than a workgroup holds, and more than a wave does; some that are not finite or beyond what is held."""
+    g = torch.Generator().manual_seed(dim)
+    page = {16: 2048, 128: 1024, 256: 64}[dim]
+    lens, news = [page // 4, 0], [n, 3]
+    table, pages, _ = table_for([a + b for a, b in zip(lens, news)], page, g)
+    pool = Pool(pages, page, 1, 2, dim, g)
+    k, v = tokens(sum(news), 2, dim, "bf16", g)
+    k, v = k.clone(), v.clone()
+    if odd:
+        k[n // 2, 0, 3], k[1, 1, 5], v[n - 1, 0, 0] = float("inf"), float("nan"), 3.3e38
+    got = put(pool, k, v, table, lens, news)
+    pool.put(k, v, table, lens, starts_of(news))
+    pool.assert_same(*got)
+
+
+def test_put_into_strided_scales():
+    """Scales whose heads are apart, blocks inside heads; the bytes between them stay."""
+    from quantexperiments_amd.kernels import put_tokens8
+    g = torch.Generator().manual_seed(15)
+    lens, news = [9, 30], [40, 3]
+    table, pages, _ = table_for([a + b for a, b in zip(lens, news)], 32, g)
+    pool = Pool(pages, 32, 2, 3, 32, g)
+    kc, vc, _, _ = pool.device()
+    wide = [torch.full((3, pages, 5), 9, dtype=torch.uint8, device="cuda") for _ in range(2)]              # [heads, pages, blocks ..]
+    scales = [w.view(torch.float8_e8m0fnu)[..., 1:3].permute(1, 2, 0) for w in wide]
+    for i, w in enumerate(wide):
+        w[..., 1:3] = pool.scales[i].permute(2, 0, 1).cuda()
+    k, v = tokens(43, 3, 32, "f16", g)
+    put_tokens8(k.cuda(), v.cuda(), kc, vc, *scales, table.cuda(), i32(lens), i32(starts_of(news)))
+    pool.put(k, v, table, lens, starts_of(news))
+    pool.assert_same(kc, vc, *scales)
+    assert all(bool((w[..., 0] == 9).all()) and bool((w[..., 3:] == 9).all()) for w in wide)
+
+
 def test_put_leaves_what_has_no_place():
     g = torch.Generator().manual_seed(6)
     lens, news = [10, 20, 5, -3], [20, 30, 0, 4]
