@@ -130,20 +130,13 @@ __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
         first = (int)min((int64_t)b * a.most_new, (int64_t)a.tokens);
         end = (int)min((int64_t)first + a.most_new, (int64_t)a.tokens);
     }
-    const int64_t len = max(a.lens[b], 0), last = len + min(end - first, a.most_new);
-    const int64_t block = len / a.c.size + run, from = max(len, block * a.c.size), to = min(last, (block + 1) * a.c.size);
+    const uint32_t size = a.c.size, page = a.c.page, cached = max(a.lens[b], 0);          // (64-bit divisions would be most of a small call's instructions)
+    const int64_t len = cached, last = len + min(end - first, a.most_new);
+    const int64_t block = (int64_t)(cached / size) + run, from = max(len, block * size), to = min(last, (block + 1) * size);
     if (from >= to) return;
-    const int64_t pg = from / a.c.page;
-    if (pg >= a.max_pages) return;
-    const int32_t id = a.table[b * a.ld_table + pg];
-    if ((uint32_t)id >= (uint32_t)a.c.pages) return;
-    const Plane8 p = plane_of(a.c, v, head);
-    const int off = (int)(from - pg * a.c.page), in_block = off % a.c.size, n = (int)(to - from), per = a.c.per, pieces = n * per;
+    const int n = (int)(to - from), per = a.c.per, pieces = n * per;
     const int64_t t_b = v ? a.v_t : a.k_t;
     const char* in = (v ? a.v + head * a.v_h : a.k + head * a.k_h) + (first + (from - len)) * t_b;
-    uint8_t* scale = p.scale + id * p.s_page + off / a.c.size * p.s_block;
-    const int was = in_block ? *scale : 0;
-
     u32x4 x[PUT8_KEEP][2];
     auto load = [&](int j0) __attribute__((always_inline)) {
 #pragma unroll
@@ -155,10 +148,23 @@ __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
                 x[j][1] = at[1];
             }
     };
+    load(0);                                                 // (beside the page and the scale, not behind them)
+    const uint32_t pg = (uint32_t)from / page;
+    if (pg >= (uint32_t)a.max_pages) return;
+    const int32_t id = a.table[b * a.ld_table + pg];
+    if ((uint32_t)id >= (uint32_t)a.c.pages) return;
+    const Plane8 p = plane_of(a.c, v, head);
+    const int off = (int)((uint32_t)from - pg * page), in_block = (int)((uint32_t)off % size);
+    uint8_t* scale = p.scale + id * p.s_page + (int)((uint32_t)off / size) * p.s_block;
+    const int was = in_block ? *scale : 0;
+    // One wave has all of its pieces; four go over them again
+    const bool again = WAVES > 1 && pieces > PUT8_KEEP * G;
+    const int rounds = WAVES > 1 ? (pieces + PUT8_KEEP * G - 1) / (PUT8_KEEP * G) : 1;
     typedef unsigned short pair __attribute__((ext_vector_type(2)));
     pair both = {0, 0};
-    for (int j0 = 0; j0 * G < pieces; j0 += PUT8_KEEP) {
-        load(j0);
+    for (int q = 0; q < rounds; ++q) {
+        const int j0 = q * PUT8_KEEP;
+        if (q) load(j0);
 #pragma unroll
         for (int j = 0; j < PUT8_KEEP; ++j)
             if ((j0 + j) * G < pieces)
@@ -180,8 +186,9 @@ __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
     const bool plain = top <= T::MOST;
     if (!plain) {                                            // the largest that is finite, or MOST
         top = 0;
-        for (int j0 = 0; j0 * G < pieces; j0 += PUT8_KEEP) {
-            if (WAVES > 1 && pieces > PUT8_KEEP * G) load(j0);          // (one wave has all of its pieces)
+        for (int q = 0; q < rounds; ++q) {
+            const int j0 = q * PUT8_KEEP;
+            if (again) load(j0);
 #pragma unroll
             for (int j = 0; j < PUT8_KEEP; ++j)
                 if ((j0 + j) * G < pieces)
@@ -199,8 +206,9 @@ __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
     if (in_block && e > was - 127) scale_slots<G>(a.c, p.at + id * p.page + (off - in_block) * p.slot, p.slot, in_block, e + 127 - was, lane);
     if (lane == 0) *scale = (uint8_t)(e + 127);
     const float by = two_to(-e), unit_of = two_to(e), most = T::get(T::MOST);
-    for (int j0 = 0; j0 * G < pieces; j0 += PUT8_KEEP) {
-        if (WAVES > 1 && pieces > PUT8_KEEP * G) load(j0);          // (one wave has all of its pieces)
+    for (int q = 0; q < rounds; ++q) {
+        const int j0 = q * PUT8_KEEP;
+        if (again) load(j0);
 #pragma unroll
         for (int j = 0; j < PUT8_KEEP; ++j)
             if ((j0 + j) * G + lane < pieces) {
@@ -216,9 +224,9 @@ __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
                     }
                     float f[4];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const float one = T::get((q & 2 ? hi : lo) >> (16 * (q & 1)) & 0xFFFF);
-                        f[q] = fabsf(one) < INFINITY ? fminf(fmaxf(one, -most), most) * by : NAN;
+                    for (int z = 0; z < 4; ++z) {
+                        const float one = T::get((z & 2 ? hi : lo) >> (16 * (z & 1)) & 0xFFFF);
+                        f[z] = fabsf(one) < INFINITY ? fminf(fmaxf(one, -most), most) * by : NAN;
                     }
                     y[d] = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
                     y[d] = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], y[d], true);
