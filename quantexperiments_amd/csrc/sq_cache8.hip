@@ -334,13 +334,28 @@ __global__ __launch_bounds__(256) void keep8_kernel(Keep8Args a) {
                 if (u + 1 < U) e[min(u + 1, U - 1)] = max(e[min(u + 1, U - 1)], most >> 16);
             }
         }
-        if (held)
+        if (held) {                                          // scaled to it, the units' pieces in flight together
+            int down[U];
+            bool any = false;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int down = (int)e[u] - (int)was[u];
+                down[u] = first + u < units ? (int)e[u] - (int)was[u] : 0;
                 e[u] = max(e[u], was[u]);
-                if (first + u < units && down > 0) scale_slots<64>(a.c, at[u] + to - held * p.slot, p.slot, held, down, lane);
+                any |= down[u] > 0;
             }
+            if (any)
+                for (int i = lane; i < held * per; i += 64) {
+                    u32x4 y[U];
+                    const int slot = row_of(a.c, i);
+                    const int64_t where = to + (slot - held) * p.slot + (i - slot * per) * 16;
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (down[u] > 0) y[u] = *reinterpret_cast<const u32x4*>(at[u] + where);
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (down[u] > 0) *reinterpret_cast<u32x4*>(at[u] + where) = scaled_codes(y[u], down[u]);
+                }
+        }
         for (int c = lo / rows; c * rows < hi; ++c) {
             at_window(c * rows / entries);
             fetch(c);
