@@ -492,7 +492,7 @@ int sq_keep_drafted(const sq_cache* cache, int32_t layers, int64_t k_layer, int6
  * sq_cache8: a layer's paged cache of keys and values as e4m3 codes (one sign, four exponent, three mantissa bits, largest 448, no infinities) and
  * one e8m0 scale (a byte, 2^(byte - 127)) for each block of tokens and head: slot s of page p, head h, element i stands for
  *     code(k + p * k_page + s * k_slot + h * k_head + i) * scale(k_scale + p * ks_page + s / (page / blocks) * ks_block + h * ks_head)
- * and values likewise.  page / blocks, the tokens of a block, is a multiple of 16; dim a multiple of 16 up to 256, heads 16-byte aligned; the
+ * and values likewise.  A scale's byte is 1 to 254 wherever a token is held (27 or more, where sq_put_tokens8 made it).  page / blocks, the tokens of a block, is a multiple of 16; dim a multiple of 16 up to 256, heads 16-byte aligned; the
  * slots of a page ascend in memory, less than 2^27 bytes from one to the next. */
 typedef struct sq_cache8 {
     void* k;

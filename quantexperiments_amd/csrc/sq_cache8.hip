@@ -108,8 +108,9 @@ template <> struct Put8Type<SQ_BF16> {
 
 // One wave per block that gets new tokens, head, and keys or values: the largest magnitude over its tokens, then the codes.  Magnitudes order as their bits, so the largest is
 // looked for two elements at a time, and v_cvt_scalef32_pk_fp8 makes two codes of the elements as they are (one by one, as where some element is beyond what is
-// held, 8000 tokens of 8 heads of 128 took 15.0 us, not 12.1).  Up to 8 pieces of 16 elements a lane stay in registers between the two: 64 tokens of 128 a wave.  WAVES: four waves share
-// a block of more than that (8000 tokens of 4 heads of 256 in blocks of 64: 12.1 us, read twice by one wave 18.0); of more than four hold, the elements are read again.
+// held, 8000 tokens of 8 heads of 128 take 3 us more).  Up to 8 pieces of 16 elements a lane stay in registers between the two: 64 tokens of 128 a wave.  WAVES: four waves share
+// a block of more than that (8000 tokens of 4 heads of 256 in blocks of 64: read twice by one wave 6 us more); of more than four hold, the elements are read again.
+// Bound by HBM: 8000 tokens of 8 heads of 128, 49 MB, 8.9 to 9.6 us (5.1 to 5.5 TB/s); a token of each of 64 sequences 4.0, of which all but a microsecond is the launch and one chain of loads.
 constexpr int64_t PUT8_CACHED = 4 << 20;         // bytes of codes up to which they stay in the caches for who reads them next (16 MB: 11.9 us, past them 10.3)
 constexpr int PUT8_KEEP = 8;
 template <int DT, int WAVES, bool PASSING>
@@ -240,8 +241,8 @@ __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
 // One wave per sequence and U units (heads of a layer's keys or values), a block that rows move to at a time.  The path ascends, so row i comes from a slot at or
 // behind lens + i: no row is read after its slot was written, and what goes to a block comes from it or from blocks behind it, whose scales have not changed yet.
 // The path and the pages are looked up once for the units; then the scales and the first rows of all of them are in flight together, whatever blocks they go to, and further rows are
-// fetched as they come.  Bound by that chain of loads (lengths, path, pages, rows) and by what is worked out along it: 64 sequences, 28 layers of 4 heads, 8 rows of 128, 11.1 us for 14.7 MB
-// read and written, with a wave per unit 17.5; 256 sequences 29.7 and 52; one sequence 4.2.
+// fetched as they come.  Bound by that chain of loads (lengths, path, pages, rows) and by what is worked out along it: 64 sequences, 28 layers of 4 heads, 8 rows of 128, 10.9 us for 21 MB
+// read and 20 written (what blocks that grow cost is in that), with a wave per unit 17.5; 256 sequences 30 and 52; one sequence 4.2.
 template <int U>
 __global__ __launch_bounds__(256) void keep8_kernel(Keep8Args a) {
     const int lane = threadIdx.x & 63, b = blockIdx.y;
