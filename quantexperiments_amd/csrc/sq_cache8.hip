@@ -40,18 +40,22 @@ __device__ __forceinline__ Plane8 plane_of(const Cache8& c, bool v, int head) {
 
 __device__ __forceinline__ float two_to(int e) { return __builtin_bit_cast(float, (uint32_t)min(max(e + 127, 1), 254) << 23); }
 
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-    const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    v = max((uint32_t)h[0], (uint32_t)h[1]);
-    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = max((uint32_t)r[0], (uint32_t)r[1]);
+// over a wave, or over each 16 lanes of it
+template <bool WAVE>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+    if constexpr (WAVE) {
+        const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = max((uint32_t)h[0], (uint32_t)h[1]);
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max((uint32_t)r[0], (uint32_t)r[1]);
+    }
     v = max(v, row_rotated_bits<8>(v));
     v = max(v, row_rotated_bits<4>(v));
     v = max(v, row_rotated_bits<2>(v));
     return max(v, row_rotated_bits<1>(v));
 }
 
-// the same of 16-bit halves
+// over a wave, of 16-bit halves
 __device__ __forceinline__ uint32_t wave_max2(uint32_t x) {
     typedef unsigned short pair __attribute__((ext_vector_type(2)));
     auto most = [](uint32_t a, uint32_t b) { return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pair, a), __builtin_bit_cast(pair, b))); };
@@ -81,16 +85,25 @@ __device__ __forceinline__ u32x4 scaled_codes(u32x4 x, int down) {
     return y;
 }
 
-// Scales n slots from `first` on down, a piece of 16 elements per lane of G
-template <int G>
+// Scales n slots from `first` on down, U pieces of 16 elements per lane of G in flight
+template <int G, int U>
 __device__ __forceinline__ void scale_slots(const Cache8& c, char* first, int64_t slot, int n, int down, int lane) {
-    for (int x = lane; x < n * c.per; x += G) {
-        const int row = row_of(c, x);
-        u32x4* at = reinterpret_cast<u32x4*>(first + row * slot + (x - row * c.per) * 16);
-        *at = scaled_codes(*at, down);
+    const int pieces = n * c.per;
+    for (int x = lane; x < pieces; x += G * U) {
+        u32x4 y[U];
+        auto at = [&](int u) __attribute__((always_inline)) {
+            const int i = min(x + u * G, pieces - 1), row = row_of(c, i);
+            return reinterpret_cast<u32x4*>(first + row * slot + (i - row * c.per) * 16);
+        };
+#pragma unroll
+        for (int u = 0; u < U; ++u) y[u] = *at(u);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (x + u * G < pieces) *at(u) = scaled_codes(y[u], down);
     }
 }
 
+constexpr int PUT8_PIECES = 8;
 // MOST: the largest magnitude that is held, 1.875 * 2^15 and 1.875 * 2^127
 template <int DT> struct Put8Type;
 template <> struct Put8Type<SQ_F16> {
@@ -108,17 +121,19 @@ template <> struct Put8Type<SQ_BF16> {
 
 // One wave per block that gets new tokens, head, and keys or values: the largest magnitude over its tokens, then the codes.  Magnitudes order as their bits, so the largest is
 // looked for two elements at a time, and v_cvt_scalef32_pk_fp8 makes two codes of the elements as they are (one by one, as where some element is beyond what is
-// held, 8000 tokens of 8 heads of 128 take 3 us more).  Up to 8 pieces of 16 elements a lane stay in registers between the two: 64 tokens of 128 a wave.  WAVES: four waves share
-// a block of more than that (8000 tokens of 4 heads of 256 in blocks of 64: read twice by one wave 6 us more); of more than four hold, the elements are read again.
-// Bound by HBM: 8000 tokens of 8 heads of 128, 49 MB, 8.9 to 9.6 us (5.1 to 5.5 TB/s); a token of each of 64 sequences 4.0, of which all but a microsecond is the launch and one chain of loads.
-constexpr int64_t PUT8_CACHED = 4 << 20;         // bytes of codes up to which they stay in the caches for who reads them next (16 MB: 11.9 us, past them 10.3)
-constexpr int PUT8_KEEP = 8;
-template <int DT, int WAVES, bool PASSING>
+// held, 8000 tokens of 8 heads of 128 take 3 us more).  Up to 8 pieces of 16 elements a lane stay in registers between the two: 64 tokens of 128 a wave.  LANES: four waves share
+// a block of more than that (8000 tokens of 4 heads of 256 in blocks of 64: read twice by one wave 6 us more); of more than four hold, the elements are read again.  One of
+// up to 16 pieces, a decode batch's single token, has 16 lanes: 1024 sequences x 8 heads of 128 4.7 us, with a
+// wave each 12.8; 64 x 4 heads 3.4 and 3.8.
+// Bound by HBM: 8000 tokens of 8 heads of 128, 49 MB, 11.0 us (4.5 TB/s; 7.1 where they still are in the caches in front of it); a token of each of 64 sequences 3.4, a launch and one chain of loads.
+constexpr int64_t PUT8_CACHED = 4 << 20;         // bytes of codes up to which heads that share lines of 128 bytes are put together in the caches; others are written past them (2000 tokens of
+                                                 // 8 heads of 128 7.0 us, so 5.5; heads of 16 4.1, so 4.4)
+template <int DT, int LANES, bool PASSING>
 __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
     typedef Put8Type<DT> T;
-    constexpr int G = 64 * WAVES;                            // lanes of a block
-    const int lane = threadIdx.x % G;
-    const uint32_t unit = blockIdx.x * (4 / WAVES) + (WAVES == 1 ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) : 0);
+    constexpr int G = LANES, WAVES = LANES > 64 ? LANES / 64 : 1, PUT8_KEEP = LANES < 64 ? 1 : PUT8_PIECES;
+    const int lane = threadIdx.x % G, mine = threadIdx.x / G;
+    const uint32_t unit = blockIdx.x * (256 / G) + (G == 64 ? __builtin_amdgcn_readfirstlane(mine) : mine);
     const bool v = unit & 1;
     const uint32_t run_of = (unit >> 1) / (uint32_t)a.c.heads;
     const int head = (int)((unit >> 1) - run_of * a.c.heads), b = (int)(run_of / (uint32_t)a.runs), run = (int)(run_of - (uint32_t)b * a.runs);
@@ -174,7 +189,7 @@ __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
     }
     __shared__ uint32_t tops[2][WAVES];
     auto most_of = [&](uint32_t v, int which) __attribute__((always_inline)) {
-        v = wave_max(v);
+        v = lanes_max<(LANES >= 64)>(v);
         if constexpr (WAVES > 1) {
             if (lane % 64 == 0) tops[which][lane / 64] = v;
             __syncthreads();                                 // (which all waves pass behind having read the block's scale)
@@ -204,7 +219,7 @@ __global__ __launch_bounds__(256) void put8_kernel(Put8Args a) {
     const uint32_t bits = __builtin_bit_cast(uint32_t, T::get(top));
     int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFF) > 0x600000);
     e = max(max(e, -100), was - 127);
-    if (in_block && e > was - 127) scale_slots<G>(a.c, p.at + id * p.page + (off - in_block) * p.slot, p.slot, in_block, e + 127 - was, lane);
+    if (in_block && e > was - 127) scale_slots<G, G == 16 ? 4 : G == 64 ? 2 : 1>(a.c, p.at + id * p.page + (off - in_block) * p.slot, p.slot, in_block, e + 127 - was, lane);
     if (lane == 0) *scale = (uint8_t)(e + 127);
     const float by = two_to(-e), unit_of = two_to(e), most = T::get(T::MOST);
     for (int q = 0; q < rounds; ++q) {
@@ -422,14 +437,15 @@ int sq_put_tokens8(const sq_heads* k, const sq_heads* v, int32_t tokens, int dty
     a.table = table; a.ld_table = ld_table; a.max_pages = max_pages; a.lens = lens; a.starts = starts;
     a.tokens = tokens; a.seqs = seqs; a.most_new = most_new;
     a.runs = (int)(((int64_t)most_new + 2 * a.c.size - 2) / a.c.size);          // the first token may be its block's last
-    const bool shared = (int64_t)(a.c.size < most_new ? a.c.size : most_new) * a.c.per > PUT8_KEEP * 64;
-    const int64_t units = 2 * (int64_t)seqs * a.runs * a.c.heads, groups = shared ? units : (units + 3) / 4;
+    const int64_t pieces = (int64_t)(a.c.size < most_new ? a.c.size : most_new) * a.c.per;
+    const int lanes = pieces > PUT8_PIECES * 64 ? 256 : pieces > 16 ? 64 : 16;
+    const int64_t units = 2 * (int64_t)seqs * a.runs * a.c.heads, groups = (units + 256 / lanes - 1) / (256 / lanes);
     if (groups > (1 << 23)) return fail(SQ_EUNSUPPORTED, "%s: %d sequences of up to %d new tokens and %d heads at once", who, seqs, most_new, cache->heads);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, a); };
     auto of = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        if ((int64_t)tokens * a.c.heads * a.c.dim * 2 > PUT8_CACHED) go(shared ? put8_kernel<DT, 4, true> : put8_kernel<DT, 1, true>);
-        else go(shared ? put8_kernel<DT, 4, false> : put8_kernel<DT, 1, false>);
+        if (a.c.dim % 128 == 0 || (int64_t)tokens * a.c.heads * a.c.dim * 2 > PUT8_CACHED) go(lanes == 256 ? put8_kernel<DT, 256, true> : lanes == 64 ? put8_kernel<DT, 64, true> : put8_kernel<DT, 16, true>);
+        else go(lanes == 256 ? put8_kernel<DT, 256, false> : lanes == 64 ? put8_kernel<DT, 64, false> : put8_kernel<DT, 16, false>);
     };
     if (dtype == SQ_F16) of(std::integral_constant<int, SQ_F16>()); else of(std::integral_constant<int, SQ_BF16>());
     return check_launch(who);
