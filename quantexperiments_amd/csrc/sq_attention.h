@@ -247,7 +247,7 @@ struct Attn8Args : AttnArgs {
     const uint8_t *ks, *vs;
     int64_t ks_page, ks_block, ks_head, vs_page, vs_block, vs_head;
     int size;                    // tokens of a block, a multiple of 16
-    int together;                // few rows: the heads of the same keys are dealt to one die
+    int inner;                   // few rows: workgroups that read the same lines (blocks of rows; heads that share lines), dealt to one die one behind the other
     int passing;                 // few rows: keys and values are read past the caches
 };
 

@@ -18,6 +18,13 @@ namespace sq {
 // eight 12.9, in four 14.3.
 // One of up to four steps a wave is not cut (a step takes 0.6 us then: one token behind 500 slots 8.7 us call by call, in four parts 10.1; captured 8.5 and 8.1; of heads of 256 12.1 and 9.9,
 // which are).
+// There the few-row kernel also takes more rows, in blocks of 32 or 16, one workgroup each, that read the same keys on one die: it has no barriers, starts and ends in 5 us where the many-row kernel
+// takes 10, and reads ahead twice as far.  Up to 128 rows always, but for the shortest tables (28 + 4 heads of 128: 8 new tokens behind 64 x 2000 slots 70.5 us in the other, 40.2 in this; 5 behind 128 x 100
+// 17.3 and 20.5).  More while the many-row kernel leaves half of the compute units idle (a batch of 4 x 250 new tokens 31.1 and 21.9, of 4 x 500 31.5 and 42.0) and a unit has at
+// most 96 products of a 16-row block with a step, 256 of sequences that are short: 48 behind 4000 27.9 and 20.2, 200 behind 4000 40 and 46; 500 behind 1000 36.4 and 27.8, 1000 behind 1000
+// 56.1 and 58.4.  Heads of 256, blocks of 16 and one workgroup a compute unit: 48 per unit and a unit per block (16 new tokens of 5 heads behind 8 x 500 26.1 and 16.6, behind 16 x 500 27.1 and 30.1), up
+// to 32 rows where there are 32 steps (4 behind 32 x 4000 94 and 61; 8 behind 64 x 200 19.6 and 30.8).  Blocks of 16 while all of them run at once and products are few: a step then takes
+// 0.6 us, of 32 1.2 (8 behind 500 9.9 and 12.3, behind 4000 11.9 and 14.0; behind 32,000 25.9 and 22.5).
 // A sequence's length is its table's width here: lengths are on the device.  Under a table of 131,072 slots one token behind 500 takes 10.2 us instead of 8.8, 48 26.7 instead of 21.4,
 // 64 sequences of 500 27.9 instead of 18.6, 64 of 2000 59.8 instead of 53.1.
 AttnPlan attn_plan(const sq_attention& a, const sq_cache& c, bool held8) {
@@ -26,9 +33,16 @@ AttnPlan attn_plan(const sq_attention& a, const sq_cache& c, bool held8) {
     const int64_t rows = (int64_t)a.most_new * (a.q_heads / c.heads), steps = ((int64_t)a.max_pages * c.page + ATTN_STEP - 1) / ATTN_STEP;
     const int waves = held8 ? ATTN8_WAVES : attn_waves(p.dp);
     int64_t per, most;
-    if (rows <= (p.dp == 256 ? 16 : 32)) {
+    const int64_t cus = device_cus(), units = (int64_t)a.seqs * c.heads * ((rows + 15) / 16), load = units * steps;
+    bool few = rows <= (p.dp == 256 ? 16 : 32);
+    if (held8 && !few) {
+        const int64_t tiles = (int64_t)a.seqs * c.heads * (rows <= 128 ? 1 : (rows + 255) / 256);
+        if (p.dp == 256) few = (units <= cus && load <= 48 * cus) || (rows <= 32 && steps >= 32);
+        else few = (rows <= 128 && steps >= 8) || (tiles * (steps < 4 ? 4 : 2) <= cus && (load <= 96 * cus || (steps <= 96 && load <= 256 * cus)));
+    }
+    if (few) {
         p.nw = 0;
-        p.mt = rows <= 16 ? 1 : 2;
+        p.mt = rows <= 16 || p.dp == 256 || (held8 && units <= 2 * cus && load <= 32 * cus) ? 1 : 2;
         per = p.mt * 16;
         most = steps / waves;
         if (most <= (held8 && p.dp < 256 ? 4 : 2)) most = 1;
@@ -39,7 +53,7 @@ AttnPlan attn_plan(const sq_attention& a, const sq_cache& c, bool held8) {
         most = steps / 4 > 8 ? steps / 4 : steps / 2 < 8 ? steps / 2 : 8;
     }
     p.row_blocks = (int)((rows + per - 1) / per);
-    const int64_t base = (int64_t)a.seqs * c.heads * p.row_blocks, cus = device_cus();
+    const int64_t base = (int64_t)a.seqs * c.heads * p.row_blocks;
     int64_t want = cus / base;
     if (held8 && !p.nw) {
         if (p.dp == 64) want = 2 * cus / base;

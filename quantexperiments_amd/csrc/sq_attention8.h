@@ -143,15 +143,17 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW * at
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     constexpr int C = T::COPIES, ROWS = MT * 16, RING = attn8_ring(DP, MT);          // (C: of a step's keys, or values)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int id = blockIdx.x, head;
-    if (a.together) {                                        // as far as eights of parts go
-        const int parts = gridDim.x / a.kv_heads, eights = parts & ~7, over = id - eights * a.kv_heads;
-        head = over < 0 ? id / 8 % a.kv_heads : over % a.kv_heads;
-        id = over < 0 ? id / 8 / a.kv_heads * 8 + id % 8 : eights + over / a.kv_heads;
+    int id = blockIdx.x, in = 0;
+    if (a.inner > 1) {                                       // as far as eights of parts go
+        const int parts = gridDim.x / a.inner, eights = parts & ~7, over = id - eights * a.inner;
+        in = over < 0 ? id / 8 % a.inner : over % a.inner;
+        id = over < 0 ? id / 8 / a.inner * 8 + id % 8 : eights + over / a.inner;
     }
-    const int split = id % a.splits; id /= a.splits;
-    if (!a.together) { head = id % a.kv_heads; id /= a.kv_heads; }
-    const int row0 = id % a.row_blocks * ROWS, b = id / a.row_blocks;
+    const int row0 = in % a.row_blocks * ROWS, split = id % a.splits;
+    id /= a.splits;
+    int head = in / a.row_blocks;
+    if (a.inner == a.row_blocks) { head = id % a.kv_heads; id /= a.kv_heads; }
+    const int b = id;
     const AttnSeq s = attn_seq(a, b);
     const int rows = s.n * a.group;
     if (row0 >= rows) return;

@@ -43,7 +43,7 @@ int sq_tree_attention8(const sq_attention* a, const sq_cache8* cache, int dtype,
     k.size = cache->page / cache->blocks;
     // Rows of heads that share lines of 128 bytes are fetched into each die's cache that reads one: 64 sequences of 4000 slots, 8 key heads of 64, 84 us, with a line's heads on
     // one die 62.  Of others, dealt out one behind the other, 32 sequences of 8192 x 8 of 128 108 us, so 115.
-    k.together = cache->dim % 128 != 0;
+    k.inner = (cache->dim % 128 ? cache->heads : 1) * p.row_blocks;
     // What is read once, and more than a few MB, is read past the dies' caches and those in front of HBM (between two calls on a layer's cache lie the other layers' and the weights): 32
     // sequences of 4000 slots x 4 key heads of 128, one set of several 32.6 us, so 28.6; the same set again and again 29.1 and 26.6; one of 131,072 35.8 and 31.5; 32 of 2,240 to 8,192 x 8
     // 74 and 62.  Less is bound by its chain of loads: 8 of 2000 9.3 us where it is still in those caches, so 10.0 (where not, 14.0 and 12.9).  (By the tables' width: lengths are on the device.)
