@@ -20,8 +20,8 @@ namespace sq {
 // which are).
 // There the few-row kernel also takes more rows, in blocks of 32 or 16, one workgroup each, that read the same keys on one die: it has no barriers, starts and ends in 5 us where the many-row kernel
 // takes 10, and reads ahead twice as far.  Up to 128 rows always, but for the shortest tables (28 + 4 heads of 128: 8 new tokens behind 64 x 2000 slots 70.5 us in the other, 40.2 in this; 5 behind 128 x 100
-// 17.3 and 20.5).  More while the many-row kernel leaves half of the compute units idle (a batch of 4 x 250 new tokens 31.1 and 21.9, of 4 x 500 31.5 and 42.0) and a unit has at
-// most 96 products of a 16-row block with a step, 256 of sequences that are short: 48 behind 4000 27.9 and 20.2, 200 behind 4000 40 and 46; 500 behind 1000 36.4 and 27.8, 1000 behind 1000
+// 17.3 and 20.5).  More while the many-row kernel leaves half of the compute units idle (a batch of 4 x 250 new tokens 31.1 and 20.8, of 4 x 500 31.5 and 42.0) and a unit has at
+// most 96 products of a 16-row block with a step, 256 of sequences that are short: 48 behind 4000 27.9 and 20.2, 200 behind 4000 40 and 46; 500 behind 1000 36.4 and 27.2, 1000 behind 1000
 // 56.1 and 58.4.  Heads of 256, blocks of 16 and one workgroup a compute unit: 48 per unit and a unit per block (16 new tokens of 5 heads behind 8 x 500 26.1 and 16.6, behind 16 x 500 27.1 and 30.1), up
 // to 32 rows where there are 32 steps (4 behind 32 x 4000 94 and 61; 8 behind 64 x 200 19.6 and 30.8).  Blocks of 16 while all of them run at once and products are few: a step then takes
 // 0.6 us, of 32 1.2 (8 behind 500 9.9 and 12.3, behind 4000 11.9 and 14.0; behind 32,000 25.9 and 22.5).
