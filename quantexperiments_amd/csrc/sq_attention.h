@@ -249,6 +249,8 @@ struct Attn8Args : AttnArgs {
     int size;                    // tokens of a block, a multiple of 16
     int inner;                   // few rows: workgroups that read the same lines (blocks of rows; heads that share lines), dealt to one die one behind the other
     int passing;                 // few rows: keys and values are read past the caches
+    int32_t* parts;              // many rows, or null: of each block of rows and sequence, into how many its keys are cut; `splits` is then the most
+    int cut, block;              // and how many there are in the mean before the last block; rows of a block are 2^block
 };
 
 // 8 codes times a power of two as a matrix instruction's operand: v_cvt_scalef32_pk takes two at a time and the scale with them, exactly
@@ -690,6 +692,62 @@ constexpr int ATTN8_STAGES = 3, ATTN8_RAW = 3;
 template <int DP, int NW> constexpr int attn8_copies() { return (attn_stage_steps(DP, NW) * ATTN_STEP / NW * DP + 1023) / 1024; }      // of a wave's keys of a stage
 template <int DP, int NW> constexpr int attn8_tile_lds() { return ATTN8_STAGES * attn_stage_bytes<DP, NW>() + ATTN8_RAW * NW * 2048 * attn8_copies<DP, NW>() + 64; }
 
+// Sequences of several lengths under one block of rows share its workgroups by their lengths, not evenly: the fewest stages T such that all of them, cut into parts of T, are
+// no more parts than there are workgroups.  Workgroup `split` of sequence b becomes part `split` of `splits` of another b.  (Lengths are on the device; up to 64 sequences, one a lane.)
+// 8 trees of 48 tokens behind 1408 to 4096 slots, 28 + 4 heads of 128: 52.2 us evenly, 47.4 so, of 20 + 4 heads of 256 67.1 and 57.4 (61 with END zero), 16 of 32
+// behind 1100 to 4000 53.2 and 49.3; where all are as long it costs 2 (8 behind 4096 51.9 and 53.7).
+template <typename F> __device__ __forceinline__ uint32_t attn8_fold(uint32_t v, F f) {          // over the wave
+    const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = f((uint32_t)h[0], (uint32_t)h[1]);
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = f((uint32_t)r[0], (uint32_t)r[1]);
+    v = f(v, row_rotated_bits<8>(v));
+    v = f(v, row_rotated_bits<4>(v));
+    v = f(v, row_rotated_bits<2>(v));
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)f(v, row_rotated_bits<1>(v)));
+}
+template <int N> __device__ __forceinline__ int attn8_from_left(int v) { return __builtin_amdgcn_update_dpp(0, v, 0x110 + N, 0xF, 0xF, false); }      // of the lane N before, in a row of 16
+// x / d rounded up, for x up to 2^21 (a 32-bit float tells it from the integers beside it), in a fifth of the instructions of a division
+__device__ __forceinline__ int attn8_parts(int x, int d, float by) {
+    const int q = (int)((float)x * by);
+    return q + (q * d < x);
+}
+template <int KEYS, int ROWS, int END>
+__device__ __forceinline__ bool attn8_share(const Attn8Args& a, int row0, int head, int lane, int& b, int& split, int& splits, AttnSeq& seq) {
+    auto sum = [](int v) __attribute__((always_inline)) { return (int)attn8_fold((uint32_t)v, [](uint32_t x, uint32_t y) { return x + y; }); };
+    const int all = a.seqs * splits, mine = b * splits + split;            // (so most stay on the die that has their sequence)
+    const AttnSeq s = attn_seq(a, min(lane, a.seqs - 1));
+    // (about how many stages: what a part has of them is worked out from the sequence itself)
+    const int rows = s.n * a.group, last = min(row0 + ROWS, rows) - 1, seen = a.mask ? s.total : min(s.total, s.len + (int)((float)last * __builtin_amdgcn_rcpf((float)a.group)) + 1);
+    const int stages = lane < a.seqs && row0 < rows ? (seen + KEYS - 1) / KEYS + END : 0;
+    const int most = (int)attn8_fold((uint32_t)stages, [](uint32_t x, uint32_t y) { return max(x, y); });
+    const float total = (float)sum(stages);
+    // (T = total / (all - seqs) is enough, since each sequence's last part may be short; fewer than two stages are not worth a part)
+    int t = max(max((int)(total * __builtin_amdgcn_rcpf((float)all)), attn8_parts(most, a.splits, __builtin_amdgcn_rcpf((float)a.splits))), 2);
+    int enough = max(t, (int)(total * __builtin_amdgcn_rcpf((float)(all - a.seqs))) + 2);
+    while (t < enough) {
+        const int half = (t + enough) / 2;
+        if (sum(attn8_parts(stages, half, __builtin_amdgcn_rcpf((float)half))) <= all) enough = half; else t = half + 1;
+    }
+    const int parts = attn8_parts(stages, t, __builtin_amdgcn_rcpf((float)t));
+    int upto = parts;
+    upto += attn8_from_left<1>(upto);
+    upto += attn8_from_left<2>(upto);
+    upto += attn8_from_left<4>(upto);
+    upto += attn8_from_left<8>(upto);
+    const int r0 = __builtin_amdgcn_readlane(upto, 15), r1 = __builtin_amdgcn_readlane(upto, 31), r2 = __builtin_amdgcn_readlane(upto, 47);
+    upto += lane < 16 ? 0 : lane < 32 ? r0 : lane < 48 ? r0 + r1 : r0 + r1 + r2;
+    if (mine == 0 && head == 0 && threadIdx.x < (unsigned)a.seqs) a.parts[row0 / ROWS * a.seqs + lane] = parts;
+    const uint64_t here = __ballot(mine >= upto - parts && mine < upto);
+    if (!here) return false;
+    b = __builtin_ctzll(here);
+    splits = __builtin_amdgcn_readlane(parts, b);
+    split = mine - __builtin_amdgcn_readlane(upto - parts, b);
+    seq = {__builtin_amdgcn_readlane(s.first, b), __builtin_amdgcn_readlane(s.n, b), __builtin_amdgcn_readlane(s.len, b), __builtin_amdgcn_readlane(s.total, b),
+           __builtin_amdgcn_readlane((int)s.over, b) != 0};
+    return true;
+}
+
 // In which order a region's instructions are issued: N times one matrix instruction, D LDS reads, V vector instructions, X exponentials
 template <int N, int V, int X, int D> __device__ __forceinline__ void attn_order() {
 #pragma unroll
@@ -731,22 +789,32 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(ARGS a) {
     constexpr bool C8 = !std::is_same_v<ARGS, AttnArgs>;
     constexpr int MT = attn_tiles(DP), SK = attn_stage_steps(DP, NW), KEYS = SK * ATTN_STEP, NB = C8 ? ATTN8_STAGES : ATTN_STAGES, STAGE = attn_stage_bytes<DP, NW>(), ROWS = NW * MT * 16;
     constexpr int MINE = KEYS / NW, C = MINE / T::ROWS, KC = DP / 32, VD = DP / 16;
+    constexpr int END = MT >= 2 ? 0 : 2;                     // (stages that a sequence's end, which goes step by step, costs beside its own)
     constexpr bool PIPELINE = MT >= 2;                       // (a tile's maximum is raised while the sums of the tile before it are outstanding)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, i16 = lane & 15;
     // the workgroups of one key head are dealt to as few dies as there are: neighbours are other heads'; last rows, which have most keys, first
     int id = blockIdx.x;
-    const int groups = a.seqs * a.kv_heads, b = id % groups / a.kv_heads, head = id % groups % a.kv_heads;
+    const int groups = a.seqs * a.kv_heads, head = id % groups % a.kv_heads;
+    int b = id % groups / a.kv_heads;
     id /= groups;
     const bool end_block = id < a.last_splits;
-    const int splits = end_block ? a.last_splits : a.splits;
+    int splits = end_block ? a.last_splits : a.splits, split;
+    if constexpr (C8) if (!end_block) splits = a.cut;
     if (!end_block) id -= a.last_splits;
-    const int split = id % splits, row0 = (a.row_blocks - (end_block ? 1 : 2) - id / splits) * ROWS;
-    const AttnSeq s = attn_seq(a, b);
+    split = id % splits;
+    const int row0 = (a.row_blocks - (end_block ? 1 : 2) - id / splits) * ROWS;
+    AttnSeq s;
+    if constexpr (C8) {
+        if (!a.parts) s = attn_seq(a, b);
+        else if (!attn8_share<KEYS, ROWS, END>(a, row0, head, lane, b, split, splits, s)) return;
+    } else s = attn_seq(a, b);
     const int rows = s.n * a.group;
     if (row0 >= rows) return;
     const int last = min(row0 + ROWS, rows) - 1;
     const int seen = a.mask ? s.total : min(s.total, s.len + last / a.group + 1);
-    const int stages = (seen + KEYS - 1) / KEYS, per = (stages + splits - 1) / splits, begin = min(split * per, stages), end = min(begin + per, stages);
+    int ending = 0;
+    if constexpr (C8) ending = a.parts ? END : 0;
+    const int stages = (seen + KEYS - 1) / KEYS, per = (stages + ending + splits - 1) / splits, begin = min(split * per, stages), end = min(begin + per, stages);
 
     AttnRows<DP, MT> r;
     const int mine = row0 + wave * MT * 16;
@@ -1031,7 +1099,9 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(ARGS a) {
         if (bad) l = NAN;
         if (row >= rows) continue;
         const int64_t tok_all = s.first + tok;
-        if (splits > 1) {
+        bool part = splits > 1;
+        if constexpr (C8) part = a.splits > 1;
+        if (part) {
             const int64_t to_row = (tok_all * a.q_heads + hq) * a.splits + split;
 #pragma unroll
             for (int d = 0; d < VD; ++d) *reinterpret_cast<float4v*>(a.po + to_row * DP + d * 16 + e) = r.o[t][d];
@@ -1054,15 +1124,16 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(ARGS a) {
 
 // The splits of a row joined: DP / 4 lanes per row and G parts of its splits, as many rows as that leaves room for.  (One row per workgroup took 15 us for
 // 10,752 rows of 4 splits, 22 MB, where this takes 6.)
-template <int DT, int DP, int G>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+template <int DT, int DP, int G, typename ARGS = AttnArgs>
+__global__ __launch_bounds__(256) void attn_join_kernel(ARGS a) {
     constexpr int Q = DP / 4, R = 256 / (Q * G);
     static_assert(R >= 1, "a workgroup holds a row");
     __shared__ __attribute__((aligned(16))) float4v part[R][G][Q];
     const int tid = threadIdx.x, q = tid % Q, g = tid / Q % G, rr = tid / (Q * G);
     const uint32_t per = (uint32_t)a.most_new * a.q_heads, i = blockIdx.x * R + rr, b = i / per, r = i - b * per, tok = r / a.q_heads, hq = r - tok * a.q_heads;
     const AttnSeq s = attn_seq(a, min((int)b, a.seqs - 1));
-    const int splits = (int)tok * a.group + (int)hq % a.group < a.last_row ? a.splits : a.last_splits;
+    int splits = (int)tok * a.group + (int)hq % a.group < a.last_row ? a.splits : a.last_splits;
+    if constexpr (!std::is_same_v<ARGS, AttnArgs>) splits = a.parts[(((int)tok * a.group + (int)hq % a.group) >> a.block) * a.seqs + min((int)b, a.seqs - 1)];
     const bool live = (int)b < a.seqs && (int)tok < s.n;
     const int64_t row = (int64_t)(s.first + tok) * a.q_heads + hq, at = row * a.splits;
     float m = ATTN_NOTHING, l = 0.f;
@@ -1148,7 +1219,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 
 // ------------------------------------------------------------------------------------------ host
 
-struct AttnPlan { int dp, mt, nw, row_blocks, splits, last_splits, last_row; };       // nw: waves of the many-row kernel; 0: the few-row one, mt tiles of rows
+// nw: waves of the many-row kernel; 0: the few-row one, mt tiles of rows.  slots: the most parts of a sequence, more than splits where sequences share workgroups by their lengths
+struct AttnPlan { int dp, mt, nw, row_blocks, splits, last_splits, last_row, slots; };
 constexpr int attn_waves(int dp) { return dp == 256 ? 2 : 4; }
 constexpr int ATTN8_WAVES = 4;
 
@@ -1175,12 +1247,12 @@ int attn_launch_many(const AttnArgs& a, unsigned grid, hipStream_t s) {
     return check_launch("sq_tree_attention");
 }
 
-template <int DT, int DP>
-int attn_launch_join(const AttnArgs& a, hipStream_t s) {
+template <int DT, int DP, typename ARGS = AttnArgs>
+int attn_launch_join(const ARGS& a, hipStream_t s) {
     const int64_t all = (int64_t)a.seqs * a.most_new * a.q_heads;
     constexpr int MOST = 1024 / DP;                          // parts of a row that fill a workgroup
-    if (a.splits > 8) hipLaunchKernelGGL((attn_join_kernel<DT, DP, MOST>), dim3((unsigned)all), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attn_join_kernel<DT, DP, 1>), dim3((unsigned)((all + MOST - 1) / MOST)), dim3(256), 0, s, a);
+    if (a.splits > 8) hipLaunchKernelGGL((attn_join_kernel<DT, DP, MOST, ARGS>), dim3((unsigned)all), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_join_kernel<DT, DP, 1, ARGS>), dim3((unsigned)((all + MOST - 1) / MOST)), dim3(256), 0, s, a);
     return check_launch("sq_tree_attention: join");
 }
 

@@ -286,7 +286,8 @@ int attn8_launch_dim(const Attn8Args& a, const AttnPlan& p, hipStream_t s) {
         constexpr bool lines = FULL && DP >= 128;            // (heads that are lines of their own: nobody else reads them)
         rc = lines && a.passing ? few(std::integral_constant<bool, lines>()) : few(std::false_type());
     }
-    return rc || p.splits == 1 ? rc : attn_launch_join<DT, DP>(a, s);
+    if (rc || p.splits == 1) return rc;
+    return a.parts ? attn_launch_join<DT, DP, Attn8Args>(a, s) : attn_launch_join<DT, DP, AttnArgs>(a, s);
 }
 template <int DT>
 int attn8_launch(const Attn8Args& a, const AttnPlan& p, hipStream_t s) {

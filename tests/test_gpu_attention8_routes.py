@@ -79,3 +79,34 @@ def test_the_same_under_a_table_of_any_width():
     for width in (0, 100, 4000):
         wide = torch.cat((s.table, torch.full((2, width), -1, dtype=torch.int32)), 1)
         s.check(*attend(s, table=wide.cuda()))
+
+
+@pytest.mark.parametrize("d,hq,hk,new,tree", [(128, 14, 2, 48, True), (64, 8, 1, 150, False), (256, 10, 2, 40, True)])
+def test_sequences_of_all_lengths_in_a_captured_call(d, hq, hk, new, tree):
+    """Parts are dealt to sequences by their lengths, which change from replay to replay: long ones beside short and empty ones, all alike, one alone."""
+    from quantexperiments_amd.kernels import tree_attention8
+    top = 4200
+    s = Setup([top] * 9, [new] * 9, hq, hk, d, 16, tree=tree, seed=d)
+    dev, lse = s.device(), torch.empty(s.n, hq, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = tree_attention8(**dev, lse=lse)
+    for lens in ([top, 3, 0, 3000, 64, 63, 2000, 1, 900], [1000] * 9, [0] * 8 + [top], [top] + [0] * 8, [top - 64 * b for b in range(9)]):
+        s.lens = lens
+        s.places = [(s.table[b, torch.arange(n + new) // 16].long(), torch.arange(n + new) % 16) for b, n in enumerate(lens)]
+        dev["lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        s.check(out, lse)
+
+
+@pytest.mark.parametrize("seqs", [63, 64, 65])
+def test_as_many_sequences_as_a_wave_has_lanes(seqs):
+    lens = [(b * 37) % 700 if b % 5 else 0 for b in range(seqs)]
+    news = [0 if b % 7 == 3 else 40 - b % 3 for b in range(seqs)]
+    s = Setup(lens, news, 4, 1, 64, 16, seed=seqs, extra_rows=3)
+    wide = torch.cat((s.table, torch.full((seqs, 200), -1, dtype=torch.int32)), 1)          # (many parts)
+    s.check(*attend(s, table=wide.cuda()))
