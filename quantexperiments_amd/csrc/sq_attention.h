@@ -249,7 +249,10 @@ struct Attn8Args : AttnArgs {
     int size;                    // tokens of a block, a multiple of 16
     int inner;                   // few rows: workgroups that read the same lines (blocks of rows; heads that share lines), dealt to one die one behind the other
     int passing;                 // few rows: keys and values are read past the caches
-    int32_t* parts;              // many rows, or null: of each block of rows and sequence, into how many its keys are cut; `splits` is then the most
+};
+// many rows of sequences that share workgroups by their lengths
+struct Attn8Shared : Attn8Args {
+    int32_t* parts;              // of each block of rows and sequence: into how many its keys are cut; `splits` is the most
     int cut, block;              // and how many there are in the mean before the last block; rows of a block are 2^block
 };
 
@@ -694,8 +697,8 @@ template <int DP, int NW> constexpr int attn8_tile_lds() { return ATTN8_STAGES *
 
 // Sequences of several lengths under one block of rows share its workgroups by their lengths, not evenly: the fewest stages T such that all of them, cut into parts of T, are
 // no more parts than there are workgroups.  Workgroup `split` of sequence b becomes part `split` of `splits` of another b.  (Lengths are on the device; up to 64 sequences, one a lane.)
-// 8 trees of 48 tokens behind 1408 to 4096 slots, 28 + 4 heads of 128: 52.2 us evenly, 47.4 so, of 20 + 4 heads of 256 67.1 and 57.4 (61 with END zero), 16 of 32
-// behind 1100 to 4000 53.2 and 49.3; where all are as long it costs 2 (8 behind 4096 51.9 and 53.7).
+// 8 trees of 48 tokens behind 1408 to 4096 slots, 28 + 4 heads of 128: 52.2 us evenly, 46.1 so, of 20 + 4 heads of 256 67.1 and 57.2 (61 with END zero), 16 of 32
+// behind 1100 to 4000 53.2 and 48.6; where all are as long it costs up to 1.5 (8 behind 4096 51.9 and 52.5).
 template <typename F> __device__ __forceinline__ uint32_t attn8_fold(uint32_t v, F f) {          // over the wave
     const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     v = f((uint32_t)h[0], (uint32_t)h[1]);
@@ -713,7 +716,7 @@ __device__ __forceinline__ int attn8_parts(int x, int d, float by) {
     return q + (q * d < x);
 }
 template <int KEYS, int ROWS, int END>
-__device__ __forceinline__ bool attn8_share(const Attn8Args& a, int row0, int head, int lane, int& b, int& split, int& splits, AttnSeq& seq) {
+__device__ __forceinline__ bool attn8_share(const Attn8Shared& a, int row0, int head, int lane, int& b, int& split, int& splits, AttnSeq& seq) {
     auto sum = [](int v) __attribute__((always_inline)) { return (int)attn8_fold((uint32_t)v, [](uint32_t x, uint32_t y) { return x + y; }); };
     const int all = a.seqs * splits, mine = b * splits + split;            // (so most stay on the die that has their sequence)
     const AttnSeq s = attn_seq(a, min(lane, a.seqs - 1));
@@ -786,10 +789,10 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(ARGS a) {
     typedef short short4v __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) short4v* tr_ptr;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    constexpr bool C8 = !std::is_same_v<ARGS, AttnArgs>;
+    constexpr bool C8 = !std::is_same_v<ARGS, AttnArgs>, SHARED = std::is_same_v<ARGS, Attn8Shared>;
     constexpr int MT = attn_tiles(DP), SK = attn_stage_steps(DP, NW), KEYS = SK * ATTN_STEP, NB = C8 ? ATTN8_STAGES : ATTN_STAGES, STAGE = attn_stage_bytes<DP, NW>(), ROWS = NW * MT * 16;
     constexpr int MINE = KEYS / NW, C = MINE / T::ROWS, KC = DP / 32, VD = DP / 16;
-    constexpr int END = MT >= 2 ? 0 : 2;                     // (stages that a sequence's end, which goes step by step, costs beside its own)
+    constexpr int END = SHARED && MT < 2 ? 2 : 0;                // (stages that a sequence's end, which goes step by step, costs beside its own)
     constexpr bool PIPELINE = MT >= 2;                       // (a tile's maximum is raised while the sums of the tile before it are outstanding)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, i16 = lane & 15;
     // the workgroups of one key head are dealt to as few dies as there are: neighbours are other heads'; last rows, which have most keys, first
@@ -799,22 +802,18 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(ARGS a) {
     id /= groups;
     const bool end_block = id < a.last_splits;
     int splits = end_block ? a.last_splits : a.splits, split;
-    if constexpr (C8) if (!end_block) splits = a.cut;
+    if constexpr (SHARED) if (!end_block) splits = a.cut;
     if (!end_block) id -= a.last_splits;
     split = id % splits;
     const int row0 = (a.row_blocks - (end_block ? 1 : 2) - id / splits) * ROWS;
     AttnSeq s;
-    if constexpr (C8) {
-        if (!a.parts) s = attn_seq(a, b);
-        else if (!attn8_share<KEYS, ROWS, END>(a, row0, head, lane, b, split, splits, s)) return;
-    } else s = attn_seq(a, b);
+    if constexpr (!SHARED) s = attn_seq(a, b);
+    else if (!attn8_share<KEYS, ROWS, END>(a, row0, head, lane, b, split, splits, s)) return;
     const int rows = s.n * a.group;
     if (row0 >= rows) return;
     const int last = min(row0 + ROWS, rows) - 1;
     const int seen = a.mask ? s.total : min(s.total, s.len + last / a.group + 1);
-    int ending = 0;
-    if constexpr (C8) ending = a.parts ? END : 0;
-    const int stages = (seen + KEYS - 1) / KEYS, per = (stages + ending + splits - 1) / splits, begin = min(split * per, stages), end = min(begin + per, stages);
+    const int stages = (seen + KEYS - 1) / KEYS, per = (stages + END + splits - 1) / splits, begin = min(split * per, stages), end = min(begin + per, stages);
 
     AttnRows<DP, MT> r;
     const int mine = row0 + wave * MT * 16;
@@ -1099,9 +1098,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(ARGS a) {
         if (bad) l = NAN;
         if (row >= rows) continue;
         const int64_t tok_all = s.first + tok;
-        bool part = splits > 1;
-        if constexpr (C8) part = a.splits > 1;
-        if (part) {
+        if (SHARED || splits > 1) {
             const int64_t to_row = (tok_all * a.q_heads + hq) * a.splits + split;
 #pragma unroll
             for (int d = 0; d < VD; ++d) *reinterpret_cast<float4v*>(a.po + to_row * DP + d * 16 + e) = r.o[t][d];
@@ -1133,7 +1130,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(ARGS a) {
     const uint32_t per = (uint32_t)a.most_new * a.q_heads, i = blockIdx.x * R + rr, b = i / per, r = i - b * per, tok = r / a.q_heads, hq = r - tok * a.q_heads;
     const AttnSeq s = attn_seq(a, min((int)b, a.seqs - 1));
     int splits = (int)tok * a.group + (int)hq % a.group < a.last_row ? a.splits : a.last_splits;
-    if constexpr (!std::is_same_v<ARGS, AttnArgs>) splits = a.parts[(((int)tok * a.group + (int)hq % a.group) >> a.block) * a.seqs + min((int)b, a.seqs - 1)];
+    if constexpr (std::is_same_v<ARGS, Attn8Shared>) splits = a.parts[(((int)tok * a.group + (int)hq % a.group) >> a.block) * a.seqs + min((int)b, a.seqs - 1)];
     const bool live = (int)b < a.seqs && (int)tok < s.n;
     const int64_t row = (int64_t)(s.first + tok) * a.q_heads + hq, at = row * a.splits;
     float m = ATTN_NOTHING, l = 0.f;

@@ -75,7 +75,7 @@ AttnPlan attn_plan(const sq_attention& a, const sq_cache& c, bool held8) {
         }
     }
     p.slots = p.splits;
-    // (fewer than 16 parts are too few to deal out: 4 x 200 tokens behind 1000 to 4000 in eight 84.4 us, so 85.0)
+    // (fewer than 16 parts are too few to deal out: 4 x 200 tokens behind 1000 to 4000 in eight 84.4 us, shared by length 85.0)
     if (held8 && p.nw && p.splits > 1 && a.seqs > 1 && a.seqs <= 64 && a.seqs * p.last_splits >= 16 && steps < (1 << 20)) p.slots = p.splits <= 4 ? 2 * p.splits : p.splits <= 8 ? 8 : 2 * p.splits < ATTN_SPLITS_MAX ? 2 * p.splits : ATTN_SPLITS_MAX;
     return p;
 }

@@ -265,19 +265,25 @@ int attn8_launch_few(const Attn8Args& a, unsigned grid, hipStream_t s) {
     hipLaunchKernelGGL((attn8_kernel<DT, DP, MT, NW, FULL, PASSING>), dim3(grid), dim3(NW * 64), LDS, s, a);
     return check_launch("sq_tree_attention8");
 }
-template <int DT, int DP, int NW, bool FULL>
-int attn8_launch_many(const Attn8Args& a, unsigned grid, hipStream_t s) {
+template <int DT, int DP, int NW, bool FULL, typename ARGS>
+int attn8_launch_many(const ARGS& a, unsigned grid, hipStream_t s) {
     constexpr int LDS = attn8_tile_lds<DP, NW>();
     static bool raised[64];
-    attn_raise((const void*)attn_tile_kernel<DT, DP, NW, FULL, Attn8Args>, LDS, raised);
-    hipLaunchKernelGGL((attn_tile_kernel<DT, DP, NW, FULL, Attn8Args>), dim3(grid), dim3(NW * 64), LDS, s, a);
+    attn_raise((const void*)attn_tile_kernel<DT, DP, NW, FULL, ARGS>, LDS, raised);
+    hipLaunchKernelGGL((attn_tile_kernel<DT, DP, NW, FULL, ARGS>), dim3(grid), dim3(NW * 64), LDS, s, a);
     return check_launch("sq_tree_attention8");
 }
 template <int DT, int DP, bool FULL>
-int attn8_launch_dim(const Attn8Args& a, const AttnPlan& p, hipStream_t s) {
+int attn8_launch_dim(const Attn8Shared& a, const AttnPlan& p, hipStream_t s) {
     const unsigned grid = (unsigned)((int64_t)a.seqs * a.kv_heads * ((p.row_blocks - 1) * p.splits + p.last_splits));
     int rc;
-    if (p.nw) rc = p.nw == 4 ? attn8_launch_many<DT, DP, 4, FULL>(a, grid, s) : attn8_launch_many<DT, DP, 8, FULL>(a, grid, s);
+    if (p.nw) {
+        auto many = [&](const auto& args) {
+            typedef std::decay_t<decltype(args)> ARGS;
+            return p.nw == 4 ? attn8_launch_many<DT, DP, 4, FULL, ARGS>(args, grid, s) : attn8_launch_many<DT, DP, 8, FULL, ARGS>(args, grid, s);
+        };
+        rc = a.parts ? many(a) : many((const Attn8Args&)a);
+    }
     else {
         auto few = [&](auto passing) {
             constexpr bool P = decltype(passing)::value;
@@ -287,17 +293,17 @@ int attn8_launch_dim(const Attn8Args& a, const AttnPlan& p, hipStream_t s) {
         rc = lines && a.passing ? few(std::integral_constant<bool, lines>()) : few(std::false_type());
     }
     if (rc || p.splits == 1) return rc;
-    return a.parts ? attn_launch_join<DT, DP, Attn8Args>(a, s) : attn_launch_join<DT, DP, AttnArgs>(a, s);
+    return a.parts ? attn_launch_join<DT, DP, Attn8Shared>(a, s) : attn_launch_join<DT, DP, AttnArgs>(a, s);
 }
 template <int DT>
-int attn8_launch(const Attn8Args& a, const AttnPlan& p, hipStream_t s) {
+int attn8_launch(const Attn8Shared& a, const AttnPlan& p, hipStream_t s) {
     auto go = [&](auto dp) {
         constexpr int DP = decltype(dp)::value;
         return a.dim == DP ? attn8_launch_dim<DT, DP, true>(a, p, s) : attn8_launch_dim<DT, DP, false>(a, p, s);
     };
     return p.dp == 64 ? go(std::integral_constant<int, 64>()) : p.dp == 128 ? go(std::integral_constant<int, 128>()) : go(std::integral_constant<int, 256>());
 }
-int attn8_launch_f16(const Attn8Args& a, const AttnPlan& p, hipStream_t s);
-int attn8_launch_bf16(const Attn8Args& a, const AttnPlan& p, hipStream_t s);
+int attn8_launch_f16(const Attn8Shared& a, const AttnPlan& p, hipStream_t s);
+int attn8_launch_bf16(const Attn8Shared& a, const AttnPlan& p, hipStream_t s);
 
 }  // namespace sq

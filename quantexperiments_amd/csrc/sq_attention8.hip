@@ -33,7 +33,7 @@ int sq_tree_attention8(const sq_attention* a, const sq_cache8* cache, int dtype,
     if (int rc = check_attention8(who, a, cache, dtype, c)) return rc;
     if (attn_nothing(*a)) return SQ_OK;
     const AttnPlan p = attn_plan(*a, c, true);
-    Attn8Args k;
+    Attn8Shared k;
     if (int rc = attn_prepare(who, *a, c, p, workspace, ws_bytes, k)) return rc;
     k.k_page = cache->k_page; k.k_slot = cache->k_slot; k.k_head = cache->k_head; k.v_page = cache->v_page; k.v_slot = cache->v_slot; k.v_head = cache->v_head;
     k.near = 1;

@@ -2,5 +2,5 @@
 #include "sq_attention8.h"
 
 namespace sq {
-int attn8_launch_bf16(const Attn8Args& a, const AttnPlan& p, hipStream_t s) { return attn8_launch<SQ_BF16>(a, p, s); }
+int attn8_launch_bf16(const Attn8Shared& a, const AttnPlan& p, hipStream_t s) { return attn8_launch<SQ_BF16>(a, p, s); }
 }  // namespace sq
