@@ -110,3 +110,10 @@ def test_as_many_sequences_as_a_wave_has_lanes(seqs):
     s = Setup(lens, news, 4, 1, 64, 16, seed=seqs, extra_rows=3)
     wide = torch.cat((s.table, torch.full((seqs, 200), -1, dtype=torch.int32)), 1)          # (many parts)
     s.check(*attend(s, table=wide.cuda()))
+
+
+@pytest.mark.parametrize("d", [16, 48, 144, 208])
+@pytest.mark.parametrize("lens,news,hq,hk,tree", [([500, 3], [1, 1], 71, 1, False), ([700, 0, 64], [2, 3, 1], 300, 1, True), ([90] * 40, [20] * 40, 9, 3, True), ([3300, 2000, 5], [60, 60, 1], 12, 1, True)])
+def test_groups_and_widths_that_fill_no_block(lens, news, hq, hk, tree, d):
+    s = Setup(lens, news, hq, hk, d, 48, blocks=3, tree=tree, seed=d + hq)
+    s.check(*attend(s))
