@@ -250,10 +250,10 @@ struct Attn8Args : AttnArgs {
     int inner;                   // few rows: workgroups that read the same lines (blocks of rows; heads that share lines), dealt to one die one behind the other
     int passing;                 // few rows: keys and values are read past the caches
 };
-// many rows of sequences that share workgroups by their lengths
+// many rows: the blocks of rows of all sequences share the workgroups of a key head by how many keys they see
 struct Attn8Shared : Attn8Args {
     int32_t* parts;              // of each block of rows and sequence: into how many its keys are cut; `splits` is the most
-    int cut, block;              // and how many there are in the mean before the last block; rows of a block are 2^block
+    int block;                   // rows of a block are 2^block
 };
 
 // 8 codes times a power of two as a matrix instruction's operand: v_cvt_scalef32_pk takes two at a time and the scale with them, exactly
@@ -695,10 +695,11 @@ constexpr int ATTN8_STAGES = 3, ATTN8_RAW = 3;
 template <int DP, int NW> constexpr int attn8_copies() { return (attn_stage_steps(DP, NW) * ATTN_STEP / NW * DP + 1023) / 1024; }      // of a wave's keys of a stage
 template <int DP, int NW> constexpr int attn8_tile_lds() { return ATTN8_STAGES * attn_stage_bytes<DP, NW>() + ATTN8_RAW * NW * 2048 * attn8_copies<DP, NW>() + 64; }
 
-// Sequences of several lengths under one block of rows share its workgroups by their lengths, not evenly: the fewest stages T such that all of them, cut into parts of T, are
-// no more parts than there are workgroups.  Workgroup `split` of sequence b becomes part `split` of `splits` of another b.  (Lengths are on the device; up to 64 sequences, one a lane.)
-// 8 trees of 48 tokens behind 1408 to 4096 slots, 28 + 4 heads of 128: 52.2 us evenly, 46.1 so, of 20 + 4 heads of 256 67.1 and 57.2 (61 with END zero), 16 of 32
-// behind 1100 to 4000 53.2 and 48.6; where all are as long it costs up to 1.5 (8 behind 4096 51.9 and 52.5).
+// The blocks of rows of all sequences share the workgroups of a key head by their work, not evenly: with the least T such that all of them, cut into parts of T, are no more parts than
+// there are workgroups.  Work is the stages that a block's rows see, of a block that fills half of its waves or less 0.6 of them.  Workgroup `which` becomes part `split` of `splits` of one.
+// (Lengths are on the device; up to 64 blocks, one a lane.)
+// 8 trees of 48 tokens behind 1408 to 4096 slots, 28 + 4 heads of 128: 52.2 us in as many parts each, 45.3 so, of 20 + 4 heads of 256 67.1 and 57.8 (61 with END zero); 4 x 200 behind 1000 to
+// 4000 84.4 and 73.5; 1500 tokens behind 2100 120 and 109, 1000 of 20 + 4 heads of 256 147 and 132; 8 trees of one length 51.9 and 53.2.
 template <typename F> __device__ __forceinline__ uint32_t attn8_fold(uint32_t v, F f) {          // over the wave
     const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     v = f((uint32_t)h[0], (uint32_t)h[1]);
@@ -716,23 +717,24 @@ __device__ __forceinline__ int attn8_parts(int x, int d, float by) {
     return q + (q * d < x);
 }
 template <int KEYS, int ROWS, int END>
-__device__ __forceinline__ bool attn8_share(const Attn8Shared& a, int row0, int head, int lane, int& b, int& split, int& splits, AttnSeq& seq) {
+__device__ __forceinline__ bool attn8_share(const Attn8Shared& a, int which, int all, int head, int lane, int& b, int& row0, int& split, int& splits, AttnSeq& seq) {
     auto sum = [](int v) __attribute__((always_inline)) { return (int)attn8_fold((uint32_t)v, [](uint32_t x, uint32_t y) { return x + y; }); };
-    const int all = a.seqs * splits, mine = b * splits + split;            // (so most stay on the die that has their sequence)
-    const AttnSeq s = attn_seq(a, min(lane, a.seqs - 1));
-    // (about how many stages: what a part has of them is worked out from the sequence itself)
-    const int rows = s.n * a.group, last = min(row0 + ROWS, rows) - 1, seen = a.mask ? s.total : min(s.total, s.len + (int)((float)last * __builtin_amdgcn_rcpf((float)a.group)) + 1);
-    const int stages = lane < a.seqs && row0 < rows ? (seen + KEYS - 1) / KEYS + END : 0;
-    const int most = (int)attn8_fold((uint32_t)stages, [](uint32_t x, uint32_t y) { return max(x, y); });
-    const float total = (float)sum(stages);
-    // (T = total / (all - seqs) is enough, since each sequence's last part may be short; fewer than two stages are not worth a part)
-    int t = max(max((int)(total * __builtin_amdgcn_rcpf((float)all)), attn8_parts(most, a.splits, __builtin_amdgcn_rcpf((float)a.splits))), 2);
-    int enough = max(t, (int)(total * __builtin_amdgcn_rcpf((float)(all - a.seqs))) + 2);
+    const int items = a.seqs * a.row_blocks, item = min(lane, items - 1), of = item / a.row_blocks, first = (a.row_blocks - 1 - (item - of * a.row_blocks)) * ROWS;
+    const AttnSeq s = attn_seq(a, of);
+    // (about how much: what a part has of it is worked out from the sequence itself)
+    const int rows = s.n * a.group, here = min(rows - first, ROWS);
+    const int seen = a.mask ? s.total : min(s.total, s.len + (int)((float)(first + here - 1) * __builtin_amdgcn_rcpf((float)a.group)) + 1);
+    const int work = lane < items && here > 0 ? ((seen + KEYS - 1) / KEYS + END) * (2 * here <= ROWS ? 3 : 5) : 0;
+    const int most = (int)attn8_fold((uint32_t)work, [](uint32_t x, uint32_t y) { return max(x, y); });
+    const float total = (float)sum(work);
+    // (T = total / (all - items) is enough, since each block's last part may be short; fewer than two stages are not worth a part)
+    int t = max(max((int)(total * __builtin_amdgcn_rcpf((float)all)), attn8_parts(most, a.splits, __builtin_amdgcn_rcpf((float)a.splits))), 10);
+    int enough = max(t, min(most, (int)(total * __builtin_amdgcn_rcpf((float)(all - items))) + 2));
     while (t < enough) {
         const int half = (t + enough) / 2;
-        if (sum(attn8_parts(stages, half, __builtin_amdgcn_rcpf((float)half))) <= all) enough = half; else t = half + 1;
+        if (sum(attn8_parts(work, half, __builtin_amdgcn_rcpf((float)half))) <= all) enough = half; else t = half + 1;
     }
-    const int parts = attn8_parts(stages, t, __builtin_amdgcn_rcpf((float)t));
+    const int parts = attn8_parts(work, t, __builtin_amdgcn_rcpf((float)t));
     int upto = parts;
     upto += attn8_from_left<1>(upto);
     upto += attn8_from_left<2>(upto);
@@ -740,14 +742,16 @@ __device__ __forceinline__ bool attn8_share(const Attn8Shared& a, int row0, int 
     upto += attn8_from_left<8>(upto);
     const int r0 = __builtin_amdgcn_readlane(upto, 15), r1 = __builtin_amdgcn_readlane(upto, 31), r2 = __builtin_amdgcn_readlane(upto, 47);
     upto += lane < 16 ? 0 : lane < 32 ? r0 : lane < 48 ? r0 + r1 : r0 + r1 + r2;
-    if (mine == 0 && head == 0 && threadIdx.x < (unsigned)a.seqs) a.parts[row0 / ROWS * a.seqs + lane] = parts;
-    const uint64_t here = __ballot(mine >= upto - parts && mine < upto);
-    if (!here) return false;
-    b = __builtin_ctzll(here);
-    splits = __builtin_amdgcn_readlane(parts, b);
-    split = mine - __builtin_amdgcn_readlane(upto - parts, b);
-    seq = {__builtin_amdgcn_readlane(s.first, b), __builtin_amdgcn_readlane(s.n, b), __builtin_amdgcn_readlane(s.len, b), __builtin_amdgcn_readlane(s.total, b),
-           __builtin_amdgcn_readlane((int)s.over, b) != 0};
+    if (which == 0 && head == 0 && threadIdx.x < (unsigned)items) a.parts[first / ROWS * a.seqs + of] = parts;
+    const uint64_t mine = __ballot(which >= upto - parts && which < upto);
+    if (!mine) return false;
+    const int l = __builtin_ctzll(mine);
+    b = __builtin_amdgcn_readlane(of, l);
+    row0 = __builtin_amdgcn_readlane(first, l);
+    splits = __builtin_amdgcn_readlane(parts, l);
+    split = which - __builtin_amdgcn_readlane(upto - parts, l);
+    seq = {__builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.n, l), __builtin_amdgcn_readlane(s.len, l), __builtin_amdgcn_readlane(s.total, l),
+           __builtin_amdgcn_readlane((int)s.over, l) != 0};
     return true;
 }
 
@@ -796,19 +800,23 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(ARGS a) {
     constexpr bool PIPELINE = MT >= 2;                       // (a tile's maximum is raised while the sums of the tile before it are outstanding)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, i16 = lane & 15;
     // the workgroups of one key head are dealt to as few dies as there are: neighbours are other heads'; last rows, which have most keys, first
-    int id = blockIdx.x;
-    const int groups = a.seqs * a.kv_heads, head = id % groups % a.kv_heads;
-    int b = id % groups / a.kv_heads;
-    id /= groups;
-    const bool end_block = id < a.last_splits;
-    int splits = end_block ? a.last_splits : a.splits, split;
-    if constexpr (SHARED) if (!end_block) splits = a.cut;
-    if (!end_block) id -= a.last_splits;
-    split = id % splits;
-    const int row0 = (a.row_blocks - (end_block ? 1 : 2) - id / splits) * ROWS;
+    int id = blockIdx.x, head, b, row0, split, splits;
     AttnSeq s;
-    if constexpr (!SHARED) s = attn_seq(a, b);
-    else if (!attn8_share<KEYS, ROWS, END>(a, row0, head, lane, b, split, splits, s)) return;
+    if constexpr (SHARED) {
+        head = id % a.kv_heads;
+        if (!attn8_share<KEYS, ROWS, END>(a, id / a.kv_heads, gridDim.x / a.kv_heads, head, lane, b, row0, split, splits, s)) return;
+    } else {
+        const int groups = a.seqs * a.kv_heads;
+        b = id % groups / a.kv_heads;
+        head = id % groups % a.kv_heads;
+        id /= groups;
+        const bool end_block = id < a.last_splits;
+        splits = end_block ? a.last_splits : a.splits;
+        if (!end_block) id -= a.last_splits;
+        split = id % splits;
+        row0 = (a.row_blocks - (end_block ? 1 : 2) - id / splits) * ROWS;
+        s = attn_seq(a, b);
+    }
     const int rows = s.n * a.group;
     if (row0 >= rows) return;
     const int last = min(row0 + ROWS, rows) - 1;
@@ -1098,7 +1106,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(ARGS a) {
         if (bad) l = NAN;
         if (row >= rows) continue;
         const int64_t tok_all = s.first + tok;
-        if (SHARED || splits > 1) {
+        if (splits > 1) {
             const int64_t to_row = (tok_all * a.q_heads + hq) * a.splits + split;
 #pragma unroll
             for (int d = 0; d < VD; ++d) *reinterpret_cast<float4v*>(a.po + to_row * DP + d * 16 + e) = r.o[t][d];
@@ -1130,8 +1138,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(ARGS a) {
     const uint32_t per = (uint32_t)a.most_new * a.q_heads, i = blockIdx.x * R + rr, b = i / per, r = i - b * per, tok = r / a.q_heads, hq = r - tok * a.q_heads;
     const AttnSeq s = attn_seq(a, min((int)b, a.seqs - 1));
     int splits = (int)tok * a.group + (int)hq % a.group < a.last_row ? a.splits : a.last_splits;
-    if constexpr (std::is_same_v<ARGS, Attn8Shared>) splits = a.parts[(((int)tok * a.group + (int)hq % a.group) >> a.block) * a.seqs + min((int)b, a.seqs - 1)];
-    const bool live = (int)b < a.seqs && (int)tok < s.n;
+    bool live = (int)b < a.seqs && (int)tok < s.n;
+    if constexpr (std::is_same_v<ARGS, Attn8Shared>) {
+        splits = live ? a.parts[(((int)tok * a.group + (int)hq % a.group) >> a.block) * a.seqs + (int)b] : 1;
+        live &= splits > 1;                                  // (a block that is not cut is written as it is)
+    }
     const int64_t row = (int64_t)(s.first + tok) * a.q_heads + hq, at = row * a.splits;
     float m = ATTN_NOTHING, l = 0.f;
     float4v v = float4v{0.f, 0.f, 0.f, 0.f};
@@ -1216,8 +1227,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(ARGS a) {
 
 // ------------------------------------------------------------------------------------------ host
 
-// nw: waves of the many-row kernel; 0: the few-row one, mt tiles of rows.  slots: the most parts of a sequence, more than splits where sequences share workgroups by their lengths
-struct AttnPlan { int dp, mt, nw, row_blocks, splits, last_splits, last_row, slots; };
+// nw: waves of the many-row kernel; 0: the few-row one, mt tiles of rows.  slots: the most parts of a row's keys; workgroups: of a key head, where they are shared by work, or 0
+struct AttnPlan { int dp, mt, nw, row_blocks, splits, last_splits, last_row, slots, workgroups; };
 constexpr int attn_waves(int dp) { return dp == 256 ? 2 : 4; }
 constexpr int ATTN8_WAVES = 4;
 

@@ -75,8 +75,15 @@ AttnPlan attn_plan(const sq_attention& a, const sq_cache& c, bool held8) {
         }
     }
     p.slots = p.splits;
-    // (fewer than 16 parts are too few to deal out: 4 x 200 tokens behind 1000 to 4000 in eight 84.4 us, shared by length 85.0)
-    if (held8 && p.nw && p.splits > 1 && a.seqs > 1 && a.seqs <= 64 && a.seqs * p.last_splits >= 16 && steps < (1 << 20)) p.slots = p.splits <= 4 ? 2 * p.splits : p.splits <= 8 ? 8 : 2 * p.splits < ATTN_SPLITS_MAX ? 2 * p.splits : ATTN_SPLITS_MAX;
+    // Over a cache held in 8 bits the blocks of rows of all sequences share a key head's workgroups by their work (attn8_share), where these are half as many again; an eighth more are enough for one
+    // sequence's, of which the last sees most: 1900 tokens behind 2100 131 us, so 129.  (16 x 100 behind 1000, 48 blocks on 64 workgroups, 49.8 and 58.6.)
+    const int64_t items = a.seqs * (int64_t)p.row_blocks, room = cus / c.heads;
+    p.workgroups = 0;
+    if (held8 && p.nw && items > 1 && items <= 64 && (a.seqs == 1 ? 8 * items <= 7 * room : 3 * items <= 2 * room) && steps < (1 << 17)) {
+        p.workgroups = (int)room;
+        const int64_t slots = 2 * p.workgroups / items;      // (two or more; the join of more than eight takes longer)
+        p.slots = (int)(slots > 8 && slots <= 16 ? 8 : slots < ATTN_SPLITS_MAX ? slots : ATTN_SPLITS_MAX);
+    }
     return p;
 }
 
@@ -100,7 +107,7 @@ int check_attention(const char* who, const sq_attention* a, const sq_cache* c) {
 bool attn_nothing(const sq_attention& a) { return a.tokens == 0 || a.seqs == 0 || a.most_new == 0; }
 
 size_t attn_workspace(const sq_attention& a, const AttnPlan& p) {
-    return p.splits == 1 ? 0 : (size_t)a.tokens * a.q_heads * p.slots * (p.dp * 4 + 8) + (p.slots > p.splits ? (size_t)p.row_blocks * a.seqs * 4 : 0);
+    return p.slots == 1 ? 0 : (size_t)a.tokens * a.q_heads * p.slots * (p.dp * 4 + 8) + (p.workgroups ? (size_t)p.row_blocks * a.seqs * 4 : 0);
 }
 
 // Everything of a call that the kernels are told but the strides of its cache
@@ -112,7 +119,7 @@ int attn_prepare(const char* who, const sq_attention& a, const sq_cache& c, cons
         return fail(SQ_EUNSUPPORTED, "%s: q, out, keys and values need 16-byte aligned heads", who);
     const int64_t ot = a.out_token < 0 ? -a.out_token : a.out_token, oh = a.out_head < 0 ? -a.out_head : a.out_head;
     if (!rows_apart(a.tokens, a.q_heads, ot, oh, c.dim)) return fail(SQ_EINVAL, "%s: rows of the output overlap (strides %lld, %lld)", who, (long long)ot, (long long)oh);
-    if ((int64_t)a.seqs * c.heads * p.row_blocks * p.splits > (1 << 23) || (p.splits > 1 && (int64_t)a.seqs * a.most_new * a.q_heads > (1 << 23)))
+    if ((int64_t)a.seqs * c.heads * p.row_blocks * p.splits > (1 << 23) || (p.slots > 1 && (int64_t)a.seqs * a.most_new * a.q_heads > (1 << 23)))
         return fail(SQ_EUNSUPPORTED, "%s: %d sequences of up to %d new tokens and %d heads at once", who, a.seqs, a.most_new, a.q_heads);
     const size_t need = attn_workspace(a, p);
     if (ws_bytes < need || (need && (!workspace || ((uintptr_t)workspace & 255))))

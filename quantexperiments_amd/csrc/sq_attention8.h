@@ -275,7 +275,7 @@ int attn8_launch_many(const ARGS& a, unsigned grid, hipStream_t s) {
 }
 template <int DT, int DP, bool FULL>
 int attn8_launch_dim(const Attn8Shared& a, const AttnPlan& p, hipStream_t s) {
-    const unsigned grid = (unsigned)((int64_t)a.seqs * a.kv_heads * ((p.row_blocks - 1) * p.splits + p.last_splits));
+    const unsigned grid = (unsigned)(p.workgroups ? (int64_t)a.kv_heads * p.workgroups : (int64_t)a.seqs * a.kv_heads * ((p.row_blocks - 1) * p.splits + p.last_splits));
     int rc;
     if (p.nw) {
         auto many = [&](const auto& args) {
@@ -292,7 +292,7 @@ int attn8_launch_dim(const Attn8Shared& a, const AttnPlan& p, hipStream_t s) {
         constexpr bool lines = FULL && DP >= 128;            // (heads that are lines of their own: nobody else reads them)
         rc = lines && a.passing ? few(std::integral_constant<bool, lines>()) : few(std::false_type());
     }
-    if (rc || p.splits == 1) return rc;
+    if (rc || p.slots == 1) return rc;
     return a.parts ? attn_launch_join<DT, DP, Attn8Shared>(a, s) : attn_launch_join<DT, DP, AttnArgs>(a, s);
 }
 template <int DT>

@@ -41,9 +41,8 @@ int sq_tree_attention8(const sq_attention* a, const sq_cache8* cache, int dtype,
     k.ks_page = cache->ks_page; k.ks_block = cache->ks_block; k.ks_head = cache->ks_head;
     k.vs_page = cache->vs_page; k.vs_block = cache->vs_block; k.vs_head = cache->vs_head;
     k.size = cache->page / cache->blocks;
-    k.cut = p.splits;
     k.block = p.nw ? __builtin_ctz((unsigned)(p.mt * 16 * p.nw)) : 0;
-    k.parts = p.slots > p.splits ? (int32_t*)(k.pml + (size_t)a->tokens * a->q_heads * p.slots) : nullptr;
+    k.parts = p.workgroups ? (int32_t*)(k.pml + (size_t)a->tokens * a->q_heads * p.slots) : nullptr;
     // Rows of heads that share lines of 128 bytes are fetched into each die's cache that reads one: 64 sequences of 4000 slots, 8 key heads of 64, 84 us, with a line's heads on
     // one die 62.  Of others, dealt out one behind the other, 32 sequences of 8192 x 8 of 128 108 us, so 115.
     k.inner = (cache->dim % 128 ? cache->heads : 1) * p.row_blocks;
