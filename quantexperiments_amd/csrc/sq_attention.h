@@ -63,10 +63,10 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, int b) {
         end = (int)min((int64_t)s.first + a.most_new, (int64_t)a.tokens);
     }
     s.n = min(end - s.first, a.most_new);
-    s.len = max(a.lens[b], 0);
-    const int64_t cap = min((int64_t)a.max_pages * a.page, (int64_t)ATTN_KEYS_MAX), want = (int64_t)s.len + s.n;
+    const int64_t cap = min((int64_t)a.max_pages * a.page, (int64_t)ATTN_KEYS_MAX), want = (int64_t)max(a.lens[b], 0) + s.n;
     s.over = want > cap;
     s.total = (int)min(want, cap);
+    s.len = max(s.total - s.n, 0);                           // (of a sequence that does not fit, which is NaN, what keeps len + n a number of 32 bits)
     return s;
 }
 
@@ -724,7 +724,7 @@ __device__ __forceinline__ bool attn8_share(const Attn8Shared& a, int which, int
     // (about how much: what a part has of it is worked out from the sequence itself)
     const int rows = s.n * a.group, here = min(rows - first, ROWS);
     const int seen = a.mask ? s.total : min(s.total, s.len + (int)((float)(first + here - 1) * __builtin_amdgcn_rcpf((float)a.group)) + 1);
-    const int work = lane < items && here > 0 ? ((seen + KEYS - 1) / KEYS + END) * (2 * here <= ROWS ? 3 : 5) : 0;
+    const int work = lane < items && here > 0 ? (max(seen + KEYS - 1, 0) / KEYS + END) * (2 * here <= ROWS ? 3 : 5) : 0;          // (never below zero: parts would be)
     const int most = (int)attn8_fold((uint32_t)work, [](uint32_t x, uint32_t y) { return max(x, y); });
     const float total = (float)sum(work);
     // (T = total / (all - items) is enough, since each block's last part may be short; fewer than two stages are not worth a part)
