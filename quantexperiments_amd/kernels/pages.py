@@ -15,7 +15,7 @@ import torch
 
 from .. import _lib
 from .._lib import SqPlane
-from .attention import _fits, _no_grad, _on_gpu, _rows2, _vector
+from .attention import _clash, _fits, _no_grad, _on_gpu, _rows2, _vector
 from .cache8 import _ld, _near
 
 
@@ -65,7 +65,8 @@ def _new(who: str, name: str, t, shape, *olds) -> None:
         raise ValueError(f"{who}: {name} must be int32 {tuple(shape)}: got {tuple(t.shape)} {t.dtype}")
     if t.dim() == 2:
         _rows2(who, name, t, shape[0], torch.int32)
-    if any(_near(t, o) for o in olds):
+    # (columns of one tensor's rows are told apart)
+    if any(_clash(t[:, None], o[:, None]) if t.dim() == o.dim() == 2 else _near(t, o) for o in olds):
         raise ValueError(f"{who}: {name} overlaps another operand")
 
 
