@@ -508,14 +508,15 @@ typedef struct sq_cache8 {
  * lens[b] cached tokens; its new token t (row starts[b] + t; starts NULL: most_new tokens each) goes to slot lens[b] + t.  For each block that gets new
  * tokens, and head:  a = the largest finite magnitude of its new tokens,  e = the smallest integer, -100 or more, with a <= 448 * 2^e, and
  * where the block holds tokens before lens[b], not less than its e; those are scaled to it where it grows (exact, but for codes
- * that fall below 2^-6: rounded to nearest even).  A code is x * 2^-e rounded to nearest even.  Elements that are not finite are held as NaN; |x| above 1.875 * 2^15 (fp16),
+ * that fall below 2^-6: rounded to nearest even).  A code is x * 2^-e rounded to nearest even: off by up to 2^-4 of x from 2^(e - 6) on, below by up to 2^(e - 10).  Elements that are not finite are held as NaN; |x| above 1.875 * 2^15 (fp16),
  * 1.875 * 2^127 (bf16) as that, so that what is read is finite in dtype.  New tokens from the most_new-th of a sequence on, whose slot lies behind the
  * table row, or whose page is not in the cache are not put anywhere.  Sequences must not share pages that are written. */
 int sq_put_tokens8(const sq_heads* k, const sq_heads* v, int32_t tokens, int dtype, const sq_cache8* cache, const int32_t* table, int64_t ld_table, int32_t max_pages,
                    const int32_t* lens, const int32_t* starts, int32_t seqs, int32_t most_new, void* stream);
 
 /* sq_tree_attention over such a cache: the same rows, masks, results, rounding and workspace rules, q and out of `dtype`.  Keys and values are code * scale as numbers
- * of dtype: exact in bf16, and in fp16 for what sq_put_tokens8 made of fp16 tokens (others: rounded to its steps of 2^-24, infinite beyond its range). */
+ * of dtype: exact in bf16, and in fp16 for what sq_put_tokens8 made of fp16 tokens (others: rounded to its steps of 2^-24, infinite beyond its range).
+ * Short sequences under a max_pages far from the truth are slower by more than over a 16-bit cache. */
 int sq_tree_attention8(const sq_attention* a, const sq_cache8* cache, int dtype, void* workspace, size_t ws_bytes, void* stream);
 size_t sq_tree_attention8_workspace_bytes(const sq_attention* a, const sq_cache8* cache, int dtype);
 

@@ -4,8 +4,10 @@ The cache is four tensors of a layer (or, with one more dimension in front, of a
   k_cache, v_cache  torch.float8_e4m3fn    [pages, slots per page, key heads, D]: codes
   k_scale, v_scale  torch.float8_e8m0fnu   [pages, blocks per page, key heads]: a power of two for each block of tokens and head
 and an element is code * scale.  A page has a multiple of 16 slots in each of its blocks; D is a multiple of 16 up to 256.  The scale of a block fits
-its largest element, and grows with it; being a power of two it costs no precision, so attention reads exactly what is held (half the bytes of a
-16-bit cache), and results differ from those of a 16-bit cache by the codes' rounding alone, up to 2^-4 of an element.
+its largest element, and grows with it.  Attention reads exactly what is held, in half the bytes of a 16-bit cache.  What is held is off by up to 2^-4 of an element of 2^-6 of its
+block's scale or more (an element alone in setting its scale is 224 to 448 times that), and of a smaller one by up to 2^-10 of the scale, which may be all of it.  Whenever the scale grows,
+elements that then lie below 2^-6 of it are rounded again, by up to 2^-10 of it once more.  Scales do not fall: a drafted token with a large element raises the scale of the
+block it lies in, and whether it is kept or not, the small elements of cached tokens there lose those bits for good, and the block's later tokens are held at that scale.
 Tables, lengths and the new tokens' rows are those of `tree_attention`; everything launches on torch's current stream, reads no device value on the host and can be
 captured.  Nothing of the reference is like it: its engine keeps its cache in 16 bits (reference shapequant/kernels/decode_e2e.py:142-225)."""
 
@@ -79,7 +81,8 @@ def put_tokens8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     """Keys and values k, v [N, Hk, D] (fp16 / bf16, 16-byte aligned heads, any strides) of new tokens put into an 8-bit cache, in place: token t of sequence b, row
     starts[b] + t (int32 [B + 1]; None: N / B each), goes to slot lens[b] + t (sq_put_tokens8); lens (int32 [B]) is left as it is.  most_new: at most so many of a sequence (default:
     N; a bound near the truth makes the launch smaller).  A block's scale is the smallest power of two by which its largest new element is not beyond 448, and not less than the one it has where it
-    holds tokens before lens[b], which are scaled to it when it grows.  Elements that are not finite become NaN.  Sequences must not share pages that are written."""
+    holds tokens before lens[b], which are scaled to it when it grows.  Elements that are not finite become NaN; larger magnitudes than 61,440 in fp16 (1.875 * 2^127 in bf16) are held as that, so that what is
+read is finite in the tokens' type.  Sequences must not share pages that are written."""
     done = _lib.native().put_tokens8(k, v, k_cache, v_cache, k_scale, v_scale, table, lens, starts, most_new)
     if done <= 0:
         if done:
@@ -111,7 +114,8 @@ def tree_attention8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     out: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
     """`tree_attention` over an 8-bit cache: attention of new tokens q [N, Hq, D] (fp16 / bf16) over lens[b] cached tokens of each sequence and, in the slots behind them, its new
     tokens' keys and values, as put_tokens8 puts them there (sq_tree_attention8).  Rows, starts, most_new, mask, scale, out, lse and what a token sees are as there.  Keys and
-    values are what the cache holds, code * scale, exactly in bf16; in fp16 as far as fp16 has them, which is all that put_tokens8 made of fp16 tokens."""
+    values are what the cache holds, code * scale, exactly in bf16; in fp16 as far as fp16 has them, which is all that put_tokens8 made of fp16 tokens.  Lengths are on the device, so work is dealt out
+for sequences that fill their table rows: short ones under a wide table take several times as long, and table[:, :n], n pages at least of the longest one, costs nothing."""
     done = _lib.native().tree_attention8(q, k_cache, v_cache, k_scale, v_scale, table, lens, starts, most_new, mask, scale, out, lse)
     if type(done) is not int:
         return done
@@ -164,7 +168,7 @@ def keep_drafted8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.T
                   counts: torch.Tensor) -> None:
     """`keep_drafted` in 8-bit caches [pages, slots, heads, D] of one layer or [layers, pages, slots, heads, D] of all: new token path[b, i] (int32 [B, m], ascending) of sequence
     b, i < counts[b] (int32 [B]), moves from slot lens[b] + path[b, i] to slot lens[b] + i (sq_keep_drafted8).  A block that tokens move to takes the largest scale of theirs and, where it
-    holds cached tokens, its own.  Entries from the first one on that does not ascend or has no slot are ignored; lens is left as it is.  Sequences must not
+    holds cached tokens, its own (which drafts that are not kept may have raised).  Entries from the first one on that does not ascend or has no slot are ignored; lens is left as it is.  Sequences must not
     share the pages that are written."""
     done = _lib.native().keep_drafted8(k_cache, v_cache, k_scale, v_scale, table, lens, path, counts)
     if done <= 0:
