@@ -13,7 +13,7 @@ namespace sq {
 // A last block of rows that fills at most half of its waves takes 0.6 of the time, and gets as many fewer parts: 8 trees of 32 tokens of 5 heads of 256 per
 // key head (160 rows in blocks of 128) 42.3 us evenly, 39.3 so; with 0.75 42.1.
 // (All times of captured calls, one behind the other; calls back to back take up to 4 % less.)
-// Over a cache held in 8 bits a compute unit holds two of the few-row workgroups (four of heads up to 64), and sequences are also cut into parts of 20 steps a wave, which ends
+// Over a cache held in 8 bits a compute unit holds two of the few-row workgroups (four of heads up to 64 in blocks of 16 rows), and sequences are also cut into parts of 20 steps a wave, which ends
 // them closer together: 64 sequences of 8192 slots x 8 key heads in three parts 205 us, whole 218; of 2,240 to 8,192 131 and 152; 32 of those 72 and 91; 32 of 4000 x 2 key heads of 64 in
 // eight 12.9, in four 14.3.
 // One of up to four steps a wave is not cut (a step takes 0.6 us then: one token behind 500 slots 8.7 us call by call, in four parts 10.1; captured 8.5 and 8.1; of heads of 256 12.1 and 9.9,
@@ -25,8 +25,9 @@ namespace sq {
 // 56.1 and 58.4.  Heads of 256, blocks of 16 and one workgroup a compute unit: 48 per unit and a unit per block (16 new tokens of 5 heads behind 8 x 500 26.1 and 16.6, behind 16 x 500 27.1 and 30.1), up
 // to 32 rows where there are 32 steps (4 behind 32 x 4000 94 and 61; 8 behind 64 x 200 19.6 and 30.8).  Blocks of 16 while all of them run at once and products are few: a step then takes
 // 0.6 us, of 32 1.2 (8 behind 500 9.9 and 12.3, behind 4000 11.9 and 14.0; behind 32,000 25.9 and 22.5).
-// A sequence's length is its table's width here: lengths are on the device.  Under a table of 131,072 slots one token behind 500 takes 10.2 us instead of 8.8, 48 26.7 instead of 21.4,
-// 64 sequences of 500 27.9 instead of 18.6, 64 of 2000 59.8 instead of 53.1.
+// A sequence's length is its table's width here: lengths are on the device.  Under a table of 131,072 slots, over a 16-bit cache, one token behind 500 takes 10.0 us instead of 8.9, 48 25.0 instead
+// of 20.3, 64 sequences of 500 27.1 instead of 18.3, 32 of 4000 57.7 instead of 53.2; over one held in 8 bits, where a batch is then cut into 51 parts and drafts go to tiles, 9.7 instead of 8.3, 21.2 and
+// 10.2, 85.8 and 11.1, 64.9 and 28.3; 64 of 2000 102 and 25.5, 8 new tokens behind 8 x 4000 57 and 21.7, 64 of 500 with heads of 64 50 and 9.3.
 AttnPlan attn_plan(const sq_attention& a, const sq_cache& c, bool held8) {
     AttnPlan p;
     p.dp = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
